@@ -3,7 +3,8 @@
     python -m pulsar_amd.build
 
 produces, next to this file,
-  libpulsar_w4a16.so          HIP kernels + the C ABI of include/pulsar_w4a16.h
+  libpulsar_w4a16.so          HIP kernels + the C ABI of include/pulsar_w4a16.h and
+                              include/pulsar_paged.h
   _pulsar_w4a16_torch.so      at::Tensor API + torch.ops.pulsar registration, and the
                               C++ model layer of include/pulsar_w4a16_model.hpp
                               (torch.classes.pulsar.Qwen3W4A16Layer)
@@ -31,10 +32,11 @@ BUILD = os.path.join(HERE, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ["repack.hip", "gemm_decode.hip", "gemm_prefill.hip", "gemm_prefill_256.hip", "gemm_kwave.hip",
-               "gemm_kwave_f16.hip", "gemm_kwave_bf16.hip", "capi.hip"]
+               "gemm_kwave_f16.hip", "gemm_kwave_bf16.hip", "capi.hip", "paged_attention.hip", "paged_cache.hip",
+               "token_logprobs.hip"]
 LIB_NAME = "libpulsar_w4a16.so"
 TORCH_LIB_NAME = "_pulsar_w4a16_torch.so"
-TORCH_SOURCES = ["torch_ops.cpp", "model.cpp"]
+TORCH_SOURCES = ["torch_ops.cpp", "model.cpp", "paged_ops.cpp"]
 PROBE_SOURCE = "probe.hip"
 PROBE_LIB_NAME = "libpw4_probe.so"
 SELFTEST_SOURCE = "capi_selftest.cpp"

@@ -11,6 +11,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "paged_common.h"
 #include "w4a16_common.h"
 #include "w4a16_kernels.h"
 
@@ -49,6 +50,15 @@ int cu_count() {
     }
     return v;
 }
+
+}  // namespace
+
+namespace pw4 {
+int report_hip_error(hipError_t e) { return hip_fail(e); }
+int device_cus() { return cu_count(); }
+}  // namespace pw4
+
+namespace {
 
 constexpr size_t kAlign = 256;
 size_t align_up(size_t v) { return (v + kAlign - 1) / kAlign * kAlign; }
