@@ -86,10 +86,12 @@ def _run_parallel(cmds: list[list[str]], verbose: bool) -> None:
 
 
 # Per-file extras.  The decode GEMM keeps its small MFMA accumulators in
-# VGPRs (no v_accvgpr moves around every 128-K step); the prefill GEMM needs
-# the AGPRs for its large accumulator tile.
+# VGPRs (no v_accvgpr moves around every 128-K step), and so does the attention
+# (its softmax rescales them); the prefill GEMM needs the AGPRs for its large
+# accumulator tile.
 HIPCC_FILE_FLAGS = {
     "gemm_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -1,12 +1,33 @@
-// Attention of new tokens over a paged cache.
+// Attention of new tokens over a paged cache (the definition: pulsar_paged.h).
 //
-// One wave a query and head.  Keys go by in blocks of 64, a key a lane: the lane
-// sums q . k_j over its key's row, the block's largest score updates the running
-// maximum (running sum and output scaled by e^(old - new)), and the output, four
-// elements of the head a lane at most, takes p_j v_j key by key.
+// Rows.  The `group` query heads that share a key-value head and the new tokens
+// of a sequence make one matrix of n * group query rows (token-major) against
+// the same keys, so one token's group is already a matrix product.  A tile is up
+// to 16 (32) rows of a few-rows call, one tile a sequence, or 128 rows else.
+//
+// Transposed products.  Scores are computed as S^T = K Q^T and outputs as
+// O^T = V^T P^T: in the MFMA result layout a lane then holds scores of one query
+// row only, so the running maximum and sum of the softmax are a lane's own (and
+// one or two half-wave exchanges), and the scores a lane holds are, rounded, the
+// very P^T operand that it has to supply next -- nothing goes through LDS.  K
+// rows are the A operand as they lie; V^T is read by the transposing LDS loads.
+//
+// Keys reach LDS by direct copies (no registers), each lane naming its own
+// source address, so a page may end anywhere.  Page ids come the same way, two
+// blocks ahead.  LDS rows are XOR-swizzled in 16-byte units by permuting the
+// source, so that K's ds_read_b128 and V's transposing reads spread over the
+// banks.  A key index outside what some row of the tile sees is clamped to one
+// that is seen: what lies in unused slots is never read, and masked scores meet
+// only values of seen keys.
+//
+// Splitting.  Where tiles are few, the blocks of keys of all tiles and heads are
+// laid end to end and dealt to the workgroups in equal runs, whatever the
+// lengths; a tile that falls to several is joined by a second launch from fp32
+// partial outputs with their maxima and sums.
 #include "pulsar_paged.h"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "paged_common.h"
@@ -15,7 +36,109 @@ using namespace pw4;
 
 namespace {
 
-using Args = pw4_paged_attention_args;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Params {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    const int32_t* tables;
+    const int32_t* lens;
+    const int32_t* cu;
+    uint16_t* out;
+    float* lse;
+    float* part_o;    // [2 * workgroups, rows of a tile, dim]
+    float* part_ml;   // [2 * workgroups, rows of a tile, 2]: maximum (base 2), sum
+    int64_t q_token, q_head, table_stride;            // elements
+    uint32_t page_stride, row_stride, head_stride;    // elements
+    int32_t* plan;           // split: what the second launch has to know (PlanOut)
+    int32_t num_tokens, batch, q_heads, kv_heads, group, dim, num_pages, page_size, page_shift;
+    int32_t max_q, max_len;  // max_len: keys that tables and caller allow
+    int32_t window;
+    float scale2;            // scale * log2(e); with a cap, scale / cap
+    float cap2;              // cap * log2(e)
+    int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
+    int32_t split;           // 1: runs of units over the grid; 0: a workgroup a tile and head
+};
+
+// ---- small device parts ------------------------------------------------------
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)p; }
+
+// One LDS copy instruction: lane l copies 16 (or 4) bytes from its own address to
+// LDS[lds + l * 16 (or 4)].  Issued from assembly so that the compiler does not
+// wait for it before LDS reads: the kernels count the copies (wait_copies).
+__device__ __forceinline__ void lds_copy16(const void* from, uint32_t lds) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(from), "s"(lds)
+        : "memory");
+}
+__device__ __forceinline__ void lds_copy4(const void* from, uint32_t lds) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %2\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dword %1, off\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(from), "s"(lds)
+        : "memory");
+}
+
+// Until at most N of this wave's copies (and older loads) are under way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ u32x2 read_transposed(const uint8_t* p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    using Lds = __attribute__((address_space(3))) s16x4*;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)(uint32_t)(uintptr_t)p));
+}
+
+// A value of lanes l and l ^ 32, in both lanes; or of l and l ^ 16.  (The elements
+// are copied out first: a bit cast of a vector's element takes its first one.)
+__device__ __forceinline__ f32x2 with_half(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    return f32x2{__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1)};
+}
+__device__ __forceinline__ f32x2 with_quarter(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t r0 = r[0], r1 = r[1];
+    return f32x2{__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1)};
+}
+__device__ __forceinline__ float max_halves(float v) {
+    const f32x2 r = with_half(v);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum_halves(float v) {
+    const f32x2 r = with_half(v);
+    return r[0] + r[1];
+}
+__device__ __forceinline__ float max_quarters(float v) {
+    const f32x2 r = with_quarter(v);
+    return fmaxf(r[0], r[1]);
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+    const f32x2 r = with_quarter(v);
+    return r[0] + r[1];
+}
 
 template <bool BF16>
 __device__ __forceinline__ float to_float(uint16_t u) {
@@ -27,65 +150,1000 @@ __device__ __forceinline__ float to_float(uint16_t u) {
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(64) void simple_kernel(const Args a) {
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    const int group = (int)(a.q_heads / a.kv_heads), D = (int)a.head_dim;
-    int lo = 0, hi = (int)a.batch;  // the row with cu_q[row] <= t < cu_q[row + 1]
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF16) {
+        return pack_bf16x2_rne(lo, hi);
+    } else {
+        return as_u32(f16x2{(_Float16)lo, (_Float16)hi});
+    }
+}
+
+__device__ __forceinline__ int first_above(const int* ends, int n, int v) {
+    int lo = 0, hi = n;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (a.cu_q[mid + 1] > t) {
+        if (ends[mid] > v) {
             hi = mid;
         } else {
             lo = mid + 1;
         }
     }
-    const int b = lo;
-    int begin = 0, end = 0;
-    if (b < a.batch && t >= a.cu_q[b] && t - a.cu_q[b] < a.max_q_len) {
-        const int len = min((int)a.seq_lens[b], (int)a.max_seq_len);
-        const int p = a.seq_lens[b] - (a.cu_q[b + 1] - a.cu_q[b]) + (t - a.cu_q[b]);
-        end = max(0, min(p + 1, min(len, (int)min((int64_t)INT_MAX, a.table_width * a.page_size))));
-        begin = a.window > 0 ? (int)max((int64_t)0, p + 1 - a.window) : 0;
+    return lo;
+}
+
+// A score in units of log2: scale * log2(e) * s, or the capped one.  cap tanh(x) =
+// cap (1 - 2 / (e^2x + 1)).
+template <bool CAP>
+__device__ __forceinline__ float score2(const Params& a, float s) {
+    if constexpr (CAP) {
+        const float e = __builtin_amdgcn_exp2f(s * a.scale2 * (2.f * kLog2e));
+        return a.cap2 - 2.f * a.cap2 * __builtin_amdgcn_rcpf(e + 1.f);
+    } else {
+        return s * a.scale2;
     }
-    const int64_t kv_head = (int64_t)(h / group) * a.kv_head_stride;
-    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + t * a.q_token_stride + h * a.q_head_stride;
-    const uint16_t* const kc = static_cast<const uint16_t*>(a.k_cache) + kv_head;
-    const uint16_t* const vc = static_cast<const uint16_t*>(a.v_cache) + kv_head;
-    float m = -__builtin_inff(), z = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+}
+
+// fp16 probabilities are held times 2^10, so that those of keys far below the
+// maximum are not subnormal; the sum is held the same way, so outputs need nothing.
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.f : 10.f;
+
+// ---- tiles -------------------------------------------------------------------
+
+// The new tokens of sequence b that are computed, and the keys it has.
+struct Sequence {
+    int q0, n, first_pos, len;
+};
+__device__ __forceinline__ Sequence sequence(const Params& a, int b) {
+    const int c0 = a.cu[b], c1 = a.cu[b + 1], l = a.lens[b];
+    Sequence s;
+    s.q0 = min(max(c0, 0), a.num_tokens);
+    s.n = min(max(min(c1, a.num_tokens) - s.q0, 0), a.max_q);
+    s.first_pos = l - (c1 - c0);
+    s.len = min(max(l, 0), a.max_len);
+    return s;
+}
+
+// A tile: query rows [row0, row0 + rows) of a sequence; keys [lo, hi) are those
+// that some row sees, and blocks of keys start at `base`.
+struct Tile {
+    int b, q0, first_pos, len, row0, rows, lo, hi, base;
+};
+template <int MR, int KEYS>
+__device__ __forceinline__ Tile tile_of(const Params& a, int b, int t, const Sequence& s) {
+    Tile r;
+    r.b = b;
+    r.q0 = s.q0;
+    r.first_pos = s.first_pos;
+    r.len = s.len;
+    r.row0 = t * MR;
+    r.rows = min(MR, s.n * a.group - r.row0);
+    const int first = s.first_pos + r.row0 / a.group, last = s.first_pos + (r.row0 + max(r.rows, 1) - 1) / a.group;
+    r.hi = max(0, min(last + 1, s.len));
+    r.lo = a.window > 0 ? max(0, first + 1 - a.window) : 0;
+    if (r.lo >= r.hi) r.lo = r.hi = 0;  // no key
+    r.base = r.lo / KEYS * KEYS;
+    return r;
+}
+// Units of UNIT keys; a tile without keys still has one, whose result is empty.
+template <int UNIT>
+__device__ __forceinline__ int units_of(const Tile& t) {
+    return t.rows <= 0 ? 0 : t.hi > t.lo ? (t.hi - t.base + UNIT - 1) / UNIT : 1;
+}
+
+constexpr int kMaxSplitTiles = 1024;  // tiles and sequences of a split call
+
+// The units of every tile, ascending sums, in LDS: tiles of sequence b are [seq_end[b - 1], seq_end[b]).
+struct Plan {
+    int seq_end[kMaxSplitTiles];
+    int unit_end[kMaxSplitTiles];
+    int scratch[16];
+};
+// Fills the plan; returns the number of tiles.  Every thread of the workgroup calls it.
+template <int MR, int KEYS, int UNIT, int WAVES>
+__device__ __forceinline__ int make_plan(const Params& a, Plan& p) {
+    int tiles = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += WAVES * 64) {
+        const int b = b0 + (int)threadIdx.x;
+        const int mine = b < a.batch ? (sequence(a, b).n * a.group + MR - 1) / MR : 0;
+        int total;
+        const int upto = block_inclusive_scan<WAVES>(mine, p.scratch, total);
+        if (b < a.batch) p.seq_end[b] = tiles + upto;
+        tiles += total;
+    }
+    tiles = min(tiles, kMaxSplitTiles);
+    __syncthreads();
+    int units = 0;
+    for (int t0 = 0; t0 < tiles; t0 += WAVES * 64) {
+        const int t = t0 + (int)threadIdx.x;
+        int mine = 0;
+        if (t < tiles) {
+            const int b = first_above(p.seq_end, a.batch, t);
+            mine = units_of<UNIT>(tile_of<MR, KEYS>(a, b, t - (b ? p.seq_end[b - 1] : 0), sequence(a, b)));
+        }
+        int total;
+        const int upto = block_inclusive_scan<WAVES>(mine, p.scratch, total);
+        if (t < tiles) p.unit_end[t] = units + upto;
+        units += total;
+    }
+    __syncthreads();
+    return tiles;
+}
+
+// Runs of units: workgroup w of `parts` takes [total w / parts, total (w + 1) / parts).
+__device__ __forceinline__ int64_t run_begin(int64_t total, int parts, int w) { return total * w / parts; }
+__device__ __forceinline__ int run_of(int64_t total, int parts, int64_t unit) {
+    return (int)(((unit + 1) * parts + total - 1) / total) - 1;
+}
+__device__ __forceinline__ int split_parts(const Params& a, int64_t total, int grid) {
+    return (int)max((int64_t)1, min((int64_t)grid, total / a.min_units));
+}
+
+// ---- one query row without matrix instructions ---------------------------------
+
+// A wave's pass over keys [begin, end) for one query: for rows that a value which
+// is not finite has reached through a key that they do not see (0 * NaN in a
+// matrix product).  Lane l holds output elements l, l + 64, ...
+struct RowResult {
+    float m2, z, o[4];
+};
+template <bool BF16, bool CAP>
+__device__ __forceinline__ RowResult plain_row(const Params& a, int b, int token, int head, int begin, int end) {
+    const int lane = threadIdx.x & 63;
+    const int64_t kv = (int64_t)((uint64_t)(head / a.group) * a.head_stride);
+    const uint16_t* const q = a.q + token * a.q_token + head * a.q_head;
+    RowResult r{-kInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int j0 = begin; j0 < end; j0 += 64) {
         const int j = j0 + lane;
-        float s = -__builtin_inff();
+        float s = -kInf;
         int64_t at = 0;
         if (j < end) {
-            const int page = a.block_tables[b * a.table_stride + j / a.page_size];
-            at = ((uint32_t)page < (uint64_t)a.num_pages ? page : 0) * a.page_stride + j % a.page_size * a.row_stride;
+            const uint32_t page = min((uint32_t)a.tables[b * a.table_stride + j / a.page_size], (uint32_t)a.num_pages - 1);
+            at = (int64_t)((uint64_t)page * a.page_stride + (uint64_t)(j % a.page_size) * a.row_stride) + kv;
             float dot = 0.f;
-            for (int d = 0; d < D; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(kc[at + d]);
-            s = dot * a.scale;
-            if (a.softcap > 0.f) s = a.softcap * tanhf(s / a.softcap);
+            for (int d = 0; d < a.dim; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(a.k[at + d]);
+            s = score2<CAP>(a, dot);
         }
-        const float m_new = fmaxf(m, wave_max(s));
-        const float shift = m_new == -__builtin_inff() ? 0.f : m_new;
-        const float p = expf(s - shift), scale = expf(m - shift);
-        m = m_new;
-        z = z * scale + wave_sum(p);
-        for (int e = 0; e < 4; ++e) o[e] *= scale;
+        const float m = fmaxf(r.m2, wave_max(s)), shift = m == -kInf ? 0.f : m;
+        const float p = __builtin_amdgcn_exp2f(s - shift), scale = __builtin_amdgcn_exp2f(r.m2 - shift);
+        r.m2 = m;
+        r.z = r.z * scale + wave_sum(p);
+        for (int e = 0; e < 4; ++e) r.o[e] *= scale;
         for (int k = 0; k < 64 && j0 + k < end; ++k) {
             const float pk = __shfl(p, k);
             const int64_t from = __shfl((long long)at, k);
             for (int e = 0; e < 4; ++e) {
-                if (lane + 64 * e < D) o[e] += pk * to_float<BF16>(vc[from + lane + 64 * e]);
+                if (lane + 64 * e < a.dim) r.o[e] += pk * to_float<BF16>(a.v[from + lane + 64 * e]);
             }
         }
     }
-    uint16_t* const out = static_cast<uint16_t*>(a.out) + ((int64_t)t * a.q_heads + h) * D;
-    for (int e = 0; e < 4; ++e) {
-        if (lane + 64 * e < D) out[lane + 64 * e] = f32_to_out<BF16>(z > 0.f ? o[e] / z : z == 0.f ? 0.f : z);
-    }
-    if (a.lse != nullptr && lane == 0) a.lse[(int64_t)t * a.q_heads + h] = m + logf(z);
+    return r;
 }
 
-int check(const Args* a) {
+// ---- copying a block of keys into LDS --------------------------------------------
+
+// 16-byte units of a row, and the XOR that places unit c of row r at c ^ swizzle.
+// K: the 16 lanes of a phase read one unit of 16 rows.  V: the transposing reads of
+// a phase take, of rows that differ in their low bits, 64 bytes of 4 rows (tiles of
+// 32 columns, WIDE) or 32 bytes of 8.  Rows of 128 bytes lie two to the 256 of a phase.
+template <int DP>
+__device__ __forceinline__ int k_swizzle(int r) {
+    return DP == 64 ? (r >> 1) & 7 : r & 15;
+}
+template <int DP, bool WIDE>
+__device__ __forceinline__ int v_swizzle(int r) {
+    if constexpr (WIDE) return DP == 64 ? ((r >> 1) & 1) * 4 : (r & 3) * 4;
+    return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
+}
+
+// Source addresses of a tile's keys.
+struct Source {
+    const uint16_t* k;        // + the key-value head
+    int64_t v_minus_k;        // bytes
+    const int32_t* table;     // the sequence's row
+    uint32_t pages1;          // pages - 1
+    int lo, last;             // keys are clamped to [lo, last]
+};
+__device__ __forceinline__ Source source_of(const Params& a, const Tile& t, int head) {
+    Source s;
+    s.k = a.k + (uint64_t)head * a.head_stride;
+    s.v_minus_k = reinterpret_cast<const uint8_t*>(a.v) - reinterpret_cast<const uint8_t*>(a.k);
+    s.table = a.tables + t.b * a.table_stride;
+    s.pages1 = (uint32_t)a.num_pages - 1;
+    s.lo = t.lo;
+    s.last = t.hi - 1;
+    return s;
+}
+__device__ __forceinline__ int clamp_key(const Source& s, int key) { return min(max(key, s.lo), s.last); }
+__device__ __forceinline__ int page_index(const Params& a, int key) {
+    return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+}
+
+// The page ids of keys first, first + 1, ... (one a lane) into LDS[lds + 4 lane].
+__device__ __forceinline__ void copy_pages(const Params& a, const Source& s, int first, uint32_t lds) {
+    const int key = clamp_key(s, first + (int)(threadIdx.x & 63));
+    lds_copy4(s.table + page_index(a, key), lds);
+}
+
+// ROWS keys from `first` on into K and V stages, `ids` their page ids; a wave's work.
+template <int DP, int ROWS, bool WIDE>
+__device__ __forceinline__ void copy_rows(const Params& a, const Source& s, int first, int row_in_stage, const int* ids,
+                                          uint8_t* k_stage, uint8_t* v_stage) {
+    constexpr int RC = DP / 8;         // units of a row
+    constexpr int PER = 64 / RC;       // rows of an instruction
+    const int lane = threadIdx.x & 63, sub = lane / RC, c = lane % RC;
+    const int valid = a.dim / 8;
+#pragma unroll
+    for (int i = 0; i < ROWS / PER; ++i) {
+        const int r = i * PER + sub, rs = row_in_stage + r;
+        const int key = clamp_key(s, first + r);
+        const uint32_t page = min((uint32_t)ids[r], s.pages1);
+        const int in_page = key - page_index(a, key) * a.page_size;
+        const uint16_t* const row = s.k + ((uint64_t)page * a.page_stride + (uint64_t)(uint32_t)in_page * a.row_stride);
+        int ck = c ^ k_swizzle<DP>(rs), cv = c ^ v_swizzle<DP, WIDE>(rs);
+        if (DP / 8 != valid) {  // a narrower head: the units past it repeat its first ones
+            ck = ck < valid ? ck : ck % valid;
+            cv = cv < valid ? cv : cv % valid;
+        }
+        lds_copy16(row + ck * 8, lds_addr(k_stage) + (row_in_stage + i * PER) * DP * 2);
+        lds_copy16(reinterpret_cast<const uint8_t*>(row + cv * 8) + s.v_minus_k,
+                   lds_addr(v_stage) + (row_in_stage + i * PER) * DP * 2);
+    }
+}
+
+// Query row `row` of the tile as the B operand of K Q^T: 16 bytes of each step of
+// the head, from unit `unit` on, `step` units apart; zeros past the head or the tile.
+template <int STEPS>
+__device__ __forceinline__ void load_query(const Params& a, const Tile& t, int head, int row, int unit, int step,
+                                           u32x4 (&q)[STEPS]) {
+    const bool in = row < t.rows;
+    const int r = t.row0 + min(row, max(t.rows - 1, 0)), i = r / a.group;
+    const uint16_t* const from = a.q + (t.q0 + i) * a.q_token + (head * a.group + r - i * a.group) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+        const int u = unit + s * step;
+        q[s] = u32x4{0, 0, 0, 0};
+        if (in && u * 8 < a.dim) q[s] = *reinterpret_cast<const u32x4*>(from + u * 8);
+    }
+}
+
+// Whether a value of keys [begin, end) is not finite (a wave's scan).
+template <bool BF16>
+__device__ __forceinline__ bool values_not_finite(const Params& a, const Tile& t, int head, int begin, int end) {
+    bool bad = false;
+    for (int key = max(begin, t.lo); key < min(end, t.hi); ++key) {
+        const uint32_t page = min((uint32_t)a.tables[t.b * a.table_stride + page_index(a, key)], (uint32_t)a.num_pages - 1);
+        const uint16_t* const v = a.v + (uint64_t)page * a.page_stride + (uint64_t)head * a.head_stride +
+                                  (uint64_t)(uint32_t)(key - page_index(a, key) * a.page_size) * a.row_stride;
+        for (int d = threadIdx.x & 63; d < a.dim; d += 64) {
+            const float x = to_float<BF16>(v[d]);
+            bad |= x - x != 0.f;
+        }
+    }
+    return __any(bad);
+}
+
+// Whether rows whose output is not finite have to be computed again one by one: some
+// key of [t.lo, t.hi) that not every row sees has a value that is not finite, or the head
+// is narrower than the kernel's (its padding repeats key elements against zeros).
+template <bool BF16>
+__device__ __forceinline__ bool must_repeat(const Params& a, const Tile& t, int head, int dp) {
+    if (a.dim != dp) return true;
+    const int first = t.first_pos + t.row0 / a.group, last = t.first_pos + (t.row0 + t.rows - 1) / a.group;
+    if (values_not_finite<BF16>(a, t, head, first + 1, t.hi)) return true;
+    return a.window > 0 && values_not_finite<BF16>(a, t, head, t.lo, last + 1 - a.window);
+}
+
+// Where a piece of a tile goes: the call's outputs, or partial slot `slot` >= 0.
+template <int MR, bool BF16>
+__device__ __forceinline__ void store_stats(const Params& a, const Tile& t, int head, int row, int slot, float m2, float z) {
+    if (slot >= 0) {
+        float* const ml = a.part_ml + ((int64_t)slot * MR + row) * 2;
+        ml[0] = m2;
+        ml[1] = z;
+    } else if (a.lse != nullptr) {
+        const int r = t.row0 + row, i = r / a.group;
+        a.lse[(int64_t)(t.q0 + i) * a.q_heads + head * a.group + r - i * a.group] =
+            m2 == -kInf ? -kInf : (m2 + (__builtin_amdgcn_logf(z) - kLift<BF16>)) * kLn2;
+    }
+}
+__device__ __forceinline__ uint16_t* out_row(const Params& a, const Tile& t, int head, int row) {
+    const int r = t.row0 + row, i = r / a.group;
+    return a.out + ((int64_t)(t.q0 + i) * a.q_heads + head * a.group + r - i * a.group) * a.dim;
+}
+
+// Rows of out past the last sequence.
+__device__ __forceinline__ void clear_tail(const Params& a) {
+    const int first = a.batch > 0 ? min(max(a.cu[a.batch], 0), a.num_tokens) : 0;
+    const int64_t per_token = (int64_t)a.q_heads * a.dim;
+    for (int t = first + (int)blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+        for (int64_t e = (int64_t)threadIdx.x * 8; e < per_token; e += blockDim.x * 8) {
+            *reinterpret_cast<u32x4*>(a.out + t * per_token + e) = u32x4{0, 0, 0, 0};
+        }
+        if (a.lse != nullptr) {
+            for (int h = threadIdx.x; h < a.q_heads; h += blockDim.x) a.lse[(int64_t)t * a.q_heads + h] = -kInf;
+        }
+    }
+}
+
+// What the second launch of a split call reads: the number of tiles, then for each
+// its ascending units, sequence and place in it.
+struct PlanOut {
+    static constexpr int kTiles = 0, kEnd = 4, kSeq = 4 + kMaxSplitTiles, kPlace = 4 + 2 * kMaxSplitTiles;
+    static constexpr int kInts = 4 + 3 * kMaxSplitTiles;
+};
+
+// A workgroup's pieces of work, one after the other: units [u0, u1) of a tile and
+// head, for partial slot `slot`, or the whole of it (-1).
+template <int MR, int KEYS, int UNIT, int WAVES>
+struct Pieces {
+    Tile t;
+    int head, u0, u1, slot;
+    int64_t at = 0, end = 0;
+    int tiles = 0, units = 0, w = 0;
+    bool fresh = true;
+
+    __device__ __forceinline__ void set_tile(const Params& a, int b, int place) {
+        b = __builtin_amdgcn_readfirstlane(b);
+        t = tile_of<MR, KEYS>(a, b, __builtin_amdgcn_readfirstlane(place), sequence(a, b));
+        t.q0 = __builtin_amdgcn_readfirstlane(t.q0);
+        t.first_pos = __builtin_amdgcn_readfirstlane(t.first_pos);
+        t.len = __builtin_amdgcn_readfirstlane(t.len);
+        t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
+        t.rows = __builtin_amdgcn_readfirstlane(t.rows);
+        t.lo = __builtin_amdgcn_readfirstlane(t.lo);
+        t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+        t.base = __builtin_amdgcn_readfirstlane(t.base);
+    }
+
+    // Every thread of the workgroup calls these two.
+    __device__ __forceinline__ void start(const Params& a, Plan& plan) {
+        if (!a.split) return;
+        tiles = __builtin_amdgcn_readfirstlane(make_plan<MR, KEYS, UNIT, WAVES>(a, plan));
+        units = tiles > 0 ? __builtin_amdgcn_readfirstlane(plan.unit_end[tiles - 1]) : 0;
+        if (blockIdx.x == 0) {
+            if (threadIdx.x == 0) a.plan[PlanOut::kTiles] = tiles;
+            for (int i = threadIdx.x; i < tiles; i += WAVES * 64) {
+                const int b = first_above(plan.seq_end, a.batch, i);
+                a.plan[PlanOut::kEnd + i] = plan.unit_end[i];
+                a.plan[PlanOut::kSeq + i] = b;
+                a.plan[PlanOut::kPlace + i] = i - (b ? plan.seq_end[b - 1] : 0);
+            }
+        }
+        if (units == 0) return;
+        const int64_t total = (int64_t)units * a.kv_heads;
+        const int parts = split_parts(a, total, gridDim.x);
+        // runs side by side on one XCD: workgroups go to the XCDs in turn
+        w = gridDim.x % 8 == 0 ? (int)(blockIdx.x % 8) * ((int)gridDim.x / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+        if (w >= parts) return;
+        at = run_begin(total, parts, w);
+        end = run_begin(total, parts, w + 1);
+    }
+    __device__ __forceinline__ bool next(const Params& a, const Plan& plan) {
+        if (!a.split) {  // tile blockIdx / heads, counted over the sequences, a sequence's last first
+            if (!fresh) return false;
+            fresh = false;
+            head = blockIdx.x % a.kv_heads;
+            const int rank = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63;
+            int before = 0;
+            for (int b0 = 0; b0 < a.batch; b0 += 64) {
+                const int b = b0 + lane;
+                const int mine = b < a.batch ? (sequence(a, b).n * a.group + MR - 1) / MR : 0;
+                const int upto = before + wave_inclusive_scan(mine);
+                const uint64_t past = __ballot(upto > rank);
+                if (past != 0) {
+                    const int l = __builtin_ctzll(past);
+                    set_tile(a, b0 + l, __builtin_amdgcn_readlane(upto, l) - 1 - rank);
+                    u0 = 0;
+                    u1 = units_of<UNIT>(t);
+                    slot = -1;
+                    return true;
+                }
+                before = __builtin_amdgcn_readlane(upto, 63);
+            }
+            return false;
+        }
+        if (at >= end) return false;
+        head = __builtin_amdgcn_readfirstlane((int)(at / units));
+        const int r = (int)(at - (int64_t)head * units);
+        const int ti = __builtin_amdgcn_readfirstlane(first_above(plan.unit_end, tiles, r));
+        const int b = __builtin_amdgcn_readfirstlane(first_above(plan.seq_end, a.batch, ti));
+        const int first = ti ? plan.unit_end[ti - 1] : 0, all = plan.unit_end[ti] - first;
+        set_tile(a, b, ti - (b ? plan.seq_end[b - 1] : 0));
+        u0 = __builtin_amdgcn_readfirstlane(r - first);
+        u1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)all, u0 + (end - at)));
+        slot = __builtin_amdgcn_readfirstlane(u0 == 0 && u1 == all ? -1 : 2 * w + (u0 == 0 ? 1 : 0));
+        at += u1 - u0;
+        return true;
+    }
+};
+
+// ---- few rows --------------------------------------------------------------------
+
+// Up to 16 MT query rows, bound by reading the keys.  Each wave takes blocks of 32
+// keys of its own, through a ring of two stages of its own (no barrier), and the
+// waves' outputs meet in LDS at the end of a piece.
+constexpr int kFewKeys = 32;
+template <int DP>
+constexpr int kFewWaves = DP == 256 ? 2 : 4;
+template <int DP>
+constexpr int kFewUnit = kFewKeys * kFewWaves<DP>;
+template <int DP>
+constexpr int kFewStage = 2 * kFewKeys * DP * 2;  // K and V of a block, bytes
+template <int DP>
+constexpr int kFewRing = 2 * kFewStage<DP> + 4 * 256;  // a wave's: two stages, four sets of page ids
+
+template <int DP, int MT>
+constexpr int few_stage_bytes() {
+    const int ring = kFewWaves<DP> * kFewRing<DP>, join = kFewWaves<DP> * 16 * MT * (DP + 4) * 4;
+    return ring > join ? ring : join;
+}
+
+template <bool BF16, int DP, int MT, bool CAP>
+__global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Params a) {
+    constexpr int WAVES = kFewWaves<DP>, MR = 16 * MT, UNIT = kFewUnit<DP>;
+    constexpr int KS = DP / 32;       // steps of 32 head elements
+    constexpr int DT = DP / 16;       // tiles of 16 output elements
+    constexpr int kCopies = 2 * kFewKeys * DP * 2 / 1024 + 1;  // of a batch: a block, and the ids of the next but one
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
+    uint8_t* const ring = smem + wave * kFewRing<DP>;
+    int* const ids = reinterpret_cast<int*>(ring + 2 * kFewStage<DP>);
+
+    Pieces<MR, kFewKeys, UNIT, WAVES> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, u0 = piece.u0, u1 = piece.u1, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const int begin = t.base + u0 * UNIT, end = min(t.hi, t.base + u1 * UNIT);
+        const int blocks = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
+        const int mine = (blocks - wave + WAVES - 1) / WAVES;  // blocks wave, wave + WAVES, ...
+        u32x4 q[MT][KS];
+        int row_lo[MT], row_hi[MT];  // keys that the lane's row sees
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            load_query<KS>(a, t, head, mt * 16 + c, g, 4, q[mt]);
+            const int pos = t.first_pos + (t.row0 + mt * 16 + c) / a.group;
+            row_hi[mt] = min(pos + 1, t.hi);
+            row_lo[mt] = a.window > 0 ? pos + 1 - a.window : 0;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[mt][st]));  // here, not waited for in the loop
+        }
+        // blocks inside [all_lo, all_hi) are seen by every row of the tile
+        const int all_hi = min(t.first_pos + t.row0 / a.group + 1, t.hi);
+        const int all_lo = a.window > 0 ? t.first_pos + (t.row0 + t.rows - 1) / a.group + 1 - a.window : 0;
+        f32x4 o[MT][DT];
+        float m[MT], z[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -kInf;
+            z[mt] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
+        auto issue = [&](int i) {  // batch i: block i, and the page ids of block i + 2
+            uint8_t* const st = ring + (i & 1) * kFewStage<DP>;
+            copy_rows<DP, kFewKeys, false>(a, src, first_of(i), 0, ids + (i & 3) * 64, st, st + kFewStage<DP> / 2);
+            copy_pages(a, src, first_of(i + 2), lds_addr(ids + ((i + 2) & 3) * 64));
+        };
+        if (mine > 0) {
+            copy_pages(a, src, first_of(0), lds_addr(ids));
+            copy_pages(a, src, first_of(1), lds_addr(ids + 64));
+            wait_copies<0>();
+            issue(0);
+            if (mine > 1) issue(1);
+        }
+        for (int i = 0; i < mine; ++i) {
+            if (i + 1 < mine) {
+                wait_copies<kCopies>();
+            } else {
+                wait_copies<0>();
+            }
+            const uint8_t* const ks = ring + (i & 1) * kFewStage<DP>;
+            const uint8_t* const vs = ks + kFewStage<DP> / 2;
+            const int key0 = first_of(i);
+            f32x4 s[MT][2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                const int r = kt * 16 + c;
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(
+                        ks + r * DP * 2 + (((4 * st + g) ^ k_swizzle<DP>(r)) * 16));
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, q[mt][st], s[mt][kt]);
+                }
+            }
+            const bool masked = key0 < all_lo || key0 + kFewKeys > all_hi;
+            u32x4 p[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float x[8], top = -kInf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = score2<CAP>(a, s[mt][e / 4][e % 4]);
+                    const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
+                    x[e] = masked & ((key < row_lo[mt]) | (key >= row_hi[mt])) ? -kInf : x[e];
+                    top = fmaxf(top, x[e]);
+                }
+                top = max_halves(max_quarters(top));
+                const float m_new = fmaxf(m[mt], top), shift = (m_new == -kInf ? 0.f : m_new) - kLift<BF16>;
+                if (__any(m_new != m[mt])) {
+                    const float scale = __builtin_amdgcn_exp2f(m[mt] - (m_new == -kInf ? 0.f : m_new));
+                    z[mt] *= scale;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[mt][d] *= scale;
+                    m[mt] = m_new;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] - shift);
+                    z[mt] += x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[mt][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+            }
+            // O^T += V^T P^T: step slot 8 g + j is key 4 g + j (j < 4) or 16 + 4 g + j - 4
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                u32x4 vf;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const int r = kt * 16 + 4 * g + c / 4, unit = 2 * d + (c % 4) / 2;
+                    const u32x2 h = read_transposed(vs + r * DP * 2 + ((unit ^ v_swizzle<DP, false>(r)) * 16) + (c & 1) * 8);
+                    vf[2 * kt] = h[0];
+                    vf[2 * kt + 1] = h[1];
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][d] = mfma16x16x32<BF16>(vf, p[mt], o[mt][d]);
+            }
+            // the stage's reads are done (the products have taken them) before it is filled again
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (i + 2 < mine) issue(i + 2);
+        }
+        __syncthreads();  // every wave is done with its ring
+        // ---- join the waves: rows of dim + 4 floats (maximum, sum behind the outputs)
+        constexpr int kRow = DP + 4;
+        float* const join = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float* const row = join + (wave * MR + mt * 16 + c) * kRow;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + 4 * g) = o[mt][d];
+            const float all = sum_halves(sum_quarters(z[mt]));
+            if (g == 0) {
+                row[DP] = m[mt];
+                row[DP + 1] = all;
+            }
+        }
+        __syncthreads();
+        bool bad = false;
+        for (int row = wave; row < t.rows; row += WAVES) {
+            float m2 = -kInf, sum = 0.f, w[WAVES];
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) m2 = fmaxf(m2, join[(v * MR + row) * kRow + DP]);
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) {
+                const float mv = join[(v * MR + row) * kRow + DP];
+                w[v] = mv == -kInf ? 0.f : __builtin_amdgcn_exp2f(mv - m2);
+                sum += w[v] * join[(v * MR + row) * kRow + DP + 1];
+            }
+            const float inv = slot >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+            uint16_t* const to = slot >= 0 ? nullptr : out_row(a, t, head, row);
+            for (int d = lane; d < a.dim; d += 64) {
+                float x = 0.f;
+#pragma unroll
+                for (int v = 0; v < WAVES; ++v) {
+                    if (w[v] != 0.f) x += w[v] * join[(v * MR + row) * kRow + d];
+                }
+                bad |= x - x != 0.f;
+                if (slot >= 0) {
+                    a.part_o[((int64_t)slot * MR + row) * a.dim + d] = x;
+                } else {
+                    to[d] = f32_to_out<BF16>(x * inv);
+                }
+            }
+            if (lane == 0) store_stats<MR, BF16>(a, t, head, row, slot, m2, sum);
+            bad |= sum - sum != 0.f;
+        }
+        if (__any(bad) && must_repeat<BF16>(a, t, head, DP)) {
+            for (int row = wave; row < t.rows; row += WAVES) {
+                const int r = t.row0 + row, i = r / a.group, pos = t.first_pos + i;
+                const int from = max(begin, a.window > 0 ? pos + 1 - a.window : 0), to = min(end, pos + 1);
+                const RowResult x = plain_row<BF16, CAP>(a, t.b, t.q0 + i, head * a.group + r - i * a.group, max(from, 0), to);
+                const float lift = __builtin_amdgcn_exp2f(kLift<BF16>);
+                for (int e = 0; e < 4; ++e) {
+                    const int d = lane + 64 * e;
+                    if (d >= a.dim) continue;
+                    if (slot >= 0) {
+                        a.part_o[((int64_t)slot * MR + row) * a.dim + d] = x.o[e] * lift;
+                    } else {
+                        out_row(a, t, head, row)[d] = f32_to_out<BF16>(x.z == 0.f ? 0.f : x.o[e] / x.z);
+                    }
+                }
+                if (lane == 0) store_stats<MR, BF16>(a, t, head, row, slot, x.m2, x.z * lift);
+            }
+        }
+        __syncthreads();  // the ring is used again
+    }
+    clear_tail(a);
+}
+
+// ---- many rows --------------------------------------------------------------------
+
+// Four waves of 32 query rows each over blocks of 64 keys that they share in LDS,
+// two stages: block i + 1 is copied while block i is worked on.
+constexpr int kManyKeys = 64, kManyWaves = 4, kManyRows = 32 * kManyWaves;
+template <int DP>
+constexpr int kManyStage = 2 * kManyKeys * DP * 2;
+template <int DP>
+constexpr int many_stage_bytes() { return 2 * kManyStage<DP> + kManyWaves * 2 * 256; }
+
+template <bool BF16, int DP, bool CAP>
+__global__ __launch_bounds__(kManyWaves * 64) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
+void many_rows_kernel(const Params a) {
+    constexpr int WAVES = kManyWaves, MR = kManyRows, KEYS = kManyKeys;
+    constexpr int KS = DP / 16;      // steps of 16 head elements
+    constexpr int DT = DP / 32;      // tiles of 32 output elements
+    constexpr int COPY = KEYS / WAVES;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
+    int* const ids = reinterpret_cast<int*>(smem + 2 * kManyStage<DP>) + wave * 128;
+    Pieces<MR, KEYS, KEYS, WAVES> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
+        const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        // the wave's own rows
+        Tile mine = t;
+        mine.row0 = t.row0 + wave * 32;
+        mine.rows = max(0, min(32, t.rows - wave * 32));
+        const int pos0 = t.first_pos + mine.row0 / a.group;
+        const int pos1 = t.first_pos + (mine.row0 + max(mine.rows, 1) - 1) / a.group;
+        mine.hi = mine.rows > 0 ? max(0, min(pos1 + 1, t.hi)) : 0;
+        mine.lo = a.window > 0 ? max(0, pos0 + 1 - a.window) : 0;
+        const int all_hi = min(pos0 + 1, t.hi), all_lo = a.window > 0 ? pos1 + 1 - a.window : 0;
+        const int pos = t.first_pos + (mine.row0 + c) / a.group;
+        const int row_hi = min(pos + 1, t.hi), row_lo = a.window > 0 ? pos + 1 - a.window : 0;
+        u32x4 q[KS];
+        load_query<KS>(a, mine, head, c, h, 2, q);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[st]));  // here, not waited for in the loop
+        f32x16 o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        float m = -kInf, z = 0.f;
+        auto issue = [&](int i) {  // batch i: the wave's rows of block i, and their page ids of block i + 1
+            uint8_t* const st = smem + (i & 1) * kManyStage<DP>;
+            const int first = begin + i * KEYS + wave * COPY;
+            copy_rows<DP, COPY, true>(a, src, first, wave * COPY, ids + (i & 1) * 64, st, st + kManyStage<DP> / 2);
+            copy_pages(a, src, first + KEYS, lds_addr(ids + ((i + 1) & 1) * 64));
+        };
+        if (blocks > 0) {
+            copy_pages(a, src, begin + wave * COPY, lds_addr(ids));
+            wait_copies<0>();
+            issue(0);
+        }
+        for (int i = 0; i < blocks; ++i) {
+            // block i is there, and every wave is done with block i - 1 (in one statement: no
+            // LDS read may move in between)
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (i + 1 < blocks) issue(i + 1);
+            const int key0 = begin + i * KEYS;
+            if (key0 >= mine.hi || key0 + KEYS <= mine.lo) continue;  // no row of the wave sees the block
+            const uint8_t* const ks = smem + (i & 1) * kManyStage<DP>;
+            const uint8_t* const vs = ks + kManyStage<DP> / 2;
+            f32x16 s[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+                const int r = kt * 32 + c;
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(
+                        ks + r * DP * 2 + (((2 * st + h) ^ k_swizzle<DP>(r)) * 16));
+                    s[kt] = mfma32x32x16<BF16>(kf, q[st], s[kt]);
+                }
+            }
+            const bool masked = key0 < all_lo || key0 + KEYS > all_hi;
+            float top = -kInf;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s[kt][e] = score2<CAP>(a, s[kt][e]);
+                }
+            if (masked) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = key0 + kt * 32 + 8 * (e / 4) + 4 * h + e % 4;
+                        s[kt][e] = (key < row_lo) | (key >= row_hi) ? -kInf : s[kt][e];
+                    }
+            }
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kt][e]);
+            top = max_halves(top);
+            const float m_new = fmaxf(m, top), shift = (m_new == -kInf ? 0.f : m_new) - kLift<BF16>;
+            if (__any(m_new != m)) {
+                const float scale = __builtin_amdgcn_exp2f(m - (m_new == -kInf ? 0.f : m_new));
+                z *= scale;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= scale;
+                m = m_new;
+            }
+            u32x4 p[4];  // step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] - shift);
+                    z += x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[st][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+#pragma unroll
+                for (int st = 0; st < 4; ++st) {
+                    u32x4 vf;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int r = st * 16 + half * 8 + 4 * h + (c & 15) / 4;
+                        const int unit = 4 * d + (c >> 4) * 2 + (c & 3) / 2;
+                        const u32x2 x = read_transposed(vs + r * DP * 2 + ((unit ^ v_swizzle<DP, true>(r)) * 16) + (c & 1) * 8);
+                        vf[2 * half] = x[0];
+                        vf[2 * half + 1] = x[1];
+                    }
+                    o[d] = mfma32x32x16<BF16>(vf, p[st], o[d]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        // ---- the lane's row: elements 32 d + 8 (e / 4) + 4 h + e % 4
+        z = sum_halves(z);
+        const bool in = c < mine.rows;
+        const float inv = slot >= 0 ? 1.f : z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
+        bool bad = z - z != 0.f;
+        float* const part = slot >= 0 ? a.part_o + ((int64_t)slot * MR + wave * 32 + c) * a.dim : nullptr;
+        uint16_t* const to = slot >= 0 || !in ? nullptr : out_row(a, mine, head, c);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+#pragma unroll
+            for (int e4 = 0; e4 < 4; ++e4) {
+                const int at = d * 32 + e4 * 8 + h * 4;
+                const f32x4 x{o[d][4 * e4], o[d][4 * e4 + 1], o[d][4 * e4 + 2], o[d][4 * e4 + 3]};
+                if (!in || at >= a.dim) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= x[e] - x[e] != 0.f;
+                if (slot >= 0) {
+                    *reinterpret_cast<f32x4*>(part + at) = x;
+                } else {
+                    *reinterpret_cast<u32x2*>(to + at) = u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
+                }
+            }
+        }
+        if (in && h == 0) {
+            if (slot >= 0) {
+                store_stats<MR, BF16>(a, t, head, wave * 32 + c, slot, m, z);
+            } else {
+                store_stats<MR, BF16>(a, mine, head, c, slot, m, z);
+            }
+        }
+        Tile met = mine;  // the keys that its products met: whole blocks
+        met.lo = max(t.lo, mine.lo - (KEYS - 1));
+        met.hi = min(t.hi, mine.hi + (KEYS - 1));
+        if (__any(in && bad) && must_repeat<BF16>(a, met, head, DP)) {
+            const float lift = __builtin_amdgcn_exp2f(kLift<BF16>);
+            for (int row = 0; row < mine.rows; ++row) {
+                const int r = mine.row0 + row, i = r / a.group, at = t.first_pos + i;
+                const int from = max(begin, a.window > 0 ? at + 1 - a.window : 0);
+                const RowResult x = plain_row<BF16, CAP>(a, t.b, t.q0 + i, head * a.group + r - i * a.group, from, min(end, at + 1));
+                for (int e = 0; e < 4; ++e) {
+                    const int d = lane + 64 * e;
+                    if (d >= a.dim) continue;
+                    if (slot >= 0) {
+                        a.part_o[((int64_t)slot * MR + wave * 32 + row) * a.dim + d] = x.o[e] * lift;
+                    } else {
+                        out_row(a, mine, head, row)[d] = f32_to_out<BF16>(x.z == 0.f ? 0.f : x.o[e] / x.z);
+                    }
+                }
+                if (lane == 0) store_stats<MR, BF16>(a, slot >= 0 ? t : mine, head, slot >= 0 ? wave * 32 + row : row, slot, x.m2, x.z * lift);
+            }
+        }
+        __syncthreads();  // every wave is done with the stages
+    }
+    clear_tail(a);
+}
+
+// ---- joining partial results --------------------------------------------------------
+
+// Tile blockIdx.x / heads, rows blockIdx.y * 4 + wave, + 4 gridDim.y, ...: a wave a row.
+template <int MR, bool BF16>
+__global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
+    const int tiles = a.plan[PlanOut::kTiles], ti = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
+    if (ti >= tiles) return;
+    const int first = ti ? a.plan[PlanOut::kEnd + ti - 1] : 0, last = a.plan[PlanOut::kEnd + ti] - 1;
+    const int units = a.plan[PlanOut::kEnd + tiles - 1];
+    const int64_t total = (int64_t)units * a.kv_heads;
+    const int parts = split_parts(a, total, grid);
+    if (last < first) return;
+    const int w0 = run_of(total, parts, (int64_t)head * units + first), w1 = run_of(total, parts, (int64_t)head * units + last);
+    if (w0 == w1) return;
+    const int lane = threadIdx.x & 63, b = a.plan[PlanOut::kSeq + ti];
+    const Tile t = tile_of<MR, 1>(a, b, a.plan[PlanOut::kPlace + ti], sequence(a, b));
+    const int n = w1 - w0 + 1;
+    auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0); };
+    for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += 4 * gridDim.y) {
+        float m2 = -kInf;
+        for (int i = lane; i < n; i += 64) m2 = fmaxf(m2, a.part_ml[(slot(i) * MR + row) * 2]);
+        m2 = wave_max(m2);
+        float z = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            float w = 0.f;
+            if (i0 + lane < n) {
+                const float* const ml = a.part_ml + (slot(i0 + lane) * MR + row) * 2;
+                w = ml[0] == -kInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m2);
+                z += ml[0] == -kInf && ml[1] == 0.f ? 0.f : w * ml[1];
+            }
+            const int here = min(64, n - i0);
+            for (int i = 0; i < here; ++i) {
+                const float wi = __shfl(w, i);
+                if (wi == 0.f) continue;
+                const float* const o = a.part_o + (slot(i0 + i) * MR + row) * a.dim;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (lane + 64 * e < a.dim) x[e] += wi * o[lane + 64 * e];
+                }
+            }
+        }
+        z = wave_sum(z);
+        const float inv = z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
+        uint16_t* const to = out_row(a, t, head, row);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (lane + 64 * e < a.dim) to[lane + 64 * e] = f32_to_out<BF16>(x[e] * inv);
+        }
+        if (lane == 0) store_stats<MR, BF16>(a, t, head, row, -1, m2, z);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+struct Call {
+    Params p;
+    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), or 128
+    int64_t tiles;             // at most
+    size_t bytes;
+};
+
+int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+
+// Which kernel, tiles and split, from what the host knows.  `a` has passed check().
+Call plan_call(const pw4_paged_attention_args* a) {
+    Call c{};
+    Params& p = c.p;
+    p.q = static_cast<const uint16_t*>(a->q);
+    p.k = static_cast<const uint16_t*>(a->k_cache);
+    p.v = static_cast<const uint16_t*>(a->v_cache);
+    p.tables = a->block_tables;
+    p.lens = a->seq_lens;
+    p.cu = a->cu_q;
+    p.out = static_cast<uint16_t*>(a->out);
+    p.lse = a->lse;
+    p.q_token = a->q_token_stride;
+    p.q_head = a->q_head_stride;
+    p.page_stride = (uint32_t)a->page_stride;
+    p.row_stride = (uint32_t)a->row_stride;
+    p.head_stride = (uint32_t)a->kv_head_stride;
+    p.table_stride = a->table_stride;
+    p.num_tokens = (int32_t)a->num_tokens;
+    p.batch = (int32_t)a->batch;
+    p.q_heads = (int32_t)a->q_heads;
+    p.kv_heads = (int32_t)a->kv_heads;
+    p.group = (int32_t)(a->q_heads / a->kv_heads);
+    p.dim = (int32_t)a->head_dim;
+    p.num_pages = (int32_t)a->num_pages;
+    p.page_size = (int32_t)a->page_size;
+    p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctzll((uint64_t)a->page_size) : -1;
+    p.max_q = (int32_t)std::min(a->max_q_len, a->num_tokens);
+    const int64_t held = a->num_pages == 0 ? 0 : std::min<int64_t>(INT_MAX, a->table_width * a->page_size);
+    p.max_len = (int32_t)std::min(a->max_seq_len, held);
+    p.window = (int32_t)a->window;
+    p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : a->scale * kLog2e;
+    p.cap2 = a->softcap * kLog2e;
+    c.dp = padded_dim(a->head_dim);
+    const int64_t rows = (int64_t)p.max_q * p.group;
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
+    const bool few = c.tile_rows != kManyRows;
+    c.tiles = few ? p.batch
+                  : std::min(a->num_tokens * p.group / kManyRows + p.batch, p.batch * ceil_div(rows, kManyRows));
+    const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
+    const int cus = device_cus();
+    // workgroups that run at once
+    const int slots = few ? (c.dp == 64 ? 2 * cus : cus) : (c.dp == 256 ? cus : 2 * cus);
+    p.min_units = 2;
+    const int64_t most_units = ceil_div(p.max_len, unit) + 1;  // of a tile: its first block may begin early
+    p.split = p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && most_units > 2 * p.min_units &&
+              (few || c.tiles * p.kv_heads < 4 * slots);
+    c.grid = (int)(c.tiles * p.kv_heads);
+    if (p.split) {
+        c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
+        const int64_t rows_held = 2 * (int64_t)c.grid * c.tile_rows;
+        c.bytes = (size_t)(rows_held * (p.dim + 2) + PlanOut::kInts) * 4;
+    }
+    return c;
+}
+
+// Runs a kernel with more LDS than a kernel may have unasked; the permission is
+// asked for once a kernel and device.
+template <auto Kernel>
+hipError_t run(const Call& c, int waves, int stages, hipStream_t s) {
+    const int most = stages + (int)sizeof(Plan), lds = c.p.split ? most : stages;
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+    if (dev < 0 || dev >= 64 || (allowed.load(std::memory_order_relaxed) >> dev & 1) == 0) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != hipSuccess) return e;
+        if (dev >= 0 && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    hipLaunchKernelGGL(Kernel, dim3((unsigned)std::max(c.grid, 1)), dim3(waves * 64), lds, s, c.p);
+    return hipGetLastError();
+}
+
+template <bool BF16, int DP, bool CAP>
+hipError_t launch(const Call& c, hipStream_t s) {
+    hipError_t e;
+    if (c.tile_rows == 16) {
+        e = run<few_rows_kernel<BF16, DP, 1, CAP>>(c, kFewWaves<DP>, few_stage_bytes<DP, 1>(), s);
+    } else if (c.tile_rows == 32) {
+        e = run<few_rows_kernel<BF16, DP, 2, CAP>>(c, kFewWaves<DP>, few_stage_bytes<DP, 2>(), s);
+    } else {
+        e = run<many_rows_kernel<BF16, DP, CAP>>(c, kManyWaves, many_stage_bytes<DP>(), s);
+    }
+    if (e != hipSuccess || !c.p.split) return e;
+    const dim3 grid((unsigned)(c.tiles * c.p.kv_heads), c.tile_rows == kManyRows ? 8 : c.tile_rows / 16);
+    if (c.tile_rows == 16) {
+        hipLaunchKernelGGL((join_kernel<16, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
+    } else if (c.tile_rows == 32) {
+        hipLaunchKernelGGL((join_kernel<32, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
+    } else {
+        hipLaunchKernelGGL((join_kernel<kManyRows, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
+    }
+    return hipGetLastError();
+}
+
+template <bool BF16, int DP>
+hipError_t launch_cap(const Call& c, hipStream_t s) {
+    return c.p.cap2 > 0.f ? launch<BF16, DP, true>(c, s) : launch<BF16, DP, false>(c, s);
+}
+template <bool BF16>
+hipError_t launch_dim(const Call& c, hipStream_t s) {
+    return c.dp == 64 ? launch_cap<BF16, 64>(c, s) : c.dp == 128 ? launch_cap<BF16, 128>(c, s) : launch_cap<BF16, 256>(c, s);
+}
+
+int check(const pw4_paged_attention_args* a) {
     if (a == nullptr) return PW4_ERR_ARG;
     if (a->dtype != PW4_DTYPE_F16 && a->dtype != PW4_DTYPE_BF16) return PW4_ERR_ARG;
     for (int64_t v : {a->num_tokens, a->batch, a->num_pages, a->table_width, a->max_q_len, a->max_seq_len, a->window}) {
@@ -106,6 +1164,10 @@ int check(const Args* a) {
     const uint64_t strides = (uint64_t)(a->q_token_stride | a->q_head_stride | a->page_stride | a->row_stride |
                                         a->kv_head_stride);
     if ((addresses & 15) != 0 || (strides & 7) != 0) return PW4_ERR_ARG;
+    for (int64_t v : {a->page_stride, a->row_stride, a->kv_head_stride}) {
+        if (v < 0) return PW4_ERR_ARG;
+        if (v > INT_MAX) return PW4_ERR_SHAPE;
+    }
     return PW4_OK;
 }
 
@@ -114,24 +1176,26 @@ int check(const Args* a) {
 extern "C" {
 
 size_t pw4_paged_attention_workspace_size(const pw4_paged_attention_args* args) {
-    (void)args;
-    return 0;
+    return check(args) != PW4_OK || args->num_tokens == 0 ? 0 : plan_call(args).bytes;
 }
 
 int pw4_paged_attention(const pw4_paged_attention_args* args, void* workspace, size_t workspace_bytes,
                         pw4_stream_t stream) {
     if (const int rc = check(args)) return rc;
     if (args->num_tokens == 0) return PW4_OK;
-    (void)workspace;
-    (void)workspace_bytes;
-    const dim3 grid((unsigned)args->num_tokens, (unsigned)args->q_heads);
-    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (args->dtype == PW4_DTYPE_BF16) {
-        hipLaunchKernelGGL(simple_kernel<true>, grid, dim3(64), 0, s, *args);
-    } else {
-        hipLaunchKernelGGL(simple_kernel<false>, grid, dim3(64), 0, s, *args);
+    Call c = plan_call(args);
+    if (c.grid > 65535 * 4096 || c.tiles * c.p.kv_heads > INT_MAX) return PW4_ERR_SHAPE;
+    if (c.bytes > 0) {
+        if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < c.bytes) {
+            return PW4_ERR_WORKSPACE;
+        }
+        const int64_t rows = 2 * (int64_t)c.grid * c.tile_rows;
+        c.p.part_o = static_cast<float*>(workspace);
+        c.p.part_ml = c.p.part_o + rows * c.p.dim;
+        c.p.plan = reinterpret_cast<int32_t*>(c.p.part_ml + rows * 2);
     }
-    const hipError_t e = hipGetLastError();
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const hipError_t e = args->dtype == PW4_DTYPE_BF16 ? launch_dim<true>(c, s) : launch_dim<false>(c, s);
     return e == hipSuccess ? PW4_OK : report_hip_error(e);
 }
 
