@@ -53,7 +53,7 @@ extern "C" {
  *            sized by them, longer sequences are cut to them (keys past
  *            max_seq_len are not seen, queries past max_q_len not computed)
  * head_dim: a multiple of 8 up to 256.  Pointers 16-byte aligned, strides
- * multiples of 8. */
+ * multiples of 8, row_stride below 2^24. */
 typedef struct pw4_paged_attention_args {
     const void* q;
     const void* k_cache;

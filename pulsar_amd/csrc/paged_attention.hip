@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 
 #include "paged_common.h"
 
@@ -58,8 +59,10 @@ struct Params {
     int32_t num_tokens, batch, q_heads, kv_heads, group, dim, num_pages, page_size, page_shift;
     int32_t max_q, max_len;  // max_len: keys that tables and caller allow
     int32_t window;
-    float scale2;            // scale * log2(e); with a cap, scale / cap
+    float scale2;            // |scale| log2(e), above 0; with a cap, scale / cap
     float cap2;              // cap * log2(e)
+    uint32_t flip;           // sign bits of q's elements to turn over: a negative scale without a cap
+    int32_t flat;            // 16 keys from a multiple of 16 on lie in one page
     int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
     int32_t split;           // 1: runs of units over the grid; 0: a workgroup a tile and head
 };
@@ -81,6 +84,19 @@ __device__ __forceinline__ void lds_copy16(const void* from, uint32_t lds) {
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
         : "v"(from), "s"(lds)
+        : "memory");
+}
+// The same with a wave-uniform base and a 32-bit byte offset a lane.
+__device__ __forceinline__ void lds_copy16(const void* base, uint32_t offset, uint32_t lds) {
+    uint32_t saved;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(saved)
+        : "v"(offset), "s"(base), "s"(lds)
         : "memory");
 }
 __device__ __forceinline__ void lds_copy4(const void* from, uint32_t lds) {
@@ -171,22 +187,29 @@ __device__ __forceinline__ int first_above(const int* ends, int n, int v) {
     return lo;
 }
 
-// A score in units of log2: scale * log2(e) * s, or the capped one.  cap tanh(x) =
-// cap (1 - 2 / (e^2x + 1)).
+// Scores are held raw, their factor `unit()` (to units of log2) going into the
+// exponent's fma; or, with a cap, in units of log2: cap tanh(x) = cap (1 - 2 / (e^2x + 1)).
 template <bool CAP>
-__device__ __forceinline__ float score2(const Params& a, float s) {
+__device__ __forceinline__ float score(const Params& a, float s) {
     if constexpr (CAP) {
-        const float e = __builtin_amdgcn_exp2f(s * a.scale2 * (2.f * kLog2e));
+        const float e = __builtin_amdgcn_exp2f(s * (a.scale2 * (2.f * kLog2e)));
         return a.cap2 - 2.f * a.cap2 * __builtin_amdgcn_rcpf(e + 1.f);
     } else {
-        return s * a.scale2;
+        return s;
     }
 }
+template <bool CAP>
+__device__ __forceinline__ float unit(const Params& a) {
+    return CAP ? 1.f : a.scale2;
+}
 
-// fp16 probabilities are held times 2^10, so that those of keys far below the
+// fp16 probabilities are held times 2^6, so that those of keys far below the
 // maximum are not subnormal; the sum is held the same way, so outputs need nothing.
 template <bool BF16>
-constexpr float kLift = BF16 ? 0.f : 10.f;
+constexpr float kLift = BF16 ? 0.f : 6.f;
+// The running maximum is renewed, and sums and outputs scaled, once a score is
+// above it by this much (in units of log2): a probability is at most 2^(8 + lift).
+constexpr float kSlack = 8.f;
 
 // ---- tiles -------------------------------------------------------------------
 
@@ -302,7 +325,7 @@ __device__ __forceinline__ RowResult plain_row(const Params& a, int b, int token
             at = (int64_t)((uint64_t)page * a.page_stride + (uint64_t)(j % a.page_size) * a.row_stride) + kv;
             float dot = 0.f;
             for (int d = 0; d < a.dim; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(a.k[at + d]);
-            s = score2<CAP>(a, dot);
+            s = score<CAP>(a, a.flip ? -dot : dot) * unit<CAP>(a);
         }
         const float m = fmaxf(r.m2, wave_max(s)), shift = m == -kInf ? 0.f : m;
         const float p = __builtin_amdgcn_exp2f(s - shift), scale = __builtin_amdgcn_exp2f(r.m2 - shift);
@@ -365,29 +388,59 @@ __device__ __forceinline__ void copy_pages(const Params& a, const Source& s, int
     lds_copy4(s.table + page_index(a, key), lds);
 }
 
-// ROWS keys from `first` on into K and V stages, `ids` their page ids; a wave's work.
-template <int DP, int ROWS, bool WIDE>
-__device__ __forceinline__ void copy_rows(const Params& a, const Source& s, int first, int row_in_stage, const int* ids,
-                                          uint8_t* k_stage, uint8_t* v_stage) {
-    constexpr int RC = DP / 8;         // units of a row
-    constexpr int PER = 64 / RC;       // rows of an instruction
-    const int lane = threadIdx.x & 63, sub = lane / RC, c = lane % RC;
-    const int valid = a.dim / 8;
+// What a lane's 16-byte units of a key's row are, for 16 keys whose first row in the
+// stage is a multiple of 16: the byte offsets of K and V from the 16 keys' first row.
+template <int DP>
+struct Lanes {
+    static constexpr int kUnits = DP / 8, kPer = 64 / kUnits, kSteps = 16 / kPer;  // rows an instruction
+    uint32_t k[kSteps], v[kSteps];
+};
+template <int DP>
+__device__ __forceinline__ int in_head(int unit, int valid) {
+    return DP / 8 == valid || unit < valid ? unit : unit % valid;  // a narrower head: its units again
+}
+template <int DP, bool WIDE>
+__device__ __forceinline__ Lanes<DP> lanes_of(const Params& a) {
+    Lanes<DP> l;
+    const int lane = threadIdx.x & 63, sub = lane / Lanes<DP>::kUnits, c = lane % Lanes<DP>::kUnits;
 #pragma unroll
-    for (int i = 0; i < ROWS / PER; ++i) {
-        const int r = i * PER + sub, rs = row_in_stage + r;
-        const int key = clamp_key(s, first + r);
-        const uint32_t page = min((uint32_t)ids[r], s.pages1);
-        const int in_page = key - page_index(a, key) * a.page_size;
-        const uint16_t* const row = s.k + ((uint64_t)page * a.page_stride + (uint64_t)(uint32_t)in_page * a.row_stride);
-        int ck = c ^ k_swizzle<DP>(rs), cv = c ^ v_swizzle<DP, WIDE>(rs);
-        if (DP / 8 != valid) {  // a narrower head: the units past it repeat its first ones
-            ck = ck < valid ? ck : ck % valid;
-            cv = cv < valid ? cv : cv % valid;
+    for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
+        const int r = i * Lanes<DP>::kPer + sub;
+        const uint32_t row = (uint32_t)r * a.row_stride;
+        l.k[i] = (row + in_head<DP>(c ^ k_swizzle<DP>(r), a.dim / 8) * 8) * 2;
+        l.v[i] = (row + in_head<DP>(c ^ v_swizzle<DP, WIDE>(r), a.dim / 8) * 8) * 2;
+    }
+    return l;
+}
+
+// 16 keys from `first` on (a multiple of 16) into the stages at row `row_in_stage` (one
+// too), `ids` their page ids in LDS; a wave's work, K or V alone or both.
+template <int DP, bool WIDE, bool K, bool V>
+__device__ __forceinline__ void copy_rows(const Params& a, const Source& s, const Lanes<DP>& l, int first, int row_in_stage,
+                                          const int* ids, uint32_t k_stage, uint32_t v_stage) {
+    constexpr int PER = Lanes<DP>::kPer;
+    const uint32_t to = row_in_stage * DP * 2;
+    if (a.flat && first >= s.lo && first + 15 <= s.last) {
+        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(ids[0]), s.pages1);
+        const uint32_t in_page = first - page_index(a, first) * a.page_size;
+        const uint16_t* const row = s.k + ((uint64_t)page * a.page_stride + (uint64_t)in_page * a.row_stride);
+#pragma unroll
+        for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
+            if (K) lds_copy16(row, l.k[i], k_stage + to + i * 1024);
+            if (V) lds_copy16(reinterpret_cast<const uint8_t*>(row) + s.v_minus_k, l.v[i], v_stage + to + i * 1024);
         }
-        lds_copy16(row + ck * 8, lds_addr(k_stage) + (row_in_stage + i * PER) * DP * 2);
-        lds_copy16(reinterpret_cast<const uint8_t*>(row + cv * 8) + s.v_minus_k,
-                   lds_addr(v_stage) + (row_in_stage + i * PER) * DP * 2);
+        return;
+    }
+    const int sub = (threadIdx.x & 63) / Lanes<DP>::kUnits;
+#pragma unroll
+    for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
+        const int r = i * PER + sub, key = clamp_key(s, first + r);
+        const uint32_t page = min((uint32_t)ids[r], s.pages1);
+        const uint32_t in_page = key - page_index(a, key) * a.page_size;
+        const uint8_t* const row = reinterpret_cast<const uint8_t*>(
+            s.k + ((uint64_t)page * a.page_stride + (uint64_t)in_page * a.row_stride - (uint64_t)r * a.row_stride));
+        if (K) lds_copy16(row + l.k[i], k_stage + to + i * 1024);
+        if (V) lds_copy16(row + l.v[i] + s.v_minus_k, v_stage + to + i * 1024);
     }
 }
 
@@ -403,7 +456,7 @@ __device__ __forceinline__ void load_query(const Params& a, const Tile& t, int h
     for (int s = 0; s < STEPS; ++s) {
         const int u = unit + s * step;
         q[s] = u32x4{0, 0, 0, 0};
-        if (in && u * 8 < a.dim) q[s] = *reinterpret_cast<const u32x4*>(from + u * 8);
+        if (in && u * 8 < a.dim) q[s] = *reinterpret_cast<const u32x4*>(from + u * 8) ^ a.flip;
     }
 }
 
@@ -591,6 +644,8 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
     Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
     uint8_t* const ring = smem + wave * kFewRing<DP>;
     int* const ids = reinterpret_cast<int*>(ring + 2 * kFewStage<DP>);
+    const Lanes<DP> lanes = lanes_of<DP, false>(a);
+    const float k = unit<CAP>(a);
 
     Pieces<MR, kFewKeys, UNIT, WAVES> piece;
     piece.start(a, plan);
@@ -626,8 +681,12 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
         }
         auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
         auto issue = [&](int i) {  // batch i: block i, and the page ids of block i + 2
-            uint8_t* const st = ring + (i & 1) * kFewStage<DP>;
-            copy_rows<DP, kFewKeys, false>(a, src, first_of(i), 0, ids + (i & 3) * 64, st, st + kFewStage<DP> / 2);
+            const uint32_t st = lds_addr(ring) + (i & 1) * kFewStage<DP>;
+#pragma unroll
+            for (int r = 0; r < kFewKeys; r += 16) {
+                copy_rows<DP, false, true, true>(a, src, lanes, first_of(i) + r, r, ids + (i & 3) * 64 + r, st,
+                                                 st + kFewStage<DP> / 2);
+            }
             copy_pages(a, src, first_of(i + 2), lds_addr(ids + ((i + 2) & 3) * 64));
         };
         if (mine > 0) {
@@ -667,23 +726,24 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
                 float x[8], top = -kInf;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = score2<CAP>(a, s[mt][e / 4][e % 4]);
+                    x[e] = score<CAP>(a, s[mt][e / 4][e % 4]);
                     const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
                     x[e] = masked & ((key < row_lo[mt]) | (key >= row_hi[mt])) ? -kInf : x[e];
                     top = fmaxf(top, x[e]);
                 }
                 top = max_halves(max_quarters(top));
-                const float m_new = fmaxf(m[mt], top), shift = (m_new == -kInf ? 0.f : m_new) - kLift<BF16>;
-                if (__any(m_new != m[mt])) {
-                    const float scale = __builtin_amdgcn_exp2f(m[mt] - (m_new == -kInf ? 0.f : m_new));
+                const float m_new = fmaxf(m[mt], top);
+                if (__any((m_new - m[mt]) * k > kSlack)) {
+                    const float scale = __builtin_amdgcn_exp2f((m[mt] - (m_new == -kInf ? 0.f : m_new)) * k);
                     z[mt] *= scale;
 #pragma unroll
                     for (int d = 0; d < DT; ++d) o[mt][d] *= scale;
                     m[mt] = m_new;
                 }
+                const float shift = (m[mt] == -kInf ? 0.f : m[mt] * k) - kLift<BF16>;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(x[e] - shift);
+                    x[e] = __builtin_amdgcn_exp2f(x[e] * k - shift);
                     z[mt] += x[e];
                 }
 #pragma unroll
@@ -718,7 +778,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
             for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + 4 * g) = o[mt][d];
             const float all = sum_halves(sum_quarters(z[mt]));
             if (g == 0) {
-                row[DP] = m[mt];
+                row[DP] = m[mt] * k;
                 row[DP + 1] = all;
             }
         }
@@ -797,6 +857,14 @@ void many_rows_kernel(const Params a) {
     const int c = lane & 31, h = lane >> 5;
     Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
     int* const ids = reinterpret_cast<int*>(smem + 2 * kManyStage<DP>) + wave * 128;
+    const Lanes<DP> lanes = lanes_of<DP, true>(a);
+    const float k = unit<CAP>(a);
+    // LDS places of the lane's operands in a stage: K's unit 2 st + h of row c lies st << 5 (in
+    // bits 5 up) away by XOR; V's 4 rows from 4 h on, at columns of tile d, d << 6 away
+    const uint32_t k_at = (uint32_t)(c * DP * 2 + ((h ^ k_swizzle<DP>(c)) * 16));
+    const int vr = 4 * h + ((c & 15) >> 2);
+    const uint32_t v_at = (uint32_t)(kManyStage<DP> / 2 + vr * DP * 2 +
+                                     ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) + (c & 1) * 8);
     Pieces<MR, KEYS, KEYS, WAVES> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
@@ -827,9 +895,10 @@ void many_rows_kernel(const Params a) {
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
         float m = -kInf, z = 0.f;
         auto issue = [&](int i) {  // batch i: the wave's rows of block i, and their page ids of block i + 1
-            uint8_t* const st = smem + (i & 1) * kManyStage<DP>;
+            const uint32_t st = lds_addr(smem) + (i & 1) * kManyStage<DP>;
             const int first = begin + i * KEYS + wave * COPY;
-            copy_rows<DP, COPY, true>(a, src, first, wave * COPY, ids + (i & 1) * 64, st, st + kManyStage<DP> / 2);
+            copy_rows<DP, true, true, true>(a, src, lanes, first, wave * COPY, ids + (i & 1) * 64, st,
+                                            st + kManyStage<DP> / 2);
             copy_pages(a, src, first + KEYS, lds_addr(ids + ((i + 1) & 1) * 64));
         };
         if (blocks > 0) {
@@ -844,30 +913,28 @@ void many_rows_kernel(const Params a) {
             if (i + 1 < blocks) issue(i + 1);
             const int key0 = begin + i * KEYS;
             if (key0 >= mine.hi || key0 + KEYS <= mine.lo) continue;  // no row of the wave sees the block
-            const uint8_t* const ks = smem + (i & 1) * kManyStage<DP>;
-            const uint8_t* const vs = ks + kManyStage<DP> / 2;
+            const uint8_t* const st_at = smem + (i & 1) * kManyStage<DP>;
             f32x16 s[2];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
-                const int r = kt * 32 + c;
-#pragma unroll
-                for (int st = 0; st < KS; ++st) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(
-                        ks + r * DP * 2 + (((2 * st + h) ^ k_swizzle<DP>(r)) * 16));
-                    s[kt] = mfma32x32x16<BF16>(kf, q[st], s[kt]);
-                }
-            }
-            const bool masked = key0 < all_lo || key0 + KEYS > all_hi;
-            float top = -kInf;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[kt][e] = score2<CAP>(a, s[kt][e]);
+                for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) {
+                const uint8_t* const at = st_at + (k_at ^ (st << 5));
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const u32x4 kf = *reinterpret_cast<const u32x4*>(at + kt * 32 * DP * 2);
+                    s[kt] = mfma32x32x16<BF16>(kf, q[st], s[kt]);
                 }
-            if (masked) {
+            }
+            if constexpr (CAP) {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) s[kt][e] = score<CAP>(a, s[kt][e]);
+            }
+            if (key0 < all_lo || key0 + KEYS > all_hi) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -876,26 +943,28 @@ void many_rows_kernel(const Params a) {
                         s[kt][e] = (key < row_lo) | (key >= row_hi) ? -kInf : s[kt][e];
                     }
             }
+            float top = -kInf;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kt][e]);
             top = max_halves(top);
-            const float m_new = fmaxf(m, top), shift = (m_new == -kInf ? 0.f : m_new) - kLift<BF16>;
-            if (__any(m_new != m)) {
-                const float scale = __builtin_amdgcn_exp2f(m - (m_new == -kInf ? 0.f : m_new));
+            const float m_new = fmaxf(m, top);
+            if (__any((m_new - m) * k > kSlack)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (m_new == -kInf ? 0.f : m_new)) * k);
                 z *= scale;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) o[d] *= scale;
                 m = m_new;
             }
+            const float shift = (m == -kInf ? 0.f : m * k) - kLift<BF16>;
             u32x4 p[4];  // step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] - shift);
+                    x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
                     z += x[e];
                 }
 #pragma unroll
@@ -903,14 +972,13 @@ void many_rows_kernel(const Params a) {
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
+                const uint8_t* const at = st_at + (v_at ^ (d << 6));
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
                     u32x4 vf;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const int r = st * 16 + half * 8 + 4 * h + (c & 15) / 4;
-                        const int unit = 4 * d + (c >> 4) * 2 + (c & 3) / 2;
-                        const u32x2 x = read_transposed(vs + r * DP * 2 + ((unit ^ v_swizzle<DP, true>(r)) * 16) + (c & 1) * 8);
+                        const u32x2 x = read_transposed(at + (st * 16 + half * 8) * DP * 2);
                         vf[2 * half] = x[0];
                         vf[2 * half + 1] = x[1];
                     }
@@ -919,6 +987,7 @@ void many_rows_kernel(const Params a) {
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
+        m = m == -kInf ? m : m * k;
         // ---- the lane's row: elements 32 d + 8 (e / 4) + 4 h + e % 4
         z = sum_halves(z);
         const bool in = c < mine.rows;
@@ -1069,7 +1138,10 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const int64_t held = a->num_pages == 0 ? 0 : std::min<int64_t>(INT_MAX, a->table_width * a->page_size);
     p.max_len = (int32_t)std::min(a->max_seq_len, held);
     p.window = (int32_t)a->window;
-    p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : a->scale * kLog2e;
+    // a scale of 0 is held as one that leaves nothing of a score either, so that -inf stays -inf
+    p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : std::max(std::fabs(a->scale) * kLog2e, 0x1p-100f);
+    p.flip = a->softcap > 0.f || a->scale >= 0.f ? 0 : 0x80008000u;
+    p.flat = a->page_size % 16 == 0;
     p.cap2 = a->softcap * kLog2e;
     c.dp = padded_dim(a->head_dim);
     const int64_t rows = (int64_t)p.max_q * p.group;
@@ -1168,6 +1240,7 @@ int check(const pw4_paged_attention_args* a) {
         if (v < 0) return PW4_ERR_ARG;
         if (v > INT_MAX) return PW4_ERR_SHAPE;
     }
+    if (a->row_stride >= 1 << 24) return PW4_ERR_SHAPE;
     return PW4_OK;
 }
 
