@@ -54,7 +54,7 @@ struct Params {
     float* part_o;    // [2 * workgroups, rows of a tile, dim]
     float* part_ml;   // [2 * workgroups, rows of a tile, 2]: maximum (base 2), sum
     int64_t q_token, q_head, table_stride;            // elements
-    uint32_t page_stride, row_stride, head_stride;    // elements
+    uint32_t page_bytes, row_bytes, head_bytes;       // the caches' strides
     int32_t* plan;           // split: what the second launch has to know (PlanOut)
     int32_t num_tokens, batch, q_heads, kv_heads, group, dim, num_pages, page_size, page_shift;
     int32_t max_q, max_len;  // max_len: keys that tables and caller allow
@@ -62,7 +62,7 @@ struct Params {
     float scale2;            // |scale| log2(e), above 0; with a cap, scale / cap
     float cap2;              // cap * log2(e)
     uint32_t flip;           // sign bits of q's elements to turn over: a negative scale without a cap
-    int32_t flat;            // 16 keys from a multiple of 16 on lie in one page
+    int32_t flat;            // pages of a power of two of keys, 16 at least
     int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
     int32_t split;           // 1: runs of units over the grid; 0: a workgroup a tile and head
 };
@@ -71,9 +71,10 @@ struct Params {
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)p; }
 
-// One LDS copy instruction: lane l copies 16 (or 4) bytes from its own address to
-// LDS[lds + l * 16 (or 4)].  Issued from assembly so that the compiler does not
-// wait for it before LDS reads: the kernels count the copies (wait_copies).
+// One LDS copy instruction: lane l copies 16 (or 4) bytes to LDS[lds + l * 16 (or 4)],
+// from its own address, or from a wave-uniform base and its own byte offset.  Issued
+// from assembly so that the compiler does not wait for it before LDS reads: the kernels
+// count the copies (wait_copies).
 __device__ __forceinline__ void lds_copy16(const void* from, uint32_t lds) {
     uint32_t saved;
     asm volatile(
@@ -86,7 +87,6 @@ __device__ __forceinline__ void lds_copy16(const void* from, uint32_t lds) {
         : "v"(from), "s"(lds)
         : "memory");
 }
-// The same with a wave-uniform base and a 32-bit byte offset a lane.
 __device__ __forceinline__ void lds_copy16(const void* base, uint32_t offset, uint32_t lds) {
     uint32_t saved;
     asm volatile(
@@ -313,18 +313,19 @@ struct RowResult {
 template <bool BF16, bool CAP>
 __device__ __forceinline__ RowResult plain_row(const Params& a, int b, int token, int head, int begin, int end) {
     const int lane = threadIdx.x & 63;
-    const int64_t kv = (int64_t)((uint64_t)(head / a.group) * a.head_stride);
+    const uint64_t kv = (uint64_t)(head / a.group) * a.head_bytes;
     const uint16_t* const q = a.q + token * a.q_token + head * a.q_head;
     RowResult r{-kInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int j0 = begin; j0 < end; j0 += 64) {
         const int j = j0 + lane;
         float s = -kInf;
-        int64_t at = 0;
+        uint64_t at = 0;  // bytes
         if (j < end) {
             const uint32_t page = min((uint32_t)a.tables[b * a.table_stride + j / a.page_size], (uint32_t)a.num_pages - 1);
-            at = (int64_t)((uint64_t)page * a.page_stride + (uint64_t)(j % a.page_size) * a.row_stride) + kv;
+            at = (uint64_t)page * a.page_bytes + (uint64_t)(j % a.page_size) * a.row_bytes + kv;
+            const uint16_t* const key = reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.k) + at);
             float dot = 0.f;
-            for (int d = 0; d < a.dim; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(a.k[at + d]);
+            for (int d = 0; d < a.dim; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(key[d]);
             s = score<CAP>(a, a.flip ? -dot : dot) * unit<CAP>(a);
         }
         const float m = fmaxf(r.m2, wave_max(s)), shift = m == -kInf ? 0.f : m;
@@ -334,9 +335,10 @@ __device__ __forceinline__ RowResult plain_row(const Params& a, int b, int token
         for (int e = 0; e < 4; ++e) r.o[e] *= scale;
         for (int k = 0; k < 64 && j0 + k < end; ++k) {
             const float pk = __shfl(p, k);
-            const int64_t from = __shfl((long long)at, k);
+            const uint16_t* const value = reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.v) +
+                                                                            __shfl((unsigned long long)at, k));
             for (int e = 0; e < 4; ++e) {
-                if (lane + 64 * e < a.dim) r.o[e] += pk * to_float<BF16>(a.v[from + lane + 64 * e]);
+                if (lane + 64 * e < a.dim) r.o[e] += pk * to_float<BF16>(value[lane + 64 * e]);
             }
         }
     }
@@ -359,88 +361,89 @@ __device__ __forceinline__ int v_swizzle(int r) {
     return DP == 64 ? ((r >> 1) & 3) * 2 : (r & 7) * 2;
 }
 
-// Source addresses of a tile's keys.
+// Where a tile's keys are.
 struct Source {
-    const uint16_t* k;        // + the key-value head
-    int64_t v_minus_k;        // bytes
-    const int32_t* table;     // the sequence's row
-    uint32_t pages1;          // pages - 1
-    int lo, last;             // keys are clamped to [lo, last]
+    const uint8_t* k;        // of the key-value head
+    const uint8_t* v;
+    const int32_t* table;    // the sequence's row
+    uint32_t pages1;         // pages - 1
+    int lo, last;            // keys are clamped to [lo, last]
 };
 __device__ __forceinline__ Source source_of(const Params& a, const Tile& t, int head) {
-    Source s;
-    s.k = a.k + (uint64_t)head * a.head_stride;
-    s.v_minus_k = reinterpret_cast<const uint8_t*>(a.v) - reinterpret_cast<const uint8_t*>(a.k);
-    s.table = a.tables + t.b * a.table_stride;
-    s.pages1 = (uint32_t)a.num_pages - 1;
-    s.lo = t.lo;
-    s.last = t.hi - 1;
-    return s;
+    const uint64_t at = (uint64_t)head * a.head_bytes;
+    return Source{reinterpret_cast<const uint8_t*>(a.k) + at, reinterpret_cast<const uint8_t*>(a.v) + at,
+                  a.tables + t.b * a.table_stride, (uint32_t)a.num_pages - 1, t.lo, t.hi - 1};
 }
 __device__ __forceinline__ int clamp_key(const Source& s, int key) { return min(max(key, s.lo), s.last); }
 __device__ __forceinline__ int page_index(const Params& a, int key) {
     return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
 }
 
-// The page ids of keys first, first + 1, ... (one a lane) into LDS[lds + 4 lane].
-__device__ __forceinline__ void copy_pages(const Params& a, const Source& s, int first, uint32_t lds) {
-    const int key = clamp_key(s, first + (int)(threadIdx.x & 63));
-    lds_copy4(s.table + page_index(a, key), lds);
+// The lane's key's page id into LDS[lds + 4 lane].
+__device__ __forceinline__ void copy_pages(const Params& a, const Source& s, int key, uint32_t lds) {
+    lds_copy4(s.table + page_index(a, clamp_key(s, key)), lds);
 }
 
 // What a lane's 16-byte units of a key's row are, for 16 keys whose first row in the
-// stage is a multiple of 16: the byte offsets of K and V from the 16 keys' first row.
+// stage is a multiple of 16: byte offsets from the 16 keys' first row.
 template <int DP>
 struct Lanes {
     static constexpr int kUnits = DP / 8, kPer = 64 / kUnits, kSteps = 16 / kPer;  // rows an instruction
-    uint32_t k[kSteps], v[kSteps];
+    uint32_t at[kSteps];
 };
-template <int DP>
-__device__ __forceinline__ int in_head(int unit, int valid) {
-    return DP / 8 == valid || unit < valid ? unit : unit % valid;  // a narrower head: its units again
-}
-template <int DP, bool WIDE>
-__device__ __forceinline__ Lanes<DP> lanes_of(const Params& a) {
+template <int DP, typename F>
+__device__ __forceinline__ Lanes<DP> lanes_of(const Params& a, F swizzle) {
     Lanes<DP> l;
-    const int lane = threadIdx.x & 63, sub = lane / Lanes<DP>::kUnits, c = lane % Lanes<DP>::kUnits;
+    const int lane = threadIdx.x & 63, sub = lane / Lanes<DP>::kUnits, c = lane % Lanes<DP>::kUnits, valid = a.dim / 8;
 #pragma unroll
     for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
         const int r = i * Lanes<DP>::kPer + sub;
-        const uint32_t row = (uint32_t)r * a.row_stride;
-        l.k[i] = (row + in_head<DP>(c ^ k_swizzle<DP>(r), a.dim / 8) * 8) * 2;
-        l.v[i] = (row + in_head<DP>(c ^ v_swizzle<DP, WIDE>(r), a.dim / 8) * 8) * 2;
+        int unit = c ^ swizzle(r);
+        if (DP / 8 != valid && unit >= valid) unit %= valid;  // a narrower head: its units again
+        l.at[i] = (uint32_t)r * a.row_bytes + unit * 16;
     }
     return l;
 }
 
-// 16 keys from `first` on (a multiple of 16) into the stages at row `row_in_stage` (one
-// too), `ids` their page ids in LDS; a wave's work, K or V alone or both.
-template <int DP, bool WIDE, bool K, bool V>
-__device__ __forceinline__ void copy_rows(const Params& a, const Source& s, const Lanes<DP>& l, int first, int row_in_stage,
-                                          const int* ids, uint32_t k_stage, uint32_t v_stage) {
-    constexpr int PER = Lanes<DP>::kPer;
-    const uint32_t to = row_in_stage * DP * 2;
-    if (a.flat && first >= s.lo && first + 15 <= s.last) {
-        const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(ids[0]), s.pages1);
-        const uint32_t in_page = first - page_index(a, first) * a.page_size;
-        const uint16_t* const row = s.k + ((uint64_t)page * a.page_stride + (uint64_t)in_page * a.row_stride);
+// 16 keys from `first` on (a multiple of 16): the byte offset of the first one's row where
+// they lie in one page and all are seen (uniform), `id` being its page's.
+__device__ __forceinline__ bool in_one_page(const Params& a, const Source& s, int first) {
+    return a.flat && first >= s.lo && first + 15 <= s.last;
+}
+__device__ __forceinline__ uint64_t row_of(const Params& a, const Source& s, int first, int id) {
+    const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(id), s.pages1);
+    return (uint64_t)page * a.page_bytes + (uint32_t)(first & (a.page_size - 1)) * a.row_bytes;
+}
+// One plane's rows of 16 keys to LDS[to], from the common row `base`, or (the other keys)
+// each lane from its own page, `ids` being the keys' page ids in LDS.
+template <int DP>
+__device__ __forceinline__ void copy_rows(const uint8_t* base, const Lanes<DP>& l, uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
-            if (K) lds_copy16(row, l.k[i], k_stage + to + i * 1024);
-            if (V) lds_copy16(reinterpret_cast<const uint8_t*>(row) + s.v_minus_k, l.v[i], v_stage + to + i * 1024);
-        }
-        return;
-    }
+    for (int i = 0; i < Lanes<DP>::kSteps; ++i) lds_copy16(base, l.at[i], to + i * 1024);
+}
+template <int DP>
+__device__ __forceinline__ void copy_rows_apart(const Params& a, const Source& s, const uint8_t* plane, const Lanes<DP>& l,
+                                                int first, const int* ids, uint32_t to) {
     const int sub = (threadIdx.x & 63) / Lanes<DP>::kUnits;
 #pragma unroll
     for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
-        const int r = i * PER + sub, key = clamp_key(s, first + r);
-        const uint32_t page = min((uint32_t)ids[r], s.pages1);
-        const uint32_t in_page = key - page_index(a, key) * a.page_size;
-        const uint8_t* const row = reinterpret_cast<const uint8_t*>(
-            s.k + ((uint64_t)page * a.page_stride + (uint64_t)in_page * a.row_stride - (uint64_t)r * a.row_stride));
-        if (K) lds_copy16(row + l.k[i], k_stage + to + i * 1024);
-        if (V) lds_copy16(row + l.v[i] + s.v_minus_k, v_stage + to + i * 1024);
+        const int r = i * Lanes<DP>::kPer + sub, key = clamp_key(s, first + r);
+        const uint32_t page = min((uint32_t)ids[r], s.pages1), in_page = key - page_index(a, key) * a.page_size;
+        const uint64_t at = (uint64_t)page * a.page_bytes + (uint64_t)in_page * a.row_bytes - (uint32_t)r * a.row_bytes;
+        lds_copy16(plane + at + l.at[i], to + i * 1024);
+    }
+}
+// K and V of 16 keys.
+template <int DP>
+__device__ __forceinline__ void copy_both(const Params& a, const Source& s, const Lanes<DP>& lk, const Lanes<DP>& lv, int first,
+                                          const int* ids, uint32_t k_to, uint32_t v_to) {
+    if (in_one_page(a, s, first)) {
+        const uint64_t row = row_of(a, s, first, ids[0]);
+        copy_rows<DP>(s.k + row, lk, k_to);
+        copy_rows<DP>(s.v + row, lv, v_to);
+    } else {
+        copy_rows_apart<DP>(a, s, s.k, lk, first, ids, k_to);
+        copy_rows_apart<DP>(a, s, s.v, lv, first, ids, v_to);
     }
 }
 
@@ -466,8 +469,9 @@ __device__ __forceinline__ bool values_not_finite(const Params& a, const Tile& t
     bool bad = false;
     for (int key = max(begin, t.lo); key < min(end, t.hi); ++key) {
         const uint32_t page = min((uint32_t)a.tables[t.b * a.table_stride + page_index(a, key)], (uint32_t)a.num_pages - 1);
-        const uint16_t* const v = a.v + (uint64_t)page * a.page_stride + (uint64_t)head * a.head_stride +
-                                  (uint64_t)(uint32_t)(key - page_index(a, key) * a.page_size) * a.row_stride;
+        const uint16_t* const v = reinterpret_cast<const uint16_t*>(
+            reinterpret_cast<const uint8_t*>(a.v) + (uint64_t)page * a.page_bytes + (uint64_t)head * a.head_bytes +
+            (uint64_t)(uint32_t)(key - page_index(a, key) * a.page_size) * a.row_bytes);
         for (int d = threadIdx.x & 63; d < a.dim; d += 64) {
             const float x = to_float<BF16>(v[d]);
             bad |= x - x != 0.f;
@@ -644,7 +648,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
     Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
     uint8_t* const ring = smem + wave * kFewRing<DP>;
     int* const ids = reinterpret_cast<int*>(ring + 2 * kFewStage<DP>);
-    const Lanes<DP> lanes = lanes_of<DP, false>(a);
+    const auto lanes_k = lanes_of<DP>(a, k_swizzle<DP>), lanes_v = lanes_of<DP>(a, v_swizzle<DP, false>);
     const float k = unit<CAP>(a);
 
     Pieces<MR, kFewKeys, UNIT, WAVES> piece;
@@ -684,14 +688,14 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
             const uint32_t st = lds_addr(ring) + (i & 1) * kFewStage<DP>;
 #pragma unroll
             for (int r = 0; r < kFewKeys; r += 16) {
-                copy_rows<DP, false, true, true>(a, src, lanes, first_of(i) + r, r, ids + (i & 3) * 64 + r, st,
-                                                 st + kFewStage<DP> / 2);
+                copy_both<DP>(a, src, lanes_k, lanes_v, first_of(i) + r, ids + (i & 3) * 64 + r, st + r * DP * 2,
+                              st + kFewStage<DP> / 2 + r * DP * 2);
             }
-            copy_pages(a, src, first_of(i + 2), lds_addr(ids + ((i + 2) & 3) * 64));
+            copy_pages(a, src, first_of(i + 2) + lane, lds_addr(ids + ((i + 2) & 3) * 64));
         };
         if (mine > 0) {
-            copy_pages(a, src, first_of(0), lds_addr(ids));
-            copy_pages(a, src, first_of(1), lds_addr(ids + 64));
+            copy_pages(a, src, first_of(0) + lane, lds_addr(ids));
+            copy_pages(a, src, first_of(1) + lane, lds_addr(ids + 64));
             wait_copies<0>();
             issue(0);
             if (mine > 1) issue(1);
@@ -840,10 +844,105 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
 // Four waves of 32 query rows each over blocks of 64 keys that they share in LDS,
 // two stages: block i + 1 is copied while block i is worked on.
 constexpr int kManyKeys = 64, kManyWaves = 4, kManyRows = 32 * kManyWaves;
+constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
 constexpr int kManyStage = 2 * kManyKeys * DP * 2;
 template <int DP>
 constexpr int many_stage_bytes() { return 2 * kManyStage<DP> + kManyWaves * 2 * 256; }
+
+// A wave's 32 rows of a tile, a row a lane (and the lane 32 from it).
+template <int KEYS>
+struct WaveRows {
+    Tile mine;             // the rows, and the keys that some of them see
+    int all_lo, all_hi;    // keys that all of them see
+    int row_lo, row_hi;    // keys that the lane's row sees
+    __device__ __forceinline__ WaveRows(const Params& a, const Tile& t, int wave) : mine(t) {
+        mine.row0 = t.row0 + wave * 32;
+        mine.rows = max(0, min(32, t.rows - wave * 32));
+        const int pos0 = t.first_pos + mine.row0 / a.group;
+        const int pos1 = t.first_pos + (mine.row0 + max(mine.rows, 1) - 1) / a.group;
+        const int pos = t.first_pos + (mine.row0 + (int)(threadIdx.x & 31)) / a.group;
+        mine.hi = mine.rows > 0 ? max(0, min(pos1 + 1, t.hi)) : 0;
+        mine.lo = a.window > 0 ? max(0, pos0 + 1 - a.window) : 0;
+        all_hi = min(pos0 + 1, t.hi);
+        all_lo = a.window > 0 ? pos1 + 1 - a.window : 0;
+        row_hi = min(pos + 1, t.hi);
+        row_lo = a.window > 0 ? pos + 1 - a.window : 0;
+    }
+    // Whether some row sees a key of the block from key0 on.
+    __device__ __forceinline__ bool sees(int key0) const { return key0 < mine.hi && key0 + KEYS > mine.lo; }
+    // Scores of keys that the lane's row does not see become -inf: s[kt][e] is key 32 kt +
+    // 8 (e / 4) + 4 h + e % 4 of the block.
+    __device__ __forceinline__ void mask(int key0, int h, f32x16 (&s)[2]) const {
+        if (key0 >= all_lo && key0 + KEYS <= all_hi) return;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int key = key0 + kt * 32 + 8 * (e / 4) + 4 * h + e % 4;
+                s[kt][e] = ((key < row_lo) | (key >= row_hi)) ? -kInf : s[kt][e];
+            }
+    }
+};
+
+// The end of a wave's rows: o[d][e] is element 32 d + 8 (e / 4) + 4 h + e % 4 of the lane's row,
+// m its maximum in units of log2, z the lane's half of its sum, over keys [begin, end).
+template <bool BF16, int DP, int MR, bool CAP>
+__device__ __forceinline__ void store_rows(const Params& a, const Tile& t, const WaveRows<kManyKeys>& r, int wave, int head,
+                                           int slot, int begin, int end, float m, float z, const f32x16 (&o)[DP / 32]) {
+    constexpr int DT = DP / 32;
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    z = sum_halves(z);
+    const bool in = c < r.mine.rows;
+    const float inv = slot >= 0 ? 1.f : z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
+    bool bad = z - z != 0.f;
+    float* const part = slot >= 0 ? a.part_o + ((int64_t)slot * MR + wave * 32 + c) * a.dim : nullptr;
+    uint16_t* const to = slot >= 0 || !in ? nullptr : out_row(a, r.mine, head, c);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+            const int at = d * 32 + e4 * 8 + h * 4;
+            const f32x4 x{o[d][4 * e4], o[d][4 * e4 + 1], o[d][4 * e4 + 2], o[d][4 * e4 + 3]};
+            if (!in || at >= a.dim) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= x[e] - x[e] != 0.f;
+            if (slot >= 0) {
+                *reinterpret_cast<f32x4*>(part + at) = x;
+            } else {
+                *reinterpret_cast<u32x2*>(to + at) = u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
+            }
+        }
+    }
+    if (in && h == 0) {
+        if (slot >= 0) {
+            store_stats<MR, BF16>(a, t, head, wave * 32 + c, slot, m, z);
+        } else {
+            store_stats<MR, BF16>(a, r.mine, head, c, slot, m, z);
+        }
+    }
+    Tile met = r.mine;  // the keys that its products met: whole blocks
+    met.lo = max(t.lo, r.mine.lo - (kManyKeys - 1));
+    met.hi = min(t.hi, r.mine.hi + (kManyKeys - 1));
+    if (__any(in && bad) && must_repeat<BF16>(a, met, head, DP)) {
+        const float lift = __builtin_amdgcn_exp2f(kLift<BF16>);
+        for (int row = 0; row < r.mine.rows; ++row) {
+            const int at_row = r.mine.row0 + row, i = at_row / a.group, at = t.first_pos + i;
+            const int from = max(begin, a.window > 0 ? at + 1 - a.window : 0);
+            const RowResult x = plain_row<BF16, CAP>(a, t.b, t.q0 + i, head * a.group + at_row - i * a.group, from, min(end, at + 1));
+            for (int e = 0; e < 4; ++e) {
+                const int d = lane + 64 * e;
+                if (d >= a.dim) continue;
+                if (slot >= 0) {
+                    a.part_o[((int64_t)slot * MR + wave * 32 + row) * a.dim + d] = x.o[e] * lift;
+                } else {
+                    out_row(a, r.mine, head, row)[d] = f32_to_out<BF16>(x.z == 0.f ? 0.f : x.o[e] / x.z);
+                }
+            }
+            if (lane == 0) store_stats<MR, BF16>(a, slot >= 0 ? t : r.mine, head, slot >= 0 ? wave * 32 + row : row, slot, x.m2, x.z * lift);
+        }
+    }
+}
 
 template <bool BF16, int DP, bool CAP>
 __global__ __launch_bounds__(kManyWaves * 64) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
@@ -857,7 +956,7 @@ void many_rows_kernel(const Params a) {
     const int c = lane & 31, h = lane >> 5;
     Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
     int* const ids = reinterpret_cast<int*>(smem + 2 * kManyStage<DP>) + wave * 128;
-    const Lanes<DP> lanes = lanes_of<DP, true>(a);
+    const auto lanes_k = lanes_of<DP>(a, k_swizzle<DP>), lanes_v = lanes_of<DP>(a, v_swizzle<DP, true>);
     const float k = unit<CAP>(a);
     // LDS places of the lane's operands in a stage: K's unit 2 st + h of row c lies st << 5 (in
     // bits 5 up) away by XOR; V's 4 rows from 4 h on, at columns of tile d, d << 6 away
@@ -873,19 +972,9 @@ void many_rows_kernel(const Params a) {
         const Source src = source_of(a, t, head);
         const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
         const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
-        // the wave's own rows
-        Tile mine = t;
-        mine.row0 = t.row0 + wave * 32;
-        mine.rows = max(0, min(32, t.rows - wave * 32));
-        const int pos0 = t.first_pos + mine.row0 / a.group;
-        const int pos1 = t.first_pos + (mine.row0 + max(mine.rows, 1) - 1) / a.group;
-        mine.hi = mine.rows > 0 ? max(0, min(pos1 + 1, t.hi)) : 0;
-        mine.lo = a.window > 0 ? max(0, pos0 + 1 - a.window) : 0;
-        const int all_hi = min(pos0 + 1, t.hi), all_lo = a.window > 0 ? pos1 + 1 - a.window : 0;
-        const int pos = t.first_pos + (mine.row0 + c) / a.group;
-        const int row_hi = min(pos + 1, t.hi), row_lo = a.window > 0 ? pos + 1 - a.window : 0;
+        const WaveRows<KEYS> r(a, t, wave);
         u32x4 q[KS];
-        load_query<KS>(a, mine, head, c, h, 2, q);
+        load_query<KS>(a, r.mine, head, c, h, 2, q);
 #pragma unroll
         for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[st]));  // here, not waited for in the loop
         f32x16 o[DT];
@@ -894,15 +983,19 @@ void many_rows_kernel(const Params a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
         float m = -kInf, z = 0.f;
-        auto issue = [&](int i) {  // batch i: the wave's rows of block i, and their page ids of block i + 1
-            const uint32_t st = lds_addr(smem) + (i & 1) * kManyStage<DP>;
-            const int first = begin + i * KEYS + wave * COPY;
-            copy_rows<DP, true, true, true>(a, src, lanes, first, wave * COPY, ids + (i & 1) * 64, st,
-                                            st + kManyStage<DP> / 2);
-            copy_pages(a, src, first + KEYS, lds_addr(ids + ((i + 1) & 1) * 64));
+        // page ids come for four blocks of the wave's 16 keys at a time, two sets in LDS
+        auto pages = [&](int set) {
+            copy_pages(a, src, begin + (set * 4 + (lane >> 4)) * KEYS + wave * COPY + (lane & 15), lds_addr(ids + (set & 1) * 64));
+        };
+        auto issue = [&](int i) {  // the wave's rows of block i
+            const uint32_t st = lds_addr(smem) + (i & 1) * kManyStage<DP> + wave * COPY * DP * 2;
+            copy_both<DP>(a, src, lanes_k, lanes_v, begin + i * KEYS + wave * COPY, ids + (i & 7) * 16, st,
+                          st + kManyStage<DP> / 2);
+            if ((i & 3) == 0 && i > 0) pages(i / 4 + 1);  // into the place of set i / 4 - 1, which is done with
         };
         if (blocks > 0) {
-            copy_pages(a, src, begin + wave * COPY, lds_addr(ids));
+            pages(0);
+            pages(1);
             wait_copies<0>();
             issue(0);
         }
@@ -912,21 +1005,25 @@ void many_rows_kernel(const Params a) {
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (i + 1 < blocks) issue(i + 1);
             const int key0 = begin + i * KEYS;
-            if (key0 >= mine.hi || key0 + KEYS <= mine.lo) continue;  // no row of the wave sees the block
+            if (!r.sees(key0)) continue;
             const uint8_t* const st_at = smem + (i & 1) * kManyStage<DP>;
             f32x16 s[2];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+            // products n = (st, kt) in turn, each with the read of an operand kAhead products on behind it
+            auto read_k = [&](int n) {
+                return *reinterpret_cast<const u32x4*>(st_at + (k_at ^ ((n / 2) << 5)) + (n % 2) * 32 * DP * 2);
+            };
+            u32x4 kf[kAhead];
 #pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                const uint8_t* const at = st_at + (k_at ^ (st << 5));
+            for (int n = 0; n < kAhead; ++n) kf[n] = read_k(n);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    const u32x4 kf = *reinterpret_cast<const u32x4*>(at + kt * 32 * DP * 2);
-                    s[kt] = mfma32x32x16<BF16>(kf, q[st], s[kt]);
-                }
+            for (int n = 0; n < 2 * KS; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
+                if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
             }
             if constexpr (CAP) {
 #pragma unroll
@@ -934,15 +1031,7 @@ void many_rows_kernel(const Params a) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) s[kt][e] = score<CAP>(a, s[kt][e]);
             }
-            if (key0 < all_lo || key0 + KEYS > all_hi) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = key0 + kt * 32 + 8 * (e / 4) + 4 * h + e % 4;
-                        s[kt][e] = (key < row_lo) | (key >= row_hi) ? -kInf : s[kt][e];
-                    }
-            }
+            r.mask(key0, h, s);
             float top = -kInf;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -958,88 +1047,224 @@ void many_rows_kernel(const Params a) {
                 m = m_new;
             }
             const float shift = (m == -kInf ? 0.f : m * k) - kLift<BF16>;
-            u32x4 p[4];  // step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4
+            // Step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4.
+            // Products n = (st, d) in turn, each with the read of an operand kAhead products on and a
+            // share of the next step's probabilities behind it.
+            float x[8];
+            auto probability = [&](int st, int e) {
+                x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
+                z += x[e];
+            };
+            auto read_v = [&](int n) {
+                const uint8_t* const at = st_at + (v_at ^ ((n % DT) << 6)) + (n / DT) * 16 * DP * 2;
+                const u32x2 y0 = read_transposed(at), y1 = read_transposed(at + 8 * DP * 2);
+                return u32x4{y0[0], y0[1], y1[0], y1[1]};
+            };
+            u32x4 vf[kAhead], p;
 #pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                float x[8];
+            for (int n = 0; n < kAhead; ++n) vf[n] = read_v(n);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
-                    z += x[e];
+            for (int e = 0; e < 8; ++e) probability(0, e);
+#pragma unroll
+            for (int n = 0; n < 4 * DT; ++n) {
+                const int st = n / DT, d = n % DT;
+                if (d == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+                o[d] = mfma32x32x16<BF16>(vf[n % kAhead], p, o[d]);
+                if (n + kAhead < 4 * DT) vf[n % kAhead] = read_v(n + kAhead);
+                if (st < 3) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[st][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const uint8_t* const at = st_at + (v_at ^ (d << 6));
-#pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    u32x4 vf;
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const u32x2 x = read_transposed(at + (st * 16 + half * 8) * DP * 2);
-                        vf[2 * half] = x[0];
-                        vf[2 * half + 1] = x[1];
-                    }
-                    o[d] = mfma32x32x16<BF16>(vf, p[st], o[d]);
+                    for (int e = d * 8 / DT; e < (d + 1) * 8 / DT; ++e) probability(st + 1, e);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        m = m == -kInf ? m : m * k;
-        // ---- the lane's row: elements 32 d + 8 (e / 4) + 4 h + e % 4
-        z = sum_halves(z);
-        const bool in = c < mine.rows;
-        const float inv = slot >= 0 ? 1.f : z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
-        bool bad = z - z != 0.f;
-        float* const part = slot >= 0 ? a.part_o + ((int64_t)slot * MR + wave * 32 + c) * a.dim : nullptr;
-        uint16_t* const to = slot >= 0 || !in ? nullptr : out_row(a, mine, head, c);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-#pragma unroll
-            for (int e4 = 0; e4 < 4; ++e4) {
-                const int at = d * 32 + e4 * 8 + h * 4;
-                const f32x4 x{o[d][4 * e4], o[d][4 * e4 + 1], o[d][4 * e4 + 2], o[d][4 * e4 + 3]};
-                if (!in || at >= a.dim) continue;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) bad |= x[e] - x[e] != 0.f;
-                if (slot >= 0) {
-                    *reinterpret_cast<f32x4*>(part + at) = x;
-                } else {
-                    *reinterpret_cast<u32x2*>(to + at) = u32x2{pack2<BF16>(x[0] * inv, x[1] * inv), pack2<BF16>(x[2] * inv, x[3] * inv)};
-                }
-            }
-        }
-        if (in && h == 0) {
-            if (slot >= 0) {
-                store_stats<MR, BF16>(a, t, head, wave * 32 + c, slot, m, z);
+        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
+        __syncthreads();  // every wave is done with the stages
+    }
+    clear_tail(a);
+}
+
+// ---- a great many rows -----------------------------------------------------------------
+
+// Eight waves of 32 rows, two on each SIMD, that take turns: while waves 0 to 3 are in
+// their products (scores of block i + 1, outputs of block i), waves 4 to 7 make the
+// probabilities of a block, and the other way round.  Both phases take about as long, so
+// the matrix cores and the vector units are busy together; the same work in any order of
+// the waves' own left each idle half of the time (one prompt of 8192 tokens, 32 heads of
+// 128: 562 us in four-wave workgroups, two a CU).  Waves 0 to 3 copy K, waves 4 to 7 copy
+// V, three blocks of each in LDS.
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideRing = 3;
+template <int DP>
+constexpr int kWideBlock = kManyKeys * DP * 2;  // bytes of K, or of V
+template <int DP>
+constexpr int wide_stage_bytes() { return 2 * kWideRing * kWideBlock<DP> + kWideWaves * 2 * 256; }
+
+template <bool BF16, int DP, bool CAP>
+__global__ __launch_bounds__(kWideWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void wide_rows_kernel(const Params a) {
+    constexpr int MR = kWideRows, KEYS = kManyKeys, KS = DP / 16, DT = DP / 32;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    Plan& plan = *reinterpret_cast<Plan*>(smem + wide_stage_bytes<DP>());
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const bool late = wave >= 4;  // half a turn behind, and copies V
+    int* const ids = reinterpret_cast<int*>(smem + 2 * kWideRing * kWideBlock<DP>) + wave * 128;
+    const uint32_t my_ring = lds_addr(smem) + (late ? kWideRing * kWideBlock<DP> : 0) + (wave & 3) * 16 * DP * 2;
+    const auto lanes = lanes_of<DP>(a, [&](int row) { return late ? v_swizzle<DP, true>(row) : k_swizzle<DP>(row); });
+    const float k = unit<CAP>(a);
+    const uint32_t k_at = (uint32_t)(c * DP * 2 + ((h ^ k_swizzle<DP>(c)) * 16));
+    const int vr = 4 * h + ((c & 15) >> 2);
+    const uint32_t v_at = (uint32_t)(vr * DP * 2 + ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) +
+                                     (c & 1) * 8);
+    Pieces<MR, KEYS, KEYS, kWideWaves> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
+        const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        const WaveRows<KEYS> r(a, t, wave);
+        const uint8_t* const plane = late ? src.v : src.k;
+        const int mine0 = begin + (wave & 3) * 16;  // of block 0, the first key that the wave copies
+        // page ids come for four blocks of the wave's 16 keys at a time, two sets in LDS
+        auto pages = [&](int set) {
+            copy_pages(a, src, mine0 + (set * 4 + (lane >> 4)) * KEYS + (lane & 15), lds_addr(ids + (set & 1) * 64));
+        };
+        auto copy = [&](int j, int place, int id) {  // the wave's keys of block j, `id` the first one's page
+            const int first = mine0 + j * KEYS;
+            const uint32_t to = my_ring + place * kWideBlock<DP>;
+            if (in_one_page(a, src, first)) {
+                copy_rows<DP>(plane + row_of(a, src, first, id), lanes, to);
             } else {
-                store_stats<MR, BF16>(a, mine, head, c, slot, m, z);
+                copy_rows_apart<DP>(a, src, plane, lanes, first, ids + (j & 7) * 16, to);
             }
+        };
+        if (blocks > 0) {
+            pages(0);
+            pages(1);
         }
-        Tile met = mine;  // the keys that its products met: whole blocks
-        met.lo = max(t.lo, mine.lo - (KEYS - 1));
-        met.hi = min(t.hi, mine.hi + (KEYS - 1));
-        if (__any(in && bad) && must_repeat<BF16>(a, met, head, DP)) {
-            const float lift = __builtin_amdgcn_exp2f(kLift<BF16>);
-            for (int row = 0; row < mine.rows; ++row) {
-                const int r = mine.row0 + row, i = r / a.group, at = t.first_pos + i;
-                const int from = max(begin, a.window > 0 ? at + 1 - a.window : 0);
-                const RowResult x = plain_row<BF16, CAP>(a, t.b, t.q0 + i, head * a.group + r - i * a.group, from, min(end, at + 1));
-                for (int e = 0; e < 4; ++e) {
-                    const int d = lane + 64 * e;
-                    if (d >= a.dim) continue;
-                    if (slot >= 0) {
-                        a.part_o[((int64_t)slot * MR + wave * 32 + row) * a.dim + d] = x.o[e] * lift;
-                    } else {
-                        out_row(a, mine, head, row)[d] = f32_to_out<BF16>(x.z == 0.f ? 0.f : x.o[e] / x.z);
+        u32x4 q[KS];
+        load_query<KS>(a, r.mine, head, c, h, 2, q);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[st]));  // here, not waited for in the loop
+        f32x16 o[DT], s[2];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        u32x4 p[4];
+        float m = -kInf, z = 0.f;
+        if (blocks > 0) {
+            wait_copies<0>();
+            copy(0, 0, ids[0]);
+            if (blocks > 1) copy(1, 1, ids[16]);
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (late) asm volatile("s_barrier" ::: "memory");
+            int place = 2;  // ring place of block i + 3
+            for (int i = -1; i < blocks; ++i) {
+                // ---- products: scores of block i + 1, outputs of block i
+                const int next = begin + (i + 1) * KEYS;
+                const int place_next = place == 2 ? 0 : place + 1;  // of blocks i + 1 (and i + 4)
+                const int place_now = place;                        // of blocks i (and i + 3)
+                const bool do_next = i + 1 < blocks && r.sees(next), do_now = i >= 0 && r.sees(next - KEYS);
+                const int id = ids[((i + 3) & 7) * 16];
+                __builtin_amdgcn_s_setprio(1);
+                if (do_next) {
+                    const uint8_t* const st_at = smem + place_next * kWideBlock<DP>;
+                    auto read_k = [&](int n) {
+                        return *reinterpret_cast<const u32x4*>(st_at + (k_at ^ ((n / 2) << 5)) + (n % 2) * 32 * DP * 2);
+                    };
+                    u32x4 kf[kAhead];
+#pragma unroll
+                    for (int n = 0; n < kAhead; ++n) kf[n] = read_k(n);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+#pragma unroll
+                    for (int n = 0; n < 2 * KS; ++n) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
+                        if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
                     }
                 }
-                if (lane == 0) store_stats<MR, BF16>(a, slot >= 0 ? t : mine, head, slot >= 0 ? wave * 32 + row : row, slot, x.m2, x.z * lift);
+                if (do_now) {
+                    const uint8_t* const st_at = smem + (kWideRing + place_now) * kWideBlock<DP>;
+                    auto read_v = [&](int n) {
+                        const uint8_t* const at = st_at + (v_at ^ ((n % DT) << 6)) + (n / DT) * 16 * DP * 2;
+                        const u32x2 y0 = read_transposed(at), y1 = read_transposed(at + 8 * DP * 2);
+                        return u32x4{y0[0], y0[1], y1[0], y1[1]};
+                    };
+                    u32x4 vf[kAhead];
+#pragma unroll
+                    for (int n = 0; n < kAhead; ++n) vf[n] = read_v(n);
+#pragma unroll
+                    for (int n = 0; n < 4 * DT; ++n) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        o[n % DT] = mfma32x32x16<BF16>(vf[n % kAhead], p[n / DT], o[n % DT]);
+                        if (n + kAhead < 4 * DT) vf[n % kAhead] = read_v(n + kAhead);
+                    }
+                }
+                __builtin_amdgcn_s_setprio(0);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                // ---- probabilities of block i + 1; copies of block i + 3
+                if (i + 3 < blocks) {
+                    if (((i + 3) & 3) == 0) pages((i + 3) / 4 + 1);  // into the place of the set before, which is done with
+                    copy(i + 3, place_now, id);
+                }
+                if (do_next) {
+                    if constexpr (CAP) {
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) s[kt][e] = score<CAP>(a, s[kt][e]);
+                    }
+                    r.mask(next, h, s);
+                    float top = -kInf;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kt][e]);
+                    top = max_halves(top);
+                    const float m_new = fmaxf(m, top);
+                    if (__any((m_new - m) * k > kSlack)) {
+                        const float scale = __builtin_amdgcn_exp2f((m - (m_new == -kInf ? 0.f : m_new)) * k);
+                        z *= scale;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) o[d] *= scale;
+                        m = m_new;
+                    }
+                    const float shift = (m == -kInf ? 0.f : m * k) - kLift<BF16>;
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
+                            z += x[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[st][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+                    }
+                }
+                // the last turn's copies have landed; this turn's may be under way
+                if (i + 3 < blocks) {
+                    wait_copies<Lanes<DP>::kSteps>();
+                } else {
+                    wait_copies<0>();
+                }
+                asm volatile("s_barrier" ::: "memory");
+                place = place_next;
             }
+            if (!late) asm volatile("s_barrier" ::: "memory");
         }
-        __syncthreads();  // every wave is done with the stages
+        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
+        __syncthreads();  // every wave is done with the ring
     }
     clear_tail(a);
 }
@@ -1100,7 +1325,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
 
 struct Call {
     Params p;
-    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), or 128
+    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128 or 256
     int64_t tiles;             // at most
     size_t bytes;
 };
@@ -1121,9 +1346,9 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.lse = a->lse;
     p.q_token = a->q_token_stride;
     p.q_head = a->q_head_stride;
-    p.page_stride = (uint32_t)a->page_stride;
-    p.row_stride = (uint32_t)a->row_stride;
-    p.head_stride = (uint32_t)a->kv_head_stride;
+    p.page_bytes = (uint32_t)a->page_stride * 2;
+    p.row_bytes = (uint32_t)a->row_stride * 2;
+    p.head_bytes = (uint32_t)a->kv_head_stride * 2;
     p.table_stride = a->table_stride;
     p.num_tokens = (int32_t)a->num_tokens;
     p.batch = (int32_t)a->batch;
@@ -1141,18 +1366,18 @@ Call plan_call(const pw4_paged_attention_args* a) {
     // a scale of 0 is held as one that leaves nothing of a score either, so that -inf stays -inf
     p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : std::max(std::fabs(a->scale) * kLog2e, 0x1p-100f);
     p.flip = a->softcap > 0.f || a->scale >= 0.f ? 0 : 0x80008000u;
-    p.flat = a->page_size % 16 == 0;
+    p.flat = p.page_shift >= 4 && (uint64_t)a->page_size * p.row_bytes <= UINT32_MAX;
     p.cap2 = a->softcap * kLog2e;
-    c.dp = padded_dim(a->head_dim);
     const int64_t rows = (int64_t)p.max_q * p.group;
-    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
-    const bool few = c.tile_rows != kManyRows;
+    c.dp = padded_dim(a->head_dim);
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= kManyRows || c.dp == 256 ? kManyRows : kWideRows;
+    const bool few = c.tile_rows <= 32;
     c.tiles = few ? p.batch
-                  : std::min(a->num_tokens * p.group / kManyRows + p.batch, p.batch * ceil_div(rows, kManyRows));
+                  : std::min(a->num_tokens * p.group / c.tile_rows + p.batch, p.batch * ceil_div(rows, c.tile_rows));
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     const int cus = device_cus();
     // workgroups that run at once
-    const int slots = few ? (c.dp == 64 ? 2 * cus : cus) : (c.dp == 256 ? cus : 2 * cus);
+    const int slots = few ? (c.dp == 64 ? 2 * cus : cus) : c.tile_rows == kManyRows && c.dp != 256 ? 2 * cus : cus;
     p.min_units = 2;
     const int64_t most_units = ceil_div(p.max_len, unit) + 1;  // of a tile: its first block may begin early
     p.split = p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && most_units > 2 * p.min_units &&
@@ -1191,17 +1416,23 @@ hipError_t launch(const Call& c, hipStream_t s) {
         e = run<few_rows_kernel<BF16, DP, 1, CAP>>(c, kFewWaves<DP>, few_stage_bytes<DP, 1>(), s);
     } else if (c.tile_rows == 32) {
         e = run<few_rows_kernel<BF16, DP, 2, CAP>>(c, kFewWaves<DP>, few_stage_bytes<DP, 2>(), s);
-    } else {
+    } else if (c.tile_rows == kManyRows) {
         e = run<many_rows_kernel<BF16, DP, CAP>>(c, kManyWaves, many_stage_bytes<DP>(), s);
+    } else if constexpr (DP < 256) {
+        e = run<wide_rows_kernel<BF16, DP, CAP>>(c, kWideWaves, wide_stage_bytes<DP>(), s);
+    } else {
+        e = hipErrorInvalidValue;  // no such tile: plan_call
     }
     if (e != hipSuccess || !c.p.split) return e;
-    const dim3 grid((unsigned)(c.tiles * c.p.kv_heads), c.tile_rows == kManyRows ? 8 : c.tile_rows / 16);
+    const dim3 grid((unsigned)(c.tiles * c.p.kv_heads), c.tile_rows / 16);
     if (c.tile_rows == 16) {
         hipLaunchKernelGGL((join_kernel<16, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
     } else if (c.tile_rows == 32) {
         hipLaunchKernelGGL((join_kernel<32, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
-    } else {
+    } else if (c.tile_rows == kManyRows) {
         hipLaunchKernelGGL((join_kernel<kManyRows, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
+    } else {
+        hipLaunchKernelGGL((join_kernel<kWideRows, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
     }
     return hipGetLastError();
 }
