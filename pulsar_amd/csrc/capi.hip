@@ -86,6 +86,11 @@ bool plan_overrides() {
     return enabled;
 }
 const char* plan_env(const char* name) { return plan_overrides() ? std::getenv(name) : nullptr; }
+}  // namespace
+namespace pw4 {
+const char* plan_override(const char* name) { return plan_env(name); }
+}  // namespace pw4
+namespace {
 
 // Act-order repack overrides for tuning sweeps and tests: the column block
 // width (8, 16, 32 or 64) and the number of workgroups; unset = heuristic.

@@ -30,6 +30,7 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 #include "paged_common.h"
 
@@ -56,13 +57,16 @@ struct Params {
     int64_t q_token, q_head, table_stride;            // elements
     uint32_t page_bytes, row_bytes, head_bytes;       // the caches' strides
     int32_t* plan;           // split: what the second launch has to know (PlanOut)
-    int32_t num_tokens, batch, q_heads, kv_heads, group, dim, num_pages, page_size, page_shift;
+    int32_t num_tokens, batch, q_heads, kv_heads, group, dim, num_pages, page_size;
+    int32_t page_shift;      // of a page size that is a power of two, else -1
+    uint32_t page_magic;     // else key / page_size = (key * page_magic) >> (32 + page_magic_shift)
+    int32_t page_magic_shift;
     int32_t max_q, max_len;  // max_len: keys that tables and caller allow
     int32_t window;
     float scale2;            // |scale| log2(e), above 0; with a cap, scale / cap
     float cap2;              // cap * log2(e)
     uint32_t flip;           // sign bits of q's elements to turn over: a negative scale without a cap
-    int32_t flat;            // pages of a power of two of keys, 16 at least
+    int32_t flat;            // 2: pages of a power of two of keys, 16 at least; 1: of a multiple of 8
     int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
     int32_t split;           // 1: runs of units over the grid; 0: a workgroup a tile and head
 };
@@ -170,7 +174,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     if constexpr (BF16) {
         return pack_bf16x2_rne(lo, hi);
     } else {
-        return as_u32(f16x2{(_Float16)lo, (_Float16)hi});
+        return as_u32(__builtin_convertvector((f32x2{lo, hi}), f16x2));
     }
 }
 
@@ -293,14 +297,21 @@ __device__ __forceinline__ int make_plan(const Params& a, Plan& p) {
     return tiles;
 }
 
-// Runs of units: workgroup w of `parts` takes [total w / parts, total (w + 1) / parts).
-__device__ __forceinline__ int64_t run_begin(int64_t total, int parts, int w) { return total * w / parts; }
-__device__ __forceinline__ int run_of(int64_t total, int parts, int64_t unit) {
-    return (int)(((unit + 1) * parts + total - 1) / total) - 1;
-}
-__device__ __forceinline__ int split_parts(const Params& a, int64_t total, int grid) {
-    return (int)max((int64_t)1, min((int64_t)grid, total / a.min_units));
-}
+// The units of all tiles and heads, `total` of them, in `parts` runs that differ by one at
+// most.  (The host keeps total below 2^31.)
+struct Runs {
+    int parts, each, more;  // the first `more` runs have each + 1 units
+    __device__ __forceinline__ Runs(const Params& a, int total, int grid) {
+        parts = max(1, min(grid, total / a.min_units));
+        each = total / parts;
+        more = total - each * parts;
+    }
+    __device__ __forceinline__ int begin(int w) const { return w * each + min(w, more); }
+    __device__ __forceinline__ int of(int unit) const {  // the run that a unit is in
+        const int longer = more * (each + 1);
+        return unit < longer ? unit / (each + 1) : more + (unit - longer) / max(each, 1);
+    }
+};
 
 // ---- one query row without matrix instructions ---------------------------------
 
@@ -376,7 +387,7 @@ __device__ __forceinline__ Source source_of(const Params& a, const Tile& t, int 
 }
 __device__ __forceinline__ int clamp_key(const Source& s, int key) { return min(max(key, s.lo), s.last); }
 __device__ __forceinline__ int page_index(const Params& a, int key) {
-    return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+    return a.page_shift >= 0 ? key >> a.page_shift : (int)(__umulhi((uint32_t)key, a.page_magic) >> a.page_magic_shift);
 }
 
 // The lane's key's page id into LDS[lds + 4 lane].
@@ -405,32 +416,51 @@ __device__ __forceinline__ Lanes<DP> lanes_of(const Params& a, F swizzle) {
     return l;
 }
 
-// 16 keys from `first` on (a multiple of 16): the byte offset of the first one's row where
-// they lie in one page and all are seen (uniform), `id` being its page's.
+// 16 keys from `first` on (a multiple of 16).  Where they lie in one page and all are seen,
+// the byte offset of the first one's row (uniform), `id` being its page's, is all there is
+// to find out.
+__device__ __forceinline__ bool all_seen(const Source& s, int first) { return first >= s.lo && first + 15 <= s.last; }
 __device__ __forceinline__ bool in_one_page(const Params& a, const Source& s, int first) {
-    return a.flat && first >= s.lo && first + 15 <= s.last;
+    return a.flat == 2 && all_seen(s, first);
 }
 __device__ __forceinline__ uint64_t row_of(const Params& a, const Source& s, int first, int id) {
     const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(id), s.pages1);
     return (uint64_t)page * a.page_bytes + (uint32_t)(first & (a.page_size - 1)) * a.row_bytes;
 }
-// One plane's rows of 16 keys to LDS[to], from the common row `base`, or (the other keys)
-// each lane from its own page, `ids` being the keys' page ids in LDS.
+// A plane's rows of 16 keys to LDS[to], from the common row `base`.
 template <int DP>
 __device__ __forceinline__ void copy_rows(const uint8_t* base, const Lanes<DP>& l, uint32_t to) {
 #pragma unroll
     for (int i = 0; i < Lanes<DP>::kSteps; ++i) lds_copy16(base, l.at[i], to + i * 1024);
 }
-template <int DP>
+// One or two planes' rows of 16 keys that lie in several pages or are not all seen, `ids`
+// being the keys' page ids in LDS: an instruction's rows from their common page (pages of
+// multiples of 8 keys; an instruction takes 8, 4 or 2), or each lane's from its own.
+template <int DP, bool BOTH>
 __device__ __forceinline__ void copy_rows_apart(const Params& a, const Source& s, const uint8_t* plane, const Lanes<DP>& l,
-                                                int first, const int* ids, uint32_t to) {
+                                                uint32_t to, const uint8_t* plane2, const Lanes<DP>& l2, uint32_t to2,
+                                                int first, const int* ids) {
+    constexpr int PER = Lanes<DP>::kPer;
+    if (a.flat && all_seen(s, first)) {
+#pragma unroll
+        for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
+            const int key = first + i * PER;
+            const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(ids[i * PER]), s.pages1);
+            const uint32_t in_page = key - page_index(a, key) * a.page_size;
+            const uint64_t at = (uint64_t)page * a.page_bytes + in_page * a.row_bytes - (uint64_t)(i * PER) * a.row_bytes;
+            lds_copy16(plane + at, l.at[i], to + i * 1024);
+            if (BOTH) lds_copy16(plane2 + at, l2.at[i], to2 + i * 1024);
+        }
+        return;
+    }
     const int sub = (threadIdx.x & 63) / Lanes<DP>::kUnits;
 #pragma unroll
     for (int i = 0; i < Lanes<DP>::kSteps; ++i) {
-        const int r = i * Lanes<DP>::kPer + sub, key = clamp_key(s, first + r);
+        const int r = i * PER + sub, key = clamp_key(s, first + r);
         const uint32_t page = min((uint32_t)ids[r], s.pages1), in_page = key - page_index(a, key) * a.page_size;
         const uint64_t at = (uint64_t)page * a.page_bytes + (uint64_t)in_page * a.row_bytes - (uint32_t)r * a.row_bytes;
         lds_copy16(plane + at + l.at[i], to + i * 1024);
+        if (BOTH) lds_copy16(plane2 + at + l2.at[i], to2 + i * 1024);
     }
 }
 // K and V of 16 keys.
@@ -442,8 +472,7 @@ __device__ __forceinline__ void copy_both(const Params& a, const Source& s, cons
         copy_rows<DP>(s.k + row, lk, k_to);
         copy_rows<DP>(s.v + row, lv, v_to);
     } else {
-        copy_rows_apart<DP>(a, s, s.k, lk, first, ids, k_to);
-        copy_rows_apart<DP>(a, s, s.v, lv, first, ids, v_to);
+        copy_rows_apart<DP, true>(a, s, s.k, lk, k_to, s.v, lv, v_to, first, ids);
     }
 }
 
@@ -523,22 +552,32 @@ __device__ __forceinline__ void clear_tail(const Params& a) {
     }
 }
 
-// What the second launch of a split call reads: the number of tiles, then for each
-// its ascending units, sequence and place in it.
+// What the second launch of a split call reads: the tiles and units there are, then for
+// each tile its ascending units and where its rows lie.
 struct PlanOut {
-    static constexpr int kTiles = 0, kEnd = 4, kSeq = 4 + kMaxSplitTiles, kPlace = 4 + 2 * kMaxSplitTiles;
-    static constexpr int kInts = 4 + 3 * kMaxSplitTiles;
+    static constexpr int kTiles = 0, kUnits = 1, kEntries = 4;
+    struct Entry {
+        int begin, end, q0, row0, rows, pad[3];
+    };
+    static constexpr int kInts = kEntries + 8 * kMaxSplitTiles;
 };
+__device__ __forceinline__ void write_plan(const Params& a, int i, int begin, int end, const Tile& t) {
+    reinterpret_cast<PlanOut::Entry*>(a.plan + PlanOut::kEntries)[i] = PlanOut::Entry{begin, end, t.q0, t.row0, t.rows, {}};
+}
 
 // A workgroup's pieces of work, one after the other: units [u0, u1) of a tile and
-// head, for partial slot `slot`, or the whole of it (-1).
-template <int MR, int KEYS, int UNIT, int WAVES>
+// head, for partial slot `slot`, or the whole of it (-1).  ONE: a sequence has one tile.
+template <int MR, int KEYS, int UNIT, int WAVES, bool ONE>
 struct Pieces {
     Tile t;
     int head, u0, u1, slot;
-    int64_t at = 0, end = 0;
-    int tiles = 0, units = 0, w = 0;
+    int at = 0, end = 0, tiles = 0, units = 0, w = 0;
+    // ONE, up to 64 sequences: the tile of sequence `lane` and its ascending units, and no plan in LDS
+    Tile my;
+    int my_end = 0;
     bool fresh = true;
+
+    __device__ __forceinline__ bool in_wave(const Params& a) const { return ONE && a.batch <= 64; }
 
     __device__ __forceinline__ void set_tile(const Params& a, int b, int place) {
         b = __builtin_amdgcn_readfirstlane(b);
@@ -556,25 +595,40 @@ struct Pieces {
     // Every thread of the workgroup calls these two.
     __device__ __forceinline__ void start(const Params& a, Plan& plan) {
         if (!a.split) return;
-        tiles = __builtin_amdgcn_readfirstlane(make_plan<MR, KEYS, UNIT, WAVES>(a, plan));
-        units = tiles > 0 ? __builtin_amdgcn_readfirstlane(plan.unit_end[tiles - 1]) : 0;
-        if (blockIdx.x == 0) {
-            if (threadIdx.x == 0) a.plan[PlanOut::kTiles] = tiles;
-            for (int i = threadIdx.x; i < tiles; i += WAVES * 64) {
-                const int b = first_above(plan.seq_end, a.batch, i);
-                a.plan[PlanOut::kEnd + i] = plan.unit_end[i];
-                a.plan[PlanOut::kSeq + i] = b;
-                a.plan[PlanOut::kPlace + i] = i - (b ? plan.seq_end[b - 1] : 0);
+        if (in_wave(a)) {
+            const int b = threadIdx.x & 63;
+            my = Tile{};
+            int n = 0;
+            if (b < a.batch) {
+                my = tile_of<MR, KEYS>(a, b, 0, sequence(a, b));
+                n = units_of<UNIT>(my);
+            }
+            my_end = wave_inclusive_scan(n);
+            tiles = a.batch;
+            units = __builtin_amdgcn_readlane(my_end, 63);
+            if (blockIdx.x == 0 && threadIdx.x < 64 && b < a.batch) write_plan(a, b, my_end - n, my_end, my);
+        } else {
+            tiles = __builtin_amdgcn_readfirstlane(make_plan<MR, KEYS, UNIT, WAVES>(a, plan));
+            units = tiles > 0 ? __builtin_amdgcn_readfirstlane(plan.unit_end[tiles - 1]) : 0;
+            if (blockIdx.x == 0) {
+                for (int i = threadIdx.x; i < tiles; i += WAVES * 64) {
+                    const int b = first_above(plan.seq_end, a.batch, i);
+                    const Tile mine = tile_of<MR, KEYS>(a, b, i - (b ? plan.seq_end[b - 1] : 0), sequence(a, b));
+                    write_plan(a, i, i ? plan.unit_end[i - 1] : 0, plan.unit_end[i], mine);
+                }
             }
         }
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            a.plan[PlanOut::kTiles] = tiles;
+            a.plan[PlanOut::kUnits] = units;
+        }
         if (units == 0) return;
-        const int64_t total = (int64_t)units * a.kv_heads;
-        const int parts = split_parts(a, total, gridDim.x);
+        const Runs runs(a, units * a.kv_heads, gridDim.x);
         // runs side by side on one XCD: workgroups go to the XCDs in turn
         w = gridDim.x % 8 == 0 ? (int)(blockIdx.x % 8) * ((int)gridDim.x / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-        if (w >= parts) return;
-        at = run_begin(total, parts, w);
-        end = run_begin(total, parts, w + 1);
+        if (w >= runs.parts) return;
+        at = __builtin_amdgcn_readfirstlane(runs.begin(w));
+        end = __builtin_amdgcn_readfirstlane(runs.begin(w + 1));
     }
     __device__ __forceinline__ bool next(const Params& a, const Plan& plan) {
         if (!a.split) {  // tile blockIdx / heads, counted over the sequences, a sequence's last first
@@ -601,14 +655,32 @@ struct Pieces {
             return false;
         }
         if (at >= end) return false;
-        head = __builtin_amdgcn_readfirstlane((int)(at / units));
-        const int r = (int)(at - (int64_t)head * units);
-        const int ti = __builtin_amdgcn_readfirstlane(first_above(plan.unit_end, tiles, r));
-        const int b = __builtin_amdgcn_readfirstlane(first_above(plan.seq_end, a.batch, ti));
-        const int first = ti ? plan.unit_end[ti - 1] : 0, all = plan.unit_end[ti] - first;
-        set_tile(a, b, ti - (b ? plan.seq_end[b - 1] : 0));
+        head = __builtin_amdgcn_readfirstlane(at / units);
+        const int r = at - head * units;
+        int first, last;
+        if (in_wave(a)) {
+            const int b = __builtin_ctzll(__ballot(my_end > r));
+            first = b ? __builtin_amdgcn_readlane(my_end, b - 1) : 0;
+            last = __builtin_amdgcn_readlane(my_end, b);
+            t.b = b;
+            t.q0 = __builtin_amdgcn_readlane(my.q0, b);
+            t.first_pos = __builtin_amdgcn_readlane(my.first_pos, b);
+            t.len = __builtin_amdgcn_readlane(my.len, b);
+            t.row0 = 0;
+            t.rows = __builtin_amdgcn_readlane(my.rows, b);
+            t.lo = __builtin_amdgcn_readlane(my.lo, b);
+            t.hi = __builtin_amdgcn_readlane(my.hi, b);
+            t.base = __builtin_amdgcn_readlane(my.base, b);
+        } else {
+            const int ti = __builtin_amdgcn_readfirstlane(first_above(plan.unit_end, tiles, r));
+            const int b = __builtin_amdgcn_readfirstlane(first_above(plan.seq_end, a.batch, ti));
+            first = ti ? plan.unit_end[ti - 1] : 0;
+            last = plan.unit_end[ti];
+            set_tile(a, b, ti - (b ? plan.seq_end[b - 1] : 0));
+        }
+        const int all = last - first;
         u0 = __builtin_amdgcn_readfirstlane(r - first);
-        u1 = __builtin_amdgcn_readfirstlane((int)min((int64_t)all, u0 + (end - at)));
+        u1 = __builtin_amdgcn_readfirstlane(min(all, u0 + (end - at)));
         slot = __builtin_amdgcn_readfirstlane(u0 == 0 && u1 == all ? -1 : 2 * w + (u0 == 0 ? 1 : 0));
         at += u1 - u0;
         return true;
@@ -651,7 +723,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
     const auto lanes_k = lanes_of<DP>(a, k_swizzle<DP>), lanes_v = lanes_of<DP>(a, v_swizzle<DP, false>);
     const float k = unit<CAP>(a);
 
-    Pieces<MR, kFewKeys, UNIT, WAVES> piece;
+    Pieces<MR, kFewKeys, UNIT, WAVES, true> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
@@ -660,11 +732,19 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
         const int begin = t.base + u0 * UNIT, end = min(t.hi, t.base + u1 * UNIT);
         const int blocks = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
         const int mine = (blocks - wave + WAVES - 1) / WAVES;  // blocks wave, wave + WAVES, ...
+        auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
+        if (mine > 0) {
+            copy_pages(a, src, first_of(0) + lane, lds_addr(ids));
+            copy_pages(a, src, first_of(1) + lane, lds_addr(ids + 64));
+        }
         u32x4 q[MT][KS];
         int row_lo[MT], row_hi[MT];  // keys that the lane's row sees
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             load_query<KS>(a, t, head, mt * 16 + c, g, 4, q[mt]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
             const int pos = t.first_pos + (t.row0 + mt * 16 + c) / a.group;
             row_hi[mt] = min(pos + 1, t.hi);
             row_lo[mt] = a.window > 0 ? pos + 1 - a.window : 0;
@@ -683,7 +763,6 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
         auto issue = [&](int i) {  // batch i: block i, and the page ids of block i + 2
             const uint32_t st = lds_addr(ring) + (i & 1) * kFewStage<DP>;
 #pragma unroll
@@ -694,8 +773,6 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
             copy_pages(a, src, first_of(i + 2) + lane, lds_addr(ids + ((i + 2) & 3) * 64));
         };
         if (mine > 0) {
-            copy_pages(a, src, first_of(0) + lane, lds_addr(ids));
-            copy_pages(a, src, first_of(1) + lane, lds_addr(ids + 64));
             wait_copies<0>();
             issue(0);
             if (mine > 1) issue(1);
@@ -964,7 +1041,7 @@ void many_rows_kernel(const Params a) {
     const int vr = 4 * h + ((c & 15) >> 2);
     const uint32_t v_at = (uint32_t)(kManyStage<DP> / 2 + vr * DP * 2 +
                                      ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) + (c & 1) * 8);
-    Pieces<MR, KEYS, KEYS, WAVES> piece;
+    Pieces<MR, KEYS, KEYS, WAVES, false> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
@@ -1120,7 +1197,7 @@ void wide_rows_kernel(const Params a) {
     const int vr = 4 * h + ((c & 15) >> 2);
     const uint32_t v_at = (uint32_t)(vr * DP * 2 + ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) +
                                      (c & 1) * 8);
-    Pieces<MR, KEYS, KEYS, kWideWaves> piece;
+    Pieces<MR, KEYS, KEYS, kWideWaves, false> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
@@ -1141,7 +1218,7 @@ void wide_rows_kernel(const Params a) {
             if (in_one_page(a, src, first)) {
                 copy_rows<DP>(plane + row_of(a, src, first, id), lanes, to);
             } else {
-                copy_rows_apart<DP>(a, src, plane, lanes, first, ids + (j & 7) * 16, to);
+                copy_rows_apart<DP, false>(a, src, plane, lanes, to, plane, lanes, to, first, ids + (j & 7) * 16);
             }
         };
         if (blocks > 0) {
@@ -1271,54 +1348,54 @@ void wide_rows_kernel(const Params a) {
 
 // ---- joining partial results --------------------------------------------------------
 
-// Tile blockIdx.x / heads, rows blockIdx.y * 4 + wave, + 4 gridDim.y, ...: a wave a row.
+// Row blockIdx.y * 4 + wave of tile and head blockIdx.x, a wave a row.
 template <int MR, bool BF16>
 __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
-    const int tiles = a.plan[PlanOut::kTiles], ti = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
-    if (ti >= tiles) return;
-    const int first = ti ? a.plan[PlanOut::kEnd + ti - 1] : 0, last = a.plan[PlanOut::kEnd + ti] - 1;
-    const int units = a.plan[PlanOut::kEnd + tiles - 1];
-    const int64_t total = (int64_t)units * a.kv_heads;
-    const int parts = split_parts(a, total, grid);
-    if (last < first) return;
-    const int w0 = run_of(total, parts, (int64_t)head * units + first), w1 = run_of(total, parts, (int64_t)head * units + last);
-    if (w0 == w1) return;
-    const int lane = threadIdx.x & 63, b = a.plan[PlanOut::kSeq + ti];
-    const Tile t = tile_of<MR, 1>(a, b, a.plan[PlanOut::kPlace + ti], sequence(a, b));
-    const int n = w1 - w0 + 1;
-    auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0); };
-    for (int row = blockIdx.y * 4 + (threadIdx.x >> 6); row < t.rows; row += 4 * gridDim.y) {
-        float m2 = -kInf;
-        for (int i = lane; i < n; i += 64) m2 = fmaxf(m2, a.part_ml[(slot(i) * MR + row) * 2]);
-        m2 = wave_max(m2);
-        float z = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            float w = 0.f;
-            if (i0 + lane < n) {
-                const float* const ml = a.part_ml + (slot(i0 + lane) * MR + row) * 2;
-                w = ml[0] == -kInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m2);
-                z += ml[0] == -kInf && ml[1] == 0.f ? 0.f : w * ml[1];
-            }
-            const int here = min(64, n - i0);
-            for (int i = 0; i < here; ++i) {
-                const float wi = __shfl(w, i);
-                if (wi == 0.f) continue;
-                const float* const o = a.part_o + (slot(i0 + i) * MR + row) * a.dim;
+    const int ti = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads;
+    const int row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const PlanOut::Entry e = reinterpret_cast<const PlanOut::Entry*>(a.plan + PlanOut::kEntries)[ti];
+    const int units = a.plan[PlanOut::kUnits];
+    if (ti >= a.plan[PlanOut::kTiles] || row >= e.rows || e.end <= e.begin) return;
+    const Runs runs(a, units * a.kv_heads, grid);
+    const int w0 = runs.of(head * units + e.begin), n = runs.of(head * units + e.end - 1) - w0 + 1;
+    if (n == 1) return;
+    // partial i: the first run's second slot, then the others' first ones
+    const auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0); };
+    float m2 = -kInf;
+    for (int i = lane; i < n; i += 64) m2 = fmaxf(m2, a.part_ml[(slot(i) * MR + row) * 2]);
+    m2 = wave_max(m2);
+    float z = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        float w = 0.f;
+        if (i0 + lane < n) {
+            const float* const ml = a.part_ml + (slot(i0 + lane) * MR + row) * 2;
+            w = ml[0] == -kInf ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m2);
+            z += ml[0] == -kInf && ml[1] == 0.f ? 0.f : w * ml[1];
+        }
+        const int here = min(64, n - i0);
+        for (int i = 0; i < here; ++i) {
+            const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+            const float* const o = a.part_o + (slot(i0 + i) * MR + row) * a.dim;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (lane + 64 * e < a.dim) x[e] += wi * o[lane + 64 * e];
+            for (int j = 0; j < 4; ++j) {
+                if (lane + 64 * j < a.dim) {
+                    const float v = o[lane + 64 * j];
+                    x[j] += wi == 0.f ? 0.f : wi * v;  // a run of no weight may hold anything
                 }
             }
         }
-        z = wave_sum(z);
-        const float inv = z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
-        uint16_t* const to = out_row(a, t, head, row);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (lane + 64 * e < a.dim) to[lane + 64 * e] = f32_to_out<BF16>(x[e] * inv);
-        }
-        if (lane == 0) store_stats<MR, BF16>(a, t, head, row, -1, m2, z);
     }
+    z = wave_sum(z);
+    const float inv = z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
+    Tile t{};
+    t.q0 = e.q0;
+    t.row0 = e.row0;
+    uint16_t* const to = out_row(a, t, head, row);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (lane + 64 * j < a.dim) to[lane + 64 * j] = f32_to_out<BF16>(x[j] * inv);
+    }
+    if (lane == 0) store_stats<MR, BF16>(a, t, head, row, -1, m2, z);
 }
 
 // ---- host ----------------------------------------------------------------------------
@@ -1359,6 +1436,11 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.num_pages = (int32_t)a->num_pages;
     p.page_size = (int32_t)a->page_size;
     p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? __builtin_ctzll((uint64_t)a->page_size) : -1;
+    if (p.page_shift < 0) {  // 2^(31 + s) / size, rounded up, for 2^(s - 1) < size < 2^s: exact for keys below 2^31
+        const int bits = 64 - __builtin_clzll((uint64_t)a->page_size);
+        p.page_magic = (uint32_t)(((1ull << (31 + bits)) + a->page_size - 1) / a->page_size);
+        p.page_magic_shift = bits - 1;
+    }
     p.max_q = (int32_t)std::min(a->max_q_len, a->num_tokens);
     const int64_t held = a->num_pages == 0 ? 0 : std::min<int64_t>(INT_MAX, a->table_width * a->page_size);
     p.max_len = (int32_t)std::min(a->max_seq_len, held);
@@ -1366,22 +1448,39 @@ Call plan_call(const pw4_paged_attention_args* a) {
     // a scale of 0 is held as one that leaves nothing of a score either, so that -inf stays -inf
     p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : std::max(std::fabs(a->scale) * kLog2e, 0x1p-100f);
     p.flip = a->softcap > 0.f || a->scale >= 0.f ? 0 : 0x80008000u;
-    p.flat = p.page_shift >= 4 && (uint64_t)a->page_size * p.row_bytes <= UINT32_MAX;
+    p.flat = (uint64_t)a->page_size * p.row_bytes > UINT32_MAX ? 0 : p.page_shift >= 4 ? 2 : a->page_size % 8 == 0 ? 1 : 0;
     p.cap2 = a->softcap * kLog2e;
     const int64_t rows = (int64_t)p.max_q * p.group;
     c.dp = padded_dim(a->head_dim);
-    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= kManyRows || c.dp == 256 ? kManyRows : kWideRows;
-    const bool few = c.tile_rows <= 32;
-    c.tiles = few ? p.batch
-                  : std::min(a->num_tokens * p.group / c.tile_rows + p.batch, p.batch * ceil_div(rows, c.tile_rows));
-    const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     const int cus = device_cus();
+    const auto tiles_of = [&](int tile_rows) {
+        return std::min(a->num_tokens * p.group / tile_rows + p.batch, p.batch * ceil_div(rows, tile_rows));
+    };
+    // 256-row tiles run at the higher rate, but only one to a CU
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32
+                  : c.dp == 256 || tiles_of(kWideRows) * p.kv_heads < cus ? kManyRows : kWideRows;
+    if (const char* const forced = plan_override("PW4_ATTN_TILE"); forced && c.tile_rows > 32 && c.dp != 256) {
+        c.tile_rows = forced[0] == '2' ? kWideRows : kManyRows;
+    }
+    const bool few = c.tile_rows <= 32;
+    c.tiles = few ? p.batch : tiles_of(c.tile_rows);
+    const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     // workgroups that run at once
     const int slots = few ? (c.dp == 64 ? 2 * cus : cus) : c.tile_rows == kManyRows && c.dp != 256 ? 2 * cus : cus;
-    p.min_units = 2;
     const int64_t most_units = ceil_div(p.max_len, unit) + 1;  // of a tile: its first block may begin early
-    p.split = p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && most_units > 2 * p.min_units &&
-              (few || c.tiles * p.kv_heads < 4 * slots);
+    const char* const forced = plan_override("PW4_ATTN_UNITS");
+    const int forced_units = forced ? std::atoi(forced) : 0;
+    // A few rows: a unit of 128 keys takes a workgroup 1.16 us, the split with its second launch
+    // 6 us more: measured even at about 1200 keys where the pieces find idle CUs (one sequence,
+    // 8 heads), at about 2500 where half of the CUs have a tile of their own (16 sequences).
+    // Else where the tiles leave at least half of the chip idle and are long: a piece's
+    // partial outputs are written and read again.
+    p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
+    const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
+    const bool wanted = forced_split ? forced_split[0] == '1'
+                        : few ? most_units > (2 * c.tiles * p.kv_heads >= cus ? 20 : 10)
+                              : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
+    p.split = wanted && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     c.grid = (int)(c.tiles * p.kv_heads);
     if (p.split) {
         c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
@@ -1424,7 +1523,7 @@ hipError_t launch(const Call& c, hipStream_t s) {
         e = hipErrorInvalidValue;  // no such tile: plan_call
     }
     if (e != hipSuccess || !c.p.split) return e;
-    const dim3 grid((unsigned)(c.tiles * c.p.kv_heads), c.tile_rows / 16);
+    const dim3 grid((unsigned)(c.tiles * c.p.kv_heads), c.tile_rows / 4);
     if (c.tile_rows == 16) {
         hipLaunchKernelGGL((join_kernel<16, BF16>), grid, dim3(256), 0, s, c.p, c.grid);
     } else if (c.tile_rows == 32) {

@@ -14,6 +14,9 @@ int report_hip_error(hipError_t e);
 // Compute units of the current device (256 when no device answers).
 int device_cus();
 
+// A plan override of the environment (tests and sweeps; null where they are not enabled).
+const char* plan_override(const char* name);
+
 constexpr int kWave = 64;
 
 __device__ __forceinline__ float wave_max(float v) {

@@ -1,18 +1,21 @@
 // Log probabilities of given tokens, with rank, entropy and top alternatives.
 //
-// Bound by one read of the logits.  A row is cut into slices of up to 16384
-// logits, one workgroup of 256 threads each, which holds its slice in registers
-// (64 logits a thread, packed as they came): the largest logit, then sum e^(x-m)
-// and sum e^(x-m) (x-m) with the slice's own m, the rank and the top candidates
-// all come from one trip to memory.  A second launch joins a row's slices, a wave
-// a row: with M = max m and the slices' sums scaled by e^(m-M),
+// Bound by one read of the logits.  A row is cut into slices, one workgroup of 256
+// threads each, which holds its slice in registers, packed as it came: 64 logits a
+// thread, or 16 where the tokens are so few that slices of 16384 leave CUs idle.  The
+// largest logit, then sum e^(x-m) and sum e^(x-m) (x-m) with the slice's own m, the rank
+// and the top candidates come from one trip to memory.  A second launch joins a row's
+// slices, a wave a row: with M = max m and the slices' sums scaled by e^(m-M),
 //   lse = M + ln Z,  entropy = ln Z - T / Z,  Z = sum e^(x-M), T = sum e^(x-M) (x-M)
-// Short slices give eight logits rows of a decode step 64 workgroups.
 //
-// Top candidates.  The k-th largest of 64 groups' maxima (four threads a group)
-// is a bound that at least k logits reach, and few more: those are listed in LDS
-// and ranked against each other.  Where ties make the list longer than it holds,
+// Top candidates.  A number that the largest logits of at least k of 64 groups reach
+// (four threads a group) is a bound that at least k logits reach, and few more: those
+// are listed in LDS and ranked against each other.  Where ties make the list longer than
+// it holds, those above the exact bound and the first k that equal it are; failing that,
 // k rounds of a workgroup-wide maximum find the same tokens.
+//
+// A row may begin at any address: vectors cover the 16-byte aligned part of a slice, and
+// what is before and behind it, 14 logits at most, are the first threads' odd ones.
 #include "pulsar_paged.h"
 
 #include <algorithm>
@@ -24,7 +27,7 @@ using namespace pw4;
 
 namespace {
 
-constexpr int kThreads = 256, kPerThread = 64, kSlice = kThreads * kPerThread;
+constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;
 constexpr int kList = 1024;  // a slice's candidates that are ranked at once
 constexpr int kJoin = 512;   // a row's
@@ -45,7 +48,7 @@ struct LogprobArgs {
     float* top_logprobs;
     int64_t* top_ids;
     int64_t row_stride;
-    int32_t tokens, vocab, top_k, slices, slice;  // slice: logits of one, a multiple of 8
+    int32_t tokens, vocab, top_k, slices, slice;  // slice: logits of one
 };
 
 __device__ __forceinline__ float lowest_if_nan(float x) { return x == x ? x : -__builtin_inff(); }
@@ -92,13 +95,14 @@ __device__ __forceinline__ float logit_at(const void* row, int64_t i) {
     return Logits<DT>::value(x, 0);
 }
 
-template <int DT>
+template <int DT, int PER>
 __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     using L = Logits<DT>;
     using T = typename L::T;
     constexpr int kVec = 16 / sizeof(T);           // logits of a 16-byte vector
-    constexpr int kVecs = kPerThread / kVec;       // vectors of a thread
+    constexpr int kVecs = PER / kVec;              // vectors of a thread
     constexpr int kPerWord = 4 / sizeof(T);
+    constexpr float kLog2e = 1.4426950408889634f, kInf = __builtin_inff();
     __shared__ uint32_t s_group[64];
     __shared__ float s_sum[8];
     __shared__ int s_ahead[4], s_count;
@@ -108,43 +112,46 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     const int row = blockIdx.y;
     const T* const x = static_cast<const T*>(a.logits) + (int64_t)row * a.row_stride;
     const int begin = blockIdx.x * a.slice, end = min(begin + a.slice, a.vocab);
-    // Vectors start at 16-byte addresses, so the first may begin before the slice.
-    const int skew = (int)((reinterpret_cast<uintptr_t>(x + begin) & 15) / sizeof(T));
-    const int first = begin - skew + tid * kVec;  // index of vector 0's first logit
+    const int64_t target = a.targets[row];
+    const bool given = target >= 0 && target < a.vocab;
+    const float mine = given ? lowest_if_nan(logit_at<DT>(x, target)) : kInf;
+    // the aligned part, and the odd logits around it
+    const int to_aligned = (int)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16 / sizeof(T));
+    const int first = min(begin + to_aligned, end), vectors = (end - first) / kVec;
+    const int head = first - begin, tail = first + vectors * kVec;
+    const int odd_at = tid < head ? begin + tid : tail + tid - head;
+    const bool has_odd = odd_at < end && (tid < head || odd_at >= tail);
+    const float odd = has_odd ? logit_at<DT>(x, odd_at) : -kInf;
     u32x4 held[kVecs];
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
-        const int i = first + v * kThreads * kVec;
-        if (i >= begin && i + kVec <= end) {
-            held[v] = *reinterpret_cast<const u32x4*>(x + i);
-        } else {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = 0;
-#pragma unroll
-                for (int h = 0; h < kPerWord; ++h) {
-                    const int at = i + j * kPerWord + h;
-                    const uint32_t raw = at >= begin && at < end ? (uint32_t)x[at] : (uint32_t)L::kLowest;
-                    w[j] |= raw << (16 * h);
-                }
-            }
-            held[v] = u32x4{w[0], w[1], w[2], w[3]};
+        constexpr uint32_t low = sizeof(T) == 2 ? L::kLowest * 0x10001u : (uint32_t)L::kLowest;
+        held[v] = u32x4{low, low, low, low};
+        if (v * kThreads + tid < vectors) {
+            held[v] = *reinterpret_cast<const u32x4*>(x + first + (v * kThreads + tid) * kVec);
         }
     }
+    const int my_first = first + tid * kVec;  // index of vector 0's first logit
+    // f(logit) of every held one.  Opaque words: a pass takes them apart again, rather than
+    // have every value of the thread held from one pass to the next.
     auto each = [&](auto&& f) {
 #pragma unroll
         for (int v = 0; v < kVecs; ++v) {
-            // opaque: a pass takes the packed words apart again, rather than have
-            // every value of the thread held from one pass to the next
+            __builtin_amdgcn_sched_barrier(0);
             asm volatile("" : "+v"(held[v]));
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                f(L::value(held[v][e / kPerWord], e % kPerWord), first + v * kThreads * kVec + e);
-            }
+            for (int e = 0; e < kVec; ++e) f(L::value(held[v][e / kPerWord], e % kPerWord), my_first + v * kThreads * kVec + e);
         }
     };
-    float m = -__builtin_inff();
+    // f(logit, index) of the thread's own logits, from memory: for what is rare
+    auto each_again = [&](auto&& f) {
+        for (int i = my_first; i < tail; i += kThreads * kVec) {
+#pragma clang loop unroll(disable)
+            for (int e = 0; e < kVec; ++e) f(logit_at<DT>(x, i + e), i + e);
+        }
+        if (has_odd) f(odd, odd_at);
+    };
+    float m = lowest_if_nan(odd);
     each([&](float l, int) { m = fmaxf(m, l); });  // passes over NaN
     // ---- the slice's largest logit, and a bound that its top_k reach
     uint32_t g = ordered(m);
@@ -156,46 +163,67 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     g = s_group[lane];
     m = wave_max(unordered(g));
     uint32_t bound = 0;
-    if (a.top_k > 0) {  // the greatest number that top_k groups reach
-        for (int bit = 31; bit >= 0; --bit) {
+    if (a.top_k > 0) {  // the greatest number of 16 bits, and then zeros, that top_k groups reach
+        for (int bit = 31; bit >= 16; --bit) {
             const uint32_t higher = bound | 1u << bit;
             if (__popcll(__ballot(g >= higher)) >= a.top_k) bound = higher;
         }
     }
-    // ---- sums and rank
-    const float shift = m == -__builtin_inff() ? 0.f : m;
-    const int64_t target = a.targets[row];
-    const bool given = target >= 0 && target < a.vocab;
-    const float mine = given ? lowest_if_nan(logit_at<DT>(x, target)) : 0.f;
-    const uint32_t ties = (uint32_t)(max(begin, min(end, (int)target)) - begin);  // places of the slice below it
+    const float lowest = a.top_k > 0 ? unordered(max(bound, 0x007fffffu)) : kInf;
+    // ---- sums, rank, and the logits that reach the bound
+    const float shift = m == -kInf ? 0.f : m;
     float z = 0.f, t = 0.f;
     int ahead = 0;
-    constexpr float kLog2e = 1.4426950408889634f;
-    each([&](float l, int) {
+    bool tie = false;
+    auto add = [&](float l) {
+        // the difference first: l * log2(e) alone would round, and overflow, by the logit's size
         const float d = l - shift, e = __builtin_amdgcn_exp2f(d * kLog2e);
         z += e;
-        t += e * fmaxf(d, -1e30f);  // 0 * -inf is no term
-    });
-    if (given) {
-        each([&](float l, int i) { ahead += l > mine || (l == mine && (uint32_t)(i - begin) < ties); });
+        t = __builtin_fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf is no term
+    };
+    auto candidate = [&](float l, int i) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kList) s_list[at] = key_of(l, (uint32_t)i);
+    };
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+        __builtin_amdgcn_sched_barrier(0);  // a vector at a time
+        asm volatile("" : "+v"(held[v]));
+        bool reaches = false;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+            const float l = L::value(held[v][e / kPerWord], e % kPerWord);
+            add(l);
+            ahead += __popcll(__ballot(l > mine));
+            tie |= l == mine;
+            reaches |= !(l < lowest);
+        }
+        if (reaches && a.top_k > 0) {  // few vectors do
+#pragma clang loop unroll(disable)
+            for (int e = 0; e < kVec; ++e) {
+                const int n = e / kPerWord;
+                const uint32_t w = n == 0 ? held[v][0] : n == 1 ? held[v][1] : n == 2 ? held[v][2] : held[v][3];
+                const float l = L::value(w, e % kPerWord);
+                const int i = my_first + v * kThreads * kVec + e;
+                if (!(l < lowest) && i < tail) candidate(l, i);
+            }
+        }
+    }
+    add(odd);
+    ahead += __popcll(__ballot(odd > mine));
+    tie |= odd == mine;
+    if (has_odd && a.top_k > 0 && !(odd < lowest)) candidate(odd, odd_at);
+    if (given && __any(tie)) {
+        int before = 0;
+        each_again([&](float l, int i) { before += l == mine && i < (int)target; });
+        ahead += wave_sum(before);
     }
     z = wave_sum(z);
     t = wave_sum(t);
-    ahead = wave_sum(ahead);
     if (lane == 0) {
         s_sum[wave] = z;
         s_sum[4 + wave] = t;
         s_ahead[wave] = ahead;
-    }
-    // ---- the logits that reach the bound
-    if (a.top_k > 0) {
-        const float lowest = unordered(bound);
-        each([&](float l, int i) {
-            if (!(l < lowest) && i >= begin && i < end) {
-                const int at = atomicAdd(&s_count, 1);
-                if (at < kList) s_list[at] = key_of(l, (uint32_t)i);
-            }
-        });
     }
     __syncthreads();
     const int64_t out = (int64_t)row * a.slices + blockIdx.x;
@@ -206,7 +234,34 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     }
     if (a.top_k == 0) return;
     uint64_t* const top = a.top + out * a.top_k;
-    const int count = s_count;
+    int count = s_count;
+    if (count > kList) {
+        // Ties, as masks make them.  With the bound's last bits, what is above it lies in fewer
+        // than top_k groups; of what equals it the first top_k are enough.
+        for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t higher = bound | 1u << bit;
+            if (__popcll(__ballot(g >= higher)) >= a.top_k) bound = higher;
+        }
+        __syncthreads();
+        if (tid == 0) s_count = 0;
+        __syncthreads();
+        each_again([&](float l, int i) {
+            if (ordered(l) > bound) candidate(l, i);
+        });
+        if (wave == 0) {
+            int found = 0;
+            for (int i0 = begin; i0 < end && found < a.top_k; i0 += 64) {
+                const int i = i0 + lane;
+                const float l = i < end ? logit_at<DT>(x, i) : 0.f;
+                const bool equal = i < end && ordered(l) == bound;
+                const uint64_t all = __ballot(equal);
+                if (equal && found + __popcll(all & ((1ull << lane) - 1)) < a.top_k) candidate(l, i);
+                found += __popcll(all);
+            }
+        }
+        __syncthreads();
+        count = s_count;
+    }
     if (count <= kList) {
         for (int i = tid; i < max(count, a.top_k); i += kThreads) {
             if (i >= count) {
@@ -220,12 +275,12 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
         }
         return;
     }
-    uint64_t below = ~0ull;  // more ties than the list holds: one token a round
+    uint64_t below = ~0ull;  // more above the bound than the list holds: one token a round
     for (int k = 0; k < a.top_k; ++k) {
         uint64_t best = 0;
-        each([&](float l, int i) {
+        each_again([&](float l, int i) {
             const uint64_t key = key_of(l, (uint32_t)i);
-            if (i >= begin && i < end && key < below && key > best) best = key;
+            if (key < below && key > best) best = key;
         });
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
@@ -312,11 +367,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LogprobArgs a) {
     }
 }
 
-int slices_of(int64_t vocab) { return (int)ceil_div(vocab, kSlice - 8); }
-
-// Slices of one size, a multiple of 8 logits; the 16-byte alignment of the first
-// vector may cost a slice up to 7 places.
-int slice_of(int64_t vocab, int slices) { return (int)round_up(ceil_div(vocab, slices), 8); }
+// Logits of a thread: 64, or 16 where slices of 64 leave half of the CUs without one.
+int per_thread(int64_t tokens, int64_t vocab) {
+    return 2 * tokens * ceil_div(vocab, kThreads * 64) <= device_cus() ? 16 : 64;
+}
+// Slices of one size; the odd logits come on top of the vectors.
+int slices_of(int64_t tokens, int64_t vocab) { return (int)ceil_div(vocab, kThreads * per_thread(tokens, vocab)); }
 
 size_t sums_bytes(int64_t tokens, int64_t slices) { return (size_t)round_up(tokens * slices * (int64_t)sizeof(SliceSums), 16); }
 
@@ -326,7 +382,7 @@ extern "C" {
 
 size_t pw4_token_logprobs_workspace_size(int64_t num_tokens, int64_t vocab, int64_t top_k) {
     if (num_tokens <= 0 || vocab <= 0 || vocab > INT_MAX / 2 || top_k < 0 || top_k > kMaxTop) return 0;
-    const int64_t slices = slices_of(vocab);
+    const int64_t slices = slices_of(num_tokens, vocab);
     return sums_bytes(num_tokens, slices) + (size_t)(num_tokens * slices * top_k) * 8;
 }
 
@@ -350,11 +406,12 @@ int pw4_token_logprobs(const void* logits, int dtype, int64_t num_tokens, int64_
         workspace_bytes < pw4_token_logprobs_workspace_size(num_tokens, vocab, top_k)) {
         return PW4_ERR_WORKSPACE;
     }
-    const int slices = slices_of(vocab);
+    const int slices = slices_of(num_tokens, vocab);
+    const bool few = per_thread(num_tokens, vocab) == 16;
     LogprobArgs a{logits, targets, static_cast<SliceSums*>(workspace),
                   reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + sums_bytes(num_tokens, slices)),
                   logprobs, ranks, entropy, top_logprobs, top_ids, row_stride, 0, (int32_t)vocab, (int32_t)top_k,
-                  slices, slice_of(vocab, slices)};
+                  slices, (int32_t)ceil_div(vocab, slices)};
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     auto run = [&](auto dt) {
         constexpr int DT = decltype(dt)::value;
@@ -372,7 +429,11 @@ int pw4_token_logprobs(const void* logits, int dtype, int64_t num_tokens, int64_
             part.top_logprobs += r * top_k;
             part.top_ids += r * top_k;
             part.tokens = (int32_t)n;
-            hipLaunchKernelGGL(slice_kernel<DT>, dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
+            if (few) {
+                hipLaunchKernelGGL((slice_kernel<DT, 16>), dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
+            } else {
+                hipLaunchKernelGGL((slice_kernel<DT, 64>), dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
+            }
             hipLaunchKernelGGL(join_kernel<DT>, dim3((unsigned)ceil_div(n, kThreads / 64)), dim3(kThreads), 0, s, part);
         }
     };
