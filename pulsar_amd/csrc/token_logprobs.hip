@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     constexpr float kLog2e = 1.4426950408889634f, kInf = __builtin_inff();
     __shared__ uint32_t s_group[64];
     __shared__ float s_sum[8];
-    __shared__ int s_ahead[4], s_count;
+    __shared__ int s_ahead[4], s_count, s_vectors, s_vector[kList];
     __shared__ uint64_t s_list[kList];
     __shared__ uint64_t s_best[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     g = max(g, (uint32_t)__shfl_xor((int)g, 1));
     g = max(g, (uint32_t)__shfl_xor((int)g, 2));
     if ((tid & 3) == 0) s_group[tid >> 2] = g;
-    if (tid == 0) s_count = 0;
+    if (tid == 0) s_count = s_vectors = 0;
     __syncthreads();
     g = s_group[lane];
     m = wave_max(unordered(g));
@@ -181,6 +181,8 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
         z += e;
         t = __builtin_fmaf(e, fmaxf(d, -1e30f), t);  // 0 * -inf is no term
     };
+    const bool listing = a.top_k > 0;
+    auto reaching = [&](float l) { return listing && !(l < lowest); };
     auto candidate = [&](float l, int i) {
         const int at = atomicAdd(&s_count, 1);
         if (at < kList) s_list[at] = key_of(l, (uint32_t)i);
@@ -196,23 +198,17 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
             add(l);
             ahead += __popcll(__ballot(l > mine));
             tie |= l == mine;
-            reaches |= !(l < lowest);
+            reaches |= reaching(l);
         }
-        if (reaches && a.top_k > 0) {  // few vectors do
-#pragma clang loop unroll(disable)
-            for (int e = 0; e < kVec; ++e) {
-                const int n = e / kPerWord;
-                const uint32_t w = n == 0 ? held[v][0] : n == 1 ? held[v][1] : n == 2 ? held[v][2] : held[v][3];
-                const float l = L::value(w, e % kPerWord);
-                const int i = my_first + v * kThreads * kVec + e;
-                if (!(l < lowest) && i < tail) candidate(l, i);
-            }
+        if (reaches && v * kThreads + tid < vectors) {  // few vectors do
+            const int at = atomicAdd(&s_vectors, 1);
+            if (at < kList) s_vector[at] = my_first + v * kThreads * kVec;
         }
     }
     add(odd);
     ahead += __popcll(__ballot(odd > mine));
     tie |= odd == mine;
-    if (has_odd && a.top_k > 0 && !(odd < lowest)) candidate(odd, odd_at);
+    if (has_odd && reaching(odd)) candidate(odd, odd_at);
     if (given && __any(tie)) {
         int before = 0;
         each_again([&](float l, int i) { before += l == mine && i < (int)target; });
@@ -234,7 +230,17 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     }
     if (a.top_k == 0) return;
     uint64_t* const top = a.top + out * a.top_k;
-    int count = s_count;
+    // the candidates of the vectors that reach the bound, a logit a thread
+    int count = s_vectors;
+    if (count <= kList) {
+        for (int j = tid; j < count * kVec; j += kThreads) {
+            const int i = s_vector[j / kVec] + j % kVec;
+            const float l = logit_at<DT>(x, i);
+            if (!(l < lowest)) candidate(l, i);
+        }
+        __syncthreads();
+        count = s_count;
+    }
     if (count > kList) {
         // Ties, as masks make them.  With the bound's last bits, what is above it lies in fewer
         // than top_k groups; of what equals it the first top_k are enough.
@@ -338,15 +344,33 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LogprobArgs a) {
         a.top_logprobs[(int64_t)row * a.top_k + place] = logprob(unordered((uint32_t)(key >> 32)));
         a.top_ids[(int64_t)row * a.top_k + place] = (uint32_t)~key;
     };
-    if (keys <= kJoin) {  // every key against every other
-        uint64_t* const mine = s_keys[threadIdx.x >> 6];
-        for (int i = lane; i < keys; i += 64) mine[i] = tops[i];
-        __builtin_amdgcn_wave_barrier();
-        for (int i = lane; i < keys; i += 64) {
+    // A number that the greatest keys of at least top_k slices reach (all keys where there are
+    // fewer slices) is a bound for the row: the few keys that reach it are ranked.
+    uint32_t bound = 0;
+    if (a.slices >= a.top_k && a.slices <= 64) {
+        const uint32_t g = lane < a.slices ? (uint32_t)(tops[(int64_t)lane * a.top_k] >> 32) : 0;
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t higher = bound | 1u << bit;
+            if (__popcll(__ballot(g >= higher)) >= a.top_k) bound = higher;
+        }
+    }
+    uint64_t* const mine = s_keys[threadIdx.x >> 6];
+    int count = 0;
+    for (int i0 = 0; i0 < keys; i0 += 64) {
+        const uint64_t key = i0 + lane < keys ? tops[i0 + lane] : 0;
+        const bool reaches = key != 0 && (uint32_t)(key >> 32) >= bound;
+        const uint64_t all = __ballot(reaches);
+        const int at = count + __popcll(all & ((1ull << lane) - 1));
+        if (reaches && at < kJoin) mine[at] = key;
+        count += __popcll(all);
+    }
+    if (count <= kJoin) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int i = lane; i < count; i += 64) {
             const uint64_t key = mine[i];
             int place = 0;
-            for (int j = 0; j < keys; ++j) place += mine[j] > key;
-            if (key != 0 && place < a.top_k) store(place, key);
+            for (int j = 0; j < count; ++j) place += mine[j] > key;
+            if (place < a.top_k) store(place, key);
         }
         return;
     }
