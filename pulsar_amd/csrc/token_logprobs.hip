@@ -1,8 +1,9 @@
 // Log probabilities of given tokens, with rank, entropy and top alternatives.
 //
 // Bound by one read of the logits.  A row is cut into slices, one workgroup of 256
-// threads each, which holds its slice in registers, packed as it came: 64 logits a
-// thread, or 16 where the tokens are so few that slices of 16384 leave CUs idle.  The
+// threads each, which holds its slice in registers, packed as it came: 32 logits a
+// thread (188 us for 2048 tokens of 100003 bf16 logits; 64 a thread, at five waves a SIMD
+// instead of eight: 206), or 16 where the tokens are so few that CUs would be idle.  The
 // largest logit, then sum e^(x-m) and sum e^(x-m) (x-m) with the slice's own m, the rank
 // and the top candidates come from one trip to memory.  A second launch joins a row's
 // slices, a wave a row: with M = max m and the slices' sums scaled by e^(m-M),
@@ -112,16 +113,12 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     const int row = blockIdx.y;
     const T* const x = static_cast<const T*>(a.logits) + (int64_t)row * a.row_stride;
     const int begin = blockIdx.x * a.slice, end = min(begin + a.slice, a.vocab);
-    const int64_t target = a.targets[row];
-    const bool given = target >= 0 && target < a.vocab;
-    const float mine = given ? lowest_if_nan(logit_at<DT>(x, target)) : kInf;
     // the aligned part, and the odd logits around it
     const int to_aligned = (int)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16 / sizeof(T));
     const int first = min(begin + to_aligned, end), vectors = (end - first) / kVec;
     const int head = first - begin, tail = first + vectors * kVec;
     const int odd_at = tid < head ? begin + tid : tail + tid - head;
     const bool has_odd = odd_at < end && (tid < head || odd_at >= tail);
-    const float odd = has_odd ? logit_at<DT>(x, odd_at) : -kInf;
     u32x4 held[kVecs];
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -131,18 +128,15 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
             held[v] = *reinterpret_cast<const u32x4*>(x + first + (v * kThreads + tid) * kVec);
         }
     }
+    const float odd = has_odd ? logit_at<DT>(x, odd_at) : -kInf;
+    __builtin_amdgcn_sched_barrier(0);  // nothing waits for the target ahead of the loads
+    const int64_t target = a.targets[row];
+    const bool given = target >= 0 && target < a.vocab;
+    const float mine = given ? lowest_if_nan(logit_at<DT>(x, target)) : kInf;
     const int my_first = first + tid * kVec;  // index of vector 0's first logit
-    // f(logit) of every held one.  Opaque words: a pass takes them apart again, rather than
-    // have every value of the thread held from one pass to the next.
-    auto each = [&](auto&& f) {
-#pragma unroll
-        for (int v = 0; v < kVecs; ++v) {
-            __builtin_amdgcn_sched_barrier(0);
-            asm volatile("" : "+v"(held[v]));
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) f(L::value(held[v][e / kPerWord], e % kPerWord), my_first + v * kThreads * kVec + e);
-        }
-    };
+    // Logit e of vector v.  (Its words are made opaque before each use of a vector, so that a
+    // later one takes them apart again, rather than have every value held in between.)
+    auto logit = [&](int v, int e) { return L::value(held[v][e / kPerWord], e % kPerWord); };
     // f(logit, index) of the thread's own logits, from memory: for what is rare
     auto each_again = [&](auto&& f) {
         for (int i = my_first; i < tail; i += kThreads * kVec) {
@@ -151,8 +145,15 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
         }
         if (has_odd) f(odd, odd_at);
     };
-    float m = lowest_if_nan(odd);
-    each([&](float l, int) { m = fmaxf(m, l); });  // passes over NaN
+    float m = lowest_if_nan(odd), peak[kVecs];  // the vectors' largest logits (NaN passed over)
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+        asm volatile("" : "+v"(held[v]));
+        peak[v] = -kInf;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) peak[v] = fmaxf(peak[v], logit(v, e));
+        m = fmaxf(m, peak[v]);
+    }
     // ---- the slice's largest logit, and a bound that its top_k reach
     uint32_t g = ordered(m);
     g = max(g, (uint32_t)__shfl_xor((int)g, 1));
@@ -191,16 +192,16 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const LogprobArgs a) {
     for (int v = 0; v < kVecs; ++v) {
         __builtin_amdgcn_sched_barrier(0);  // a vector at a time
         asm volatile("" : "+v"(held[v]));
-        bool reaches = false;
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-            const float l = L::value(held[v][e / kPerWord], e % kPerWord);
-            add(l);
-            ahead += __popcll(__ballot(l > mine));
-            tie |= l == mine;
-            reaches |= reaching(l);
+        for (int e = 0; e < kVec; ++e) add(logit(v, e));
+        if (__any(peak[v] >= mine)) {  // for a likely token, few vectors
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                ahead += __popcll(__ballot(logit(v, e) > mine));
+                tie |= logit(v, e) == mine;
+            }
         }
-        if (reaches && v * kThreads + tid < vectors) {  // few vectors do
+        if (reaching(peak[v]) && v * kThreads + tid < vectors) {
             const int at = atomicAdd(&s_vectors, 1);
             if (at < kList) s_vector[at] = my_first + v * kThreads * kVec;
         }
@@ -391,9 +392,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LogprobArgs a) {
     }
 }
 
-// Logits of a thread: 64, or 16 where slices of 64 leave half of the CUs without one.
+// Logits of a thread: 32, or 16 where slices of 32 leave half of the CUs without one.
 int per_thread(int64_t tokens, int64_t vocab) {
-    return 2 * tokens * ceil_div(vocab, kThreads * 64) <= device_cus() ? 16 : 64;
+    return 2 * tokens * ceil_div(vocab, kThreads * 32) <= device_cus() ? 16 : 32;
 }
 // Slices of one size; the odd logits come on top of the vectors.
 int slices_of(int64_t tokens, int64_t vocab) { return (int)ceil_div(vocab, kThreads * per_thread(tokens, vocab)); }
@@ -456,7 +457,7 @@ int pw4_token_logprobs(const void* logits, int dtype, int64_t num_tokens, int64_
             if (few) {
                 hipLaunchKernelGGL((slice_kernel<DT, 16>), dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
             } else {
-                hipLaunchKernelGGL((slice_kernel<DT, 64>), dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
+                hipLaunchKernelGGL((slice_kernel<DT, 32>), dim3(slices, (unsigned)n), dim3(kThreads), 0, s, part);
             }
             hipLaunchKernelGGL(join_kernel<DT>, dim3((unsigned)ceil_div(n, kThreads / 64)), dim3(kThreads), 0, s, part);
         }
