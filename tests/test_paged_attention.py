@@ -109,6 +109,59 @@ def test_long_context_is_split():
     _run([5000, 70], [60, 60], heads=1, group=2, seed=3)
 
 
+@pytest.fixture
+def plan(monkeypatch):
+    """Pins the split, the units of a piece and the tile rows (the library reads these in tests)."""
+    def pin(split=None, units=None, tile=None):
+        for name, value in (("SPLIT", split), ("UNITS", units), ("TILE", tile)):
+            if value is None:
+                monkeypatch.delenv(f"PW4_ATTN_{name}", raising=False)
+            else:
+                monkeypatch.setenv(f"PW4_ATTN_{name}", str(value))
+    return pin
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split,units", [(0, None), (1, 1), (1, 3)])
+@pytest.mark.parametrize("new", [1, 6])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_few_rows_whole_and_split(plan, dim, new, split, units):
+    plan(split, units)
+    _run([1500, 40, 0, 777, 3], [new, new, 0, new, min(new, 3)], heads=2, group=4, dim=dim, seed=dim + new)
+    _run([900, 1300], [new, new], heads=1, group=3, dim=dim, window=200, cap=3.0, dtype=H, seed=dim)
+    _run([700] * 70, [new] * 70, heads=1, group=2, dim=dim, page=24, seed=dim)  # more sequences than lanes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split,units", [(0, None), (1, 1), (1, 3)])
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("dim,dtype", [(64, H), (128, B), (96, B), (256, H)])
+def test_many_rows_whole_and_split(plan, dim, dtype, tile, split, units):
+    plan(split, units, tile)
+    _run([600, 257, 64, 400], [600, 129, 1, 90], heads=2, group=2, dim=dim, dtype=dtype, seed=dim)
+    _run([900, 333], [200, 333], heads=1, group=3, dim=dim, dtype=dtype, window=150, cap=4.0, page=8, seed=dim)
+    _run([1000, 50], [70, 50], heads=1, group=7, dim=dim, dtype=dtype, page=24, window=300, seed=dim)
+    _run([500], [499], heads=3, group=1, dim=dim, dtype=dtype, page=7, extra=5, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("split", [0, 1])
+def test_nonfinite_values_in_wide_and_split_tiles(plan, tile, split):
+    plan(split, 1, tile)
+    lens, page, dim, new = [700], 16, 128, 400
+    kc, vc, tables, ks, vs = paged_kv(lens, page, 1, dim, B, 8)
+    for j, bad in ((310, math.nan), (480, math.inf), (650, -math.inf)):
+        vs[0][j, 0, j % dim] = bad
+        vc[int(tables[0, j // page]), j % page, 0, j % dim] = bad
+    q = torch.randn(new, 2, dim, generator=gen(9)).to(B).to(DEV)
+    for window in (0, 120):
+        out, lse = ops.paged_attention(q, kc, vc, tables, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                       offsets([new]).to(DEV), new, lens[0], window=window, return_lse=True)
+        ref = attention_ref(q.cpu(), ks[0], vs[0], lens[0], new, dim ** -0.5, window, 0.0)
+        check_attention(out, lse, ref, dim, lens[0], B)
+
+
 @pytest.mark.gpu
 def test_rows_past_the_last_sequence_are_empty():
     _run([50, 20], [3, 1], extra=7)
