@@ -636,6 +636,14 @@ struct Pieces {
             fresh = false;
             head = blockIdx.x % a.kv_heads;
             const int rank = blockIdx.x / a.kv_heads, lane = threadIdx.x & 63;
+            u0 = 0;
+            slot = -1;
+            if (ONE) {  // the rank is the sequence
+                if (rank >= a.batch) return false;
+                set_tile(a, rank, 0);
+                u1 = units_of<UNIT>(t);
+                return t.rows > 0;
+            }
             int before = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 64) {
                 const int b = b0 + lane;
@@ -645,9 +653,7 @@ struct Pieces {
                 if (past != 0) {
                     const int l = __builtin_ctzll(past);
                     set_tile(a, b0 + l, __builtin_amdgcn_readlane(upto, l) - 1 - rank);
-                    u0 = 0;
                     u1 = units_of<UNIT>(t);
-                    slot = -1;
                     return true;
                 }
                 before = __builtin_amdgcn_readlane(upto, 63);
@@ -689,9 +695,12 @@ struct Pieces {
 
 // ---- few rows --------------------------------------------------------------------
 
-// Up to 16 MT query rows, bound by reading the keys.  Each wave takes blocks of 32
-// keys of its own, through a ring of two stages of its own (no barrier), and the
-// waves' outputs meet in LDS at the end of a piece.
+// Up to 16 MT query rows, bound by reading the keys: 16 sequences of 2 to 32 thousand
+// keys, 8 heads of 128, 754 MB, take 140 us and 6 for the join (5.2 TB/s; a copy of 4 GiB
+// reads and writes 4.7).  Each wave takes blocks of 32 keys of its own, through a ring of
+// two stages of its own (no barrier), and the waves' outputs meet in LDS at the end of a
+// piece.  Four waves and their rings fill a CU's LDS; 64 KB are under way in it, three
+// times what the memory's latency asks for at that rate.
 constexpr int kFewKeys = 32;
 template <int DP>
 constexpr int kFewWaves = DP == 256 ? 2 : 4;
@@ -919,7 +928,10 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
 // ---- many rows --------------------------------------------------------------------
 
 // Four waves of 32 query rows each over blocks of 64 keys that they share in LDS,
-// two stages: block i + 1 is copied while block i is worked on.
+// two stages: block i + 1 is copied while block i is worked on.  For calls with too few
+// tiles of 256 rows to fill the chip, and heads wider than 128; two workgroups to a CU
+// (one prompt of 8192 tokens, 32 heads of 128: 562 us, where 256-row tiles take 511).
+// With a cap the vector units bound it: three transcendental instructions a score.
 constexpr int kManyKeys = 64, kManyWaves = 4, kManyRows = 32 * kManyWaves;
 constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
@@ -1173,7 +1185,9 @@ void many_rows_kernel(const Params a) {
 // the matrix cores and the vector units are busy together; the same work in any order of
 // the waves' own left each idle half of the time (one prompt of 8192 tokens, 32 heads of
 // 128: 562 us in four-wave workgroups, two a CU).  Waves 0 to 3 copy K, waves 4 to 7 copy
-// V, three blocks of each in LDS.
+// V, three blocks of each in LDS.  511 us, 1076 TFLOP/s, where the library's large matrix
+// product reaches 1184: the products' turn takes 1320 cycles (1024 are the matrix cores'
+// own), the other one 1100 for the probabilities and 600 for the copies.
 constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideRing = 3;
 template <int DP>
 constexpr int kWideBlock = kManyKeys * DP * 2;  // bytes of K, or of V
@@ -1364,6 +1378,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
     float m2 = -kInf;
     for (int i = lane; i < n; i += 64) m2 = fmaxf(m2, a.part_ml[(slot(i) * MR + row) * 2]);
     m2 = wave_max(m2);
+    constexpr int kAtOnce = 8;
     float z = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0; i0 < n; i0 += 64) {
         float w = 0.f;
@@ -1373,15 +1388,19 @@ __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
             z += ml[0] == -kInf && ml[1] == 0.f ? 0.f : w * ml[1];
         }
         const int here = min(64, n - i0);
-        for (int i = 0; i < here; ++i) {
-            const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
-            const float* const o = a.part_o + (slot(i0 + i) * MR + row) * a.dim;
+        for (int i = 0; i < here; i += kAtOnce) {  // so many loads under way
+            float v[kAtOnce][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (lane + 64 * j < a.dim) {
-                    const float v = o[lane + 64 * j];
-                    x[j] += wi == 0.f ? 0.f : wi * v;  // a run of no weight may hold anything
-                }
+            for (int u = 0; u < kAtOnce; ++u) {
+                const float* const o = a.part_o + (slot(i0 + min(i + u, here - 1)) * MR + row) * a.dim;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[u][j] = lane + 64 * j < a.dim ? o[lane + 64 * j] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) {
+                const float wi = __shfl(w, min(i + u, 63));  // 0 past the last
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] += wi == 0.f ? 0.f : wi * v[u][j];  // a run of no weight may hold anything
             }
         }
     }
@@ -1471,14 +1490,16 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
     // A few rows: a unit of 128 keys takes a workgroup 1.16 us, the split with its second launch
-    // 6 us more: measured even at about 1200 keys where the pieces find idle CUs (one sequence,
-    // 8 heads), at about 2500 where half of the CUs have a tile of their own (16 sequences).
-    // Else where the tiles leave at least half of the chip idle and are long: a piece's
-    // partial outputs are written and read again.
+    // some 6 us.  One sequence, 8 heads, whole and split: 777 keys 14.1 and 15.0 us, 1100 keys
+    // 16.2 and 14.4, 8000 keys 72 and 23.  Where half of the CUs have a tile of their own (16
+    // sequences) there is less to gain: 2400 keys 27.8 and 29.8, 4000 keys 56.5 and 48.1.
+    // Else where the tiles leave at least half of the chip idle and are long, since a piece's
+    // partial outputs are written and read again: 270 tiles of 128 rows on 512 places, 18 blocks
+    // each, took 49 us whole and 65 split.
     p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
     const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
     const bool wanted = forced_split ? forced_split[0] == '1'
-                        : few ? most_units > (2 * c.tiles * p.kv_heads >= cus ? 20 : 10)
+                        : few ? most_units > (2 * c.tiles * p.kv_heads >= cus ? 22 : 8)
                               : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
     p.split = wanted && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     c.grid = (int)(c.tiles * p.kv_heads);

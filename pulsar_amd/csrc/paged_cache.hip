@@ -10,8 +10,13 @@
 // page contents, table rows -- is left to a second launch of many workgroups,
 // which reads what the first decided from the workspace.
 //
+// (1000 pages dealt of 4000: 6.3 us.)
+//
 // Page moves are bound by HBM: each byte is read and written once, in 16 KB
-// pieces of 64 bytes a thread, so a pool of any page size keeps every CU busy.
+// pieces of 64 bytes a thread, so a pool of any page size keeps every CU busy:
+// compacting 1.1 GB of moves takes 213 us (5.0 TB/s, both ways counted; a copy of
+// 4 GiB reaches 4.7), forking 48 rows of 32 planes 61 us.  Storing 65 MB of new
+// keys and values takes 13.5 us.
 #include "pulsar_paged.h"
 
 #include <algorithm>

@@ -2,6 +2,7 @@
 // registration, in the manner of torch_ops.cpp.
 #include "pulsar_paged_ops.hpp"
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -26,8 +27,14 @@ void check_status(int rc, const char* op) {
     TORCH_CHECK(rc == PW4_OK, op, ": ", pw4_status_string(rc));
 }
 
+// at::empty on like's device without the dispatcher's way there: a call of the small
+// operators is as long as its host side, and some have six outputs.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), std::nullopt));
+}
+
 at::Tensor scratch(size_t bytes, const at::Tensor& like) {
-    return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, like.options().dtype(at::kByte));
+    return fresh({(int64_t)std::max<size_t>(bytes, 16)}, at::kByte, like);
 }
 
 void check_device(const char* op, const at::Tensor& first, std::initializer_list<const at::Tensor*> others) {
@@ -135,8 +142,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, con
     const bool in_place = q.numel() == 0 || (q.stride(2) == 1 && aligned16(q) && stride_of(q, 0) % 8 == 0 &&
                                              stride_of(q, 1) % 8 == 0);
     const at::Tensor qc = in_place ? q : q.contiguous();
-    at::Tensor out = at::empty({T, Hq, D}, q.options());
-    at::Tensor lse = at::empty({return_lse ? T : 0, Hq}, q.options().dtype(at::kFloat));
+    at::Tensor out = fresh({T, Hq, D}, q.scalar_type(), q);
+    at::Tensor lse = fresh({return_lse ? T : 0, Hq}, at::kFloat, q);
     if (T == 0) return {out, lse};
     pw4_paged_attention_args a{};
     a.q = qc.data_ptr();
@@ -184,8 +191,8 @@ std::tuple<at::Tensor, at::Tensor> paged_cache_extend_cuda(at::Tensor& ref_count
     TORCH_CHECK(num_tokens >= 0, op, ": num_tokens must not be negative");
     TORCH_CHECK(page_size > 0, op, ": page_size must be positive");
     DeviceGuard guard(block_tables.device());
-    at::Tensor slots = at::empty({num_tokens}, block_tables.options().dtype(at::kLong));
-    at::Tensor missing = at::empty({1}, block_tables.options());
+    at::Tensor slots = fresh({num_tokens}, at::kLong, block_tables);
+    at::Tensor missing = fresh({1}, at::kInt, block_tables);
     check_status(pw4_paged_cache_extend(ref_counts.data_ptr<int32_t>(), ref_counts.size(0),
                                         block_tables.data_ptr<int32_t>(), block_tables.size(1),
                                         table_stride(block_tables), seq_lens.data_ptr<int32_t>(),
@@ -247,7 +254,7 @@ at::Tensor paged_cache_fork_cuda(at::Tensor& pool, at::Tensor& ref_counts, at::T
     TORCH_CHECK(src_rows.size(0) == dst_rows.size(0), op, ": src_rows and dst_rows differ in length");
     TORCH_CHECK(pool.size(2) > 0, op, ": page_size must be positive");
     DeviceGuard guard(pool.device());
-    at::Tensor missing = at::empty({1}, block_tables.options());
+    at::Tensor missing = fresh({1}, at::kInt, block_tables);
     const size_t bytes = pw4_paged_cache_fork_workspace_size(src_rows.size(0));
     const at::Tensor ws = scratch(bytes, pool);
     check_status(pw4_paged_cache_fork(&p, ref_counts.data_ptr<int32_t>(), block_tables.data_ptr<int32_t>(),
@@ -280,7 +287,7 @@ at::Tensor paged_cache_compact_cuda(at::Tensor& pool, at::Tensor& ref_counts, at
     check_tables(op, &ref_counts, block_tables, nullptr);
     TORCH_CHECK(ref_counts.size(0) == pool.size(1), op, ": ref_counts must be [pages of pool]");
     DeviceGuard guard(pool.device());
-    at::Tensor used = at::empty({1}, block_tables.options());
+    at::Tensor used = fresh({1}, at::kInt, block_tables);
     const size_t bytes = pw4_paged_cache_compact_workspace_size(pool.size(1));
     const at::Tensor ws = scratch(bytes, pool);
     check_status(pw4_paged_cache_compact(&p, ref_counts.data_ptr<int32_t>(), block_tables.data_ptr<int32_t>(),
@@ -305,9 +312,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log
     const int64_t T = logits.size(0), V = logits.size(1);
     const at::Tensor x = (V == 1 || logits.stride(1) == 1) && (T <= 1 || logits.stride(0) >= V) ? logits
                                                                                               : logits.contiguous();
-    const auto f = logits.options().dtype(at::kFloat), l = targets.options();
-    at::Tensor lp = at::empty({T}, f), ranks = at::empty({T}, l), ent = at::empty({T}, f);
-    at::Tensor top = at::empty({T, top_k}, f), ids = at::empty({T, top_k}, l);
+    at::Tensor lp = fresh({T}, at::kFloat, logits), ranks = fresh({T}, at::kLong, logits);
+    at::Tensor ent = fresh({T}, at::kFloat, logits);
+    at::Tensor top = fresh({T, top_k}, at::kFloat, logits), ids = fresh({T, top_k}, at::kLong, logits);
     if (T == 0) return {lp, ranks, ent, top, ids};
     const size_t bytes = pw4_token_logprobs_workspace_size(T, V, top_k);
     const at::Tensor ws = scratch(bytes, logits);

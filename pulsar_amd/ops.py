@@ -199,6 +199,17 @@ def gemm_w4a16_silu_mul(x: torch.Tensor, weight_marlin: torch.Tensor, scales: to
     return torch.ops.pulsar.gemm_w4a16_silu_mul(x, weight_marlin, scales, qzeros, perm, group_size)
 
 
+# The overloads themselves: looking one up costs as much as a small operator's checks.
+_paged_attention = torch.ops.pulsar.paged_attention.default
+_paged_cache_compact = torch.ops.pulsar.paged_cache_compact.default
+_paged_cache_copy = torch.ops.pulsar.paged_cache_copy.default
+_paged_cache_extend = torch.ops.pulsar.paged_cache_extend.default
+_paged_cache_fork = torch.ops.pulsar.paged_cache_fork.default
+_paged_cache_free = torch.ops.pulsar.paged_cache_free.default
+_paged_cache_write = torch.ops.pulsar.paged_cache_write.default
+_token_logprobs = torch.ops.pulsar.token_logprobs.default
+
+
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                     seq_lens: torch.Tensor, cu_q: torch.Tensor, max_q_len: int, max_seq_len: int,
                     scale: float | None = None, window: int = 0, softcap: float = 0.0, return_lse: bool = False):
@@ -222,7 +233,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out like q (contiguous), and with return_lse also lse = ln sum e^s, fp32 [T, q_heads].  A
         query that sees no key, and a row of q past cu_q[-1], has out 0 and lse -inf.
     """
-    out, lse = torch.ops.pulsar.paged_attention(q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len,
+    out, lse = _paged_attention(q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len,
                                                 max_seq_len, scale, window, softcap, return_lse)
     return (out, lse) if return_lse else out
 
@@ -233,20 +244,20 @@ def paged_cache_extend(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq
     the rows in order.  Returns (slots int64 [num_tokens], missing int32 [1]): token t's place
     page * page_size + row.  Where pages or table columns lack nothing changes, the slots are -1 and
     missing says how many."""
-    return torch.ops.pulsar.paged_cache_extend(ref_counts, block_tables, seq_lens, cu_q, num_tokens, page_size)
+    return _paged_cache_extend(ref_counts, block_tables, seq_lens, cu_q, num_tokens, page_size)
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       slots: torch.Tensor) -> None:
     """Stores k and v [T, kv_heads, head_dim] in the slots of one layer's caches (fp16 or bf16); a
     slot outside the caches (-1) is passed over."""
-    torch.ops.pulsar.paged_cache_write(k, v, k_cache, v_cache, slots)
+    _paged_cache_write(k, v, k_cache, v_cache, slots)
 
 
 def paged_cache_copy(pool: torch.Tensor, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
     """pool[:, dst_pages[i]] = pool[:, src_pages[i]] over a pool [planes, pages, page_size, ...] of any
     dtype with contiguous pages.  No page may be a destination twice, or a destination and a source."""
-    torch.ops.pulsar.paged_cache_copy(pool, src_pages, dst_pages)
+    _paged_cache_copy(pool, src_pages, dst_pages)
 
 
 def paged_cache_fork(pool: torch.Tensor, ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -255,19 +266,19 @@ def paged_cache_fork(pool: torch.Tensor, ref_counts: torch.Tensor, block_tables:
     filled is copied into a free one in every plane of the pool.  A source may come many times; the
     destinations are empty rows, each named once.  Returns missing int32 [1]: the free pages that
     lacked, in which case nothing changed."""
-    return torch.ops.pulsar.paged_cache_fork(pool, ref_counts, block_tables, seq_lens, src_rows, dst_rows)
+    return _paged_cache_fork(pool, ref_counts, block_tables, seq_lens, src_rows, dst_rows)
 
 
 def paged_cache_free(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                      rows: torch.Tensor) -> None:
     """The rows give their pages back: a page is free once no row holds it."""
-    torch.ops.pulsar.paged_cache_free(ref_counts, block_tables, seq_lens, rows)
+    _paged_cache_free(ref_counts, block_tables, seq_lens, rows)
 
 
 def paged_cache_compact(pool: torch.Tensor, ref_counts: torch.Tensor, block_tables: torch.Tensor) -> torch.Tensor:
     """Moves pages so that those in use are the pool's first, and renames them in the tables: the i-th
     free page among them takes the i-th used page behind them.  Returns how many are in use, int32 [1]."""
-    return torch.ops.pulsar.paged_cache_compact(pool, ref_counts, block_tables)
+    return _paged_cache_compact(pool, ref_counts, block_tables)
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int):
@@ -278,4 +289,4 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int):
     logits stand by index.  targets int64 [T]; one outside the vocabulary has logprob 0 and rank -1.
     top_k is 0 to 32.
     """
-    return torch.ops.pulsar.token_logprobs(logits, targets, top_k)
+    return _token_logprobs(logits, targets, top_k)
