@@ -931,7 +931,9 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
 // two stages: block i + 1 is copied while block i is worked on.  For calls with too few
 // tiles of 256 rows to fill the chip, and heads wider than 128; two workgroups to a CU
 // (one prompt of 8192 tokens, 32 heads of 128: 562 us, where 256-row tiles take 511).
-// With a cap the vector units bound it: three transcendental instructions a score.
+// Tiles too few to give a SIMD its second wave leave it bound by latency: chunks of 707 and
+// 101 tokens, 14 heads of 64, a window of 1024 and a cap (three transcendental instructions
+// a score) take 48 us, the vector units busy 24% of it.
 constexpr int kManyKeys = 64, kManyWaves = 4, kManyRows = 32 * kManyWaves;
 constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
@@ -1186,8 +1188,8 @@ void many_rows_kernel(const Params a) {
 // the waves' own left each idle half of the time (one prompt of 8192 tokens, 32 heads of
 // 128: 562 us in four-wave workgroups, two a CU).  Waves 0 to 3 copy K, waves 4 to 7 copy
 // V, three blocks of each in LDS.  511 us, 1076 TFLOP/s, where the library's large matrix
-// product reaches 1184: the products' turn takes 1320 cycles (1024 are the matrix cores'
-// own), the other one 1100 for the probabilities and 600 for the copies.
+// product reaches 1184; by the counters the matrix cores are busy 51% of the cycles and
+// vector instructions take 49%.
 constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideRing = 3;
 template <int DP>
 constexpr int kWideBlock = kManyKeys * DP * 2;  // bytes of K, or of V
@@ -1489,17 +1491,19 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const int64_t most_units = ceil_div(p.max_len, unit) + 1;  // of a tile: its first block may begin early
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
-    // A few rows: a unit of 128 keys takes a workgroup 1.16 us, the split with its second launch
-    // some 6 us.  One sequence, 8 heads, whole and split: 777 keys 14.1 and 15.0 us, 1100 keys
-    // 16.2 and 14.4, 8000 keys 72 and 23.  Where half of the CUs have a tile of their own (16
-    // sequences) there is less to gain: 2400 keys 27.8 and 29.8, 4000 keys 56.5 and 48.1.
+    // A few rows: a workgroup takes about 1.1 us a unit of 128 keys, the split a second launch
+    // and the partial outputs' way through memory, which grow with the tiles.  Heads of 128, 8
+    // of them, whole and split, us: 1 sequence of 640 keys 11.5 and 13.4, 777 14.1 and 13.2,
+    // 8000 72 and 23; 4 of 777 14.0 and 14.1, 900 15.1 and 14.0; 8 of 1100 16.9 and 19.9, 1600
+    // 20.5 and 21.4, 2400 26.7 and 24.2; 12 of 2400 27.1 and 27.5; 16 of 2400 27.7 and 29.4,
+    // 4000 56.1 and 47.0.
     // Else where the tiles leave at least half of the chip idle and are long, since a piece's
     // partial outputs are written and read again: 270 tiles of 128 rows on 512 places, 18 blocks
     // each, took 49 us whole and 65 split.
     p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
     const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
     const bool wanted = forced_split ? forced_split[0] == '1'
-                        : few ? most_units > (2 * c.tiles * p.kv_heads >= cus ? 22 : 8)
+                        : few ? most_units > (8 * c.tiles * p.kv_heads <= cus ? 7 : 4 * c.tiles * p.kv_heads <= cus ? 16 : 22)
                               : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
     p.split = wanted && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     c.grid = (int)(c.tiles * p.kv_heads);

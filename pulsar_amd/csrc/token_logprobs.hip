@@ -15,8 +15,9 @@
 // it holds, those above the exact bound and the first k that equal it are; failing that,
 // k rounds of a workgroup-wide maximum find the same tokens.
 //
-// 2048 tokens of 100003 bf16 logits (410 MB) take 171 us and 12 for the join (2.2 TB/s):
-// bound by the vector units, which spend about 16 instructions on a logit (unpacking
+// 2048 tokens of 100003 bf16 logits (410 MB) take 159 us and 28 for the join under a
+// profiler, 184 a call (2.2 TB/s): bound by the vector units, busy 74% of the first
+// launch's cycles, which spend about 21 instructions on a logit (unpacking
 // twice, the maximum, six for the sums with one transcendental, the rank's two where a
 // vector holds a logit that is ahead).
 //
