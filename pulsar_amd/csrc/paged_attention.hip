@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdlib>
@@ -64,7 +65,7 @@ struct Params {
     int32_t max_q, max_len;  // max_len: keys that tables and caller allow
     int32_t window;
     float scale2;            // |scale| log2(e), above 0; with a cap, scale / cap
-    float cap2;              // cap * log2(e)
+    float cap2;              // cap log2(e), 0 without a cap
     uint32_t flip;           // sign bits of q's elements to turn over: a negative scale without a cap
     int32_t flat;            // 2: pages of a power of two of keys, 16 at least; 1: of a multiple of 8
     int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
@@ -191,20 +192,51 @@ __device__ __forceinline__ int first_above(const int* ends, int n, int v) {
     return lo;
 }
 
-// Scores are held raw, their factor `unit()` (to units of log2) going into the
-// exponent's fma; or, with a cap, in units of log2: cap tanh(x) = cap (1 - 2 / (e^2x + 1)).
-template <bool CAP>
-__device__ __forceinline__ float score(const Params& a, float s) {
-    if constexpr (CAP) {
-        const float e = __builtin_amdgcn_exp2f(s * (a.scale2 * (2.f * kLog2e)));
-        return a.cap2 - 2.f * a.cap2 * __builtin_amdgcn_rcpf(e + 1.f);
-    } else {
-        return s;
-    }
-}
+// Scores are held raw, or with a cap as tanh(s scale / cap); their factor `unit()` (to
+// units of log2) goes into the exponent's fma.
 template <bool CAP>
 __device__ __forceinline__ float unit(const Params& a) {
-    return CAP ? 1.f : a.scale2;
+    return CAP ? a.cap2 : a.scale2;
+}
+
+// tanh for |x| < kSeries by its Taylor series, the next term of which is below 2^-24 x
+// there: 1 - 2 / (e^2x + 1) subtracts two numbers near 1, so its error is 2^-24 of 1 at
+// least, which a cap far above the scores would make an error of 2^-24 of the cap.
+constexpr float kSeries = 0.5f;
+__device__ __forceinline__ float tanh_series(float x) {
+    const float y = x * x;
+    float p = 21844.f / 6081075;
+    p = __builtin_fmaf(p, y, -1382.f / 155925);
+    p = __builtin_fmaf(p, y, 62.f / 2835);
+    p = __builtin_fmaf(p, y, -17.f / 315);
+    p = __builtin_fmaf(p, y, 2.f / 15);
+    p = __builtin_fmaf(p, y, -1.f / 3);
+    return __builtin_fmaf(x * y, p, x);
+}
+__device__ __forceinline__ float tanh_of(float x) {
+    const float e = __builtin_amdgcn_exp2f(x * (2.f * kLog2e));
+    const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+    return fabsf(x) < kSeries ? tanh_series(x) : far;
+}
+// With a cap, N raw scores become their tanh.  Every lane of the wave calls it: mostly all
+// its scores are far below the cap, and the series is all there is to do.
+template <bool CAP, int N, typename V>
+__device__ __forceinline__ void cap_scores(const Params& a, V& s) {
+    if constexpr (CAP) {
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            s[e] *= a.scale2;
+            most = fmaxf(most, fabsf(s[e]));
+        }
+        if (__any(most >= kSeries)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = tanh_of(s[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = tanh_series(s[e]);
+        }
+    }
 }
 
 // fp16 probabilities are held times 2^6, so that those of keys far below the
@@ -337,7 +369,7 @@ __device__ __forceinline__ RowResult plain_row(const Params& a, int b, int token
             const uint16_t* const key = reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(a.k) + at);
             float dot = 0.f;
             for (int d = 0; d < a.dim; ++d) dot += to_float<BF16>(q[d]) * to_float<BF16>(key[d]);
-            s = score<CAP>(a, a.flip ? -dot : dot) * unit<CAP>(a);
+            s = (CAP ? tanh_of(dot * a.scale2) : a.flip ? -dot : dot) * unit<CAP>(a);
         }
         const float m = fmaxf(r.m2, wave_max(s)), shift = m == -kInf ? 0.f : m;
         const float p = __builtin_amdgcn_exp2f(s - shift), scale = __builtin_amdgcn_exp2f(r.m2 - shift);
@@ -815,8 +847,10 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
             for (int mt = 0; mt < MT; ++mt) {
                 float x[8], top = -kInf;
 #pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[mt][e / 4][e % 4];
+                cap_scores<CAP, 8>(a, x);
+#pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    x[e] = score<CAP>(a, s[mt][e / 4][e % 4]);
                     const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
                     x[e] = masked & ((key < row_lo[mt]) | (key >= row_hi[mt])) ? -kInf : x[e];
                     top = fmaxf(top, x[e]);
@@ -1116,12 +1150,8 @@ void many_rows_kernel(const Params a) {
                 s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
                 if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
             }
-            if constexpr (CAP) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[kt][e] = score<CAP>(a, s[kt][e]);
-            }
+            cap_scores<CAP, 16>(a, s[0]);
+            cap_scores<CAP, 16>(a, s[1]);
             r.mask(key0, h, s);
             float top = -kInf;
 #pragma unroll
@@ -1311,12 +1341,8 @@ void wide_rows_kernel(const Params a) {
                     copy(i + 3, place_now, id);
                 }
                 if (do_next) {
-                    if constexpr (CAP) {
-#pragma unroll
-                        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) s[kt][e] = score<CAP>(a, s[kt][e]);
-                    }
+                    cap_scores<CAP, 16>(a, s[0]);
+                    cap_scores<CAP, 16>(a, s[1]);
                     r.mask(next, h, s);
                     float top = -kInf;
 #pragma unroll
@@ -1467,10 +1493,14 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.max_len = (int32_t)std::min(a->max_seq_len, held);
     p.window = (int32_t)a->window;
     // a scale of 0 is held as one that leaves nothing of a score either, so that -inf stays -inf
-    p.scale2 = a->softcap > 0.f ? a->scale / a->softcap : std::max(std::fabs(a->scale) * kLog2e, 0x1p-100f);
+    // Caps are held between 2^-100 and 2^100: no e^s tells a smaller one from 0, and what a
+    // larger one takes off a score below 2^88 is lost in the score's own rounding.
+    const float cap = std::min(std::max(a->softcap, 0x1p-100f), 0x1p100f);
+    p.scale2 = a->softcap > 0.f ? std::min(std::max(a->scale / cap, -FLT_MAX), FLT_MAX)
+                                : std::max(std::fabs(a->scale) * kLog2e, 0x1p-100f);
     p.flip = a->softcap > 0.f || a->scale >= 0.f ? 0 : 0x80008000u;
     p.flat = (uint64_t)a->page_size * p.row_bytes > UINT32_MAX ? 0 : p.page_shift >= 4 ? 2 : a->page_size % 8 == 0 ? 1 : 0;
-    p.cap2 = a->softcap * kLog2e;
+    p.cap2 = a->softcap > 0.f ? cap * kLog2e : 0.f;
     const int64_t rows = (int64_t)p.max_q * p.group;
     c.dp = padded_dim(a->head_dim);
     const int cus = device_cus();

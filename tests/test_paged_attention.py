@@ -441,3 +441,44 @@ def test_fake_kernel():
 def test_opcheck():
     torch.library.opcheck(torch.ops.pulsar.paged_attention.default, tuple(_good().values()),
                           test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"))
+
+
+def _one_key(values, dtype, n=1, **options):
+    """lse of queries that see one key each, whose score before scale and cap is values[h] exactly: a
+    head a value, the query 1 in one element and 0 else.  n > 1: the first query of a prompt of n."""
+    heads, dim, page = len(values), 64, 16
+    kc = torch.zeros(-(-n // page), page, heads, dim, dtype=dtype)
+    kc[0, 0, :, 3] = values.to(dtype)
+    q = torch.zeros(n, heads, dim, dtype=dtype)
+    q[:, :, 3] = 1
+    kc, q = kc.to(DEV), q.to(DEV)
+    tables = torch.arange(kc.shape[0], dtype=torch.int32, device=DEV)[None]
+    _, lse = ops.paged_attention(q, kc, torch.zeros_like(kc), tables, torch.tensor([n], dtype=torch.int32, device=DEV),
+                                 offsets([n]).to(DEV), n, n, return_lse=True, **options)
+    return lse[0].cpu().double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("cap", [1e-3, 0.5, 30.0, 1e3, 1e6, 1e12, 3e38])
+@pytest.mark.parametrize("n,tile", [(1, None), (70, 128), (300, 256)])
+def test_softcap_of_any_size(plan, n, tile, cap, dtype):
+    """The capped score of one key is its lse.  c tanh(s / c): s / c has a relative error of 2 eps, the
+    tanh 8 (the hardware's exp2 and reciprocal at s / c = 1/2, its worst place), units of log2 and back
+    5: 15 eps of the score; e^0 and its logarithm, whatever factor a sum is held with, some 20 eps."""
+    plan(tile=tile)
+    scale = 0.75
+    s = torch.cat([torch.logspace(-6, 4, 31), -torch.logspace(-6, 4, 31), torch.zeros(1)]).to(dtype)
+    got = _one_key(s, dtype, n, softcap=cap, scale=scale)
+    c = float(torch.tensor(cap, dtype=torch.float32))
+    want = c * torch.tanh(s.double() * scale / c)
+    eps = 2.0 ** -24
+    assert bool(((got - want).abs() <= (20 * want.abs() + 24) * eps).all()), float((got - want).abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e7])
+@pytest.mark.parametrize("new", [1, 100])
+def test_softcap_far_above_the_scores(new, cap):
+    _run([400, 123], [new, new], cap=cap, seed=7)
+    _run([90, 300], [new, new], heads=1, group=3, dim=80, cap=cap, dtype=H, seed=8)
