@@ -81,11 +81,14 @@ class PagedKVCache:
         return torch.tensor(rows, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
 
     def fork(self, src: list[int], dst: list[int]) -> torch.Tensor:
-        """Rows dst become copies of rows src; returns the free pages that lacked (int32 [1])."""
+        """Rows dst become copies of rows src; returns the free pages that lacked (int32 [1]).  What the
+        rows dst held is given back first, whether or not there is room for the copies."""
         if len(src) != len(dst) or len(set(dst)) != len(dst) or set(src) & set(dst):
             raise ValueError("PagedKVCache.fork: as many sources as destinations, each destination once and no source")
-        missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens,
-                                       self._rows(src, "fork"), self._rows(dst, "fork"))
+        src_rows, dst_rows = self._rows(src, "fork"), self._rows(dst, "fork")
+        if any(self._most[d] for d in dst):
+            ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, dst_rows)
+        missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens, src_rows, dst_rows)
         for s, d in zip(src, dst):
             self._most[d] = self._most[s]
         return missing

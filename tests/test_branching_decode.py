@@ -87,3 +87,18 @@ def test_refusals():
         cache.free([2])
     with pytest.raises(ValueError, match="destination"):
         cache.fork([0, 1], [1, 0])
+
+
+@pytest.mark.gpu
+def test_forking_onto_rows_in_use_gives_their_pages_back():
+    cache = PagedKVCache(layers=1, pages=12, page_size=8, kv_heads=1, head_dim=64, rows=4, max_seq_len=64)
+    cache.extend([20, 17, 9, 0])
+    assert int((cache.ref_counts > 0).sum()) == 8
+    assert int(cache.fork([0, 0], [1, 3])) == 0
+    assert cache.seq_lens.tolist() == [20, 20, 9, 20]
+    tables = [[p for p in r if p >= 0] for r in cache.block_tables.tolist()]
+    assert tables[1][:2] == tables[3][:2] == tables[0][:2] and [len(t) for t in tables] == [3, 3, 2, 3]
+    held = torch.bincount(torch.tensor([p for r in tables for p in r]), minlength=12)
+    assert torch.equal(held.int(), cache.ref_counts.cpu())  # every count is of a row that is there
+    cache.free([0, 1, 2, 3])
+    assert int(cache.ref_counts.abs().sum()) == 0
