@@ -37,7 +37,7 @@ extern "C" {
  *   s_j = scale * q . k_j       with softcap c > 0:  c * tanh(s_j / c)
  *   lse = ln sum_j e^{s_j},  out = sum_j e^{s_j - lse} v_j
  * A query that sees no key gets out = 0 and lse = -inf, and so do the rows of q
- * past cu_q[batch].  Keys that no query of their sequence sees may hold
+ * past cu_q[batch] and those of queries past max_q_len.  Keys that no query of their sequence sees may hold
  * anything, NaN included.
  *
  * Heads are grouped: query head h reads key-value head h / (q_heads / kv_heads).
@@ -51,7 +51,7 @@ extern "C" {
  *            q_heads] fp32 or NULL
  *   max_q_len, max_seq_len  upper bounds of n_b and seq_lens[b]: the grid is
  *            sized by them, longer sequences are cut to them (keys past
- *            max_seq_len are not seen, queries past max_q_len not computed)
+ *            max_seq_len are not seen, queries past max_q_len come out empty)
  * head_dim: a multiple of 8 up to 256.  Pointers 16-byte aligned, strides
  * multiples of 8, row_stride below 2^24. */
 typedef struct pw4_paged_attention_args {

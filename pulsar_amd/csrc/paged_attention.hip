@@ -570,11 +570,10 @@ __device__ __forceinline__ uint16_t* out_row(const Params& a, const Tile& t, int
     return a.out + ((int64_t)(t.q0 + i) * a.q_heads + head * a.group + r - i * a.group) * a.dim;
 }
 
-// Rows of out past the last sequence.
-__device__ __forceinline__ void clear_tail(const Params& a) {
-    const int first = a.batch > 0 ? min(max(a.cu[a.batch], 0), a.num_tokens) : 0;
+// Tokens begin, begin + step, ... of [begin, end): out 0, lse -inf.
+__device__ __forceinline__ void clear_tokens(const Params& a, int begin, int end, int step) {
     const int64_t per_token = (int64_t)a.q_heads * a.dim;
-    for (int t = first + (int)blockIdx.x; t < a.num_tokens; t += gridDim.x) {
+    for (int t = begin; t < end; t += step) {
         for (int64_t e = (int64_t)threadIdx.x * 8; e < per_token; e += blockDim.x * 8) {
             *reinterpret_cast<u32x4*>(a.out + t * per_token + e) = u32x4{0, 0, 0, 0};
         }
@@ -582,6 +581,18 @@ __device__ __forceinline__ void clear_tail(const Params& a) {
             for (int h = threadIdx.x; h < a.q_heads; h += blockDim.x) a.lse[(int64_t)t * a.q_heads + h] = -kInf;
         }
     }
+}
+// Rows of out that no tile has: past the last sequence, and of each sequence past the
+// max_q tokens that are computed (a workgroup a sequence).
+__device__ __forceinline__ void clear_rest(const Params& a) {
+    const int first = a.batch > 0 ? min(max(a.cu[a.batch], 0), a.num_tokens) : 0;
+    if (a.max_q < a.num_tokens) {
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            const int c0 = min(max(a.cu[b], 0), a.num_tokens), c1 = min(a.cu[b + 1], a.num_tokens);
+            if (c1 - c0 > a.max_q) clear_tokens(a, c0 + a.max_q, c1, 1);
+        }
+    }
+    if (first < a.num_tokens) clear_tokens(a, first + (int)blockIdx.x, a.num_tokens, gridDim.x);
 }
 
 // What the second launch of a split call reads: the tiles and units there are, then for
@@ -956,7 +967,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
         }
         __syncthreads();  // the ring is used again
     }
-    clear_tail(a);
+    clear_rest(a);
 }
 
 // ---- many rows --------------------------------------------------------------------
@@ -1206,7 +1217,7 @@ void many_rows_kernel(const Params a) {
         store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
         __syncthreads();  // every wave is done with the stages
     }
-    clear_tail(a);
+    clear_rest(a);
 }
 
 // ---- a great many rows -----------------------------------------------------------------
@@ -1385,7 +1396,7 @@ void wide_rows_kernel(const Params a) {
         store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
         __syncthreads();  // every wave is done with the ring
     }
-    clear_tail(a);
+    clear_rest(a);
 }
 
 // ---- joining partial results --------------------------------------------------------

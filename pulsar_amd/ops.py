@@ -225,13 +225,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         k_cache, v_cache: [pages, page_size, kv_heads, head_dim] in q's dtype, head_dim (a multiple
             of 8 up to 256) contiguous; any other strides that keep rows 16-byte aligned.
         block_tables, seq_lens, cu_q: int32 [batch, width], [batch] and [batch + 1].
-        max_q_len, max_seq_len: bounds of n and seq_lens that the host knows; what is past them is
-            cut off.
+        max_q_len, max_seq_len: bounds of n and seq_lens that the host knows; keys past the latter
+            are not seen, queries past the former come out empty.
         scale: defaults to 1 / sqrt(head_dim).
 
     Returns:
         out like q (contiguous), and with return_lse also lse = ln sum e^s, fp32 [T, q_heads].  A
-        query that sees no key, and a row of q past cu_q[-1], has out 0 and lse -inf.
+        query that sees no key or is past max_q_len, and a row of q past cu_q[-1], has out 0 and
+        lse -inf.
     """
     out, lse = _paged_attention(q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len,
                                                 max_seq_len, scale, window, softcap, return_lse)

@@ -482,3 +482,33 @@ def test_softcap_of_any_size(plan, n, tile, cap, dtype):
 def test_softcap_far_above_the_scores(new, cap):
     _run([400, 123], [new, new], cap=cap, seed=7)
     _run([90, 300], [new, new], heads=1, group=3, dim=80, cap=cap, dtype=H, seed=8)
+
+
+def _filled(shape, dtype):
+    """Leaves memory of 7s to the allocator, where the next tensor of this size is likely to lie."""
+    return torch.full(shape, 7, dtype=dtype, device=DEV).data_ptr()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("most,tile", [(0, None), (1, None), (5, None), (40, 128), (90, 256)])
+def test_queries_past_max_q_len_are_empty(plan, most, tile, split):
+    """Of more new tokens than max_q_len the first ones are computed, at their places, and the others'
+    rows are out 0 and lse -inf."""
+    plan(split, 1, tile)
+    lens, new, dim = [300, 150, 2, 40], [100, 150, 2, 0], 64
+    kc, vc, tables, ks, vs = paged_kv(lens, 16, 2, dim, B, 3)
+    q = torch.randn(sum(new) + 3, 4, dim, generator=gen(4)).to(B).to(DEV)
+    cu = offsets(new)
+    _filled(q.shape, B), _filled(q.shape[:2], torch.float32)
+    out, lse = ops.paged_attention(q, kc, vc, tables, torch.tensor(lens, dtype=torch.int32, device=DEV), cu.to(DEV),
+                                   most, max(lens), return_lse=True)
+    computed = torch.zeros(q.shape[0], dtype=torch.bool)
+    for b, n in enumerate(new):
+        c0, m = int(cu[b]), min(n, most)
+        if m == 0:
+            continue
+        computed[c0:c0 + m] = True
+        out_ref = attention_ref(q[c0:c0 + n].cpu(), ks[b], vs[b], lens[b], n, dim ** -0.5, 0, 0.0)
+        check_attention(out[c0:c0 + m], lse[c0:c0 + m], [r[:m] for r in out_ref], dim, lens[b], B)
+    assert bool((out.cpu()[~computed] == 0).all()) and bool((lse.cpu()[~computed] == -math.inf).all())
