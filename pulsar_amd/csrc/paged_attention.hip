@@ -552,7 +552,8 @@ __device__ __forceinline__ bool must_repeat(const Params& a, const Tile& t, int 
     return a.window > 0 && values_not_finite<BF16>(a, t, head, t.lo, last + 1 - a.window);
 }
 
-// Where a piece of a tile goes: the call's outputs, or partial slot `slot` >= 0.
+// Where a piece of a tile goes: the call's outputs, or partial slot `slot` >= 0.  (A row whose
+// scores are all NaN has a maximum of -inf too, but a sum of NaN, and so has its lse.)
 template <int MR, bool BF16>
 __device__ __forceinline__ void store_stats(const Params& a, const Tile& t, int head, int row, int slot, float m2, float z) {
     if (slot >= 0) {
@@ -562,7 +563,7 @@ __device__ __forceinline__ void store_stats(const Params& a, const Tile& t, int 
     } else if (a.lse != nullptr) {
         const int r = t.row0 + row, i = r / a.group;
         a.lse[(int64_t)(t.q0 + i) * a.q_heads + head * a.group + r - i * a.group] =
-            m2 == -kInf ? -kInf : (m2 + (__builtin_amdgcn_logf(z) - kLift<BF16>)) * kLn2;
+            m2 == -kInf && z == 0.f ? -kInf : (m2 + (__builtin_amdgcn_logf(z) - kLift<BF16>)) * kLn2;
     }
 }
 __device__ __forceinline__ uint16_t* out_row(const Params& a, const Tile& t, int head, int row) {

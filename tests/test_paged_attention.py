@@ -512,3 +512,44 @@ def test_queries_past_max_q_len_are_empty(plan, most, tile, split):
         out_ref = attention_ref(q[c0:c0 + n].cpu(), ks[b], vs[b], lens[b], n, dim ** -0.5, 0, 0.0)
         check_attention(out[c0:c0 + m], lse[c0:c0 + m], [r[:m] for r in out_ref], dim, lens[b], B)
     assert bool((out.cpu()[~computed] == 0).all()) and bool((lse.cpu()[~computed] == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("new,tile", [(1, None), (7, None), (60, 128), (200, 256)])
+def test_nan_scores_have_a_nan_lse(plan, new, tile, split):
+    """A query of NaN, and a key of NaN for the queries that see it: out and lse are NaN (-inf is the
+    lse of a query that sees no key), and no other row's change."""
+    plan(split, 1, tile)
+    lens, page, dim = [new + 130], 16, 64
+    kc, vc, tables, ks, vs = paged_kv(lens, page, 2, dim, B, 8)
+    q = torch.randn(new, 4, dim, generator=gen(9)).to(B)
+    args = (torch.tensor(lens, dtype=torch.int32, device=DEV), offsets([new]).to(DEV), new, lens[0])
+    ref = attention_ref(q, ks[0], vs[0], lens[0], new, dim ** -0.5, 0, 0.0)
+
+    def check(out, lse, bad):  # bad [new, 4]
+        assert torch.equal(lse.cpu().isnan(), bad) and torch.equal(out.cpu().isnan().all(-1), bad)
+        fine = ~bad
+        check_attention(out.cpu()[fine], lse.cpu()[fine], [r[fine] for r in ref], dim, lens[0], B)
+
+    bad = torch.zeros(new, 4, dtype=torch.bool)
+    bad[new // 2, 1] = True
+    broken = torch.where(bad[..., None], math.nan, q)
+    check(*ops.paged_attention(broken.to(DEV), kc, vc, tables, *args, return_lse=True), bad)
+    j = lens[0] - 1 - (new - 1) // 2  # its queries: those from new - 1 - (new - 1) // 2 on
+    kc[int(tables[0, j // page]), j % page, 1, 5] = math.nan
+    bad = torch.zeros(new, 4, dtype=torch.bool)
+    bad[new - 1 - (new - 1) // 2:, 2:] = True
+    check(*ops.paged_attention(q.to(DEV), kc, vc, tables, *args, return_lse=True), bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [0, 1])
+def test_nan_scores_only(plan, split):
+    """Every score of a row NaN, in one piece or many."""
+    plan(split, 1)
+    kc, vc, tables, _, _ = paged_kv([700, 1], 16, 1, 128, H, 8)
+    q = torch.full((2, 3, 128), math.nan, dtype=H, device=DEV)
+    out, lse = ops.paged_attention(q, kc, vc, tables, torch.tensor([700, 1], dtype=torch.int32, device=DEV),
+                                   offsets([1, 1]).to(DEV), 1, 700, return_lse=True)
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
