@@ -542,14 +542,16 @@ __device__ __forceinline__ bool values_not_finite(const Params& a, const Tile& t
 }
 
 // Whether rows whose output is not finite have to be computed again one by one: some
-// key of [t.lo, t.hi) that not every row sees has a value that is not finite, or the head
-// is narrower than the kernel's (its padding repeats key elements against zeros).
+// key of [t.lo, t.hi) that not every row sees has a value that is not finite, or the first or
+// the last one has, which stand in for the block's keys outside (a probability of 0, and
+// 0 * inf is not inf), or the head is narrower than the kernel's (its padding repeats key
+// elements against zeros).
 template <bool BF16>
 __device__ __forceinline__ bool must_repeat(const Params& a, const Tile& t, int head, int dp) {
     if (a.dim != dp) return true;
     const int first = t.first_pos + t.row0 / a.group, last = t.first_pos + (t.row0 + t.rows - 1) / a.group;
-    if (values_not_finite<BF16>(a, t, head, first + 1, t.hi)) return true;
-    return a.window > 0 && values_not_finite<BF16>(a, t, head, t.lo, last + 1 - a.window);
+    if (values_not_finite<BF16>(a, t, head, min(first + 1, t.hi - 1), t.hi)) return true;
+    return a.window > 0 && values_not_finite<BF16>(a, t, head, t.lo, max(last + 1 - a.window, t.lo + 1));
 }
 
 // Where a piece of a tile goes: the call's outputs, or partial slot `slot` >= 0.  (A row whose

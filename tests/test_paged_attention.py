@@ -553,3 +553,25 @@ def test_nan_scores_only(plan, split):
     out, lse = ops.paged_attention(q, kc, vc, tables, torch.tensor([700, 1], dtype=torch.int32, device=DEV),
                                    offsets([1, 1]).to(DEV), 1, 700, return_lse=True)
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("window", [0, 21])
+@pytest.mark.parametrize("group,tile", [(1, None), (4, None), (40, 128), (70, 256)])
+def test_infinite_values_of_the_outermost_keys(plan, group, tile, window, split):
+    """The first and the last key that a query sees hold an infinite value: its outputs there are that
+    infinity, not NaN (the keys around them in a block take no part)."""
+    plan(split, 1, tile)
+    length, page, dim = 77, 16, 64
+    first = length - window if window else 0
+    for j, bad in ((length - 1, math.inf), (first, -math.inf)):
+        kc, vc, tables, ks, vs = paged_kv([length], page, 1, dim, B, 8)
+        vs[0][j, 0, 9] = bad
+        vc[int(tables[0, j // page]), j % page, 0, 9] = bad
+        q = torch.randn(1, group, dim, generator=gen(9)).to(B).to(DEV)
+        out, lse = ops.paged_attention(q, kc, vc, tables, torch.tensor([length], dtype=torch.int32, device=DEV),
+                                       offsets([1]).to(DEV), 1, length, window=window, return_lse=True)
+        ref = attention_ref(q.cpu(), ks[0], vs[0], length, 1, dim ** -0.5, window, 0.0)
+        check_attention(out, lse, ref, dim, length, B)
+        assert bool((out[:, :, 9] == bad).all())
