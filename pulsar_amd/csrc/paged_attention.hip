@@ -1626,7 +1626,7 @@ int check(const pw4_paged_attention_args* a) {
         a->head_dim % 8 != 0 || a->page_size > INT_MAX || a->table_stride < a->table_width) {
         return PW4_ERR_SHAPE;
     }
-    if (!(a->softcap >= 0.f) || a->scale != a->scale) return PW4_ERR_ARG;
+    if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale)) return PW4_ERR_ARG;
     if (a->num_tokens == 0) return PW4_OK;
     if (!a->q || !a->out || !a->cu_q || (a->batch && !a->seq_lens)) return PW4_ERR_ARG;
     if (a->batch && a->table_width && a->num_pages && (!a->k_cache || !a->v_cache || !a->block_tables)) return PW4_ERR_ARG;

@@ -130,8 +130,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, con
     TORCH_CHECK(k_cache.size(1) > 0, op, ": page_size must be positive");
     TORCH_CHECK(max_q_len >= 0 && max_seq_len >= 0, op, ": max_q_len and max_seq_len must not be negative");
     TORCH_CHECK(window >= 0, op, ": window must not be negative");
-    TORCH_CHECK(softcap >= 0 && std::isfinite(softcap), op, ": softcap must be finite and not negative");
-    TORCH_CHECK(!scale || std::isfinite(*scale), op, ": scale must be finite");
+    TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), op, ": softcap must be finite in fp32 and not negative");
+    TORCH_CHECK(!scale || std::isfinite((float)*scale), op, ": scale must be finite in fp32");
     for (const at::Tensor* c : {&k_cache, &v_cache}) {
         TORCH_CHECK(c->numel() == 0 || (aligned16(*c) && stride_of(*c, 0) % 8 == 0 && stride_of(*c, 1) % 8 == 0 &&
                                         stride_of(*c, 2) % 8 == 0),
@@ -172,7 +172,8 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, con
     a.max_seq_len = max_seq_len;
     a.window = window;
     a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
-    a.softcap = (float)softcap;
+    // (a cap above 0 stays one: the kernel takes what is below 2^-100 as 2^-100)
+    a.softcap = softcap > 0 ? std::max((float)softcap, 0x1p-100f) : 0.f;
     a.dtype = q.scalar_type() == at::kBFloat16 ? PW4_DTYPE_BF16 : PW4_DTYPE_F16;
     const size_t bytes = pw4_paged_attention_workspace_size(&a);
     const at::Tensor ws = bytes ? scratch(bytes, q) : at::Tensor();

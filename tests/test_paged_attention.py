@@ -575,3 +575,19 @@ def test_infinite_values_of_the_outermost_keys(plan, group, tile, window, split)
         ref = attention_ref(q.cpu(), ks[0], vs[0], length, 1, dim ** -0.5, window, 0.0)
         check_attention(out, lse, ref, dim, length, B)
         assert bool((out[:, :, 9] == bad).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["softcap", "scale"])
+def test_refuses_what_32_bits_cannot_hold(name):
+    with pytest.raises(RuntimeError, match=name):
+        ops.paged_attention(**dict(_good(), **{name: 1e39}))
+
+
+def test_c_entry_refuses_infinite_factors():
+    lib = pulsar_amd.capi()
+    lib.pw4_paged_attention.argtypes = [ctypes.POINTER(_Args), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    for change in (dict(softcap=math.inf), dict(scale=math.inf), dict(scale=-math.inf)):
+        a = dict(num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, page_size=16, scale=1.0, dtype=1)
+        assert lib.pw4_paged_attention(ctypes.byref(_Args(**a)), None, 0, None) == 0
+        assert lib.pw4_paged_attention(ctypes.byref(_Args(**dict(a, **change))), None, 0, None) == -1
