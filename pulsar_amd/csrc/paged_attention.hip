@@ -1532,7 +1532,14 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     // workgroups that run at once
     const int slots = few ? (c.dp == 64 ? 2 * cus : cus) : c.tile_rows == kManyRows && c.dp != 256 ? 2 * cus : cus;
-    const int64_t most_units = ceil_div(p.max_len, unit) + 1;  // of a tile: its first block may begin early
+    // Units of a tile: of the keys that a window leaves its rows, or all.  (Its first block may begin
+    // early.)  32 query on 8 key-value heads of 128, sequences of 32768 keys, the rules below by
+    // these units and by all of the sequence's, us: 8 tokens in a window of 128 7.1 and 9.7, two
+    // chunks of 100 in one of 512 22.6 and 45.1, in one of 128 15.4 and 49.0.
+    const int64_t most_keys =
+        p.window == 0 ? p.max_len
+                      : std::min<int64_t>(p.max_len, (int64_t)p.window + (std::min<int64_t>(c.tile_rows, rows) + p.group - 2) / p.group);
+    const int64_t most_units = ceil_div(most_keys, unit) + 1;
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
     // A few rows: a workgroup takes about 1.1 us a unit of 128 keys, the split a second launch

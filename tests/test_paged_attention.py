@@ -591,3 +591,43 @@ def test_c_entry_refuses_infinite_factors():
         a = dict(num_tokens=0, q_heads=4, kv_heads=2, head_dim=64, page_size=16, scale=1.0, dtype=1)
         assert lib.pw4_paged_attention(ctypes.byref(_Args(**a)), None, 0, None) == 0
         assert lib.pw4_paged_attention(ctypes.byref(_Args(**dict(a, **change))), None, 0, None) == -1
+
+
+def _workspace(**change):
+    lib = pulsar_amd.capi()
+    lib.pw4_paged_attention_workspace_size.argtypes = [ctypes.POINTER(_Args)]
+    lib.pw4_paged_attention_workspace_size.restype = ctypes.c_size_t
+    a = dict(q=4096, k_cache=4096, v_cache=4096, block_tables=4096, seq_lens=4096, cu_q=4096, out=4096, num_tokens=8,
+             batch=8, q_heads=32, kv_heads=8, head_dim=128, num_pages=4, page_size=16, table_width=2048,
+             table_stride=2048, q_token_stride=4096, q_head_stride=128, page_stride=16384, row_stride=1024,
+             kv_head_stride=128, max_q_len=1, max_seq_len=32768, scale=1.0, dtype=1)
+    a.update(change)
+    return lib.pw4_paged_attention_workspace_size(ctypes.byref(_Args(**a)))
+
+
+def test_the_split_goes_by_the_keys_that_a_window_leaves():
+    """Workspace is asked for where the keys are split over workgroups: a tile sees `window` keys and
+    its rows' spread, however long its sequence is."""
+    chunks = dict(batch=2, num_tokens=200, max_q_len=100)
+    for case in ({}, chunks, dict(chunks, kv_heads=2, q_heads=14, head_dim=64)):
+        long = _workspace(**case)
+        assert long > 0
+        for window in (1, 128, 600):
+            short = _workspace(**case, window=window)
+            assert short == _workspace(**dict(case, max_seq_len=window + 150), window=window) == 0
+        for window in (32768, 2 ** 31 - 1):
+            assert _workspace(**case, window=window) == long
+    assert _workspace(window=30000) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [None, 1])
+@pytest.mark.parametrize("window", [1, 31, 128, 1000])
+def test_windows_in_long_sequences(plan, window, split):
+    """The newest tokens of long sequences, of which a window is seen: few rows, 128 and 256 rows."""
+    plan(split, 1 if split else None)
+    lens = [9001, 8000, 131]
+    _run(lens, [1, 2, 3], heads=2, group=4, window=window, seed=window)
+    _run(lens, [40, 1, 131], heads=1, group=3, dim=64, dtype=H, window=window, seed=window)
+    plan(split, 1 if split else None, 256)
+    _run(lens, [300, 77, 131], heads=1, group=2, dim=128, window=window, seed=window)
