@@ -47,7 +47,8 @@ void check_device(const char* op, const at::Tensor& first, std::initializer_list
 void check_ints(const char* op, const char* name, const at::Tensor& t, int64_t dim, at::ScalarType type = at::kInt) {
     TORCH_CHECK(t.scalar_type() == type && t.dim() == dim, op, ": ", name, " must be ",
                 type == at::kInt ? "int32" : "int64", " and ", dim, "-D");
-    TORCH_CHECK(t.numel() == 0 || t.stride(-1) == 1, op, ": ", name, " must be contiguous in its last dimension");
+    TORCH_CHECK(t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1, op, ": ", name,
+                " must be contiguous in its last dimension");
 }
 
 // The book-keeping of a pool: int32 ref_counts [P], block_tables [rows, width], seq_lens [rows].
@@ -73,11 +74,6 @@ void check_cache(const char* op, const char* name, const at::Tensor& c) {
                 " must be contiguous in its last dimension");
 }
 
-void check_same_layout(const char* op, const at::Tensor& k_cache, const at::Tensor& v_cache) {
-    TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.strides() == v_cache.strides() &&
-                    k_cache.scalar_type() == v_cache.scalar_type(),
-                op, ": k_cache and v_cache must have one shape, dtype and layout");
-}
 
 void check_half(const char* op, const char* name, const at::Tensor& t) {
     TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, op, ": ", name,
@@ -86,6 +82,12 @@ void check_half(const char* op, const char* name, const at::Tensor& t) {
 
 // Stride of a dimension; that of a dimension of one counts for nothing.
 int64_t stride_of(const at::Tensor& t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+void check_same_layout(const char* op, const at::Tensor& k_cache, const at::Tensor& v_cache) {
+    bool same = k_cache.sizes() == v_cache.sizes() && k_cache.scalar_type() == v_cache.scalar_type();
+    for (int64_t d = 0; same && d < k_cache.dim(); ++d) same = stride_of(k_cache, d) == stride_of(v_cache, d);
+    TORCH_CHECK(same, op, ": k_cache and v_cache must have one shape, dtype and layout");
+}
 
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 

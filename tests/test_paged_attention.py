@@ -631,3 +631,22 @@ def test_windows_in_long_sequences(plan, window, split):
     _run(lens, [40, 1, 131], heads=1, group=3, dim=64, dtype=H, window=window, seed=window)
     plan(split, 1 if split else None, 256)
     _run(lens, [300, 77, 131], heads=1, group=2, dim=128, window=window, seed=window)
+
+
+@pytest.mark.gpu
+def test_one_element_views():
+    """The stride of a dimension of one counts for nothing."""
+    args = _good()
+    want = ops.paged_attention(**args)
+    got = ops.paged_attention(**dict(args, seq_lens=args["seq_lens"].repeat(2)[::2],
+                                     block_tables=args["block_tables"].repeat(2, 1)[::2]))
+    assert torch.equal(got, want)
+    one = _good()
+    one.update(seq_lens=torch.tensor([3], dtype=torch.int32, device=DEV))
+    want = ops.paged_attention(**one)
+    got = ops.paged_attention(**dict(one, block_tables=one["block_tables"].repeat_interleave(4, 1)[:, :4:4]))
+    assert torch.equal(got, want)
+    # caches of one page, whose strides between pages differ
+    one.update(k_cache=one["k_cache"][:1], v_cache=one["v_cache"][:1], block_tables=one["block_tables"][:, :1] * 0)
+    one["v_cache"] = one["v_cache"].as_strided(one["v_cache"].shape, (8, *one["v_cache"].stride()[1:]))
+    assert ops.paged_attention(**one).shape == one["q"].shape

@@ -242,3 +242,11 @@ def test_opcheck():
     x = torch.randn(2, 50, generator=gen(1)).to(DEV)
     torch.library.opcheck(torch.ops.pulsar.token_logprobs.default, (x, torch.zeros(2, dtype=torch.int64, device=DEV), 3),
                           test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"))
+
+
+@pytest.mark.gpu
+def test_a_target_of_one_token_may_be_any_view():
+    x = torch.randn(1, 100, generator=gen(1)).to(DEV)
+    t = torch.tensor([5, 6, 7], device=DEV)
+    for a, b in zip(ops.token_logprobs(x, t[::3], 2), ops.token_logprobs(x, t[:1], 2)):
+        assert torch.equal(a, b)
