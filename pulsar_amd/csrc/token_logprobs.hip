@@ -351,15 +351,15 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LogprobArgs a) {
         a.top_logprobs[(int64_t)row * a.top_k + place] = logprob(unordered((uint32_t)(key >> 32)));
         a.top_ids[(int64_t)row * a.top_k + place] = (uint32_t)~key;
     };
-    // A number that the greatest keys of at least top_k slices reach (all keys where there are
-    // fewer slices) is a bound for the row: the few keys that reach it are ranked.
-    uint32_t bound = 0;
-    if (a.slices >= a.top_k && a.slices <= 64) {
-        const uint32_t g = lane < a.slices ? (uint32_t)(tops[(int64_t)lane * a.top_k] >> 32) : 0;
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t higher = bound | 1u << bit;
-            if (__popcll(__ballot(g >= higher)) >= a.top_k) bound = higher;
-        }
+    // A number that the q-th greatest keys of at least top_k / q slices reach is a bound for the
+    // row, which top_k keys at least reach: the few that do are ranked.  (q is 1 where there are
+    // top_k slices; a lane's number is the greatest of the slices that it has.)
+    const int q = (a.top_k + a.slices - 1) / a.slices, reach = (a.top_k + q - 1) / q;
+    uint32_t bound = 0, g = 0;
+    for (int s = lane; s < a.slices; s += 64) g = max(g, (uint32_t)(tops[(int64_t)s * a.top_k + q - 1] >> 32));
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t higher = bound | 1u << bit;
+        if (__popcll(__ballot(g >= higher)) >= reach) bound = higher;
     }
     uint64_t* const mine = s_keys[threadIdx.x >> 6];
     int count = 0;
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const LogprobArgs a) {
         }
         return;
     }
-    uint64_t below = ~0ull;  // a vocabulary of very many slices: one token a round
+    uint64_t below = ~0ull;  // many keys that tie at the bound: one token a round
     for (int k = 0; k < a.top_k; ++k) {
         uint64_t best = 0;
         for (int i = lane; i < keys; i += 64) {

@@ -250,3 +250,42 @@ def test_a_target_of_one_token_may_be_any_view():
     t = torch.tensor([5, 6, 7], device=DEV)
     for a, b in zip(ops.token_logprobs(x, t[::3], 2), ops.token_logprobs(x, t[:1], 2)):
         assert torch.equal(a, b)
+
+
+def _spread_over_few_groups(vocab, dtype, seed):
+    """A row whose larger logits, some thousand of a slice, all different, lie in the vectors that 124 of
+    a workgroup's 256 threads take (31 groups of four), and whose others are equal."""
+    vec = 128 // torch.finfo(dtype).bits
+    x = torch.zeros(vocab)
+    there = torch.nonzero((torch.arange(vocab) // (4 * vec)) % 64 < 31)[:, 0]
+    x[there] = 1 + torch.rand(len(there), generator=gen(seed)) * 6
+    return x.to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F, H, B])
+@pytest.mark.parametrize("tokens,vocab", [(1, 4096), (2, 30000), (300, 8192), (64, 30000)])
+def test_more_large_logits_than_a_list_holds(tokens, vocab, dtype):
+    x = torch.stack([_spread_over_few_groups(vocab, dtype, i) for i in range(tokens)]).to(DEV)
+    t = torch.randint(0, vocab, (tokens,), generator=gen(5)).to(DEV)
+    for top in (31, 32):
+        _check(x, t, top, ops.token_logprobs(x, t, top))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("tokens,vocab,top", [(2, 100003, 32), (2, 100003, 26), (64, 150001, 32), (64, 150001, 20),
+                                              (1, 600011, 32), (3, 600011, 5)])
+def test_rows_of_many_slices(tokens, vocab, top, dtype):
+    """More slices than top tokens and fewer, up to more slices than a wave has lanes; and the same rows
+    of a few different logits, and of almost nothing."""
+    g = gen(vocab + top)
+    t = torch.randint(0, vocab, (tokens,), generator=g).to(DEV)
+    x = (torch.randn(tokens, vocab, generator=g) * 3).to(dtype).to(DEV)
+    _check(x, t, top, ops.token_logprobs(x, t, top))
+    x = torch.randint(0, 3, (tokens, vocab), generator=g).to(dtype).to(DEV)
+    _check(x, t, top, ops.token_logprobs(x, t, top))
+    x = torch.full((tokens, vocab), -math.inf, dtype=dtype)
+    x[:, vocab // 2] = 1.0
+    x, t = x.to(DEV), torch.full_like(t, vocab // 2)
+    assert torch.equal(ops.token_logprobs(x, t, top)[4].cpu(), logprobs_ref(x.cpu(), t.cpu(), top)[4])
