@@ -73,6 +73,12 @@ def paged(cache: PagedKVCache, step: Step):
     return attend
 
 
+def room(missing: torch.Tensor, what: str) -> None:
+    """Raises where the cache had no room: it took nothing then, and the rows are as they were."""
+    if int(missing):
+        raise RuntimeError(f"{what}: {int(missing)} pages (or table columns) too few")
+
+
 def beam_search(model: Decoder, cache: PagedKVCache, prompt: torch.Tensor, beams: int, steps: int, chunk: int = 48):
     """The `beams` likeliest continuations found, [(log probability, tokens)], likeliest first, and the
     prompt's own log probabilities.  Uses rows 0 to 2 * beams - 1 of the cache."""
@@ -81,6 +87,7 @@ def beam_search(model: Decoder, cache: PagedKVCache, prompt: torch.Tensor, beams
     for at in range(0, n, chunk):  # the prompt, in chunks, into row 0
         tokens = prompt[at:at + chunk]
         step = cache.extend([tokens.numel()] + [0] * (cache.rows - 1))
+        room(step.missing, "prompt")
         logits = model.forward(tokens, torch.arange(at, at + tokens.numel(), device=dev), paged(cache, step))
         after = torch.full_like(tokens, -1)  # the token that follows each one, none behind the last
         after[:min(tokens.numel(), n - at - 1)] = prompt[at + 1:at + chunk + 1]
@@ -91,13 +98,14 @@ def beam_search(model: Decoder, cache: PagedKVCache, prompt: torch.Tensor, beams
     held = [0]
     for i in range(1, steps + 1):
         # every beam goes on in a row of its own, which shares its parent's full pages
-        cache.fork([row for _, row, _ in alive], spare)
+        room(cache.fork([row for _, row, _ in alive], spare), "fork")
         cache.free(held)
         held, spare = spare, rows
         rows = held
         if i == steps:
             break
         step = cache.extend([1 if r in held else 0 for r in range(cache.rows)])
+        room(step.missing, "next tokens")
         tokens = torch.tensor([t[-1] for _, _, t in alive], device=dev)
         logits = model.forward(tokens, torch.full((beams,), n + i - 1, device=dev), paged(cache, step))
         _, _, _, top, ids = ops.token_logprobs(logits, torch.full_like(tokens, -1), beams)

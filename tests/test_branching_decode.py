@@ -102,3 +102,21 @@ def test_forking_onto_rows_in_use_gives_their_pages_back():
     assert torch.equal(held.int(), cache.ref_counts.cpu())  # every count is of a row that is there
     cache.free([0, 1, 2, 3])
     assert int(cache.ref_counts.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+def test_a_beam_search_that_runs_out_of_pages_says_so():
+    model = example.Decoder(seed=1)
+    tokens = torch.randint(0, 1003, (33,), device="cuda:0", generator=torch.Generator("cuda:0").manual_seed(3))
+
+    def search(pages, most=64):
+        cache = PagedKVCache(layers=2, pages=pages, page_size=16, kv_heads=2, head_dim=64, rows=8, max_seq_len=most,
+                             dtype=torch.float16)
+        return example.beam_search(model, cache, tokens, beams=4, steps=3)
+
+    search(pages=10)  # 2 full pages shared by all, and a last one for each of 4 beams and each of their children
+    for pages in (9, 6, 2):  # in a later fork, in the first one, in the prompt
+        with pytest.raises(RuntimeError, match="pages"):
+            search(pages)
+    with pytest.raises(RuntimeError, match="pages"):
+        search(pages=40, most=32)  # no column for the prompt's last token
