@@ -4,7 +4,7 @@ The pool holds keys and values of every layer as planes of one tensor, [2 * laye
 page_size, kv_heads, head_dim], so a page id names the same page in all of them and forking, copying
 and compacting are one call for the whole model.  The book-keeping -- reference counts, block tables,
 lengths -- is on the device and changes in place; the host keeps only an upper bound of each row's
-length, which sizes the attention's grid.  No method waits for the device.
+length, which sizes the attention's grid.  No method but `lengths` waits for the device.
 
 The reference's engine holds such a pool behind its attention (pulsar-core's ActiveBuffer,
 active_buffer.hpp:164, and the scatter of new keys at paged_attention.cu:48).
@@ -61,9 +61,17 @@ class PagedKVCache:
         cu_q = torch.tensor(total, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
         slots, missing = ops.paged_cache_extend(self.ref_counts, self.block_tables, self.seq_lens, cu_q, total[-1],
                                                 self.page_size)
-        self._most = [m + c for m, c in zip(self._most, counts)]
+        most = self.block_tables.shape[1] * self.page_size  # an extend past a row's table is refused
+        self._most = [min(m + c, most) for m, c in zip(self._most, counts)]
         seen = [m for m, c in zip(self._most, counts) if c]
         return Step(list(counts), cu_q, slots, missing, max(counts), max(seen, default=0))
+
+    def lengths(self) -> list[int]:
+        """Each row's tokens, read from the device: this waits for it.  The host's bounds of the rows are
+        exact afterwards.  (They only grow else until a row is freed, also by what a full pool refused;
+        a bound that is too high costs speed, not results.)"""
+        self._most = self.seq_lens.tolist()
+        return list(self._most)
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """Stores the step's keys and values [T, kv_heads, head_dim] of a layer."""

@@ -120,3 +120,16 @@ def test_a_beam_search_that_runs_out_of_pages_says_so():
             search(pages)
     with pytest.raises(RuntimeError, match="pages"):
         search(pages=40, most=32)  # no column for the prompt's last token
+
+
+@pytest.mark.gpu
+def test_the_bound_of_a_row_is_held_to_its_table_and_its_length():
+    cache = PagedKVCache(layers=1, pages=3, page_size=8, kv_heads=1, head_dim=64, rows=2, max_seq_len=32)
+    cache.extend([20, 0])
+    for _ in range(5):
+        step = cache.extend([10, 0])  # refused
+        assert int(step.missing) == 1
+    assert step.max_seq_len == 32  # what the row's table holds
+    assert cache.lengths() == [20, 0]  # and after this the bounds are the lengths
+    step = cache.extend([1, 0])
+    assert int(step.missing) == 0 and step.max_seq_len == 21
