@@ -4,7 +4,9 @@ The pool holds keys and values of every layer as planes of one tensor, [2 * laye
 page_size, kv_heads, head_dim], so a page id names the same page in all of them and forking, copying
 and compacting are one call for the whole model.  The book-keeping -- reference counts, block tables,
 lengths -- is on the device and changes in place; the host keeps only an upper bound of each row's
-length, which sizes the attention's grid.  No method but `lengths` waits for the device.
+length, which sizes the attention's grid.  No method but `lengths` waits for the device.  Methods that
+take lists copy them to the device when they are called, so they do not belong into a captured graph;
+the operators may.
 
 The reference's engine holds such a pool behind its attention (pulsar-core's ActiveBuffer,
 active_buffer.hpp:164, and the scatter of new keys at paged_attention.cu:48).
@@ -51,6 +53,11 @@ class PagedKVCache:
         """Keys and values of a layer, [pages, page_size, kv_heads, head_dim]."""
         return self.pool[2 * index], self.pool[2 * index + 1]
 
+    def _ints(self, values: list[int]) -> torch.Tensor:
+        # Pageable memory: such a copy of up to 4096 rows' numbers returns at once, the device busy or
+        # not, as a test holds it to, and 3 us sooner than one from pinned memory.
+        return torch.tensor(values, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
+
     def extend(self, counts: list[int]) -> Step:
         """Takes pages for counts[b] new tokens of row b."""
         if len(counts) != self.rows or min(counts) < 0:
@@ -58,7 +65,7 @@ class PagedKVCache:
         total = [0]
         for c in counts:
             total.append(total[-1] + c)
-        cu_q = torch.tensor(total, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
+        cu_q = self._ints(total)
         slots, missing = ops.paged_cache_extend(self.ref_counts, self.block_tables, self.seq_lens, cu_q, total[-1],
                                                 self.page_size)
         most = self.block_tables.shape[1] * self.page_size  # an extend past a row's table is refused
@@ -86,7 +93,7 @@ class PagedKVCache:
     def _rows(self, rows: list[int], what: str) -> torch.Tensor:
         if any(not 0 <= r < self.rows for r in rows):
             raise ValueError(f"PagedKVCache.{what}: rows are 0 to {self.rows - 1}, got {rows}")
-        return torch.tensor(rows, dtype=torch.int32).to(self.seq_lens.device, non_blocking=True)
+        return self._ints(rows)
 
     def fork(self, src: list[int], dst: list[int]) -> torch.Tensor:
         """Rows dst become copies of rows src; returns the free pages that lacked (int32 [1]).  What the

@@ -133,3 +133,31 @@ def test_the_bound_of_a_row_is_held_to_its_table_and_its_length():
     assert cache.lengths() == [20, 0]  # and after this the bounds are the lengths
     step = cache.extend([1, 0])
     assert int(step.missing) == 0 and step.max_seq_len == 21
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 4000])
+def test_no_method_waits_for_the_device(rows):
+    """While the device is busy with something else each returns."""
+    cache = PagedKVCache(layers=1, pages=8 * rows, page_size=8, kv_heads=1, head_dim=64, rows=rows, max_seq_len=64)
+    k = torch.zeros(rows, 1, 64, dtype=torch.bfloat16, device="cuda:0")
+    half = list(range(rows // 2))
+
+    def use():
+        step = cache.extend([1] * rows)
+        cache.write(0, k, k, step)
+        cache.attend(0, k, step)
+        cache.fork(half, [r + rows // 2 for r in half])
+        cache.free(list(range(rows)))
+        cache.compact()
+
+    for _ in range(3):  # the allocators' first memory
+        use()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Event()
+    torch.cuda._sleep(1 << 28)  # a tenth of a second or more
+    busy.record()
+    use()
+    assert not busy.query()
+    torch.cuda.synchronize()
+    assert cache.lengths() == [0] * rows and int(cache.ref_counts.abs().sum()) == 0
