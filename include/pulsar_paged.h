@@ -17,7 +17,7 @@
  *   seq_lens     [rows]          tokens of each row
  * so a serving step needs no host wait.  What a kernel reads from them is
  * checked against the pool before it is used as an address: a page id outside
- * the pool reads page 0 (attention), or is passed over (everything else).
+ * the pool reads the last page (attention), or is passed over (everything else).
  */
 #ifndef PULSAR_PAGED_H
 #define PULSAR_PAGED_H

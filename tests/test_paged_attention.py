@@ -650,3 +650,18 @@ def test_one_element_views():
     one.update(k_cache=one["k_cache"][:1], v_cache=one["v_cache"][:1], block_tables=one["block_tables"][:, :1] * 0)
     one["v_cache"] = one["v_cache"].as_strided(one["v_cache"].shape, (8, *one["v_cache"].stride()[1:]))
     assert ops.paged_attention(**one).shape == one["q"].shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", [-1, 10 ** 9, -2 ** 31])
+@pytest.mark.parametrize("new", [1, 40])
+def test_page_ids_outside_the_pool_read_its_last_page(new, name):
+    lens, page = [130], 16
+    kc, vc, tables, _, _ = paged_kv(lens, page, 2, 64, B, 5, junk=1.0)
+    q = torch.randn(new, 4, 64, generator=gen(6)).to(B).to(DEV)
+    args = (torch.tensor(lens, dtype=torch.int32, device=DEV), offsets([new]).to(DEV), new, lens[0])
+    got = []
+    for page_id in (name, kc.shape[0] - 1):
+        tables[0, 2] = page_id
+        got.append(ops.paged_attention(q, kc, vc, tables, *args))
+    assert torch.equal(*got)
