@@ -243,6 +243,17 @@ __device__ __forceinline__ void cap_scores(const Params& a, V& s) {
 // maximum are not subnormal; the sum is held the same way, so outputs need nothing.
 template <bool BF16>
 constexpr float kLift = BF16 ? 0.f : 6.f;
+// What the exponents are taken against, for a maximum m of raw scores.
+template <bool BF16>
+__device__ __forceinline__ float shift_of(float m, float k) {
+    return __builtin_fmaf(m, k, -kLift<BF16>);
+}
+// The maximum (units of log2) that a row's sums are held by, to the bit: fp16's shift is rounded
+// by up to 2^-22 more than m k, which the lse would take over.
+template <bool BF16>
+__device__ __forceinline__ float held_max(float m, float k) {
+    return shift_of<BF16>(m, k) + kLift<BF16>;
+}
 // The running maximum is renewed, and sums and outputs scaled, once a score is
 // above it by this much (in units of log2): a probability is at most 2^(8 + lift).
 constexpr float kSlack = 8.f;
@@ -565,7 +576,7 @@ __device__ __forceinline__ void store_stats(const Params& a, const Tile& t, int 
     } else if (a.lse != nullptr) {
         const int r = t.row0 + row, i = r / a.group;
         a.lse[(int64_t)(t.q0 + i) * a.q_heads + head * a.group + r - i * a.group] =
-            m2 == -kInf && z == 0.f ? -kInf : (m2 + (__builtin_amdgcn_logf(z) - kLift<BF16>)) * kLn2;
+            m2 == -kInf && z == 0.f ? -kInf : (m2 + __builtin_amdgcn_logf(z * (BF16 ? 1.f : 0x1p-6f))) * kLn2;
     }
 }
 __device__ __forceinline__ uint16_t* out_row(const Params& a, const Tile& t, int head, int row) {
@@ -878,7 +889,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
                     for (int d = 0; d < DT; ++d) o[mt][d] *= scale;
                     m[mt] = m_new;
                 }
-                const float shift = (m[mt] == -kInf ? 0.f : m[mt] * k) - kLift<BF16>;
+                const float shift = m[mt] == -kInf ? -kLift<BF16> : shift_of<BF16>(m[mt], k);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     x[e] = __builtin_amdgcn_exp2f(x[e] * k - shift);
@@ -916,7 +927,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
             for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + 4 * g) = o[mt][d];
             const float all = sum_halves(sum_quarters(z[mt]));
             if (g == 0) {
-                row[DP] = m[mt] * k;
+                row[DP] = held_max<BF16>(m[mt], k);
                 row[DP + 1] = all;
             }
         }
@@ -1181,7 +1192,7 @@ void many_rows_kernel(const Params a) {
                 for (int d = 0; d < DT; ++d) o[d] *= scale;
                 m = m_new;
             }
-            const float shift = (m == -kInf ? 0.f : m * k) - kLift<BF16>;
+            const float shift = m == -kInf ? -kLift<BF16> : shift_of<BF16>(m, k);
             // Step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4.
             // Products n = (st, d) in turn, each with the read of an operand kAhead products on and a
             // share of the next step's probabilities behind it.
@@ -1217,7 +1228,7 @@ void many_rows_kernel(const Params a) {
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
+        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held_max<BF16>(m, k), z, o);
         __syncthreads();  // every wave is done with the stages
     }
     clear_rest(a);
@@ -1372,7 +1383,7 @@ void wide_rows_kernel(const Params a) {
                         for (int d = 0; d < DT; ++d) o[d] *= scale;
                         m = m_new;
                     }
-                    const float shift = (m == -kInf ? 0.f : m * k) - kLift<BF16>;
+                    const float shift = m == -kInf ? -kLift<BF16> : shift_of<BF16>(m, k);
 #pragma unroll
                     for (int st = 0; st < 4; ++st) {
                         float x[8];
@@ -1396,7 +1407,7 @@ void wide_rows_kernel(const Params a) {
             }
             if (!late) asm volatile("s_barrier" ::: "memory");
         }
-        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, m * k, z, o);
+        store_rows<BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held_max<BF16>(m, k), z, o);
         __syncthreads();  // every wave is done with the ring
     }
     clear_rest(a);

@@ -665,3 +665,25 @@ def test_page_ids_outside_the_pool_read_its_last_page(new, name):
         tables[0, 2] = page_id
         got.append(ops.paged_attention(q, kc, vc, tables, *args))
     assert torch.equal(*got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("split", [0, 1])
+def test_lse_of_two_keys(plan, dtype, split):
+    """Scores below 2 that the products give exactly, two keys a query.  Each rounding of the lse as an
+    even one: the exponents' arguments (fp16's are near 6, spaced 2^-21) 9.5e-8, exp2 7e-8, log2 of a
+    sum below 2 4e-8, the maximum's sum with it 5e-8, the lse's own 7e-8: 1.5e-7 in the mean square."""
+    plan(split, 1)
+    heads, dim = 2048, 64
+    s = (torch.rand(2, heads, generator=gen(3)) * 4 - 2).to(dtype)
+    kc = torch.zeros(1, 16, heads, dim, dtype=dtype)
+    kc[0, :2, :, 7] = s
+    q = torch.zeros(1, heads, dim, dtype=dtype)
+    q[:, :, 7] = 1
+    kc, q = kc.to(DEV), q.to(DEV)
+    _, lse = ops.paged_attention(q, kc, torch.zeros_like(kc), torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+                                 torch.tensor([2], dtype=torch.int32, device=DEV), offsets([1]).to(DEV), 1, 2,
+                                 scale=1.0, return_lse=True)
+    err = lse[0].cpu().double() - torch.logsumexp(s.double(), 0)
+    assert float(err.square().mean().sqrt()) <= 1.5e-7 and float(err.abs().max()) <= 1e-6
