@@ -52,7 +52,8 @@ extern "C" {
  *   max_q_len, max_seq_len  upper bounds of n_b and seq_lens[b]: the grid is
  *            sized by them, longer sequences are cut to them (keys past
  *            max_seq_len are not seen, queries past max_q_len come out empty)
- * scale and softcap are finite.  head_dim: a multiple of 8 up to 256.  Pointers
+ * scale and softcap are finite.  A sequence has fewer than 2^31 - 1024 rows (new
+ * tokens times the query heads of a key-value head).  head_dim: a multiple of 8 up to 256.  Pointers
  * 16-byte aligned, strides multiples of 8, row_stride below 2^24. */
 typedef struct pw4_paged_attention_args {
     const void* q;

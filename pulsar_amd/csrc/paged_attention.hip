@@ -1644,6 +1644,8 @@ int check(const pw4_paged_attention_args* a) {
         a->head_dim % 8 != 0 || a->page_size > INT_MAX || a->table_stride < a->table_width) {
         return PW4_ERR_SHAPE;
     }
+    // rows of a sequence are counted in 32 bits
+    if (std::min(a->max_q_len, a->num_tokens) * (a->q_heads / a->kv_heads) > INT_MAX - 1024) return PW4_ERR_SHAPE;
     if (!(a->softcap >= 0.f) || !std::isfinite(a->softcap) || !std::isfinite(a->scale)) return PW4_ERR_ARG;
     if (a->num_tokens == 0) return PW4_OK;
     if (!a->q || !a->out || !a->cu_q || (a->batch && !a->seq_lens)) return PW4_ERR_ARG;

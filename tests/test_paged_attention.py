@@ -687,3 +687,15 @@ def test_lse_of_two_keys(plan, dtype, split):
                                  scale=1.0, return_lse=True)
     err = lse[0].cpu().double() - torch.logsumexp(s.double(), 0)
     assert float(err.square().mean().sqrt()) <= 1.5e-7 and float(err.abs().max()) <= 1e-6
+
+
+def test_c_entry_refuses_more_rows_than_it_counts():
+    lib = pulsar_amd.capi()
+    lib.pw4_paged_attention.argtypes = [ctypes.POINTER(_Args), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+
+    def call(tokens, most):  # refused before any launch: for the rows (-2), or else for want of memory for q (-1)
+        a = dict(num_tokens=tokens, max_q_len=most, q_heads=8192, kv_heads=1, head_dim=8, page_size=16, scale=1.0, dtype=1)
+        return lib.pw4_paged_attention(ctypes.byref(_Args(**a)), None, 0, None)
+
+    assert call(2 ** 18, 2 ** 18) == -2 and call(2 ** 20, 2 ** 18) == -2
+    assert call(2 ** 18, 2 ** 17) == -1 and call(2 ** 17, 2 ** 30) == -1
