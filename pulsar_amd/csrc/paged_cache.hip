@@ -364,9 +364,9 @@ struct CompactArgs {
     int32_t* refs;
     int32_t* tables;
     int32_t* used;
-    int32_t* moves;      // workspace: how many pages move,
-    int32_t* move_src;   // [pages / 2] from where
-    int32_t* move_dst;   // [pages / 2] to where,
+    int32_t* moves;      // workspace [2]: how many pages move,
+    int32_t* move_src;   // [most_moves(pages)] from where
+    int32_t* move_dst;   // [most_moves(pages)] to where,
     int32_t* new_name;   // [pages] where each page that moves goes
     int64_t table_stride;
     int32_t pages, rows, width;
@@ -465,6 +465,9 @@ int pool_unit(const Pool& p) {
                          (uint64_t)p.page_bytes;
     return (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
 }
+
+// Pages that compacting moves at most: there is a hole for each.
+int64_t most_moves(int64_t pages) { return (pages + 1) / 2; }
 
 // Workgroups that move `pairs` pages: a piece each, up to eight a CU.
 int move_blocks(const Pool& p, int64_t pairs) {
@@ -612,7 +615,7 @@ int pw4_paged_cache_free(int32_t* ref_counts, int64_t num_pages, int32_t* block_
 }
 
 size_t pw4_paged_cache_compact_workspace_size(int64_t num_pages) {
-    return num_pages > 0 ? (size_t)(2 * num_pages + 2) * 4 : 8;
+    return num_pages > 0 ? (size_t)(2 + 2 * most_moves(num_pages) + num_pages) * 4 : 8;
 }
 
 int pw4_paged_cache_compact(const pw4_page_pool* pool, int32_t* ref_counts, int32_t* block_tables, int64_t rows,
@@ -626,8 +629,8 @@ int pw4_paged_cache_compact(const pw4_page_pool* pool, int32_t* ref_counts, int3
         return PW4_ERR_WORKSPACE;
     }
     int32_t* const ws = static_cast<int32_t*>(workspace);
-    const int64_t half = (p.pages + 1) / 2;
-    const CompactArgs a{ref_counts, block_tables, used, ws, ws + 2, ws + 2 + half, ws + 2 + 2 * half, table_stride,
+    const int64_t most = most_moves(p.pages);
+    const CompactArgs a{ref_counts, block_tables, used, ws, ws + 2, ws + 2 + most, ws + 2 + 2 * most, table_stride,
                         p.pages, (int32_t)rows, (int32_t)table_width};
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(compact_pages_kernel, dim3(1), dim3(kMetaThreads), 0, s, a);

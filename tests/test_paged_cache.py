@@ -516,3 +516,49 @@ def test_opcheck():
                      (lib.paged_cache_free, (r, t, l, _i32([0]))),
                      (lib.paged_cache_compact, (p, r, t))):
         torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def _compact_size(pages):
+    lib = pulsar_amd.capi()
+    lib.pw4_paged_cache_compact_workspace_size.argtypes = [ctypes.c_int64]
+    lib.pw4_paged_cache_compact_workspace_size.restype = ctypes.c_size_t
+    return lib.pw4_paged_cache_compact_workspace_size(pages)
+
+
+def test_compact_workspace_holds_what_is_written():
+    """A count (and a place to align), both ends of each of up to pages / 2 moves, a name for each page."""
+    for pages in (1, 2, 3, 63, 64, 575, 4095, 4096):
+        assert _compact_size(pages) >= 4 * (2 + 2 * ((pages + 1) // 2) + pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [1, 2, 63, 64, 127, 575])
+def test_compact_writes_nothing_past_its_workspace(pages):
+    page, used = 8, max(1, pages // 3)
+    rng = random.Random(pages)
+    held = rng.sample(range(pages), used)
+    tables = torch.tensor([held], dtype=torch.int32)
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[held] = 1
+    pool = torch.randn(2, pages, page, 1, 8, generator=gen(pages)).bfloat16()
+    host, want = Pages(refs, tables, torch.tensor([used * page], dtype=torch.int32), page), pool.clone()
+    p, r, t = _dev(pool, refs, tables)
+    size = _compact_size(pages)
+    ws = torch.full((size + 64,), 0x5a, dtype=torch.uint8, device=DEV)
+
+    class Pool(ctypes.Structure):
+        _fields_ = [("base", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in (
+            "planes", "num_pages", "page_bytes", "plane_stride_bytes", "page_stride_bytes")]
+
+    lib = pulsar_amd.capi()
+    P, I = ctypes.c_void_p, ctypes.c_int64
+    lib.pw4_paged_cache_compact.argtypes = [ctypes.POINTER(Pool), P, P, I, I, I, P, P, ctypes.c_size_t, P]
+    count = torch.zeros(1, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    args = Pool(p.data_ptr(), 2, pages, page * 16, pages * page * 16, page * 16)
+    assert lib.pw4_paged_cache_compact(ctypes.byref(args), r.data_ptr(), t.data_ptr(), 1, used, used, count.data_ptr(),
+                                       ws.data_ptr(), size, None) == 0
+    torch.cuda.synchronize()
+    assert count.tolist() == [host.compact(want)]
+    _same(host, r, t)
+    assert torch.equal(p.cpu(), want) and bool((ws[size:] == 0x5a).all())
