@@ -1567,7 +1567,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const bool wanted = forced_split ? forced_split[0] == '1'
                         : few ? most_units > (8 * c.tiles * p.kv_heads <= cus ? 7 : 4 * c.tiles * p.kv_heads <= cus ? 16 : 22)
                               : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
-    p.split = wanted && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
+    p.split = wanted && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     c.grid = (int)(c.tiles * p.kv_heads);
     if (p.split) {
         c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));

@@ -699,3 +699,15 @@ def test_c_entry_refuses_more_rows_than_it_counts():
 
     assert call(2 ** 18, 2 ** 18) == -2 and call(2 ** 20, 2 ** 18) == -2
     assert call(2 ** 18, 2 ** 17) == -1 and call(2 ** 17, 2 ** 30) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 100])
+def test_no_sequences_and_a_far_bound(new):
+    """Nothing to split, whatever max_seq_len is."""
+    kc = torch.zeros(40, 16, 2, 64, dtype=B, device=DEV)
+    none = torch.zeros(0, 9000, dtype=torch.int32, device=DEV)
+    q = torch.ones(new, 4, 64, dtype=B, device=DEV)
+    out, lse = ops.paged_attention(q, kc, kc, none, none[:, 0].contiguous(), offsets([]).to(DEV), new, 9000 * 16,
+                                   return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
