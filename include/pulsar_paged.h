@@ -83,8 +83,8 @@ int pw4_paged_attention(const pw4_paged_attention_args* args, void* workspace, s
  * slots[t] (int64 [num_tokens]) is token t's place page * page_size + row, -1 for
  * t past cu_q[rows].  All or nothing: where the pool has too few free pages or a
  * table too few columns nothing changes, every slot is -1 and *missing (int32) is
- * the number of pages that the pool lacks plus the columns that the tables lack;
- * else it is 0.  rows up to 4096. */
+ * the number of pages that the pool lacks plus the columns that the tables lack
+ * (2^18 of a row at most); else it is 0.  rows up to 4096. */
 int pw4_paged_cache_extend(int32_t* ref_counts, int64_t num_pages, int32_t* block_tables, int64_t table_width,
                            int64_t table_stride, int32_t* seq_lens, const int32_t* cu_q, int64_t rows,
                            int64_t num_tokens, int64_t page_size, int64_t* slots, int32_t* missing,

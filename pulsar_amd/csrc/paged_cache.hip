@@ -32,8 +32,8 @@ namespace {
 constexpr int kMetaThreads = 1024, kMetaWaves = kMetaThreads / 64;
 constexpr int kMaxRows = 4096;  // rows (extend) or pairs (fork) of a call: their prefix sums lie in LDS
 
-__device__ __forceinline__ int pages_of(uint32_t tokens, uint32_t page_size) {
-    return (int)((tokens + page_size - 1) / page_size);
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page_size) {
+    return tokens == 0 ? 0 : (tokens - 1) / page_size + 1;
 }
 
 // First i in [0, n) with ends[i] > v (ends ascending); n if none.
@@ -105,10 +105,15 @@ struct ExtendArgs {
     int32_t pages, width, rows, page_size;
 };
 
+// Tokens that row b gets.
+__device__ __forceinline__ uint32_t new_tokens(const int32_t* cu, int b) {
+    return cu[b + 1] > cu[b] ? min((uint32_t)cu[b + 1] - (uint32_t)cu[b], (uint32_t)INT_MAX) : 0;
+}
+
 __device__ __forceinline__ int64_t slot_of(const ExtendArgs& a, const int32_t* cu, int row, int t, int old_len) {
     const uint32_t pos = (uint32_t)(old_len + t - cu[row]);
     const uint32_t col = pos / (uint32_t)a.page_size;
-    const int page = a.tables[(int64_t)row * a.table_stride + min((int)col, a.width - 1)];
+    const int page = a.tables[(int64_t)row * a.table_stride + min(col, (uint32_t)a.width - 1)];
     return (int64_t)page * a.page_size + (pos - col * (uint32_t)a.page_size);
 }
 
@@ -126,10 +131,11 @@ __global__ __launch_bounds__(kMetaThreads) void extend_kernel(const ExtendArgs a
         const int b = b0 + tid;
         int mine = 0;
         if (b < a.rows) {
-            const int len = max(a.lens[b], 0), n = max(cu[b + 1] - cu[b], 0);
-            const int want = pages_of((uint32_t)len + (uint32_t)n, a.page_size);
-            mine = want - pages_of(len, a.page_size);
-            over += max(want - a.width, 0);
+            // counts below 2^31 each, so sums below 2^32, whatever lens and cu hold
+            const uint32_t len = max(a.lens[b], 0), n = new_tokens(cu, b), width = a.width;
+            const uint32_t want = pages_of(len + n, a.page_size);
+            mine = (int)min(want - pages_of(len, a.page_size), (uint32_t)INT_MAX);
+            over += want > width ? (int)min(want - width, 1u << 18) : 0;  // a sum that 4096 rows do not overflow
         }
         int total;
         const int upto = block_inclusive_scan<kMetaWaves>(mine, scratch, total);
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(kMetaThreads) void extend_kernel(const ExtendArgs a
     const bool dealing = over == 0;
     auto place = [&](int f, int& row) -> int64_t {  // the table entry that takes the f-th page
         row = first_above(need_end, a.rows, f);
-        const int col = pages_of(max(a.lens[row], 0), a.page_size) + f - (row ? need_end[row - 1] : 0);
+        const int col = (int)pages_of(max(a.lens[row], 0), a.page_size) + f - (row ? need_end[row - 1] : 0);
         return (int64_t)row * a.table_stride + col;
     };
     const int found = deal_free_pages(a.refs, a.pages, need, scratch, [&](int f, int page) {
@@ -149,7 +155,7 @@ __global__ __launch_bounds__(kMetaThreads) void extend_kernel(const ExtendArgs a
         a.tables[place(f, row)] = page;
         a.refs[page] = 1;
     });
-    const int missing = max(need - found, 0) + over;
+    const int missing = (int)min((int64_t)max(need - found, 0) + over, (int64_t)INT_MAX);
     __syncthreads();
     if (missing != 0 && dealing) {  // give back what was dealt
         for (int f = tid; f < found; f += kMetaThreads) {
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(kMetaThreads) void extend_kernel(const ExtendArgs a
     }
     __syncthreads();
     if (missing == 0) {
-        for (int b = tid; b < a.rows; b += kMetaThreads) a.lens[b] = max(a.lens[b], 0) + max(cu[b + 1] - cu[b], 0);
+        for (int b = tid; b < a.rows; b += kMetaThreads) a.lens[b] = max(a.lens[b], 0) + (int)new_tokens(cu, b);
     }
 }
 
@@ -183,7 +189,7 @@ __global__ __launch_bounds__(256) void slots_kernel(const ExtendArgs a) {
     if (t >= a.num_tokens) return;
     const int row = first_above(cu + 1, a.rows, t);
     const bool in = ok && row < a.rows && t >= cu[row];
-    a.slots[t] = in ? slot_of(a, cu, row, t, a.lens[row] - (cu[row + 1] - cu[row])) : -1;
+    a.slots[t] = in ? slot_of(a, cu, row, t, a.lens[row] - (int)new_tokens(cu, row)) : -1;
 }
 
 // ---- write --------------------------------------------------------------------

@@ -562,3 +562,22 @@ def test_compact_writes_nothing_past_its_workspace(pages):
     assert count.tolist() == [host.compact(want)]
     _same(host, r, t)
     assert torch.equal(p.cpu(), want) and bool((ws[size:] == 0x5a).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("lens,counts", [([5, 40], [2 ** 31 - 50, 0]), ([2 ** 31 - 20, 0], [30, 0]),
+                                         ([2 ** 31 - 1, 3], [2 ** 31 - 1, 0]), ([7, 9], [0, 2 ** 31 - 1])])
+def test_extend_by_more_than_any_table_holds(lens, counts, page):
+    """Tokens whose sum passes 31 or 32 bits: refused as any others that no table has room for, and
+    neither the tables nor what lies around them changes."""
+    wide = torch.full((4, 12), 99, dtype=torch.int32, device=DEV)
+    tables = wide[1:3, :8]
+    tables.fill_(-1)
+    refs = torch.zeros(64, dtype=torch.int32, device=DEV)
+    l = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    slots, missing = ops.paged_cache_extend(refs, tables, l, offsets(counts).to(DEV), 40, page)
+    assert int(missing) > 0 and set(slots.tolist()) == {-1}
+    assert l.tolist() == lens and int(refs.abs().sum()) == 0 and bool((tables == -1).all())
+    wide[1:3, :8] = 99
+    assert bool((wide == 99).all())
