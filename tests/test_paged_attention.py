@@ -711,3 +711,38 @@ def test_no_sequences_and_a_far_bound(new):
     out, lse = ops.paged_attention(q, kc, kc, none, none[:, 0].contiguous(), offsets([]).to(DEV), new, 9000 * 16,
                                    return_lse=True)
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [0, 1])
+@pytest.mark.parametrize("tile,new", [(None, 1), (None, 7), (128, 40), (256, 150)])
+@pytest.mark.parametrize("dim", [64, 96, 256])
+def test_writes_stay_in_the_outputs_and_the_workspace(plan, dim, tile, new, split):
+    """The C entry on buffers with a margin behind each."""
+    plan(split, 1, tile)
+    lens, group, heads = [900, 333, new, 61], 4, 2
+    counts = [new, min(new, 40), new, 0]
+    kc, vc, tables, _, _ = paged_kv(lens, 16, heads, dim, B, 3)
+    q = torch.randn(sum(counts) + 1, heads * group, dim, generator=gen(4)).to(B).to(DEV)
+    lens_t, cu = torch.tensor(lens, dtype=torch.int32, device=DEV), offsets(counts).to(DEV)
+    want = ops.paged_attention(q, kc, vc, tables, lens_t, cu, new, 900, return_lse=True)
+    out = torch.full((q.numel() + 64,), 3.0, dtype=B, device=DEV)
+    lse = torch.full((q.shape[0] * q.shape[1] + 64,), 3.0, device=DEV)
+    a = _Args(q=q.data_ptr(), k_cache=kc.data_ptr(), v_cache=vc.data_ptr(), block_tables=tables.data_ptr(),
+              seq_lens=lens_t.data_ptr(), cu_q=cu.data_ptr(), out=out.data_ptr(), lse=lse.data_ptr(),
+              num_tokens=q.shape[0], batch=4, q_heads=heads * group, kv_heads=heads, head_dim=dim,
+              num_pages=kc.shape[0], page_size=16, table_width=tables.shape[1], table_stride=tables.stride(0),
+              q_token_stride=q.stride(0), q_head_stride=q.stride(1), page_stride=kc.stride(0), row_stride=kc.stride(1),
+              kv_head_stride=kc.stride(2), max_q_len=new, max_seq_len=900, scale=dim ** -0.5, dtype=1)
+    lib = pulsar_amd.capi()
+    lib.pw4_paged_attention.argtypes = [ctypes.POINTER(_Args), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+    lib.pw4_paged_attention_workspace_size.argtypes = [ctypes.POINTER(_Args)]
+    lib.pw4_paged_attention_workspace_size.restype = ctypes.c_size_t
+    size = lib.pw4_paged_attention_workspace_size(ctypes.byref(a))
+    assert (size > 0) == bool(split)
+    ws = torch.full((size + 256,), 0x5a, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    assert lib.pw4_paged_attention(ctypes.byref(a), ws.data_ptr(), size, None) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(out[:q.numel()].view(q.shape), want[0]) and torch.equal(lse[:-64].view(want[1].shape), want[1])
+    assert bool((out[q.numel():] == 3).all()) and bool((lse[-64:] == 3).all()) and bool((ws[size:] == 0x5a).all())

@@ -581,3 +581,35 @@ def test_extend_by_more_than_any_table_holds(lens, counts, page):
     assert l.tolist() == lens and int(refs.abs().sum()) == 0 and bool((tables == -1).all())
     wide[1:3, :8] = 99
     assert bool((wide == 99).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 37])
+def test_fork_writes_nothing_past_its_workspace(n):
+    page, width = 8, 4
+    pool, refs, tables, lens = _state(2 * n, 6 * n, page, width, [3 + 5 * (b % 4) for b in range(n)], n)
+    host, want = Pages(refs, tables, lens, page), pool.clone()
+    p, r, t, l = _dev(pool, refs, tables, lens)
+
+    class Pool(ctypes.Structure):
+        _fields_ = [("base", ctypes.c_void_p)] + [(k, ctypes.c_int64) for k in (
+            "planes", "num_pages", "page_bytes", "plane_stride_bytes", "page_stride_bytes")]
+
+    lib = pulsar_amd.capi()
+    P, I, SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t
+    lib.pw4_paged_cache_fork_workspace_size.argtypes, lib.pw4_paged_cache_fork_workspace_size.restype = [I], SZ
+    lib.pw4_paged_cache_fork.argtypes = [ctypes.POINTER(Pool), P, P, I, I, I, P, P, P, I, I, P, P, SZ, P]
+    size = lib.pw4_paged_cache_fork_workspace_size(n)
+    ws = torch.full((size + 64,), 0x5a, dtype=torch.uint8, device=DEV)
+    src, dst = _i32(list(range(n))), _i32(list(range(n, 2 * n)))
+    missing = torch.full((16,), 77, dtype=torch.int32, device=DEV)
+    page_bytes = pool[0, 0].numel() * 2
+    args = Pool(p.data_ptr(), pool.shape[0], pool.shape[1], page_bytes, pool.shape[1] * page_bytes, page_bytes)
+    torch.cuda.synchronize()
+    assert lib.pw4_paged_cache_fork(ctypes.byref(args), r.data_ptr(), t.data_ptr(), 2 * n, width, width, l.data_ptr(),
+                                    src.data_ptr(), dst.data_ptr(), n, page, missing.data_ptr(), ws.data_ptr(), size,
+                                    None) == 0
+    torch.cuda.synchronize()
+    assert host.fork(list(range(n)), list(range(n, 2 * n)), want) == 0
+    _same(host, r, t, l)
+    assert torch.equal(p.cpu(), want) and bool((ws[size:] == 0x5a).all()) and missing.tolist() == [0] + [77] * 15

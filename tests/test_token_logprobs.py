@@ -289,3 +289,26 @@ def test_rows_of_many_slices(tokens, vocab, top, dtype):
     x[:, vocab // 2] = 1.0
     x, t = x.to(DEV), torch.full_like(t, vocab // 2)
     assert torch.equal(ops.token_logprobs(x, t, top)[4].cpu(), logprobs_ref(x.cpu(), t.cpu(), top)[4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,vocab,top", [(1, 1, 1), (3, 9000, 32), (7, 50001, 5), (300, 8193, 20), (65, 20000, 0)])
+def test_writes_stay_in_the_outputs_and_the_workspace(tokens, vocab, top):
+    """The C entry on buffers with a margin behind each."""
+    lib = pulsar_amd.capi()
+    P, I, SZ = ctypes.c_void_p, ctypes.c_int64, ctypes.c_size_t
+    lib.pw4_token_logprobs.argtypes = [P, ctypes.c_int, I, I, I, P, I, P, P, P, P, P, P, SZ, P]
+    lib.pw4_token_logprobs_workspace_size.argtypes, lib.pw4_token_logprobs_workspace_size.restype = [I] * 3, SZ
+    x = torch.randn(tokens, vocab, generator=gen(tokens)).to(B).to(DEV)
+    t = torch.randint(0, vocab, (tokens,), generator=gen(vocab)).to(DEV)
+    want = ops.token_logprobs(x, t, top)
+    got = [torch.full((w.numel() + 16,), 77, dtype=w.dtype, device=DEV) for w in want]
+    size = lib.pw4_token_logprobs_workspace_size(tokens, vocab, top)
+    ws = torch.full((size + 256,), 0x5a, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    assert lib.pw4_token_logprobs(x.data_ptr(), 1, tokens, vocab, vocab, t.data_ptr(), top, *(g.data_ptr() for g in got),
+                                  ws.data_ptr(), size, None) == 0
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert torch.equal(g[:w.numel()].view(w.shape), w) and bool((g[w.numel():] == 77).all())
+    assert bool((ws[size:] == 0x5a).all())
