@@ -229,7 +229,7 @@ __device__ __forceinline__ void cap_scores(const Params& a, V& s) {
             s[e] *= a.scale2;
             most = fmaxf(most, fabsf(s[e]));
         }
-        if (__any(most >= kSeries)) {
+        if (__builtin_expect(__any(most >= kSeries), 0)) {
 #pragma unroll
             for (int e = 0; e < N; ++e) s[e] = tanh_of(s[e]);
         } else {
