@@ -989,10 +989,10 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void few_rows_kernel(const Para
 // Four waves of 32 query rows each over blocks of 64 keys that they share in LDS,
 // two stages: block i + 1 is copied while block i is worked on.  For calls with too few
 // tiles of 256 rows to fill the chip, and heads wider than 128; two workgroups to a CU
-// (one prompt of 8192 tokens, 32 heads of 128: 562 us, where 256-row tiles take 511).
-// Tiles too few to give a SIMD its second wave leave it bound by latency: chunks of 707 and
-// 101 tokens, 14 heads of 64, a window of 1024 and a cap (three transcendental instructions
-// a score) take 48 us, the vector units busy 24% of it.
+// (one prompt of 8192 tokens, 32 heads of 128: 535 to 566 us on two cards, where 256-row
+// tiles take 510 and 544).  Tiles too few to give a SIMD its second wave leave it bound by
+// latency: chunks of 707 and 101 tokens, 14 heads of 64, a window of 1024 and a cap take
+// 49.5 us, the vector units busy 28% of it, 0.6 waves on a SIMD.
 constexpr int kManyKeys = 64, kManyWaves = 4, kManyRows = 32 * kManyWaves;
 constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
@@ -1240,11 +1240,11 @@ void many_rows_kernel(const Params a) {
 // their products (scores of block i + 1, outputs of block i), waves 4 to 7 make the
 // probabilities of a block, and the other way round.  Both phases take about as long, so
 // the matrix cores and the vector units are busy together; the same work in any order of
-// the waves' own left each idle half of the time (one prompt of 8192 tokens, 32 heads of
-// 128: 562 us in four-wave workgroups, two a CU).  Waves 0 to 3 copy K, waves 4 to 7 copy
-// V, three blocks of each in LDS.  511 us, 1076 TFLOP/s, where the library's large matrix
-// product reaches 1184; by the counters the matrix cores are busy 51% of the cycles and
-// vector instructions take 49%.
+// the waves' own left each idle half of the time (two four-wave workgroups a CU: 4% slower
+// on a prompt of 8192 tokens, 32 heads of 128).  Waves 0 to 3 copy K, waves 4 to 7 copy V,
+// three blocks of each in LDS.  510 to 544 us by the card, 1010 to 1078 TFLOP/s, where the
+// library's large matrix product reaches 1184 on the fastest; by the counters the matrix
+// cores are busy 50% of the cycles and vector instructions take 49%.
 constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideRing = 3;
 template <int DP>
 constexpr int kWideBlock = kManyKeys * DP * 2;  // bytes of K, or of V
@@ -1555,15 +1555,22 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const int64_t most_units = ceil_div(most_keys, unit) + 1;
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
-    // A few rows: a workgroup takes about 1.1 us a unit of 128 keys, the split a second launch
-    // and the partial outputs' way through memory, which grow with the tiles.  Heads of 128, 8
-    // of them, whole and split, us: 1 sequence of 640 keys 11.5 and 13.4, 777 14.1 and 13.2,
-    // 8000 72 and 23; 4 of 777 14.0 and 14.1, 900 15.1 and 14.0; 8 of 1100 16.9 and 19.9, 1600
-    // 20.5 and 21.4, 2400 26.7 and 24.2; 12 of 2400 27.1 and 27.5; 16 of 2400 27.7 and 29.4,
-    // 4000 56.1 and 47.0.
+    // A few rows: whole, a workgroup takes about 1.1 us a unit of 128 keys; the split, a second
+    // launch and the partial outputs' way through memory, which grow with the tiles.  8 key-value
+    // heads, sequences of one length, whole and split, us:
+    //   heads of 64   1 of 640 keys 9.2 and 10.9, of 777 11.1 and 10.8, of 8000 60 and 20
+    //                 8 of 1600 16.6 and 17.5, of 2400 22.4 and 20.5; 16 of 2400 22.6 and 25.2, of 4000 33.9 and 32.3
+    //   heads of 128  1 of 640 11.2 and 12.4, of 777 13.7 and 12.3, of 8000 72 and 22; 4 of 1100 16.2 and 19.0
+    //                 8 of 1600 21.3 and 22.3, of 2400 27.6 and 26.1; 16 of 2400 29.8 and 35.2, of 4000 43.8 and 48.1
+    //   heads of 256 (units of 64 keys)  1 of 400 20.5 and 15.1; 8 of 777 32.4 and 28.8, of 1100 40.9 and 31.4
+    //                 16 of 1100 41.6 and 37.5, of 1600 52.7 and 48.2
+    // Over 1 to 16 sequences of 400 to 8000 keys the thresholds' choice is within 17% of the better
+    // one, for each of these heads.  Lengths of one batch that differ are not looked at,
+    // max_seq_len is.
     // Else where the tiles leave at least half of the chip idle and are long, since a piece's
     // partial outputs are written and read again: 270 tiles of 128 rows on 512 places, 18 blocks
-    // each, took 49 us whole and 65 split.
+    // each, take 49.5 us whole and 63 split.  The rule still splits some calls that are faster
+    // whole: two chunks of 100 tokens in a window of 1024 take 32.0 us whole and 35.9 split.
     p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
     const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
     const bool wanted = forced_split ? forced_split[0] == '1'

@@ -2,8 +2,8 @@
 //
 // Bound by one read of the logits.  A row is cut into slices, one workgroup of 256
 // threads each, which holds its slice in registers, packed as it came: 32 logits a
-// thread (188 us for 2048 tokens of 100003 bf16 logits; 64 a thread, at five waves a SIMD
-// instead of eight: 206), or 16 where the tokens are so few that CUs would be idle.  The
+// thread (2048 tokens of 100003 bf16 logits took 188 us so, and 64 a thread, at five waves
+// a SIMD instead of eight, 206), or 16 where the tokens are so few that CUs would be idle.  The
 // largest logit, then sum e^(x-m) and sum e^(x-m) (x-m) with the slice's own m, the rank
 // and the top candidates come from one trip to memory.  A second launch joins a row's
 // slices, a wave a row: with M = max m and the slices' sums scaled by e^(m-M),
@@ -15,8 +15,8 @@
 // it holds, those above the exact bound and the first k that equal it are; failing that,
 // k rounds of a workgroup-wide maximum find the same tokens.
 //
-// 2048 tokens of 100003 bf16 logits (410 MB) take 159 us and 28 for the join under a
-// profiler, 184 a call (2.2 TB/s): bound by the vector units, busy 74% of the first
+// 2048 tokens of 100003 bf16 logits (410 MB) take 160 us and 8.6 for the join under a
+// profiler, 164 a call (2.5 TB/s): bound by the vector units, busy 74% of the first
 // launch's cycles, which spend about 21 instructions on a logit (unpacking
 // twice, the maximum, six for the sums with one transcendental, the rank's two where a
 // vector holds a logit that is ahead).
