@@ -405,7 +405,7 @@ def run(state: dict):
             return ops.paged_cache_append(s["q"], s["k"], s["v"], pool[0], pool[1], s["slots"], **how), pool
         q = ops.paged_cache_append_fp4(s["q"], s["k"], s["v"], pool[0], pool[1], s["slots"], **how)
         return q, *ops.paged_cache_read_fp4(pool[0], pool[1], s["slots"], s["q"].dtype)
-    picked = ops.beam_select(s["logits"], s["scores"], finished=s["ended"], end_token=s["end_token"])
+    picked = ops.beam_select(s["logits"], s["scores"], ended=s["ended"], end_token=s["end_token"])
     return [*picked, *ops.beam_reorder([s["history"]], picked[1])]
 
 
