@@ -1,6 +1,7 @@
 /*
- * pulsar_paged.h -- C ABI of the paged key-value cache operators and of the
- * log probabilities of given tokens, in libpulsar_w4a16.so (gfx950).
+ * pulsar_paged.h -- C ABI of the paged key-value cache operators (16-bit and
+ * 4-bit), of the log probabilities of given tokens and of beam search's
+ * selection, in libpulsar_w4a16.so (gfx950).
  *
  * The conventions of pulsar_w4a16.h: every tensor argument is a device pointer,
  * every size and stride an element count unless it says bytes, every call is
@@ -100,6 +101,40 @@ int pw4_paged_cache_write(const void* k, const void* v, void* k_cache, void* v_c
                           int64_t page_size, int64_t page_stride, int64_t row_stride, int64_t kv_head_stride,
                           pw4_stream_t stream);
 
+/* paged_cache_append: paged_cache_write with the position rotation on the way.
+ * Token t at position p = positions[t] has, for each pair (a, b) of a head's first
+ * rot elements and its c = rope[p][i], s = rope[p][rot / 2 + i],
+ *   (a, b) -> (a c - b s, b c + a s),
+ * pair i being elements i and rot / 2 + i, or with `interleaved` 2 i and 2 i + 1;
+ * sums are fp64 and rounded once.  q's result goes to q_out, k's and v itself into
+ * slot slots[t] of one layer's caches.  A slot outside the pool is passed over (q is
+ * rotated all the same); so is a token whose position is not one of the table's rows,
+ * and its q_out is 0.  No two tokens may name one slot.
+ *   q, k, v   [num_tokens, q_heads or kv_heads, head_dim] by their strides, head_dim
+ *             contiguous; q and q_out NULL: keys and values only
+ *   q_out     [num_tokens, q_heads, head_dim] contiguous
+ *   rope      fp32 [rope_rows, rot]: cosines, then sines
+ *   positions NULL: nothing is rotated (rope NULL then, and q too)
+ *   caches    as for paged_attention
+ * head_dim a multiple of 8 up to 256, rot even and at most head_dim. */
+typedef struct pw4_paged_append_args {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    void* k_cache;
+    void* v_cache;
+    const int64_t* slots;     /* [num_tokens] */
+    const int64_t* positions; /* [num_tokens] */
+    const float* rope;
+    int64_t num_tokens, q_heads, kv_heads, head_dim, rot, rope_rows;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t num_pages, page_size, page_stride, row_stride, kv_head_stride;
+    int interleaved;
+    int dtype; /* of q, k, v, q_out and 16-bit caches: PW4_DTYPE_F16 or PW4_DTYPE_BF16 */
+} pw4_paged_append_args;
+int pw4_paged_cache_append(const pw4_paged_append_args* args, pw4_stream_t stream);
+
 /* A pool that the page operators move whole pages of: `planes` of them (keys and
  * values of every layer), each of num_pages pages of page_bytes contiguous bytes,
  * plane_stride_bytes and page_stride_bytes apart. */
@@ -143,6 +178,38 @@ int pw4_paged_cache_compact(const pw4_page_pool* pool, int32_t* ref_counts, int3
                             size_t workspace_bytes, pw4_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * The cache in 4 bits (OCP MX blocks).  A token's head is blocks of 32 elements: an
+ * exponent byte b that stands for 2^(b - 127) (255: every element is NaN) and codes of
+ * a sign bit and three bits for 0, 1/2, 1, 3/2, 2, 3, 4, 6.  A page is, for each key-value
+ * head and token of it in turn, head_dim / 2 bytes of codes (element 2 i in the low half of
+ * byte i); then, heads and tokens in the same order, head_dim / 32 exponents:
+ * page_size * kv_heads * head_dim * 17 / 32 bytes.  head_dim is a multiple of 32 up to 256.
+ *
+ * Values round to the block 2^e whose largest magnitude is in [3.5, 7) 2^e (e from -127; with
+ * dtype fp16 up to 13, so that what is held is finite in fp16), and there to the nearest code,
+ * of two the even one: each is off by 2^e at most, half a step.  A block with a NaN or an
+ * infinity becomes NaN.
+ *
+ * Caches are pages of one layer, page_stride bytes apart, 16-byte aligned; row_stride and
+ * kv_head_stride are not read.  The page operators above move such pages as any. */
+
+/* paged_cache_append into 4-bit caches: rotated, summed in fp64, rounded to fp32, then to blocks. */
+int pw4_paged_cache_append_fp4(const pw4_paged_append_args* args, pw4_stream_t stream);
+
+/* paged_cache_read_fp4: the values that slots of one layer's 4-bit caches hold, k and v
+ * [num_tokens, kv_heads, head_dim] contiguous, each rounded once to dtype (fp16 or bf16; exact
+ * unless it is subnormal there); 0 for a slot outside the pool. */
+int pw4_paged_cache_read_fp4(const void* k_cache, const void* v_cache, const int64_t* slots, void* k, void* v,
+                             int64_t num_tokens, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
+                             int64_t page_size, int64_t page_stride, int dtype, pw4_stream_t stream);
+
+/* paged_attention over 4-bit caches of q's dtype: the same arguments but for the caches' strides, and
+ * the same results as over a 16-bit cache of the values that they hold. */
+size_t pw4_paged_attention_fp4_workspace_size(const pw4_paged_attention_args* args);
+int pw4_paged_attention_fp4(const pw4_paged_attention_args* args, void* workspace, size_t workspace_bytes,
+                            pw4_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * token_logprobs: over each row x of logits [num_tokens, vocab] (fp16, bf16 or
  * fp32, rows row_stride apart), with lse = ln sum e^x:
  *   logprobs  [num_tokens] fp32  x[targets[t]] - lse, 0 where the target is
@@ -162,6 +229,34 @@ int pw4_token_logprobs(const void* logits, int dtype, int64_t num_tokens, int64_
                        const int64_t* targets, int64_t top_k, float* logprobs, int64_t* ranks, float* entropy,
                        float* top_logprobs, int64_t* top_ids, void* workspace, size_t workspace_bytes,
                        pw4_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * beam_select: the next beams of `batch` searches.  logits [batch * beams, vocab] (fp16, bf16 or
+ * fp32, rows row_stride apart) are those of row b * beams + k, beam k of search b.  Its continuation
+ * by token v has the total
+ *   scores[b][k] + x_v - ln sum_w e^(x_w)            (sums of a row fp32, totals fp64)
+ * and the `width` best of each search are chosen, best first: out_scores their totals in fp32,
+ * out_rows the row that each continues, out_tokens its token [batch, width].  Equal totals stand by
+ * beam, then by logit, then by token, the lower first.  A total that is NaN counts as -inf.
+ * ended (bytes, NULL: none): a beam whose byte is not 0 has one continuation, end_token with its score
+ * as it is; its logits are not read.  out_ended (with ended): whether the new beam continues one that
+ * had ended, or its token is end_token.
+ * beams and width from 1 to 32, width at most beams * vocab, with ended at most beams. */
+size_t pw4_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t vocab, int64_t width);
+int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,
+                    const float* scores, const uint8_t* ended, int64_t end_token, int64_t width, float* out_scores,
+                    int32_t* out_rows, int64_t* out_tokens, uint8_t* out_ended, void* workspace,
+                    size_t workspace_bytes, pw4_stream_t stream);
+
+/* beam_reorder: dst[i] = src[rows[i]], i < n, in each of `count` states of num_rows rows; a row outside
+ * becomes zeros.  dst may not overlap src.  (states is read on the host.) */
+typedef struct pw4_beam_state {
+    const void* src;   /* [num_rows] rows of row_bytes contiguous bytes */
+    void* dst;         /* [n] of them */
+    int64_t row_bytes, num_rows;
+} pw4_beam_state;
+int pw4_beam_reorder(const pw4_beam_state* states, int64_t count, const int32_t* rows, int64_t n,
+                     pw4_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -33,7 +33,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
 HIP_SOURCES = ["repack.hip", "gemm_decode.hip", "gemm_prefill.hip", "gemm_prefill_256.hip", "gemm_kwave.hip",
                "gemm_kwave_f16.hip", "gemm_kwave_bf16.hip", "capi.hip", "paged_attention.hip", "paged_cache.hip",
-               "token_logprobs.hip"]
+               "token_logprobs.hip", "paged_append.hip", "paged_attention_fp4.hip", "beam_search.hip"]
 LIB_NAME = "libpulsar_w4a16.so"
 TORCH_LIB_NAME = "_pulsar_w4a16_torch.so"
 TORCH_SOURCES = ["torch_ops.cpp", "model.cpp", "paged_ops.cpp"]
@@ -92,6 +92,7 @@ def _run_parallel(cmds: list[list[str]], verbose: bool) -> None:
 HIPCC_FILE_FLAGS = {
     "gemm_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "paged_attention_fp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

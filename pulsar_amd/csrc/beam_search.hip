@@ -1,0 +1,239 @@
+// Beam search's selection and the reordering of the beams' states (the definitions:
+// pulsar_paged.h).
+//
+// Bound by one read of the logits: a row's slices are read once, as token_logprobs reads them,
+// and leave their largest logit, sum e^(x-m) and `width` best candidates.  The second launch has
+// a workgroup a search, whose waves join a beam's slices each: its log-sum-exp, the slices'
+// sums added in fp64, and its best candidates in order.  No beam gives more than `width` of the
+// new ones, so width times beams candidates are left, in lists that fall by total; a candidate's
+// place among all is its place in its own list and, by bisection, those ahead of it in the
+// others.  Totals are fp64: scores of some hundred tokens have fp32 steps of 1e-5, within which
+// beams would tie.
+#include "logit_slices.h"
+
+#include <type_traits>
+
+using namespace pw4;
+
+namespace {
+
+constexpr int kMaxBeams = 32;
+
+struct SelectArgs {
+    SliceArgs s;
+    const float* scores;
+    int64_t end_token;
+    float* out_scores;
+    int32_t* out_rows;
+    int64_t* out_tokens;
+    uint8_t* out_ended;
+    int32_t beams, width;
+};
+
+constexpr double kLowest = -__builtin_inf();
+
+// ln sum e^x of a row, by a wave; NaN where the row has a NaN or +inf, -inf where it is all -inf.
+__device__ __forceinline__ double join_lse(const SliceSums* sums, int slices) {
+    const int lane = threadIdx.x & 63;
+    float m = -__builtin_inff();
+    for (int s = lane; s < slices; s += 64) m = fmaxf(m, sums[s].m);
+    m = wave_max(m);
+    double z = 0;
+    for (int s = lane; s < slices; s += 64) {
+        const SliceSums p = sums[s];
+        if (p.m == -__builtin_inff() && p.z == p.z) continue;
+        z += p.z * exp((double)p.m - (double)m);
+    }
+    z = wave_sum(z);
+    return (double)m + log(z);
+}
+
+__global__ __launch_bounds__(kThreads) void select_kernel(const SelectArgs a) {
+    __shared__ uint64_t s_join[kThreads / 64][kJoin];
+    __shared__ uint64_t s_key[kMaxBeams * kMaxTop];
+    __shared__ double s_total[kMaxBeams * kMaxTop];
+    __shared__ int s_length[kMaxBeams];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row0 = blockIdx.x * a.beams, per = a.s.top_k;
+    for (int k = wave; k < a.beams; k += kThreads / 64) {
+        const int row = row0 + k;
+        const bool ended = a.s.passed != nullptr && a.s.passed[row] != 0;
+        const double score = a.scores[row];
+        uint64_t* const keys = s_key + k * per;
+        double* const totals = s_total + k * per;
+        if (lane == 0) s_length[k] = ended ? 1 : per;
+        if (ended) {
+            if (lane == 0) totals[0] = score == score ? score : kLowest;
+            continue;
+        }
+        const double lse = join_lse(a.s.sums + (int64_t)row * a.s.slices, a.s.slices);
+        join_tops(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, s_join[wave], [&](int place, uint64_t key) {
+            const double total = score + ((double)unordered((uint32_t)(key >> 32)) - lse);
+            keys[place] = key;
+            totals[place] = total == total ? total : kLowest;
+        });
+    }
+    __syncthreads();
+    for (int i = tid; i < a.beams * per; i += kThreads) {
+        const int k = i / per;
+        int place = i - k * per;
+        if (place >= s_length[k]) continue;
+        const double total = s_total[i];
+        for (int other = 0; other < a.beams && place < a.width; ++other) {
+            if (other == k) continue;
+            // how many of the other's list are ahead: greater, or equal and of a lower beam
+            int lo = 0, hi = s_length[other];
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                const double t = s_total[other * per + mid];
+                if (t > total || (t == total && other < k)) {
+                    lo = mid + 1;
+                } else {
+                    hi = mid;
+                }
+            }
+            place += lo;
+        }
+        if (place >= a.width) continue;
+        const int row = row0 + k;
+        const bool ended = a.s.passed != nullptr && a.s.passed[row] != 0;
+        const int64_t at = (int64_t)blockIdx.x * a.width + place;
+        const int64_t token = ended ? a.end_token : (int64_t)(uint32_t)~s_key[i];
+        a.out_scores[at] = (float)total;
+        a.out_rows[at] = row;
+        a.out_tokens[at] = token;
+        if (a.out_ended != nullptr) a.out_ended[at] = ended || token == a.end_token;
+    }
+}
+
+// ---- reordering -----------------------------------------------------------------
+
+constexpr int kStates = 8;            // of a launch
+constexpr int64_t kPiece = 16384;     // bytes of a row that a workgroup copies
+
+struct ReorderArgs {
+    const uint8_t* src[kStates];
+    uint8_t* dst[kStates];
+    int64_t row_bytes[kStates], num_rows[kStates];
+    int32_t pieces[kStates];          // of a row
+    int64_t end[kStates];             // ascending sums of n * pieces
+    const int32_t* rows;
+    int32_t count;
+};
+
+template <typename V>
+__global__ __launch_bounds__(kThreads) void reorder_kernel(const ReorderArgs a) {
+    int s = 0;
+    while (s + 1 < a.count && (int64_t)blockIdx.x >= a.end[s]) ++s;
+    const int64_t item = blockIdx.x - (s ? a.end[s - 1] : 0);
+    const int64_t i = item / a.pieces[s], begin = (item - i * a.pieces[s]) * kPiece;
+    const int64_t row = a.rows[i], bytes = min(kPiece, a.row_bytes[s] - begin);
+    const bool there = row >= 0 && row < a.num_rows[s];
+    const V* const from = reinterpret_cast<const V*>(a.src[s] + (there ? row : 0) * a.row_bytes[s] + begin);
+    V* const to = reinterpret_cast<V*>(a.dst[s] + i * a.row_bytes[s] + begin);
+    for (int e = threadIdx.x; e < bytes / (int)sizeof(V); e += kThreads) to[e] = there ? from[e] : V{};
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pw4_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t vocab, int64_t width) {
+    if (batch <= 0 || beams <= 0 || beams > kMaxBeams || batch > 65535 / beams || vocab <= 0 || vocab > INT_MAX / 2 ||
+        width <= 0 || width > kMaxTop) {
+        return 0;
+    }
+    const int64_t rows = batch * beams, slices = slices_of(rows, vocab);
+    return sums_bytes(rows, slices) + (size_t)(rows * slices * std::min(width, vocab)) * 8;
+}
+
+int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,
+                    const float* scores, const uint8_t* ended, int64_t end_token, int64_t width, float* out_scores,
+                    int32_t* out_rows, int64_t* out_tokens, uint8_t* out_ended, void* workspace,
+                    size_t workspace_bytes, pw4_stream_t stream) {
+    if (batch < 0 || beams <= 0 || vocab <= 0 || width <= 0) return PW4_ERR_ARG;
+    if (dtype != PW4_DTYPE_F16 && dtype != PW4_DTYPE_BF16 && dtype != PW4_DTYPE_F32) return PW4_ERR_ARG;
+    if (beams > kMaxBeams || width > kMaxTop || vocab > INT_MAX / 2 || batch > 65535 / beams || width > beams * vocab ||
+        (ended != nullptr && width > beams) || row_stride < vocab) {
+        return PW4_ERR_SHAPE;
+    }
+    if (batch == 0) return PW4_OK;
+    if (!logits || !scores || !out_scores || !out_rows || !out_tokens || (out_ended != nullptr && ended == nullptr)) return PW4_ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(logits) % (dtype == PW4_DTYPE_F32 ? 4 : 2) != 0) return PW4_ERR_ARG;
+    if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+        workspace_bytes < pw4_beam_select_workspace_size(batch, beams, vocab, width)) {
+        return PW4_ERR_WORKSPACE;
+    }
+    const int64_t rows = batch * beams;
+    const int slices = slices_of(rows, vocab);
+    const SliceArgs slicing{logits, nullptr, ended, static_cast<SliceSums*>(workspace),
+                            reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + sums_bytes(rows, slices)),
+                            row_stride, (int32_t)rows, (int32_t)vocab, (int32_t)std::min(width, vocab), slices,
+                            (int32_t)ceil_div(vocab, slices)};
+    const SelectArgs a{slicing, scores, end_token, out_scores, out_rows, out_tokens, out_ended, (int32_t)beams, (int32_t)width};
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const dim3 grid(slices, (unsigned)rows);
+    const auto run = [&](auto dt) {
+        constexpr int DT = decltype(dt)::value;
+        if (per_thread(rows, vocab) == 16) {
+            hipLaunchKernelGGL((slice_kernel<DT, 16, false>), grid, dim3(kThreads), 0, s, slicing);
+        } else {
+            hipLaunchKernelGGL((slice_kernel<DT, 32, false>), grid, dim3(kThreads), 0, s, slicing);
+        }
+    };
+    if (dtype == PW4_DTYPE_F16) {
+        run(std::integral_constant<int, PW4_DTYPE_F16>{});
+    } else if (dtype == PW4_DTYPE_BF16) {
+        run(std::integral_constant<int, PW4_DTYPE_BF16>{});
+    } else {
+        run(std::integral_constant<int, PW4_DTYPE_F32>{});
+    }
+    hipLaunchKernelGGL(select_kernel, dim3((unsigned)batch), dim3(kThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? PW4_OK : report_hip_error(e);
+}
+
+int pw4_beam_reorder(const pw4_beam_state* states, int64_t count, const int32_t* rows, int64_t n,
+                     pw4_stream_t stream) {
+    if (count < 0 || n < 0 || (count && !states)) return PW4_ERR_ARG;
+    if (n > INT_MAX) return PW4_ERR_SHAPE;
+    for (int64_t i = 0; i < count; ++i) {
+        const pw4_beam_state& st = states[i];
+        if (st.row_bytes < 0 || st.num_rows < 0) return PW4_ERR_ARG;
+        if (st.num_rows > INT_MAX || (st.row_bytes - 1) / kPiece + 1 > INT_MAX / kStates / std::max<int64_t>(n, 1)) return PW4_ERR_SHAPE;
+        if (n && st.row_bytes && (!rows || !st.dst || (st.num_rows && !st.src))) return PW4_ERR_ARG;
+    }
+    if (n == 0) return PW4_OK;
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    for (int64_t first = 0; first < count;) {
+        ReorderArgs a{};
+        a.rows = rows;
+        uint64_t all = 0;
+        int64_t items = 0;
+        for (; first < count && a.count < kStates; ++first) {
+            const pw4_beam_state& st = states[first];
+            if (st.row_bytes == 0) continue;
+            const int c = a.count++;
+            a.src[c] = static_cast<const uint8_t*>(st.src);
+            a.dst[c] = static_cast<uint8_t*>(st.dst);
+            a.row_bytes[c] = st.row_bytes;
+            a.num_rows[c] = st.num_rows;
+            a.pieces[c] = (int32_t)ceil_div(st.row_bytes, kPiece);
+            a.end[c] = items += n * a.pieces[c];
+            all |= (uint64_t)(uintptr_t)st.src | (uint64_t)(uintptr_t)st.dst | (uint64_t)st.row_bytes;
+        }
+        if (a.count == 0) break;
+        const dim3 grid((unsigned)items);
+        if ((all & 15) == 0) {
+            hipLaunchKernelGGL(reorder_kernel<u32x4>, grid, dim3(kThreads), 0, s, a);
+        } else if ((all & 3) == 0) {
+            hipLaunchKernelGGL(reorder_kernel<uint32_t>, grid, dim3(kThreads), 0, s, a);
+        } else {
+            hipLaunchKernelGGL(reorder_kernel<uint8_t>, grid, dim3(kThreads), 0, s, a);
+        }
+        if (const hipError_t e = hipGetLastError(); e != hipSuccess) return report_hip_error(e);
+    }
+    return PW4_OK;
+}
+
+}  // extern "C"

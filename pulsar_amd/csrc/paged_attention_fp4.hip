@@ -1,0 +1,611 @@
+// Attention of new tokens over a paged cache in 4 bits (the definition and the pages'
+// layout: pulsar_paged.h).
+//
+// A key is codes times powers of two, one for each 32 elements.  The conversion
+// instructions take both (v_cvt_scalef32_pk_*_fp4: two elements each), and every value
+// that a code stands for is exact in 16 bits, so the products see the cache's own
+// numbers and the rest is the attention over a 16-bit cache: rows, tiles, transposed
+// products and splitting are those of paged_attention.hip.
+//
+// Keys come into registers as they lie in the cache, a block ahead; a wave's load takes 16
+// keys, lane l a quarter (l / 16) of key l % 16's head.  Widened, that quarter is K's matrix
+// operand as it is, q's elements being put in the same order; V goes to LDS (and K too, where
+// waves share it), from where it is read transposed.  A key index outside what some row of the
+// tile sees is clamped to one that is seen, as there.
+#include "paged_attention_parts.h"
+
+using namespace pw4;
+
+namespace {
+
+struct Fp4Params : Params {
+    uint32_t row_codes, row_exps;    // bytes of a token's codes, and of its exponents
+    uint32_t head_codes, head_exps;  // of a page's of one head
+    uint32_t exps_at;                // where a page's exponents begin
+};
+
+// The cache's elements one at a time, as the products take them.
+struct Fp4Keys {
+    static constexpr bool kRepeats = false;
+    template <bool BF16>
+    static __device__ __forceinline__ float element(const Fp4Params& a, const uint16_t* plane, int head, uint32_t page,
+                                                    uint32_t row, int d) {
+        const uint8_t* const at = reinterpret_cast<const uint8_t*>(plane) + (uint64_t)page * a.page_bytes;
+        const uint32_t code = at[head * a.head_codes + row * a.row_codes + d / 2] >> (d % 2 * 4) & 15;
+        const uint32_t exp = at[a.exps_at + head * a.head_exps + row * a.row_exps + d / 32];
+        const float scale = __builtin_bit_cast(float, exp << 23);
+        const auto pair = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, scale, 0);
+        return to_float<BF16>(f32_to_out<BF16>(pair[0]));
+    }
+};
+
+// Where a tile's keys are.
+struct Source {
+    const uint8_t* k;
+    const uint8_t* v;
+    const int32_t* table;    // the sequence's row
+    uint32_t codes, exps;    // of the key-value head in a page
+    uint32_t pages1;         // pages - 1
+    int lo, last;            // keys are clamped to [lo, last]
+};
+__device__ __forceinline__ Source source_of(const Fp4Params& a, const Tile& t, int head) {
+    return Source{reinterpret_cast<const uint8_t*>(a.k), reinterpret_cast<const uint8_t*>(a.v), a.tables + t.b * a.table_stride,
+                  head * a.head_codes, a.exps_at + head * a.head_exps, (uint32_t)a.num_pages - 1, t.lo, t.hi - 1};
+}
+__device__ __forceinline__ int clamp_key(const Source& s, int key) { return min(max(key, s.lo), s.last); }
+
+// A lane's quarter of a key, as it lies in the cache: DP / 4 elements.
+template <int DP>
+struct Quarter {
+    static constexpr int kWords = DP / 32;            // of 8 codes
+    static constexpr int kExps = DP == 256 ? 2 : 1;
+    uint32_t codes[kWords], exps[kExps];
+};
+
+// Where in a token's codes and exponents a lane's quarter is.  Heads narrower than DP: a quarter, or
+// half of one, that they do not have is read from the head's start, and its exponent taken as 0.
+template <int DP>
+struct Lane {
+    uint32_t codes[Quarter<DP>::kExps], exps[Quarter<DP>::kExps];
+    bool there[Quarter<DP>::kExps];
+    __device__ __forceinline__ explicit Lane(const Fp4Params& a) {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int h = 0; h < Quarter<DP>::kExps; ++h) {
+            const int first = g * (DP / 4) + h * 32;  // element
+            there[h] = first < a.dim;
+            codes[h] = there[h] ? first / 2 : 0;
+            exps[h] = there[h] ? first / 32 : 0;
+        }
+    }
+};
+
+// The lane's key's page id.
+__device__ __forceinline__ uint32_t page_of(const Fp4Params& a, const Source& s, int key) {
+    return s.table[page_index(a, clamp_key(s, key))];
+}
+
+template <int DP>
+__device__ __forceinline__ void load_quarter(const uint8_t* codes, const uint8_t* exps, const Lane<DP>& l, Quarter<DP>& q) {
+    if constexpr (DP == 64) {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(codes + l.codes[0]);
+        q.codes[0] = x[0];
+        q.codes[1] = x[1];
+    } else {
+#pragma unroll
+        for (int h = 0; h < Quarter<DP>::kExps; ++h) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(codes + l.codes[h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q.codes[4 * h + e] = x[e];
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < Quarter<DP>::kExps; ++h) q.exps[h] = exps[l.exps[h]];
+}
+
+// Both planes' quarters of the lane's key, on page `id`.
+struct Place {
+    uint64_t page;
+    uint32_t codes, exps;
+};
+__device__ __forceinline__ Place place_of(const Fp4Params& a, const Source& s, int key, uint32_t id) {
+    key = clamp_key(s, key);
+    const uint32_t row = key - page_index(a, key) * a.page_size;
+    return Place{(uint64_t)min(id, s.pages1) * a.page_bytes, s.codes + row * a.row_codes, s.exps + row * a.row_exps};
+}
+template <int DP>
+__device__ __forceinline__ void load_plane(const uint8_t* plane, const Place& p, const Lane<DP>& l, Quarter<DP>& q) {
+    load_quarter<DP>(plane + p.page + p.codes, plane + p.page + p.exps, l, q);
+}
+
+// 16-bit elements of a quarter: word i becomes elements 8 i .. 8 i + 7.
+template <bool BF16, int DP>
+__device__ __forceinline__ u32x4 widen(const Lane<DP>& l, const Quarter<DP>& q, int i) {
+    const int h = DP == 256 ? i / 4 : 0;
+    const float scale = __builtin_bit_cast(float, (l.there[h] ? q.exps[h] : 127u) << 23);
+    const uint32_t w = q.codes[i];
+    if constexpr (BF16) {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+    } else {
+        return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
+    }
+}
+// A lane's quarter of row r of a stage (rows of DP 16-bit elements, 16-byte units placed by XOR with
+// `swizzle`), widened.
+template <bool BF16, int DP>
+__device__ __forceinline__ void store_quarter(uint8_t* stage, int r, int swizzle, const Lane<DP>& l, const Quarter<DP>& q) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int i = 0; i < Quarter<DP>::kWords; ++i) {
+        *reinterpret_cast<u32x4*>(stage + r * DP * 2 + ((g * Quarter<DP>::kWords + i) ^ swizzle) * 16) = widen<BF16, DP>(l, q, i);
+    }
+}
+
+// ---- few rows --------------------------------------------------------------------
+
+// Up to 16 MT query rows.  Each wave takes blocks of 32 keys of its own: K straight from registers,
+// V through 32 rows of LDS of its own (no barrier); the next block's codes are under way meanwhile.
+constexpr int kFewKeys = 32;
+template <int DP>
+constexpr int kFewWaves = DP == 256 ? 2 : 4;
+template <int DP>
+constexpr int kFewUnit = kFewKeys * kFewWaves<DP>;
+template <int DP>
+constexpr int kFewStage = kFewKeys * DP * 2;  // V of a block, bytes
+
+template <int DP, int MT>
+constexpr int few_stage_bytes() {
+    const int stages = kFewWaves<DP> * kFewStage<DP>, join = kFewWaves<DP> * 16 * MT * (DP + 4) * 4;
+    return stages > join ? stages : join;
+}
+
+template <bool BF16, int DP, int MT, bool CAP>
+__global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const Fp4Params a) {
+    constexpr int WAVES = kFewWaves<DP>, MR = 16 * MT, UNIT = kFewUnit<DP>;
+    constexpr int KS = DP / 32;       // steps of 32 head elements
+    constexpr int DT = DP / 16;       // tiles of 16 output elements
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
+    uint8_t* const stage = smem + wave * kFewStage<DP>;
+    const Lane<DP> at(a);
+    const float k = unit<CAP>(a);
+
+    Pieces<MR, kFewKeys, UNIT, WAVES, true> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, u0 = piece.u0, u1 = piece.u1, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const int begin = t.base + u0 * UNIT, end = min(t.hi, t.base + u1 * UNIT);
+        const int blocks = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
+        const int mine = (blocks - wave + WAVES - 1) / WAVES;  // blocks wave, wave + WAVES, ...
+        auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
+        uint32_t ids[2] = {0, 0};  // of the next block's keys c and 16 + c
+        auto pages = [&](int i) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) ids[kt] = page_of(a, src, first_of(i) + kt * 16 + c);
+        };
+        Quarter<DP> kq[2][2], vq[2][2];
+        auto load = [&](int i, int set, uint32_t id0, uint32_t id1) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const Place p = place_of(a, src, first_of(i) + kt * 16 + c, kt ? id1 : id0);
+                load_plane<DP>(src.k, p, at, kq[set][kt]);
+                load_plane<DP>(src.v, p, at, vq[set][kt]);
+            }
+        };
+        if (mine > 0) pages(0);
+        u32x4 q[MT][KS];
+        int row_lo[MT], row_hi[MT];  // keys that the lane's row sees
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            load_query<KS>(a, t, head, mt * 16 + c, g * KS, 1, q[mt]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const int pos = t.first_pos + (t.row0 + mt * 16 + c) / a.group;
+            row_hi[mt] = min(pos + 1, t.hi);
+            row_lo[mt] = a.window > 0 ? pos + 1 - a.window : 0;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[mt][st]));  // here, not waited for in the loop
+        }
+        // blocks inside [all_lo, all_hi) are seen by every row of the tile
+        const int all_hi = min(t.first_pos + t.row0 / a.group + 1, t.hi);
+        const int all_lo = a.window > 0 ? t.first_pos + (t.row0 + t.rows - 1) / a.group + 1 - a.window : 0;
+        f32x4 o[MT][DT];
+        float m[MT], z[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -kInf;
+            z[mt] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        if (mine > 0) {
+            load(0, 0, ids[0], ids[1]);
+            if (mine > 1) pages(1);
+        }
+        auto block = [&](int i, int set) {
+            // the ids of block i + 2 ahead of the codes of block i + 1: loads return in order
+            if (i + 1 < mine) {
+                const uint32_t id0 = ids[0], id1 = ids[1];
+                if (i + 2 < mine) pages(i + 2);
+                load(i + 1, set ^ 1, id0, id1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const int key0 = first_of(i);
+            f32x4 s[MT][2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    const u32x4 kf = widen<BF16, DP>(at, kq[set][kt], st);
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, q[mt][st], s[mt][kt]);
+                }
+            }
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const int r = kt * 16 + c;
+                store_quarter<BF16, DP>(stage, r, v_swizzle<DP, false>(r), at, vq[set][kt]);
+            }
+            asm volatile("" ::: "memory");  // a wave's LDS operations stay in this order
+            const bool masked = key0 < all_lo || key0 + kFewKeys > all_hi;
+            u32x4 p[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float x[8], top = -kInf;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[mt][e / 4][e % 4];
+                cap_scores<CAP, 8>(a, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
+                    x[e] = masked & ((key < row_lo[mt]) | (key >= row_hi[mt])) ? -kInf : x[e];
+                    top = fmaxf(top, x[e]);
+                }
+                top = max_halves(max_quarters(top));
+                const float m_new = fmaxf(m[mt], top);
+                if (__any((m_new - m[mt]) * k > kSlack)) {
+                    const float scale = __builtin_amdgcn_exp2f((m[mt] - (m_new == -kInf ? 0.f : m_new)) * k);
+                    z[mt] *= scale;
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) o[mt][d] *= scale;
+                    m[mt] = m_new;
+                }
+                const float shift = m[mt] == -kInf ? -kLift<BF16> : shift_of<BF16>(m[mt], k);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(x[e] * k - shift);
+                    z[mt] += x[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[mt][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+            }
+            // O^T += V^T P^T: step slot 8 g + j is key 4 g + j (j < 4) or 16 + 4 g + j - 4
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                u32x4 vf;
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const int r = kt * 16 + 4 * g + c / 4, unit = 2 * d + (c % 4) / 2;
+                    const u32x2 h = read_transposed(stage + r * DP * 2 + ((unit ^ v_swizzle<DP, false>(r)) * 16) + (c & 1) * 8);
+                    vf[2 * kt] = h[0];
+                    vf[2 * kt + 1] = h[1];
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][d] = mfma16x16x32<BF16>(vf, p[mt], o[mt][d]);
+            }
+            asm volatile("" ::: "memory");
+        };
+        for (int i = 0; i < mine; i += 2) {
+            block(i, 0);
+            if (i + 1 < mine) block(i + 1, 1);
+        }
+        __syncthreads();  // every wave is done with its stage
+        join_waves<Fp4Keys, BF16, DP, MT, WAVES, CAP>(a, t, smem, wave, head, slot, begin, end, k, m, z, o);
+        __syncthreads();  // the stages are used again
+    }
+    clear_rest(a);
+}
+
+// ---- many rows --------------------------------------------------------------------
+
+// Four waves of 32 query rows each over blocks of 64 keys that they share in LDS as 16-bit elements,
+// two stages: each wave widens 16 keys of a block, whose codes came during the block before.
+constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
+constexpr int kAhead = 4;  // operands read ahead of their products
+template <int DP>
+constexpr int kManyStage = 2 * kManyKeys * DP * 2;
+template <int DP>
+constexpr int many_stage_bytes() { return 2 * kManyStage<DP>; }
+
+template <bool BF16, int DP, bool CAP>
+__global__ __launch_bounds__(kManyWaves * 64) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
+void fp4_many_rows_kernel(const Fp4Params a) {
+    constexpr int WAVES = kManyWaves, MR = kManyRows, KEYS = kManyKeys;
+    constexpr int KS = DP / 16;      // steps of 16 head elements
+    constexpr int DT = DP / 32;      // tiles of 32 output elements
+    constexpr int COPY = KEYS / WAVES;
+    static_assert(COPY == 16, "a load takes 16 keys");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
+    const Lane<DP> at(a);
+    const int copied = wave * COPY + (lane & 15);  // the lane's key of a block
+    const float k = unit<CAP>(a);
+    // LDS places of the lane's operands in a stage: K's unit 2 st + h of row c lies st << 5 (in
+    // bits 5 up) away by XOR; V's 4 rows from 4 h on, at columns of tile d, d << 6 away
+    const uint32_t k_at = (uint32_t)(c * DP * 2 + ((h ^ k_swizzle<DP>(c)) * 16));
+    const int vr = 4 * h + ((c & 15) >> 2);
+    const uint32_t v_at = (uint32_t)(kManyStage<DP> / 2 + vr * DP * 2 +
+                                     ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) + (c & 1) * 8);
+    Pieces<MR, KEYS, KEYS, WAVES, false> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
+        const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        const WaveRows<KEYS> r(a, t, wave);
+        u32x4 q[KS];
+        load_query<KS>(a, r.mine, head, c, h, 2, q);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[st]));  // here, not waited for in the loop
+        f32x16 o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        float m = -kInf, z = 0.f;
+        uint32_t id = 0;  // the page of the lane's key of the block that is loaded next
+        Quarter<DP> kq, vq;
+        auto page = [&](int i) { return page_of(a, src, begin + i * KEYS + copied); };
+        auto load = [&](int i) {
+            const Place p = place_of(a, src, begin + i * KEYS + copied, id);
+            load_plane<DP>(src.k, p, at, kq);
+            load_plane<DP>(src.v, p, at, vq);
+        };
+        auto store = [&](int i) {
+            uint8_t* const to = smem + (i & 1) * kManyStage<DP>;
+            store_quarter<BF16, DP>(to, copied, k_swizzle<DP>(copied), at, kq);
+            store_quarter<BF16, DP>(to + kManyStage<DP> / 2, copied, v_swizzle<DP, true>(copied), at, vq);
+        };
+        if (blocks > 0) {
+            id = page(0);
+            load(0);
+            if (blocks > 1) id = page(1);
+            store(0);
+            if (blocks > 1) {
+                load(1);
+                if (blocks > 2) id = page(2);
+            }
+        }
+        for (int i = 0; i < blocks; ++i) {
+            // block i is there, and every wave is done with block i - 1
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (i + 1 < blocks) {
+                store(i + 1);
+                if (i + 2 < blocks) {
+                    const uint32_t then = i + 3 < blocks ? page(i + 3) : 0;
+                    load(i + 2);
+                    id = then;
+                }
+            }
+            const int key0 = begin + i * KEYS;
+            if (!r.sees(key0)) continue;
+            const uint8_t* const st_at = smem + (i & 1) * kManyStage<DP>;
+            f32x16 s[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+            // products n = (st, kt) in turn, each with the read of an operand kAhead products on behind it
+            auto read_k = [&](int n) {
+                return *reinterpret_cast<const u32x4*>(st_at + (k_at ^ ((n / 2) << 5)) + (n % 2) * 32 * DP * 2);
+            };
+            u32x4 kf[kAhead];
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) kf[n] = read_k(n);
+#pragma unroll
+            for (int n = 0; n < 2 * KS; ++n) {
+                __builtin_amdgcn_sched_barrier(0);
+                s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
+                if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
+            }
+            cap_scores<CAP, 16>(a, s[0]);
+            cap_scores<CAP, 16>(a, s[1]);
+            r.mask(key0, h, s);
+            float top = -kInf;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kt][e]);
+            top = max_halves(top);
+            const float m_new = fmaxf(m, top);
+            if (__any((m_new - m) * k > kSlack)) {
+                const float scale = __builtin_amdgcn_exp2f((m - (m_new == -kInf ? 0.f : m_new)) * k);
+                z *= scale;
+#pragma unroll
+                for (int d = 0; d < DT; ++d) o[d] *= scale;
+                m = m_new;
+            }
+            const float shift = m == -kInf ? -kLift<BF16> : shift_of<BF16>(m, k);
+            // Step st of 16 keys: slot 8 h + j is key 16 st + 4 h + j (j < 4) or 16 st + 8 + 4 h + j - 4.
+            // Products n = (st, d) in turn, each with the read of an operand kAhead products on and a
+            // share of the next step's probabilities behind it.
+            float x[8];
+            auto probability = [&](int st, int e) {
+                x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
+                z += x[e];
+            };
+            auto read_v = [&](int n) {
+                const uint8_t* const at_v = st_at + (v_at ^ ((n % DT) << 6)) + (n / DT) * 16 * DP * 2;
+                const u32x2 y0 = read_transposed(at_v), y1 = read_transposed(at_v + 8 * DP * 2);
+                return u32x4{y0[0], y0[1], y1[0], y1[1]};
+            };
+            u32x4 vf[kAhead], p;
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) vf[n] = read_v(n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) probability(0, e);
+#pragma unroll
+            for (int n = 0; n < 4 * DT; ++n) {
+                const int st = n / DT, d = n % DT;
+                if (d == 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                o[d] = mfma32x32x16<BF16>(vf[n % kAhead], p, o[d]);
+                if (n + kAhead < 4 * DT) vf[n % kAhead] = read_v(n + kAhead);
+                if (st < 3) {
+#pragma unroll
+                    for (int e = d * 8 / DT; e < (d + 1) * 8 / DT; ++e) probability(st + 1, e);
+                }
+            }
+        }
+        store_rows<Fp4Keys, BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held_max<BF16>(m, k), z, o);
+        __syncthreads();  // every wave is done with the stages
+    }
+    clear_rest(a);
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+struct Call {
+    Fp4Params p;
+    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128
+    int64_t tiles;             // at most
+    size_t bytes;
+};
+
+int64_t page_bytes(const pw4_paged_attention_args* a) {
+    return a->page_size * a->kv_heads * (a->head_dim / 2 + a->head_dim / 32);
+}
+
+// Which kernel, tiles and split, from what the host knows.  `a` has passed check().
+Call plan_call(const pw4_paged_attention_args* a) {
+    Call c{};
+    Fp4Params& p = c.p;
+    static_cast<Params&>(p) = params_of(a);
+    p.page_bytes = (uint32_t)a->page_stride;
+    p.row_codes = (uint32_t)(a->head_dim / 2);
+    p.row_exps = (uint32_t)(a->head_dim / 32);
+    p.head_codes = (uint32_t)a->page_size * p.row_codes;
+    p.head_exps = (uint32_t)a->page_size * p.row_exps;
+    p.exps_at = (uint32_t)a->kv_heads * p.head_codes;
+    const int64_t rows = (int64_t)p.max_q * p.group;
+    c.dp = padded_dim(a->head_dim);
+    const int cus = device_cus();
+    const auto tiles_of = [&](int tile_rows) {
+        return std::min(a->num_tokens * p.group / tile_rows + p.batch, p.batch * ceil_div(rows, tile_rows));
+    };
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
+    const bool few = c.tile_rows <= 32;
+    c.tiles = few ? p.batch : tiles_of(c.tile_rows);
+    const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
+    // workgroups that run at once
+    const int slots = few ? 3 * cus : c.dp != 256 ? 2 * cus : cus;
+    // units of a tile: of the keys that a window leaves its rows, or all
+    const int64_t most_keys =
+        p.window == 0 ? p.max_len
+                      : std::min<int64_t>(p.max_len, (int64_t)p.window + (std::min<int64_t>(c.tile_rows, rows) + p.group - 2) / p.group);
+    const int64_t most_units = ceil_div(most_keys, unit) + 1;
+    const char* const forced = plan_override("PW4_ATTN_UNITS");
+    const int forced_units = forced ? std::atoi(forced) : 0;
+    p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
+    const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
+    const bool wanted = forced_split ? forced_split[0] == '1'
+                        : few ? most_units > (8 * c.tiles * p.kv_heads <= cus ? 7 : 4 * c.tiles * p.kv_heads <= cus ? 16 : 22)
+                              : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
+    p.split = wanted && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
+    c.grid = (int)(c.tiles * p.kv_heads);
+    if (p.split) {
+        c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
+        c.bytes = partial_bytes(c.grid, c.tile_rows, p.dim);
+    }
+    return c;
+}
+
+template <bool BF16, int DP, bool CAP>
+hipError_t launch(const Call& c, hipStream_t s) {
+    hipError_t e;
+    if (c.tile_rows == 16) {
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), s);
+    } else if (c.tile_rows == 32) {
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), s);
+    } else {
+        e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), s);
+    }
+    if (e != hipSuccess || !c.p.split) return e;
+    if (c.tile_rows == 16) {
+        run_join<16, BF16>(c.p, c.tiles, c.grid, s);
+    } else if (c.tile_rows == 32) {
+        run_join<32, BF16>(c.p, c.tiles, c.grid, s);
+    } else {
+        run_join<kManyRows, BF16>(c.p, c.tiles, c.grid, s);
+    }
+    return hipGetLastError();
+}
+
+template <bool BF16, int DP>
+hipError_t launch_cap(const Call& c, hipStream_t s) {
+    return c.p.cap2 > 0.f ? launch<BF16, DP, true>(c, s) : launch<BF16, DP, false>(c, s);
+}
+template <bool BF16>
+hipError_t launch_dim(const Call& c, hipStream_t s) {
+    return c.dp == 64 ? launch_cap<BF16, 64>(c, s) : c.dp == 128 ? launch_cap<BF16, 128>(c, s) : launch_cap<BF16, 256>(c, s);
+}
+
+int check(const pw4_paged_attention_args* a) {
+    if (const int rc = check_attention(a)) return rc;
+    if (a->head_dim % 32 != 0) return PW4_ERR_SHAPE;
+    if (a->num_tokens == 0) return PW4_OK;
+    const uint64_t addresses = (uint64_t)(uintptr_t)a->q | (uint64_t)(uintptr_t)a->k_cache |
+                               (uint64_t)(uintptr_t)a->v_cache | (uint64_t)(uintptr_t)a->out;
+    if ((addresses & 15) != 0 || ((a->q_token_stride | a->q_head_stride) & 7) != 0) return PW4_ERR_ARG;
+    if (a->kv_heads > 65535 || a->page_size > INT_MAX / 256 / a->kv_heads) return PW4_ERR_SHAPE;
+    if (a->page_stride < 0 || a->page_stride % 16 != 0) return PW4_ERR_ARG;
+    if (a->page_stride > INT_MAX || (a->num_pages > 1 && a->page_stride < page_bytes(a))) return PW4_ERR_SHAPE;
+    return PW4_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t pw4_paged_attention_fp4_workspace_size(const pw4_paged_attention_args* args) {
+    return check(args) != PW4_OK || args->num_tokens == 0 ? 0 : plan_call(args).bytes;
+}
+
+int pw4_paged_attention_fp4(const pw4_paged_attention_args* args, void* workspace, size_t workspace_bytes,
+                            pw4_stream_t stream) {
+    if (const int rc = check(args)) return rc;
+    if (args->num_tokens == 0) return PW4_OK;
+    Call c = plan_call(args);
+    if (c.grid > 65535 * 4096 || c.tiles * c.p.kv_heads > INT_MAX) return PW4_ERR_SHAPE;
+    if (c.bytes > 0) {
+        if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < c.bytes) {
+            return PW4_ERR_WORKSPACE;
+        }
+        place_partials(c.p, workspace, c.grid, c.tile_rows);
+    }
+    const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const hipError_t e = args->dtype == PW4_DTYPE_BF16 ? launch_dim<true>(c, s) : launch_dim<false>(c, s);
+    return e == hipSuccess ? PW4_OK : report_hip_error(e);
+}
+
+}  // extern "C"

@@ -106,27 +106,45 @@ pw4_page_pool as_pool(const char* op, const at::Tensor& pool) {
                          stride_of(pool, 1) * e};
 }
 
-}  // namespace
+// A 4-bit cache uint8 [P, page, heads, D / 2 + D / 32], its pages in one piece each; returns D.
+int64_t check_fp4_cache(const char* op, const char* name, const at::Tensor& c) {
+    TORCH_CHECK(c.scalar_type() == at::kByte && c.dim() == 4, op, ": ", name,
+                " must be uint8 and 4-D [pages, page_size, kv_heads, head_dim / 2 + head_dim / 32]");
+    TORCH_CHECK(c.size(3) > 0 && c.size(3) % 17 == 0 && c.size(3) <= 8 * 17, op, ": ", name,
+                "'s rows must be head_dim / 2 + head_dim / 32 bytes, head_dim a multiple of 32 up to 256");
+    int64_t bytes = 1;
+    for (int64_t d = 3; d >= 1; --d) {
+        TORCH_CHECK(c.numel() == 0 || c.size(d) == 1 || c.stride(d) == bytes, op, ": ", name, "'s pages must be contiguous");
+        bytes *= c.size(d);
+    }
+    TORCH_CHECK(c.numel() == 0 || (aligned16(c) && stride_of(c, 0) % 16 == 0), op, ": ", name,
+                "'s pages must be 16-byte aligned");
+    TORCH_CHECK(c.numel() == 0 || c.size(0) == 1 || c.stride(0) >= bytes, op, ": ", name, "'s pages overlap");
+    return c.size(3) / 17 * 32;
+}
 
-std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, const at::Tensor& k_cache,
-                                                        const at::Tensor& v_cache, const at::Tensor& block_tables,
-                                                        const at::Tensor& seq_lens, const at::Tensor& cu_q,
-                                                        int64_t max_q_len, int64_t max_seq_len,
-                                                        std::optional<double> scale, int64_t window, double softcap,
-                                                        bool return_lse) {
-    const char* const op = "paged_attention";
+// paged_attention over 16-bit caches, or with fp4 over 4-bit ones.
+std::tuple<at::Tensor, at::Tensor> attend(const char* op, bool fp4, const at::Tensor& q, const at::Tensor& k_cache,
+                                          const at::Tensor& v_cache, const at::Tensor& block_tables,
+                                          const at::Tensor& seq_lens, const at::Tensor& cu_q, int64_t max_q_len,
+                                          int64_t max_seq_len, std::optional<double> scale, int64_t window,
+                                          double softcap, bool return_lse) {
     check_device(op, q, {&k_cache, &v_cache, &block_tables, &seq_lens, &cu_q});
     check_half(op, "q", q);
     TORCH_CHECK(q.dim() == 3, op, ": q must be 3-D [T, q_heads, head_dim]");
-    check_cache(op, "k_cache", k_cache);
-    check_cache(op, "v_cache", v_cache);
+    if (!fp4) {
+        check_cache(op, "k_cache", k_cache);
+        check_cache(op, "v_cache", v_cache);
+    }
+    const int64_t dim = fp4 ? check_fp4_cache(op, "k_cache", k_cache) : k_cache.size(3);
+    if (fp4) check_fp4_cache(op, "v_cache", v_cache);
     check_same_layout(op, k_cache, v_cache);
-    TORCH_CHECK(k_cache.scalar_type() == q.scalar_type(), op, ": q and the caches must have one dtype");
+    TORCH_CHECK(fp4 || k_cache.scalar_type() == q.scalar_type(), op, ": q and the caches must have one dtype");
     check_tables(op, nullptr, block_tables, &seq_lens);
     check_ints(op, "cu_q", cu_q, 1);
     const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), B = block_tables.size(0), Hkv = k_cache.size(2);
     TORCH_CHECK(cu_q.size(0) == B + 1, op, ": cu_q must be [batch + 1]");
-    TORCH_CHECK(k_cache.size(3) == D, op, ": q and the caches differ in head_dim");
+    TORCH_CHECK(dim == D, op, ": q and the caches differ in head_dim");
     TORCH_CHECK(D > 0 && D <= 256 && D % 8 == 0, op, ": head_dim must be a multiple of 8 up to 256");
     TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0, op, ": q_heads must be a multiple of kv_heads");
     TORCH_CHECK(k_cache.size(1) > 0, op, ": page_size must be positive");
@@ -135,7 +153,7 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, con
     TORCH_CHECK(softcap >= 0 && std::isfinite((float)softcap), op, ": softcap must be finite in fp32 and not negative");
     TORCH_CHECK(!scale || std::isfinite((float)*scale), op, ": scale must be finite in fp32");
     for (const at::Tensor* c : {&k_cache, &v_cache}) {
-        TORCH_CHECK(c->numel() == 0 || (aligned16(*c) && stride_of(*c, 0) % 8 == 0 && stride_of(*c, 1) % 8 == 0 &&
+        TORCH_CHECK(fp4 || c->numel() == 0 || (aligned16(*c) && stride_of(*c, 0) % 8 == 0 && stride_of(*c, 1) % 8 == 0 &&
                                         stride_of(*c, 2) % 8 == 0),
                     op, ": the caches' rows must be 16-byte aligned");
     }
@@ -177,10 +195,146 @@ std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, con
     // (a cap above 0 stays one: the kernel takes what is below 2^-100 as 2^-100)
     a.softcap = softcap > 0 ? std::max((float)softcap, 0x1p-100f) : 0.f;
     a.dtype = q.scalar_type() == at::kBFloat16 ? PW4_DTYPE_BF16 : PW4_DTYPE_F16;
-    const size_t bytes = pw4_paged_attention_workspace_size(&a);
+    const size_t bytes = fp4 ? pw4_paged_attention_fp4_workspace_size(&a) : pw4_paged_attention_workspace_size(&a);
     const at::Tensor ws = bytes ? scratch(bytes, q) : at::Tensor();
-    check_status(pw4_paged_attention(&a, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), op);
+    const auto call = fp4 ? pw4_paged_attention_fp4 : pw4_paged_attention;
+    check_status(call(&a, bytes ? ws.data_ptr() : nullptr, bytes, current_stream()), op);
     return {out, lse};
+}
+
+// paged_cache_append into 16-bit caches, or with fp4 into 4-bit ones.
+at::Tensor append(const char* op, bool fp4, const std::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
+                  at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& slots,
+                  const std::optional<at::Tensor>& rope, const std::optional<at::Tensor>& positions, bool interleaved) {
+    check_device(op, k_cache, {&k, &v, &v_cache, &slots});
+    if (q) check_device(op, k_cache, {&*q});
+    if (rope) check_device(op, k_cache, {&*rope});
+    if (positions) check_device(op, k_cache, {&*positions});
+    if (!fp4) {
+        check_cache(op, "k_cache", k_cache);
+        check_cache(op, "v_cache", v_cache);
+    }
+    const int64_t dim = fp4 ? check_fp4_cache(op, "k_cache", k_cache) : k_cache.size(3);
+    if (fp4) check_fp4_cache(op, "v_cache", v_cache);
+    check_same_layout(op, k_cache, v_cache);
+    check_half(op, "k", k);
+    check_ints(op, "slots", slots, 1, at::kLong);
+    TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes(), op, ": k and v must be 3-D [T, kv_heads, head_dim]");
+    TORCH_CHECK(v.scalar_type() == k.scalar_type() && (!q || q->scalar_type() == k.scalar_type()), op,
+                ": q, k and v must have one dtype");
+    TORCH_CHECK(fp4 || k_cache.scalar_type() == k.scalar_type(), op, ": k, v and the caches must have one dtype");
+    const int64_t T = k.size(0), Hkv = k.size(1);
+    TORCH_CHECK(slots.size(0) == T, op, ": slots must be [T]");
+    TORCH_CHECK(Hkv == k_cache.size(2) && k.size(2) == dim, op, ": k and the caches differ in kv_heads or head_dim");
+    TORCH_CHECK(dim > 0 && dim <= 256 && dim % 8 == 0, op, ": head_dim must be a multiple of 8 up to 256");
+    TORCH_CHECK(!q || (q->dim() == 3 && q->size(0) == T && q->size(2) == dim), op, ": q must be 3-D [T, q_heads, head_dim]");
+    TORCH_CHECK(k_cache.size(1) > 0, op, ": page_size must be positive");
+    TORCH_CHECK(rope.has_value() == positions.has_value(), op, ": rope and positions come together");
+    TORCH_CHECK(rope || !q, op, ": q is rotated, so it needs rope and positions");
+    if (rope) {
+        TORCH_CHECK(rope->scalar_type() == at::kFloat && rope->dim() == 2 && rope->is_contiguous(), op,
+                    ": rope must be fp32, contiguous and 2-D [positions, rot]");
+        TORCH_CHECK(rope->size(1) % 2 == 0 && rope->size(1) <= dim, op, ": rope's rows must be even in length and at most head_dim");
+        check_ints(op, "positions", *positions, 1, at::kLong);
+        TORCH_CHECK(positions->size(0) == T, op, ": positions must be [T]");
+    }
+    DeviceGuard guard(k_cache.device());
+    const auto rows = [&](const at::Tensor& t) { return t.size(2) <= 1 || t.numel() == 0 || t.stride(2) == 1 ? t : t.contiguous(); };
+    const at::Tensor kc = rows(k), vc = rows(v), qc = q ? rows(*q) : at::Tensor();
+    at::Tensor out = q ? fresh({T, q->size(1), dim}, k.scalar_type(), k) : fresh({0, 0, dim}, k.scalar_type(), k);
+    if (T == 0) return out;
+    pw4_paged_append_args a{};
+    if (q) {
+        a.q = qc.data_ptr();
+        a.q_out = out.data_ptr();
+        a.q_heads = q->size(1);
+        a.q_token_stride = stride_of(qc, 0);
+        a.q_head_stride = stride_of(qc, 1);
+    }
+    a.k = kc.data_ptr();
+    a.v = vc.data_ptr();
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.slots = slots.data_ptr<int64_t>();
+    if (rope) {
+        a.positions = positions->data_ptr<int64_t>();  // (not null: T > 0)
+        a.rope = rope->data_ptr<float>();
+        a.rot = rope->size(1);
+        a.rope_rows = rope->size(0);
+    }
+    a.num_tokens = T;
+    a.kv_heads = Hkv;
+    a.head_dim = dim;
+    a.k_token_stride = stride_of(kc, 0);
+    a.k_head_stride = stride_of(kc, 1);
+    a.v_token_stride = stride_of(vc, 0);
+    a.v_head_stride = stride_of(vc, 1);
+    a.num_pages = k_cache.size(0);
+    a.page_size = k_cache.size(1);
+    a.page_stride = stride_of(k_cache, 0);
+    a.row_stride = stride_of(k_cache, 1);
+    a.kv_head_stride = stride_of(k_cache, 2);
+    a.interleaved = interleaved;
+    a.dtype = k.scalar_type() == at::kBFloat16 ? PW4_DTYPE_BF16 : PW4_DTYPE_F16;
+    check_status((fp4 ? pw4_paged_cache_append_fp4 : pw4_paged_cache_append)(&a, current_stream()), op);
+    return out;
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_cuda(const at::Tensor& q, const at::Tensor& k_cache,
+                                                        const at::Tensor& v_cache, const at::Tensor& block_tables,
+                                                        const at::Tensor& seq_lens, const at::Tensor& cu_q,
+                                                        int64_t max_q_len, int64_t max_seq_len,
+                                                        std::optional<double> scale, int64_t window, double softcap,
+                                                        bool return_lse) {
+    return attend("paged_attention", false, q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len, max_seq_len, scale, window,
+                  softcap, return_lse);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_attention_fp4_cuda(const at::Tensor& q, const at::Tensor& k_cache,
+                                                            const at::Tensor& v_cache, const at::Tensor& block_tables,
+                                                            const at::Tensor& seq_lens, const at::Tensor& cu_q,
+                                                            int64_t max_q_len, int64_t max_seq_len,
+                                                            std::optional<double> scale, int64_t window, double softcap,
+                                                            bool return_lse) {
+    return attend("paged_attention_fp4", true, q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len, max_seq_len, scale, window,
+                  softcap, return_lse);
+}
+
+at::Tensor paged_cache_append_cuda(const std::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
+                                   at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& slots,
+                                   const std::optional<at::Tensor>& rope, const std::optional<at::Tensor>& positions,
+                                   bool interleaved) {
+    return append("paged_cache_append", false, q, k, v, k_cache, v_cache, slots, rope, positions, interleaved);
+}
+
+at::Tensor paged_cache_append_fp4_cuda(const std::optional<at::Tensor>& q, const at::Tensor& k, const at::Tensor& v,
+                                       at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& slots,
+                                       const std::optional<at::Tensor>& rope, const std::optional<at::Tensor>& positions,
+                                       bool interleaved) {
+    return append("paged_cache_append_fp4", true, q, k, v, k_cache, v_cache, slots, rope, positions, interleaved);
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_cache_read_fp4_cuda(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                             const at::Tensor& slots, at::ScalarType dtype) {
+    const char* const op = "paged_cache_read_fp4";
+    check_device(op, k_cache, {&v_cache, &slots});
+    const int64_t dim = check_fp4_cache(op, "k_cache", k_cache);
+    check_fp4_cache(op, "v_cache", v_cache);
+    check_same_layout(op, k_cache, v_cache);
+    check_ints(op, "slots", slots, 1, at::kLong);
+    TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, op, ": dtype must be fp16 or bf16");
+    TORCH_CHECK(k_cache.size(1) > 0, op, ": page_size must be positive");
+    DeviceGuard guard(k_cache.device());
+    const int64_t T = slots.size(0), Hkv = k_cache.size(2);
+    at::Tensor k = fresh({T, Hkv, dim}, dtype, k_cache), v = fresh({T, Hkv, dim}, dtype, k_cache);
+    check_status(pw4_paged_cache_read_fp4(k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr<int64_t>(), k.data_ptr(),
+                                          v.data_ptr(), T, Hkv, dim, k_cache.size(0), k_cache.size(1),
+                                          stride_of(k_cache, 0), dtype == at::kBFloat16 ? PW4_DTYPE_BF16 : PW4_DTYPE_F16,
+                                          current_stream()),
+                 op);
+    return {k, v};
 }
 
 std::tuple<at::Tensor, at::Tensor> paged_cache_extend_cuda(at::Tensor& ref_counts, at::Tensor& block_tables,
@@ -332,6 +486,70 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> token_log
     return {lp, ranks, ent, top, ids};
 }
 
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select_cuda(const at::Tensor& logits,
+                                                                            const at::Tensor& scores,
+                                                                            std::optional<int64_t> width,
+                                                                            const std::optional<at::Tensor>& ended,
+                                                                            int64_t end_token) {
+    const char* const op = "beam_select";
+    check_device(op, logits, {&scores});
+    if (ended) check_device(op, logits, {&*ended});
+    const auto dt = logits.scalar_type();
+    TORCH_CHECK(dt == at::kFloat || dt == at::kHalf || dt == at::kBFloat16, op, ": logits must be fp32, fp16 or bf16");
+    TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, op, ": logits must be 2-D [batch * beams, vocab]");
+    TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.dim() == 2, op, ": scores must be fp32 and 2-D [batch, beams]");
+    const int64_t B = scores.size(0), K = scores.size(1), V = logits.size(1), W = width.value_or(K);
+    TORCH_CHECK(K > 0 && K <= 32, op, ": beams must be 1 to 32");
+    TORCH_CHECK(logits.size(0) == B * K, op, ": logits must be [batch * beams, vocab]");
+    TORCH_CHECK(W > 0 && W <= 32 && W <= K * V, op, ": width must be 1 to 32 and at most beams * vocab");
+    TORCH_CHECK(!ended || (ended->scalar_type() == at::kBool && ended->sizes() == scores.sizes()), op,
+                ": ended must be bool [batch, beams]");
+    TORCH_CHECK(!ended || W <= K, op, ": with ended, width must be at most beams");
+    DeviceGuard guard(logits.device());
+    const at::Tensor x = (V == 1 || logits.stride(1) == 1) && (B * K <= 1 || logits.stride(0) >= V) ? logits
+                                                                                                  : logits.contiguous();
+    const at::Tensor sc = scores.contiguous(), en = ended ? ended->contiguous() : at::Tensor();
+    at::Tensor out = fresh({B, W}, at::kFloat, logits), rows = fresh({B, W}, at::kInt, logits);
+    at::Tensor tokens = fresh({B, W}, at::kLong, logits), now = fresh({ended ? B : 0, W}, at::kBool, logits);
+    if (B == 0) return {out, rows, tokens, now};
+    const size_t bytes = pw4_beam_select_workspace_size(B, K, V, W);
+    const at::Tensor ws = scratch(bytes, logits);
+    check_status(pw4_beam_select(x.data_ptr(), dt == at::kFloat ? PW4_DTYPE_F32
+                                               : dt == at::kHalf ? PW4_DTYPE_F16
+                                                                 : PW4_DTYPE_BF16,
+                                 B, K, V, B * K > 1 ? x.stride(0) : V, sc.data_ptr<float>(),
+                                 ended ? static_cast<const uint8_t*>(en.data_ptr()) : nullptr, end_token, W,
+                                 out.data_ptr<float>(), rows.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(),
+                                 ended ? static_cast<uint8_t*>(now.data_ptr()) : nullptr, ws.data_ptr(), bytes,
+                                 current_stream()),
+                 op);
+    return {out, rows, tokens, now};
+}
+
+std::vector<at::Tensor> beam_reorder_cuda(at::TensorList states, const at::Tensor& rows) {
+    const char* const op = "beam_reorder";
+    check_device(op, rows, {});
+    TORCH_CHECK(rows.scalar_type() == at::kInt, op, ": rows must be int32");
+    DeviceGuard guard(rows.device());
+    const at::Tensor which = rows.contiguous();
+    const int64_t n = which.numel();
+    std::vector<at::Tensor> in, out;
+    std::vector<pw4_beam_state> list;
+    for (const at::Tensor& t : states) {
+        check_device(op, rows, {&t});
+        TORCH_CHECK(t.dim() >= 1, op, ": states must be at least 1-D");
+        in.push_back(t.contiguous());
+        at::DimVector sizes(t.sizes());
+        sizes[0] = n;
+        out.push_back(fresh(sizes, t.scalar_type(), rows));
+        int64_t bytes = t.element_size();
+        for (int64_t d = 1; d < t.dim(); ++d) bytes *= t.size(d);
+        list.push_back(pw4_beam_state{in.back().data_ptr(), out.back().data_ptr(), bytes, t.size(0)});
+    }
+    check_status(pw4_beam_reorder(list.data(), (int64_t)list.size(), which.data_ptr<int32_t>(), n, current_stream()), op);
+    return out;
+}
+
 }  // namespace pulsar
 
 TORCH_LIBRARY_FRAGMENT(pulsar, m) {
@@ -344,6 +562,18 @@ TORCH_LIBRARY_FRAGMENT(pulsar, m) {
         "int num_tokens, int page_size) -> (Tensor, Tensor)");
     m.def(
         "paged_cache_write(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots) -> ()");
+    m.def(
+        "paged_cache_append(Tensor? q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, "
+        "Tensor? rope=None, Tensor? positions=None, bool interleaved=False) -> Tensor");
+    m.def(
+        "paged_cache_append_fp4(Tensor? q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, "
+        "Tensor? rope=None, Tensor? positions=None, bool interleaved=False) -> Tensor");
+    m.def(
+        "paged_cache_read_fp4(Tensor k_cache, Tensor v_cache, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)");
+    m.def(
+        "paged_attention_fp4(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, Tensor seq_lens, Tensor "
+        "cu_q, int max_q_len, int max_seq_len, float? scale=None, int window=0, float softcap=0., bool "
+        "return_lse=False) -> (Tensor, Tensor)");
     m.def("paged_cache_copy(Tensor(a!) pool, Tensor src_pages, Tensor dst_pages) -> ()");
     m.def(
         "paged_cache_fork(Tensor(a!) pool, Tensor(b!) ref_counts, Tensor(c!) block_tables, Tensor(d!) seq_lens, "
@@ -352,6 +582,10 @@ TORCH_LIBRARY_FRAGMENT(pulsar, m) {
         "paged_cache_free(Tensor(a!) ref_counts, Tensor(b!) block_tables, Tensor(c!) seq_lens, Tensor rows) -> ()");
     m.def("paged_cache_compact(Tensor(a!) pool, Tensor(b!) ref_counts, Tensor(c!) block_tables) -> Tensor");
     m.def("token_logprobs(Tensor logits, Tensor targets, int top_k) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+    m.def(
+        "beam_select(Tensor logits, Tensor scores, int? width=None, Tensor? ended=None, int end_token=-1) -> (Tensor, "
+        "Tensor, Tensor, Tensor)");
+    m.def("beam_reorder(Tensor[] states, Tensor rows) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(pulsar, CUDA, m) {
@@ -363,4 +597,10 @@ TORCH_LIBRARY_IMPL(pulsar, CUDA, m) {
     m.impl("paged_cache_free", TORCH_FN(pulsar::paged_cache_free_cuda));
     m.impl("paged_cache_compact", TORCH_FN(pulsar::paged_cache_compact_cuda));
     m.impl("token_logprobs", TORCH_FN(pulsar::token_logprobs_cuda));
+    m.impl("paged_cache_append", TORCH_FN(pulsar::paged_cache_append_cuda));
+    m.impl("paged_cache_append_fp4", TORCH_FN(pulsar::paged_cache_append_fp4_cuda));
+    m.impl("paged_cache_read_fp4", TORCH_FN(pulsar::paged_cache_read_fp4_cuda));
+    m.impl("paged_attention_fp4", TORCH_FN(pulsar::paged_attention_fp4_cuda));
+    m.impl("beam_select", TORCH_FN(pulsar::beam_select_cuda));
+    m.impl("beam_reorder", TORCH_FN(pulsar::beam_reorder_cuda));
 }

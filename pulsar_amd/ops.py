@@ -1,4 +1,4 @@
-"""Python wrappers and fake (meta) kernels for the W4A16, paged-cache and log-probability ops.
+"""Python wrappers and fake (meta) kernels for the W4A16, paged-cache, log-probability and beam ops.
 
 Same wrapper names, argument meaning and fake-kernel output shapes as the
 reference pulsar/src/pulsar/core/ops.py:117-165,369-445, so code written
@@ -10,6 +10,12 @@ block_tables[b, j // page_size] at place j % page_size.  The book-keeping is int
 device, changed in place: ref_counts [pages] (0: free), block_tables [rows, width] (-1 past a
 row's last page) and seq_lens [rows].  No call waits for the device, and each can be captured
 into a graph.
+
+The cache in 4 bits (the `_fp4` ops) is a pool of bytes, [.., pages, page_size, kv_heads, head_dim / 2 +
+head_dim / 32] with head_dim a multiple of 32: blocks of 32 elements as OCP MX has them, 4-bit floats
+(0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign) under a shared power of two.  Inside a page the bytes lie head by
+head, all codes ahead of all exponents (include/pulsar_paged.h); pages are 16-byte aligned.  The page
+operators move such pages as any others.
 """
 
 from __future__ import annotations
@@ -79,6 +85,15 @@ def _paged_cache_write_fake(k, v, k_cache, v_cache, slots):
     return None
 
 
+def _paged_cache_append_fake(q, k, v, k_cache, v_cache, slots, rope=None, positions=None, interleaved=False):
+    return k.new_empty(q.shape if q is not None else (0, 0, k.shape[2]))
+
+
+def _paged_cache_read_fp4_fake(k_cache, v_cache, slots, dtype):
+    shape = (slots.shape[0], k_cache.shape[2], k_cache.shape[3] // 17 * 32)
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
 def _paged_cache_copy_fake(pool, src_pages, dst_pages):
     return None
 
@@ -101,6 +116,16 @@ def _token_logprobs_fake(logits, targets, top_k):
     return f32[0], targets.new_empty((t,)), f32[1], f32[2], targets.new_empty((t, top_k))
 
 
+def _beam_select_fake(logits, scores, width=None, ended=None, end_token=-1):
+    shape = (scores.shape[0], scores.shape[1] if width is None else width)
+    return (scores.new_empty(shape), scores.new_empty(shape, dtype=torch.int32), scores.new_empty(shape, dtype=torch.int64),
+            scores.new_empty(shape if ended is not None else (0, shape[1]), dtype=torch.bool))
+
+
+def _beam_reorder_fake(states, rows):
+    return [s.new_empty((rows.numel(), *s.shape[1:])) for s in states]
+
+
 def _register_fakes() -> None:
     fakes = {
         "pulsar::gemm_w4a16": _gemm_w4a16_fake,
@@ -119,6 +144,12 @@ def _register_fakes() -> None:
         "pulsar::paged_cache_free": _paged_cache_free_fake,
         "pulsar::paged_cache_compact": _paged_cache_compact_fake,
         "pulsar::token_logprobs": _token_logprobs_fake,
+        "pulsar::paged_cache_append": _paged_cache_append_fake,
+        "pulsar::paged_cache_append_fp4": _paged_cache_append_fake,
+        "pulsar::paged_cache_read_fp4": _paged_cache_read_fp4_fake,
+        "pulsar::paged_attention_fp4": _paged_attention_fake,
+        "pulsar::beam_select": _beam_select_fake,
+        "pulsar::beam_reorder": _beam_reorder_fake,
     }
     for name, func in fakes.items():
         torch.library.register_fake(name, func)
@@ -200,6 +231,12 @@ def gemm_w4a16_silu_mul(x: torch.Tensor, weight_marlin: torch.Tensor, scales: to
 
 
 # The overloads themselves: looking one up costs as much as a small operator's checks.
+_beam_reorder = torch.ops.pulsar.beam_reorder.default
+_beam_select = torch.ops.pulsar.beam_select.default
+_paged_attention_fp4 = torch.ops.pulsar.paged_attention_fp4.default
+_paged_cache_append = torch.ops.pulsar.paged_cache_append.default
+_paged_cache_append_fp4 = torch.ops.pulsar.paged_cache_append_fp4.default
+_paged_cache_read_fp4 = torch.ops.pulsar.paged_cache_read_fp4.default
 _paged_attention = torch.ops.pulsar.paged_attention.default
 _paged_cache_compact = torch.ops.pulsar.paged_cache_compact.default
 _paged_cache_copy = torch.ops.pulsar.paged_cache_copy.default
@@ -239,6 +276,17 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     return (out, lse) if return_lse else out
 
 
+def paged_attention_fp4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                        seq_lens: torch.Tensor, cu_q: torch.Tensor, max_q_len: int, max_seq_len: int,
+                        scale: float | None = None, window: int = 0, softcap: float = 0.0, return_lse: bool = False):
+    """paged_attention over 4-bit caches uint8 [pages, page_size, kv_heads, head_dim / 2 + head_dim / 32],
+    with the results that a 16-bit cache of the values they hold has.  q is fp16 or bf16, of the dtype
+    that the cache was written in; head_dim a multiple of 32 up to 256."""
+    out, lse = _paged_attention_fp4(q, k_cache, v_cache, block_tables, seq_lens, cu_q, max_q_len, max_seq_len, scale,
+                                    window, softcap, return_lse)
+    return (out, lse) if return_lse else out
+
+
 def paged_cache_extend(ref_counts: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                        cu_q: torch.Tensor, num_tokens: int, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
     """Room for cu_q[b+1] - cu_q[b] new tokens of each row: the lowest-numbered free pages, dealt to
@@ -253,6 +301,58 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     """Stores k and v [T, kv_heads, head_dim] in the slots of one layer's caches (fp16 or bf16); a
     slot outside the caches (-1) is passed over."""
     _paged_cache_write(k, v, k_cache, v_cache, slots)
+
+
+def rope_table(positions: int, rot: int, base: float = 10000.0, device="cuda:0") -> torch.Tensor:
+    """Cosines and sines fp32 [positions, rot] of the angles p base^(-2 i / rot), i < rot / 2, as
+    paged_cache_append takes them; the angles are fp64, so far positions are as good as near ones."""
+    half = rot // 2
+    rate = base ** (-torch.arange(half, dtype=torch.float64, device=device) / max(half, 1))
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * rate
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def paged_cache_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                       v_cache: torch.Tensor, slots: torch.Tensor, rope: torch.Tensor | None = None,
+                       positions: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+    """paged_cache_write with the position rotation of q and k on the way, in one launch.
+
+    Token t at p = positions[t] has its heads' first rot elements rotated pairwise,
+    (a, b) -> (a c - b s, b c + a s) with c = rope[p, i] and s = rope[p, rot / 2 + i]: pair i is elements i
+    and rot / 2 + i, or with `interleaved` 2 i and 2 i + 1.  k rotated and v go to the token's slot.
+
+    Args:
+        q: [T, q_heads, head_dim], or None.
+        k, v: [T, kv_heads, head_dim] in q's and the caches' dtype, fp16 or bf16; like q with any strides.
+        slots: int64 [T]; a token whose slot is outside the caches (-1) is not stored.
+        rope: fp32 [positions, rot], contiguous, rot even and at most head_dim (rope_table makes one);
+            None: nothing is rotated, and q is None.
+        positions: int64 [T]; a token whose position is outside the table is not stored, and its q is 0.
+
+    Returns:
+        q rotated, contiguous; None without q.
+    """
+    out = _paged_cache_append(q, k, v, k_cache, v_cache, slots, rope, positions, interleaved)
+    return None if q is None else out
+
+
+def paged_cache_append_fp4(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, slots: torch.Tensor, rope: torch.Tensor | None = None,
+                           positions: torch.Tensor | None = None, interleaved: bool = False) -> torch.Tensor | None:
+    """paged_cache_append into 4-bit caches uint8 [pages, page_size, kv_heads, head_dim / 2 + head_dim / 32].
+
+    A block of 32 elements of k (rotated, in fp32) or v is rounded to 2^e times 4-bit floats, its largest
+    magnitude in [3.5, 7) 2^e: each element is off by 2^e at most.  In fp16 e is 13 at most, which cuts
+    magnitudes above 6 * 2^13 off.  A block with a NaN or an infinity becomes NaN."""
+    out = _paged_cache_append_fp4(q, k, v, k_cache, v_cache, slots, rope, positions, interleaved)
+    return None if q is None else out
+
+
+def paged_cache_read_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                         dtype: torch.dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    """The keys and values [T, kv_heads, head_dim] that slots of 4-bit caches hold, in fp16 or bf16; 0 for a
+    slot outside."""
+    return _paged_cache_read_fp4(k_cache, v_cache, slots, dtype)
 
 
 def paged_cache_copy(pool: torch.Tensor, src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
@@ -291,3 +391,32 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top_k: int):
     top_k is 0 to 32.
     """
     return _token_logprobs(logits, targets, top_k)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int | None = None, ended: torch.Tensor | None = None,
+                end_token: int = -1):
+    """The best continuations of each search's beams.
+
+    Beam k of search b, row b * beams + k of logits, continued by token v has the total
+    scores[b, k] + log softmax(logits row)[v]; the `width` best of a search (default: as many as it has
+    beams) are chosen, best first.  Equal totals stand by beam, then by logit, then by token; a total that
+    is NaN counts as -inf.  A beam that has ended goes on only as itself, with end_token and its score.
+
+    Args:
+        logits: [batch * beams, vocab] fp16, bf16 or fp32.
+        scores: fp32 [batch, beams], beams up to 32.
+        width: up to 32, with `ended` at most beams.
+        ended: bool [batch, beams].
+
+    Returns:
+        (scores fp32, rows int32, tokens int64), each [batch, width]: rows are those of logits that the new
+        beams continue.  With `ended` also which of them have ended, by their token or before.
+    """
+    out = _beam_select(logits, scores, width, ended, end_token)
+    return out[:3] if ended is None else out
+
+
+def beam_reorder(states: list[torch.Tensor], rows: torch.Tensor) -> list[torch.Tensor]:
+    """[s[rows] for s in states], of tensors of any dtype, in one launch for up to eight: rows is int32 of any
+    shape, taken flat; a row outside becomes zeros."""
+    return _beam_reorder(states, rows)

@@ -1,7 +1,7 @@
 """A paged key-value cache for the layers of a model, over the operators of pulsar_amd.ops.
 
 The pool holds keys and values of every layer as planes of one tensor, [2 * layers, pages,
-page_size, kv_heads, head_dim], so a page id names the same page in all of them and forking, copying
+page_size, kv_heads, head_dim] (with bits=4 bytes, the last dimension head_dim / 2 + head_dim / 32), so a page id names the same page in all of them and forking, copying
 and compacting are one call for the whole model.  The book-keeping -- reference counts, block tables,
 lengths -- is on the device and changes in place; the host keeps only an upper bound of each row's
 length, which sizes the attention's grid.  No method but `lengths` waits for the device.  Methods that
@@ -32,17 +32,26 @@ class Step:
     missing: torch.Tensor
     max_q_len: int
     max_seq_len: int
+    positions: torch.Tensor | None = None  # of the tokens, int64: PagedKVCache.positions
 
 
 class PagedKVCache:
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, rows: int,
-                 max_seq_len: int, dtype: torch.dtype = torch.bfloat16, device="cuda:0"):
+                 max_seq_len: int, dtype: torch.dtype = torch.bfloat16, device="cuda:0", bits: int = 16):
         if min(layers, pages, page_size, kv_heads, head_dim, rows, max_seq_len) <= 0:
             raise ValueError("PagedKVCache: every size must be positive")
         if dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"PagedKVCache: dtype must be fp16 or bf16, got {dtype}")
-        self.page_size, self.rows = page_size, rows
-        self.pool = torch.empty((2 * layers, pages, page_size, kv_heads, head_dim), dtype=dtype, device=device)
+        if bits not in (4, 16) or (bits == 4 and (head_dim % 32 or head_dim > 256)):
+            raise ValueError(f"PagedKVCache: bits must be 16, or 4 with head_dim a multiple of 32 up to 256, got {bits}")
+        self.page_size, self.rows, self.bits, self.dtype = page_size, rows, bits, dtype
+        if bits == 16:
+            self.pool = torch.empty((2 * layers, pages, page_size, kv_heads, head_dim), dtype=dtype, device=device)
+        else:
+            row = head_dim // 2 + head_dim // 32
+            size = page_size * kv_heads * row  # a page's; pages begin at multiples of 16
+            flat = torch.empty((2 * layers, pages, -(-size // 16) * 16), dtype=torch.uint8, device=device)
+            self.pool = flat[:, :, :size].unflatten(2, (page_size, kv_heads, row))
         ints = {"dtype": torch.int32, "device": device}
         self.ref_counts = torch.zeros(pages, **ints)
         self.block_tables = torch.full((rows, -(-max_seq_len // page_size)), -1, **ints)
@@ -50,7 +59,7 @@ class PagedKVCache:
         self._most = [0] * rows  # at most so many tokens in each row
 
     def layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values of a layer, [pages, page_size, kv_heads, head_dim]."""
+        """Keys and values of a layer, [pages, page_size, kv_heads, head_dim] (bytes with bits=4)."""
         return self.pool[2 * index], self.pool[2 * index + 1]
 
     def _ints(self, values: list[int]) -> torch.Tensor:
@@ -80,15 +89,38 @@ class PagedKVCache:
         self._most = self.seq_lens.tolist()
         return list(self._most)
 
+    def positions(self, step: Step) -> torch.Tensor:
+        """The positions of a step's tokens in their rows, int64 [T], made once a step."""
+        if step.positions is None:
+            n = step.cu_q[1:] - step.cu_q[:-1]
+            tokens = step.slots.shape[0]
+            row = torch.repeat_interleave(n, output_size=tokens)
+            # (a step that was refused has the positions it would have had, and no slots)
+            first = self.seq_lens - torch.where(step.missing == 0, n, 0) - step.cu_q[:-1]
+            step.positions = torch.arange(tokens, device=row.device) + first[row]
+        return step.positions
+
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """Stores the step's keys and values [T, kv_heads, head_dim] of a layer."""
-        ops.paged_cache_write(k, v, *self.layer(layer), step.slots)
+        if self.bits == 16:
+            ops.paged_cache_write(k, v, *self.layer(layer), step.slots)
+        else:
+            ops.paged_cache_append_fp4(None, k, v, *self.layer(layer), step.slots)
+
+    def append(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: Step, rope: torch.Tensor,
+               interleaved: bool = False) -> torch.Tensor:
+        """Rotates the step's queries and keys by their positions in their rows (ops.paged_cache_append's
+        rotation, `rope` of at least as many positions as a row has), stores the keys and values and returns
+        the queries.  The positions are taken when a step's first layer is appended: before the next step."""
+        append = ops.paged_cache_append if self.bits == 16 else ops.paged_cache_append_fp4
+        return append(q, k, v, *self.layer(layer), step.slots, rope, self.positions(step), interleaved)
 
     def attend(self, layer: int, q: torch.Tensor, step: Step, **options):
         """Attention of the step's queries [T, q_heads, head_dim] over their rows, with the options of
         ops.paged_attention."""
-        return ops.paged_attention(q, *self.layer(layer), self.block_tables, self.seq_lens, step.cu_q, step.max_q_len,
-                                   step.max_seq_len, **options)
+        attention = ops.paged_attention if self.bits == 16 else ops.paged_attention_fp4
+        return attention(q, *self.layer(layer), self.block_tables, self.seq_lens, step.cu_q, step.max_q_len,
+                         step.max_seq_len, **options)
 
     def _rows(self, rows: list[int], what: str) -> torch.Tensor:
         if any(not 0 <= r < self.rows for r in rows):
@@ -106,6 +138,24 @@ class PagedKVCache:
         missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens, src_rows, dst_rows)
         for s, d in zip(src, dst):
             self._most[d] = self._most[s]
+        return missing
+
+    def reorder(self, rows: torch.Tensor, live: list[int], spare: list[int]) -> torch.Tensor:
+        """Beams go on: row spare[i] becomes a copy of row live[rows[i]], rows being int32 on the device
+        (ops.beam_select's of one search), and the rows `live` are given back.  Returns the free pages that
+        lacked (int32 [1]), in which case nothing changed.  The rows `spare` are empty."""
+        if len(set(spare)) != len(spare) or set(live) & set(spare) or rows.numel() != len(spare):
+            raise ValueError("PagedKVCache.reorder: a spare row for each of rows, each once and not live")
+        if any(self._most[s] for s in spare):
+            raise ValueError("PagedKVCache.reorder: the spare rows must be empty")
+        from_rows, to_rows = self._rows(live, "reorder"), self._rows(spare, "reorder")
+        missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens,
+                                       ops.beam_reorder([from_rows], rows)[0], to_rows)
+        # nothing goes where nothing was copied: row -1 is none
+        ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, torch.where(missing == 0, from_rows, -1))
+        most = max((self._most[r] for r in live), default=0)
+        for r in spare:
+            self._most[r] = most
         return missing
 
     def free(self, rows: list[int]) -> None:
