@@ -5,9 +5,9 @@
 // and leave their largest logit, sum e^(x-m) and `width` best candidates.  The second launch has
 // a workgroup a search, whose waves join a beam's slices each: its log-sum-exp, the slices'
 // sums added in fp64, and its best candidates in order.  No beam gives more than `width` of the
-// new ones, so width times beams candidates are left, in lists that fall by total; a candidate's
-// place among all is its place in its own list and, by bisection, those ahead of it in the
-// others.  Totals are fp64: scores of some hundred tokens have fp32 steps of 1e-5, within which
+// new ones, so width times beams candidates are left, in lists that fall by total, which are
+// merged pair by pair: a candidate's place in the merged list is its own and, by bisection,
+// how many of the other list are ahead.  Totals are fp64: scores of some hundred tokens have fp32 steps of 1e-5, within which
 // beams would tie.
 #include "logit_slices.h"
 
@@ -48,58 +48,81 @@ __device__ __forceinline__ double join_lse(const SliceSums* sums, int slices) {
     return (double)m + log(z);
 }
 
-__global__ __launch_bounds__(kThreads) void select_kernel(const SelectArgs a) {
-    __shared__ uint64_t s_join[kThreads / 64][kJoin];
+// A list of candidates, best first: totals, and which candidate each is.
+struct Lists {
+    double total[kMaxBeams * kMaxTop];
+    int which[kMaxBeams * kMaxTop];
+    int length[kMaxBeams];
+};
+
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void select_kernel(const SelectArgs a) {
+    constexpr int JOIN = WAVES > 4 ? 128 : kJoin;
+    __shared__ uint64_t s_join[WAVES][JOIN];
     __shared__ uint64_t s_key[kMaxBeams * kMaxTop];
-    __shared__ double s_total[kMaxBeams * kMaxTop];
-    __shared__ int s_length[kMaxBeams];
+    __shared__ Lists s_lists[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row0 = blockIdx.x * a.beams, per = a.s.top_k;
-    for (int k = wave; k < a.beams; k += kThreads / 64) {
+    for (int k = wave; k < a.beams; k += WAVES) {
         const int row = row0 + k;
         const bool ended = a.s.passed != nullptr && a.s.passed[row] != 0;
         const double score = a.scores[row];
-        uint64_t* const keys = s_key + k * per;
-        double* const totals = s_total + k * per;
-        if (lane == 0) s_length[k] = ended ? 1 : per;
+        Lists& l = s_lists[0];
+        const int at = k * a.width;
+        if (lane == 0) l.length[k] = ended ? 1 : per;
         if (ended) {
-            if (lane == 0) totals[0] = score == score ? score : kLowest;
+            if (lane == 0) {
+                l.total[at] = score == score ? score : kLowest;
+                l.which[at] = at;
+            }
             continue;
         }
         const double lse = join_lse(a.s.sums + (int64_t)row * a.s.slices, a.s.slices);
-        join_tops(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, s_join[wave], [&](int place, uint64_t key) {
+        join_tops<JOIN>(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, s_join[wave], [&](int place, uint64_t key) {
             const double total = score + ((double)unordered((uint32_t)(key >> 32)) - lse);
-            keys[place] = key;
-            totals[place] = total == total ? total : kLowest;
+            s_key[at + place] = key;
+            l.total[at + place] = total == total ? total : kLowest;
+            l.which[at + place] = at + place;
         });
     }
-    __syncthreads();
-    for (int i = tid; i < a.beams * per; i += kThreads) {
-        const int k = i / per;
-        int place = i - k * per;
-        if (place >= s_length[k]) continue;
-        const double total = s_total[i];
-        for (int other = 0; other < a.beams && place < a.width; ++other) {
-            if (other == k) continue;
-            // how many of the other's list are ahead: greater, or equal and of a lower beam
-            int lo = 0, hi = s_length[other];
+    // Neighbouring lists become one, of `width` candidates at most, until one is left: a candidate's
+    // place there is its own and how many of the other list are ahead of it.
+    int from = 0;
+    for (int lists = a.beams; lists > 1; lists = (lists + 1) / 2, from ^= 1) {
+        const Lists& l = s_lists[from];
+        Lists& to = s_lists[from ^ 1];
+        __syncthreads();
+        for (int i = tid; i < lists * a.width; i += WAVES * 64) {
+            const int list = i / a.width, place = i - list * a.width, other = list ^ 1;
+            if (place >= l.length[list]) continue;
+            const double total = l.total[i];
+            int lo = 0, hi = other < lists ? l.length[other] : 0;
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                const double t = s_total[other * per + mid];
-                if (t > total || (t == total && other < k)) {
+                const double t = l.total[other * a.width + mid];
+                if (t > total || (t == total && other < list)) {
                     lo = mid + 1;
                 } else {
                     hi = mid;
                 }
             }
-            place += lo;
+            if (place + lo < a.width) {
+                const int dst = (list >> 1) * a.width + place + lo;
+                to.total[dst] = total;
+                to.which[dst] = l.which[i];
+            }
         }
-        if (place >= a.width) continue;
-        const int row = row0 + k;
+        for (int i = tid; i < (lists + 1) / 2; i += WAVES * 64) {
+            to.length[i] = min(a.width, l.length[2 * i] + (2 * i + 1 < lists ? l.length[2 * i + 1] : 0));
+        }
+    }
+    __syncthreads();
+    if (tid < min(a.width, s_lists[from].length[0])) {
+        const int which = s_lists[from].which[tid], row = row0 + which / a.width;
         const bool ended = a.s.passed != nullptr && a.s.passed[row] != 0;
-        const int64_t at = (int64_t)blockIdx.x * a.width + place;
-        const int64_t token = ended ? a.end_token : (int64_t)(uint32_t)~s_key[i];
-        a.out_scores[at] = (float)total;
+        const int64_t at = (int64_t)blockIdx.x * a.width + tid;
+        const int64_t token = ended ? a.end_token : (int64_t)(uint32_t)~s_key[which];
+        a.out_scores[at] = (float)s_lists[from].total[tid];
         a.out_rows[at] = row;
         a.out_tokens[at] = token;
         if (a.out_ended != nullptr) a.out_ended[at] = ended || token == a.end_token;
@@ -188,7 +211,12 @@ int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams,
     } else {
         run(std::integral_constant<int, PW4_DTYPE_F32>{});
     }
-    hipLaunchKernelGGL(select_kernel, dim3((unsigned)batch), dim3(kThreads), 0, s, a);
+    // a wave a beam, or two where there are more than 16
+    if (beams <= 4) {
+        hipLaunchKernelGGL(select_kernel<4>, dim3((unsigned)batch), dim3(4 * 64), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(select_kernel<16>, dim3((unsigned)batch), dim3(16 * 64), 0, s, a);
+    }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PW4_OK : report_hip_error(e);
 }

@@ -296,8 +296,8 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(const SliceArgs a) {
 }
 
 // A row's top_k keys from its slices', `tops` [slices, top_k]: store(place, key), by one wave.  `mine`
-// is kJoin keys of the wave's in LDS.
-template <typename F>
+// is JOIN keys of the wave's in LDS.
+template <int JOIN = kJoin, typename F>
 __device__ __forceinline__ void join_tops(const uint64_t* tops, int slices, int top_k, uint64_t* mine, F&& store) {
     const int lane = threadIdx.x & 63, keys = slices * top_k;
     // A number that the q-th greatest keys of at least top_k / q slices reach is a bound for the
@@ -316,10 +316,10 @@ __device__ __forceinline__ void join_tops(const uint64_t* tops, int slices, int 
         const bool reaches = key != 0 && (uint32_t)(key >> 32) >= bound;
         const uint64_t all = __ballot(reaches);
         const int at = count + __popcll(all & ((1ull << lane) - 1));
-        if (reaches && at < kJoin) mine[at] = key;
+        if (reaches && at < JOIN) mine[at] = key;
         count += __popcll(all);
     }
-    if (count <= kJoin) {
+    if (count <= JOIN) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         for (int i = lane; i < count; i += 64) {
             const uint64_t key = mine[i];

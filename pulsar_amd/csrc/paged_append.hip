@@ -2,17 +2,17 @@
 // rounded to the cache's 16 bits or to its blocks of 4; and what a 4-bit cache holds, read
 // back.  (The formulas and the pages' layout: pulsar_paged.h.)
 //
-// A workgroup has a token, a thread eight neighbouring elements of a head at a time: it loads
-// them and, of a rotated head, the eight that they are paired with (a cache line that other
-// threads of the wave load as well), and goes over the token's heads with its cosines and sines
-// in registers.  Pages and rows of the cache are a token's own, so their division is scalar.
+// A thread has sixteen elements of a head, eight and the eight that they are paired with, at a
+// number of the token's heads in turn, with the pairs' cosines and sines in registers; the next
+// head's elements are under way meanwhile.  What vectors of eight do not fit (odd rotations, odd
+// addresses) is done one element at a time by append_any_kernel.
 //
 // Rotations are fp64: the product of an element and an fp32 cosine is exact there, so the sum is
 // rounded once and a 4-bit cache's exponent and codes, which stand next to borders, do not depend
 // on the order of the operations.  fp64 vector instructions run at fp32's rate on this chip.
 //
-// Four threads hold a block of 32 elements; its largest magnitude takes two exchanges.  The
-// conversion instruction rounds to codes by the block's scale (to nearest, halves to even,
+// A block of 32 elements is four vectors of two to four threads of a wave; its largest magnitude
+// takes one or two exchanges.  The conversion instruction rounds to codes by the block's scale (to nearest, halves to even,
 // saturating), two elements each.
 #include "pulsar_paged.h"
 
@@ -46,6 +46,7 @@ struct AppendArgs {
     int64_t rope_rows;
     int32_t q_heads, kv_heads, dim, rot, page_size, interleaved;
     int32_t exp_limit;                                 // greatest exponent byte
+    int32_t tokens, abreast;                           // append_kernel: head groups of a token side by side
 };
 
 template <bool BF16>
@@ -57,34 +58,201 @@ __device__ __forceinline__ float widen16(uint16_t u) {
     }
 }
 
-// Eight elements from `from` on.  VEC: it is 16-byte aligned.
-template <bool VEC>
-__device__ __forceinline__ void load8(const uint16_t* from, uint16_t (&x)[8]) {
-    if constexpr (VEC) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(from);
+// The largest magnitude among fp32 elements, as its bits (a NaN or an infinity: 0x7f800000 or more).
+__device__ __forceinline__ uint32_t magnitude(const float (&x)[8]) {
+    uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (uint16_t)(w[e / 2] >> (e % 2 * 16));
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = from[e];
-    }
+    for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
+    return top;
 }
-template <bool VEC>
-__device__ __forceinline__ void store8(uint16_t* to, const uint16_t (&x)[8]) {
-    if constexpr (VEC) {
-        u32x4 w;
+// The exponent byte of a block whose largest magnitude is `top`: that magnitude's exponent, one more from
+// 1.75 of it on, less 2.
+__device__ __forceinline__ uint32_t exponent_of(uint32_t top, int limit) {
+    return top >= 0x7f800000u ? 255u : (uint32_t)min(max((int)((top + 0x200000u) >> 23) - 2, 0), limit);
+}
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[8], uint32_t exp) {
+    const float scale = __builtin_bit_cast(float, exp << 23);
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
+    return w;
+}
+__device__ __forceinline__ uint32_t other_lane(uint32_t v, int lane) { return (uint32_t)__shfl((int)v, lane); }
+
+// Where a token goes.
+struct Token {
+    bool known, stored;       // its position is in the table; and its slot in the pool
+    const float* table;       // its cosines and sines
+    uint32_t page, row;
+};
+__device__ __forceinline__ Token token_at(const AppendArgs& a, int token) {
+    Token t{true, false, nullptr, 0, 0};
+    const int64_t slot = a.slots[token];
+    t.stored = slot >= 0 && slot < a.places;
+    if (a.positions != nullptr) {
+        const int64_t p = a.positions[token];
+        t.known = p >= 0 && p < a.rope_rows;
+        if (t.known) t.table = a.rope + p * a.rot;
+        t.stored &= t.known;
+    }
+    if (t.stored) {
+        t.page = (uint32_t)slot / (uint32_t)a.page_size;
+        t.row = (uint32_t)slot - t.page * (uint32_t)a.page_size;
+    }
+    return t;
+}
+// Head h of a token's: q's first, then k's, then v's.
+struct Head {
+    bool is_q, is_v;
+    int at;
+    const uint16_t* from;
+    __device__ __forceinline__ Head(const AppendArgs& a, int token, int h) {
+        is_q = h < a.q_heads;
+        is_v = h >= a.q_heads + a.kv_heads;
+        at = is_q ? h : is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
+        const Heads& heads = is_q ? a.q : is_v ? a.v : a.k;
+        from = heads.from + token * heads.token + at * heads.head;
+    }
+};
+
+template <bool BF16>
+__device__ __forceinline__ void widen8(u32x4 w, float (&x)[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = x[2 * e] | (uint32_t)x[2 * e + 1] << 16;
-        *reinterpret_cast<u32x4*>(to) = w;
-    } else {
+    for (int e = 0; e < 8; ++e) x[e] = widen16<BF16>((uint16_t)(w[e / 2] >> (e % 2 * 16)));
+}
+template <bool BF16>
+__device__ __forceinline__ u32x4 round8(const float (&x)[8]) {
+    u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[e] = x[e];
+    for (int e = 0; e < 4; ++e) w[e] = f32_to_out<BF16>(x[2 * e]) | (uint32_t)f32_to_out<BF16>(x[2 * e + 1]) << 16;
+    return w;
+}
+
+// Everything 16-byte aligned, head_dim and rot multiples of 16.  A wave is 64 / U rows of U = dim / 16
+// lanes; a row of lanes goes over heads first, first + abreast, ... of its token, its lane u having
+// elements 8 u .. + 7 and their mates rot / 2 further on, or (PAIRS, values, and what is not rotated)
+// 16 u .. + 15.
+template <bool BF16, bool FP4, bool PAIRS>
+__global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
+    const int lane = threadIdx.x & 63, units = a.dim / 16, in_wave = 64 / units;
+    const int r = lane / units, u = lane - r * units, row0 = lane - u;
+    const int group = ((int)threadIdx.x >> 6) * in_wave + r, side = group / a.abreast;
+    const int at_once = kThreads / 64 * in_wave / a.abreast;  // tokens
+    const int token = (int)blockIdx.x * at_once + side;
+    if (r >= in_wave || side >= at_once || token >= a.tokens) return;
+    const int heads = a.q_heads + 2 * a.kv_heads, step = a.abreast * (int)gridDim.y;
+    int h = group - side * a.abreast + (int)blockIdx.y * a.abreast;
+    if (h >= heads) return;
+    const int half = a.rot / 2;
+    const bool turns = a.positions != nullptr && 16 * u < a.rot, split = !PAIRS && turns;
+    const int d0 = split ? 8 * u : 16 * u, d1 = split ? half + 8 * u : 16 * u + 8;
+    const auto load = [&](int head, u32x4 (&w)[2]) {
+        const Head x(a, token, head);
+        w[0] = *reinterpret_cast<const u32x4*>(x.from + (x.is_v ? 16 * u : d0));
+        w[1] = *reinterpret_cast<const u32x4*>(x.from + (x.is_v ? 16 * u + 8 : d1));
+    };
+    u32x4 next[2];
+    load(h, next);
+    const Token t = token_at(a, token);
+    double c[8], s[8];
+    if (turns && t.known) {
+        float cf[8], sf[8];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {  // (a row of the table is only 4-byte aligned where rot is)
+            *reinterpret_cast<f32x4*>(cf + e) = *reinterpret_cast<const f32x4*>(t.table + 8 * u + e);
+            *reinterpret_cast<f32x4*>(sf + e) = *reinterpret_cast<const f32x4*>(t.table + half + 8 * u + e);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            c[e] = cf[e];
+            s[e] = sf[e];
+        }
+    }
+    // the lanes and halves that hold the neighbours of the lane's two vectors in a block of 32
+    int near0[2], near1[2];      // by 8 elements and by 16: lane
+    bool late0[2], late1[2];     // whether it is that lane's second vector
+    if (FP4 && !PAIRS) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const auto owner = [&](int d, int& where, bool& late) {
+                const bool turned = a.positions != nullptr && d < a.rot;
+                late = turned ? d >= half : d % 16 != 0;
+                where = row0 + (turned ? (d - (late ? half : 0)) / 8 : d / 16);
+            };
+            owner(d0 ^ (8 << i), near0[i], late0[i]);
+            owner(d1 ^ (8 << i), near1[i], late1[i]);
+        }
+    }
+    while (true) {
+        const u32x4 w[2] = {next[0], next[1]};
+        const Head x(a, token, h);
+        const bool more = h + step < heads;
+        if (more) load(h + step, next);
+        const bool turned = turns && t.known && !x.is_v;
+        float x0[8], x1[8];
+        if (turned || (FP4 && !x.is_q)) {
+            widen8<BF16>(w[0], x0);
+            widen8<BF16>(w[1], x1);
+        }
+        if (turned) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float& fa = PAIRS ? (e < 4 ? x0 : x1)[e % 4 * 2] : x0[e];
+                float& fb = PAIRS ? (e < 4 ? x0 : x1)[e % 4 * 2 + 1] : x1[e];
+                const double da = fa, db = fb;
+                fa = (float)__builtin_fma(da, c[e], -(db * s[e]));
+                fb = (float)__builtin_fma(db, c[e], da * s[e]);
+            }
+        }
+        if (x.is_q || (!FP4 && t.stored)) {
+            u32x4 out0 = w[0], out1 = w[1];
+            if (turned) {
+                out0 = round8<BF16>(x0);
+                out1 = round8<BF16>(x1);
+            } else if (!t.known) {
+                out0 = out1 = u32x4{0, 0, 0, 0};
+            }
+            const int64_t in_cache = t.page * a.page_bytes + t.row * a.row_bytes + x.at * a.head_bytes;
+            uint16_t* const to = x.is_q ? a.q_out + ((int64_t)token * a.q_heads + x.at) * a.dim
+                                        : reinterpret_cast<uint16_t*>((x.is_v ? a.v_cache : a.k_cache) + in_cache);
+            *reinterpret_cast<u32x4*>(to + (x.is_v ? 16 * u : d0)) = out0;
+            *reinterpret_cast<u32x4*>(to + (x.is_v ? 16 * u + 8 : d1)) = out1;
+        } else if (FP4 && t.stored) {
+            uint32_t m0 = magnitude(x0), m1 = magnitude(x1);
+            if (PAIRS || x.is_v || a.positions == nullptr) {  // (a row's lanes agree)
+                m0 = max(m0, m1);
+                m0 = m1 = max(m0, other_lane(m0, lane ^ 1));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t a0 = other_lane(m0, near0[i]), a1 = other_lane(m1, near0[i]);
+                    const uint32_t b0 = other_lane(m0, near1[i]), b1 = other_lane(m1, near1[i]);
+                    m0 = max(m0, late0[i] ? a1 : a0);
+                    m1 = max(m1, late1[i] ? b1 : b0);
+                }
+            }
+            const int at0 = x.is_v ? 16 * u : d0, at1 = x.is_v ? 16 * u + 8 : d1;
+            const uint32_t e0 = exponent_of(m0, a.exp_limit), e1 = exponent_of(m1, a.exp_limit);
+            uint8_t* const to = (x.is_v ? a.v_cache : a.k_cache) + t.page * a.page_bytes;
+            const uint32_t place = x.at * a.page_size + t.row;
+            uint8_t* const codes = to + place * a.row_codes;
+            uint8_t* const exps = to + a.exps_at + place * a.row_exps;
+            *reinterpret_cast<uint32_t*>(codes + at0 / 2) = to_codes(x0, e0);
+            *reinterpret_cast<uint32_t*>(codes + at1 / 2) = to_codes(x1, e1);
+            if (at0 % 32 == 0) exps[at0 / 32] = (uint8_t)e0;
+            if (at1 % 32 == 0) exps[at1 / 32] = (uint8_t)e1;
+        }
+        if (!more) return;
+        h += step;
     }
 }
 
-// What a thread's eight elements, from element d0 of a head on, are rotated by: element e becomes
+// ---- one element at a time -------------------------------------------------------
+
+// What eight neighbouring elements, from element d0 of a head on, are rotated by: element e becomes
 // own * c[e] + mate * s[e], its mate being element mate(e) of the head.
-template <bool VEC>
 struct Turn {
     float c[8], s[8];
     int d0, rot, half;
@@ -107,107 +275,60 @@ struct Turn {
         if (d >= rot) return d;
         return pairs ? d ^ 1 : d < half ? d + half : d - half;
     }
-    // The rotated elements of a head, rounded to fp32.  VEC: the mates of eight lie side by side,
-    // and so do their cosines.
+    // The rotated elements of a head, rounded to fp32.
     template <bool BF16>
-    __device__ __forceinline__ void apply(const uint16_t* head, const uint16_t (&own)[8], float (&out)[8]) const {
-        uint16_t other[8];
-        if (VEC && !pairs) {
-            load8<true>(head + mate(0), other);
-        } else if (VEC) {
+    __device__ __forceinline__ void apply(const uint16_t* head, float (&x)[8]) const {
+        float other[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) other[e] = own[e ^ 1];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) other[e] = head[mate(e)];
-        }
+        for (int e = 0; e < 8; ++e) other[e] = widen16<BF16>(head[mate(e)]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = widen16<BF16>(own[e]);
-            const double turned = __builtin_fma((double)x, (double)c[e], (double)widen16<BF16>(other[e]) * (double)s[e]);
-            out[e] = VEC || d0 + e < rot ? (float)turned : x;
+            const double turned = __builtin_fma((double)x[e], (double)c[e], (double)other[e] * (double)s[e]);
+            x[e] = d0 + e < rot ? (float)turned : x[e];
         }
     }
 };
 
-// Eight fp32 elements of a block that this thread and the three beside it hold, to codes; the block's
-// exponent byte goes to the first of the four's `exp`.
-__device__ __forceinline__ uint32_t to_codes(const float (&x)[8], int limit, uint32_t& exp) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    // the exponent of the largest magnitude, one more from 1.75 of it on, less 2
-    exp = top >= 0x7f800000u ? 255u : (uint32_t)min(max((int)((top + 0x200000u) >> 23) - 2, 0), limit);
-    const float scale = __builtin_bit_cast(float, exp << 23);
-    uint32_t w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], scale, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], scale, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], scale, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], scale, 3);
-    return w;
-}
-
-// Token blockIdx.x; of its heads (q's, k's, v's) blockIdx.y's share.
-template <bool BF16, bool VEC, bool FP4>
-__global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
+// Token blockIdx.x; of its heads blockIdx.y's share.  A thread has eight neighbouring elements of a head;
+// four threads have a block of 32.
+template <bool BF16, bool FP4>
+__global__ __launch_bounds__(kThreads) void append_any_kernel(const AppendArgs a) {
     const int token = blockIdx.x;
     const int units = a.dim / 8, at_once = kThreads / units;
     const int first = threadIdx.x / units, d0 = (threadIdx.x - first * units) * 8;
     if (first >= at_once) return;
-    const int64_t slot = a.slots[token];
-    bool stored = slot >= 0 && slot < a.places, known = true;
-    const float* table = nullptr;
-    if (a.positions != nullptr) {
-        const int64_t p = a.positions[token];
-        known = p >= 0 && p < a.rope_rows;
-        if (known) table = a.rope + p * a.rot;
-        stored &= known;
-    }
-    const uint32_t page = stored ? (uint32_t)slot / (uint32_t)a.page_size : 0;
-    const uint32_t row = stored ? (uint32_t)slot - page * (uint32_t)a.page_size : 0;
-    const Turn<VEC> turn(a, table, d0);
+    const Token t = token_at(a, token);
+    const Turn turn(a, t.table, d0);
     const int heads = a.q_heads + 2 * a.kv_heads;
     for (int h = first + blockIdx.y * at_once; h < heads; h += at_once * gridDim.y) {
-        const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv_heads;
-        if (!is_q && !stored) continue;
-        const int at = is_q ? h : is_v ? h - a.q_heads - a.kv_heads : h - a.q_heads;
-        const Heads& from = is_q ? a.q : is_v ? a.v : a.k;
-        const uint16_t* const head = from.from + token * from.token + at * from.head;
+        const Head x(a, token, h);
+        if (!x.is_q && !t.stored) continue;
         uint16_t own[8];
-        float x[8];
-        load8<VEC>(head + d0, own);
-        const bool turns = turn.any && !is_v;
-        if (turns) {
-            turn.template apply<BF16>(head, own, x);
-        } else if (FP4) {
+        float f[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = widen16<BF16>(own[e]);
-        }
-        if (FP4 && !is_q) {
-            uint32_t exp;
-            const uint32_t codes = to_codes(x, a.exp_limit, exp);
-            uint8_t* const to = (is_v ? a.v_cache : a.k_cache) + page * a.page_bytes;
-            const uint32_t place = at * a.page_size + row;
-            *reinterpret_cast<uint32_t*>(to + place * a.row_codes + d0 / 2) = codes;
+        for (int e = 0; e < 8; ++e) own[e] = x.from[d0 + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = widen16<BF16>(own[e]);
+        const bool turns = turn.any && !x.is_v;
+        if (turns) turn.template apply<BF16>(x.from, f);
+        if (FP4 && !x.is_q) {
+            uint32_t top = magnitude(f);
+            top = max(top, other_lane(top, (threadIdx.x & 63) ^ 1));
+            top = max(top, other_lane(top, (threadIdx.x & 63) ^ 2));
+            const uint32_t exp = exponent_of(top, a.exp_limit);
+            uint8_t* const to = (x.is_v ? a.v_cache : a.k_cache) + t.page * a.page_bytes;
+            const uint32_t place = x.at * a.page_size + t.row;
+            *reinterpret_cast<uint32_t*>(to + place * a.row_codes + d0 / 2) = to_codes(f, exp);
             if (d0 % 32 == 0) to[a.exps_at + place * a.row_exps + d0 / 32] = (uint8_t)exp;
             continue;
         }
-        if (turns) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) own[e] = f32_to_out<BF16>(x[e]);
+        uint16_t* to = a.q_out + ((int64_t)token * a.q_heads + x.at) * a.dim;
+        if (!x.is_q) {
+            to = reinterpret_cast<uint16_t*>((x.is_v ? a.v_cache : a.k_cache) + t.page * a.page_bytes + t.row * a.row_bytes +
+                                             x.at * a.head_bytes);
         }
-        if (is_q) {
-            if (!known) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) own[e] = 0;
-            }
-            store8<true>(a.q_out + ((int64_t)token * a.q_heads + at) * a.dim + d0, own);
-        } else {
-            uint8_t* const to = (is_v ? a.v_cache : a.k_cache) + page * a.page_bytes + row * a.row_bytes + at * a.head_bytes;
-            store8<VEC>(reinterpret_cast<uint16_t*>(to) + d0, own);
-        }
+        for (int e = 0; e < 8; ++e) to[d0 + e] = !t.known ? 0 : turns ? f32_to_out<BF16>(f[e]) : own[e];
     }
 }
 
@@ -222,7 +343,7 @@ struct ReadArgs {
     int32_t kv_heads, dim, page_size;
 };
 
-// Token blockIdx.x: its keys' and values' words of eight codes.
+// A token's keys' and values' words of eight codes.
 template <bool BF16>
 __global__ __launch_bounds__(kThreads) void read_kernel(const ReadArgs a) {
     const int token = blockIdx.x, units = a.dim / 8, items = 2 * a.kv_heads * units;
@@ -298,8 +419,9 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
     const uint64_t strides = (q ? (uint64_t)(a->q_token_stride | a->q_head_stride) : 0) |
                              (uint64_t)(a->k_token_stride | a->k_head_stride | a->v_token_stride | a->v_head_stride) | cache_strides;
     if (addresses & 1) return PW4_ERR_ARG;
-    // vectors of eight: everything aligned, and the mates of eight elements side by side
-    const bool vec = (addresses & 15) == 0 && (strides & 7) == 0 && (!turns || a->rot % (a->interleaved ? 8 : 16) == 0);
+    // vectors of eight: everything aligned, and whole vectors rotated or not
+    const bool vec = (addresses & 15) == 0 && (strides & 7) == 0 && a->head_dim % 16 == 0 &&
+                     (!turns || (a->rot % 16 == 0 && (uintptr_t)a->rope % 16 == 0));
     AppendArgs p{};
     p.q = Heads{static_cast<const uint16_t*>(a->q), a->q_token_stride, a->q_head_stride};
     p.k = Heads{static_cast<const uint16_t*>(a->k), a->k_token_stride, a->k_head_stride};
@@ -325,21 +447,31 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
     p.page_size = (int32_t)a->page_size;
     p.interleaved = a->interleaved != 0;
     p.exp_limit = a->dtype == PW4_DTYPE_F16 ? 127 + 13 : 254;
-    const int64_t passes = ceil_div(heads, kThreads / (a->head_dim / 8));
-    // few tokens: a workgroup a pass over the heads; many: one goes over them all
-    const int64_t shares = a->num_tokens * passes <= 8 * device_cus() ? passes : 1;
-    const dim3 grid((unsigned)a->num_tokens, (unsigned)std::min<int64_t>(shares, 65535));
+    p.tokens = (int32_t)a->num_tokens;
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    auto run = [&](auto bf16, auto wide) {
-        constexpr bool BF16 = decltype(bf16)::value, VEC = decltype(wide)::value;
-        if (fp4) {
-            hipLaunchKernelGGL((append_kernel<BF16, VEC, true>), grid, dim3(kThreads), 0, s, p);
+    const auto run = [&](auto bf16, auto four) {
+        constexpr bool BF16 = decltype(bf16)::value, FP4 = decltype(four)::value;
+        if (!vec) {
+            const int64_t passes = ceil_div(heads, kThreads / (a->head_dim / 8));
+            const int64_t shares = a->num_tokens * passes <= 8 * device_cus() ? passes : 1;
+            hipLaunchKernelGGL((append_any_kernel<BF16, FP4>), dim3((unsigned)a->num_tokens, (unsigned)shares), dim3(kThreads), 0,
+                               s, p);
+            return;
+        }
+        // Rows of lanes of a workgroup, and how many of them share a token: all, each with a head, where
+        // tokens are few; else 8, so that a row's cosines serve several heads.
+        const int64_t rows = kThreads / 64 * (64 / (a->head_dim / 16));
+        const bool few = a->num_tokens * heads <= 8 * device_cus() * rows;
+        p.abreast = (int32_t)std::min<int64_t>(few ? rows : std::min<int64_t>(8, rows), heads);
+        const dim3 grid((unsigned)ceil_div(a->num_tokens, rows / p.abreast), (unsigned)(few ? ceil_div(heads, p.abreast) : 1));
+        if (p.interleaved || !turns) {
+            hipLaunchKernelGGL((append_kernel<BF16, FP4, true>), grid, dim3(kThreads), 0, s, p);
         } else {
-            hipLaunchKernelGGL((append_kernel<BF16, VEC, false>), grid, dim3(kThreads), 0, s, p);
+            hipLaunchKernelGGL((append_kernel<BF16, FP4, false>), grid, dim3(kThreads), 0, s, p);
         }
     };
-    const auto with_vec = [&](auto bf16) { vec ? run(bf16, std::true_type{}) : run(bf16, std::false_type{}); };
-    a->dtype == PW4_DTYPE_BF16 ? with_vec(std::true_type{}) : with_vec(std::false_type{});
+    const auto with_bits = [&](auto bf16) { fp4 ? run(bf16, std::true_type{}) : run(bf16, std::false_type{}); };
+    a->dtype == PW4_DTYPE_BF16 ? with_bits(std::true_type{}) : with_bits(std::false_type{});
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PW4_OK : report_hip_error(e);
 }
