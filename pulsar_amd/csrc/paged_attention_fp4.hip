@@ -22,6 +22,7 @@ struct Fp4Params : Params {
     uint32_t row_codes, row_exps;    // bytes of a token's codes, and of its exponents
     uint32_t head_codes, head_exps;  // of a page's of one head
     uint32_t exps_at;                // where a page's exponents begin
+    int32_t flat;                    // pages hold whole runs of 16 keys
 };
 
 // The cache's elements one at a time, as the products take them.
@@ -80,11 +81,6 @@ struct Lane {
     }
 };
 
-// The lane's key's page id.
-__device__ __forceinline__ uint32_t page_of(const Fp4Params& a, const Source& s, int key) {
-    return s.table[page_index(a, clamp_key(s, key))];
-}
-
 template <int DP>
 __device__ __forceinline__ void load_quarter(const uint8_t* codes, const uint8_t* exps, const Lane<DP>& l, Quarter<DP>& q) {
     if constexpr (DP == 64) {
@@ -103,20 +99,46 @@ __device__ __forceinline__ void load_quarter(const uint8_t* codes, const uint8_t
     for (int h = 0; h < Quarter<DP>::kExps; ++h) q.exps[h] = exps[l.exps[h]];
 }
 
-// Both planes' quarters of the lane's key, on page `id`.
-struct Place {
-    uint64_t page;
-    uint32_t codes, exps;
-};
-__device__ __forceinline__ Place place_of(const Fp4Params& a, const Source& s, int key, uint32_t id) {
-    key = clamp_key(s, key);
-    const uint32_t row = key - page_index(a, key) * a.page_size;
-    return Place{(uint64_t)min(id, s.pages1) * a.page_bytes, s.codes + row * a.row_codes, s.exps + row * a.row_exps};
-}
+// The lane's quarters of K and V of key c of 16 that begin with `first`, `id` being its page.  Where the
+// 16 lie in one page and all are seen, the row they begin with is uniform.
 template <int DP>
-__device__ __forceinline__ void load_plane(const uint8_t* plane, const Place& p, const Lane<DP>& l, Quarter<DP>& q) {
-    load_quarter<DP>(plane + p.page + p.codes, plane + p.page + p.exps, l, q);
-}
+struct Loader {
+    Lane<DP> lane;
+    Lane<DP> rows;  // with row c of 16 ahead
+    int c;
+    __device__ __forceinline__ explicit Loader(const Fp4Params& a) : lane(a), rows(a), c(threadIdx.x & 15) {
+#pragma unroll
+        for (int h = 0; h < Quarter<DP>::kExps; ++h) {
+            rows.codes[h] += c * a.row_codes;
+            rows.exps[h] += c * a.row_exps;
+        }
+    }
+    __device__ __forceinline__ uint32_t page(const Fp4Params& a, const Source& s, int first) const {
+        return s.table[page_index(a, clamp_key(s, first + c))];
+    }
+    __device__ __forceinline__ bool in_one_page(const Fp4Params& a, const Source& s, int first) const {
+        return a.flat && first >= s.lo && first + 15 <= s.last;
+    }
+    template <bool K, bool V>
+    __device__ __forceinline__ void load(const Fp4Params& a, const Source& s, int first, uint32_t id, Quarter<DP>& k,
+                                         Quarter<DP>& v) const {
+        if (in_one_page(a, s, first)) {
+            const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(id), s.pages1);
+            const uint32_t row = first - page_index(a, first) * a.page_size;
+            const uint64_t codes = (uint64_t)page * a.page_bytes + (s.codes + row * a.row_codes);
+            const uint64_t exps = (uint64_t)page * a.page_bytes + (s.exps + row * a.row_exps);
+            if (K) load_quarter<DP>(s.k + codes, s.k + exps, rows, k);
+            if (V) load_quarter<DP>(s.v + codes, s.v + exps, rows, v);
+        } else {
+            const int key = clamp_key(s, first + c);
+            const uint32_t row = key - page_index(a, key) * a.page_size;
+            const uint64_t page = (uint64_t)min(id, s.pages1) * a.page_bytes;
+            const uint64_t codes = page + (s.codes + row * a.row_codes), exps = page + (s.exps + row * a.row_exps);
+            if (K) load_quarter<DP>(s.k + codes, s.k + exps, lane, k);
+            if (V) load_quarter<DP>(s.v + codes, s.v + exps, lane, v);
+        }
+    }
+};
 
 // 16-bit elements of a quarter: word i becomes elements 8 i .. 8 i + 7.
 template <bool BF16, int DP>
@@ -150,7 +172,8 @@ __device__ __forceinline__ void store_quarter(uint8_t* stage, int r, int swizzle
 // ---- few rows --------------------------------------------------------------------
 
 // Up to 16 MT query rows.  Each wave takes blocks of 32 keys of its own: K straight from registers,
-// V through 32 rows of LDS of its own (no barrier); the next block's codes are under way meanwhile.
+// V through 32 rows of LDS of its own (no barrier); the next block's codes are under way during the
+// softmax and the second product.
 constexpr int kFewKeys = 32;
 template <int DP>
 constexpr int kFewWaves = DP == 256 ? 2 : 4;
@@ -165,8 +188,13 @@ constexpr int few_stage_bytes() {
     return stages > join ? stages : join;
 }
 
+// Waves on a SIMD that a kernel's registers are held to.
+template <int DP, int MT>
+constexpr int kFewOccupancy = DP == 256 ? 1 : DP == 128 ? MT == 1 ? 3 : 2 : MT == 1 ? 4 : 2;
+
 template <bool BF16, int DP, int MT, bool CAP>
-__global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const Fp4Params a) {
+__global__ __launch_bounds__(kFewWaves<DP> * 64) __attribute__((amdgpu_waves_per_eu(kFewOccupancy<DP, MT>)))
+void fp4_few_rows_kernel(const Fp4Params a) {
     constexpr int WAVES = kFewWaves<DP>, MR = 16 * MT, UNIT = kFewUnit<DP>;
     constexpr int KS = DP / 32;       // steps of 32 head elements
     constexpr int DT = DP / 16;       // tiles of 16 output elements
@@ -175,7 +203,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
     const int c = lane & 15, g = lane >> 4;
     Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
     uint8_t* const stage = smem + wave * kFewStage<DP>;
-    const Lane<DP> at(a);
+    const Loader<DP> from(a);
     const float k = unit<CAP>(a);
 
     Pieces<MR, kFewKeys, UNIT, WAVES, true> piece;
@@ -191,15 +219,13 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
         uint32_t ids[2] = {0, 0};  // of the next block's keys c and 16 + c
         auto pages = [&](int i) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) ids[kt] = page_of(a, src, first_of(i) + kt * 16 + c);
+            for (int kt = 0; kt < 2; ++kt) ids[kt] = from.page(a, src, first_of(i) + kt * 16);
         };
-        Quarter<DP> kq[2][2], vq[2][2];
-        auto load = [&](int i, int set, uint32_t id0, uint32_t id1) {
+        Quarter<DP> kq[2], vq[2];
+        auto load = [&](int i, uint32_t id0, uint32_t id1) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                const Place p = place_of(a, src, first_of(i) + kt * 16 + c, kt ? id1 : id0);
-                load_plane<DP>(src.k, p, at, kq[set][kt]);
-                load_plane<DP>(src.v, p, at, vq[set][kt]);
+                from.template load<true, true>(a, src, first_of(i) + kt * 16, kt ? id1 : id0, kq[kt], vq[kt]);
             }
         };
         if (mine > 0) pages(0);
@@ -230,17 +256,10 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
             for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (mine > 0) {
-            load(0, 0, ids[0], ids[1]);
+            load(0, ids[0], ids[1]);
             if (mine > 1) pages(1);
         }
-        auto block = [&](int i, int set) {
-            // the ids of block i + 2 ahead of the codes of block i + 1: loads return in order
-            if (i + 1 < mine) {
-                const uint32_t id0 = ids[0], id1 = ids[1];
-                if (i + 2 < mine) pages(i + 2);
-                load(i + 1, set ^ 1, id0, id1);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < mine; ++i) {
             const int key0 = first_of(i);
             f32x4 s[MT][2];
 #pragma unroll
@@ -249,7 +268,7 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
                 for (int mt = 0; mt < MT; ++mt) s[mt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
-                    const u32x4 kf = widen<BF16, DP>(at, kq[set][kt], st);
+                    const u32x4 kf = widen<BF16, DP>(from.lane, kq[kt], st);
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, q[mt][st], s[mt][kt]);
                 }
@@ -257,8 +276,14 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 const int r = kt * 16 + c;
-                store_quarter<BF16, DP>(stage, r, v_swizzle<DP, false>(r), at, vq[set][kt]);
+                store_quarter<BF16, DP>(stage, r, v_swizzle<DP, false>(r), from.lane, vq[kt]);
             }
+            if (i + 1 < mine) {  // the ids of the block after next ahead of the next one's codes: loads return in order
+                const uint32_t id0 = ids[0], id1 = ids[1];
+                if (i + 2 < mine) pages(i + 2);
+                load(i + 1, id0, id1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");  // a wave's LDS operations stay in this order
             const bool masked = key0 < all_lo || key0 + kFewKeys > all_hi;
             u32x4 p[MT];
@@ -307,10 +332,6 @@ __global__ __launch_bounds__(kFewWaves<DP> * 64) void fp4_few_rows_kernel(const 
                 for (int mt = 0; mt < MT; ++mt) o[mt][d] = mfma16x16x32<BF16>(vf, p[mt], o[mt][d]);
             }
             asm volatile("" ::: "memory");
-        };
-        for (int i = 0; i < mine; i += 2) {
-            block(i, 0);
-            if (i + 1 < mine) block(i + 1, 1);
         }
         __syncthreads();  // every wave is done with its stage
         join_waves<Fp4Keys, BF16, DP, MT, WAVES, CAP>(a, t, smem, wave, head, slot, begin, end, k, m, z, o);
@@ -342,7 +363,7 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
     Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
-    const Lane<DP> at(a);
+    const Loader<DP> from(a);
     const int copied = wave * COPY + (lane & 15);  // the lane's key of a block
     const float k = unit<CAP>(a);
     // LDS places of the lane's operands in a stage: K's unit 2 st + h of row c lies st << 5 (in
@@ -372,16 +393,12 @@ void fp4_many_rows_kernel(const Fp4Params a) {
         float m = -kInf, z = 0.f;
         uint32_t id = 0;  // the page of the lane's key of the block that is loaded next
         Quarter<DP> kq, vq;
-        auto page = [&](int i) { return page_of(a, src, begin + i * KEYS + copied); };
-        auto load = [&](int i) {
-            const Place p = place_of(a, src, begin + i * KEYS + copied, id);
-            load_plane<DP>(src.k, p, at, kq);
-            load_plane<DP>(src.v, p, at, vq);
-        };
+        auto page = [&](int i) { return from.page(a, src, begin + i * KEYS + wave * COPY); };
+        auto load = [&](int i) { from.template load<true, true>(a, src, begin + i * KEYS + wave * COPY, id, kq, vq); };
         auto store = [&](int i) {
             uint8_t* const to = smem + (i & 1) * kManyStage<DP>;
-            store_quarter<BF16, DP>(to, copied, k_swizzle<DP>(copied), at, kq);
-            store_quarter<BF16, DP>(to + kManyStage<DP> / 2, copied, v_swizzle<DP, true>(copied), at, vq);
+            store_quarter<BF16, DP>(to, copied, k_swizzle<DP>(copied), from.lane, kq);
+            store_quarter<BF16, DP>(to + kManyStage<DP> / 2, copied, v_swizzle<DP, true>(copied), from.lane, vq);
         };
         if (blocks > 0) {
             id = page(0);
@@ -507,6 +524,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.head_codes = (uint32_t)a->page_size * p.row_codes;
     p.head_exps = (uint32_t)a->page_size * p.row_exps;
     p.exps_at = (uint32_t)a->kv_heads * p.head_codes;
+    p.flat = a->page_size % 16 == 0;
     const int64_t rows = (int64_t)p.max_q * p.group;
     c.dp = padded_dim(a->head_dim);
     const int cus = device_cus();
@@ -518,7 +536,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
     c.tiles = few ? p.batch : tiles_of(c.tile_rows);
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     // workgroups that run at once
-    const int slots = few ? 3 * cus : c.dp != 256 ? 2 * cus : cus;
+    const int slots = few ? (c.dp == 256 ? 2 : c.tile_rows == 32 ? 2 : c.dp == 128 ? 3 : 4) * cus : c.dp != 256 ? 2 * cus : cus;
     // units of a tile: of the keys that a window leaves its rows, or all
     const int64_t most_keys =
         p.window == 0 ? p.max_len
