@@ -32,7 +32,7 @@ namespace {
 
 // The cache's elements one at a time.
 struct HalfKeys {
-    static constexpr bool kRepeats = true;
+    static constexpr bool kRepeats = true, kFresh = false;
     template <bool BF16>
     static __device__ __forceinline__ float element(const Params& a, const uint16_t* plane, int head, uint32_t page,
                                                     uint32_t row, int d) {
@@ -733,13 +733,13 @@ template <bool BF16, int DP, bool CAP>
 hipError_t launch(const Call& c, hipStream_t s) {
     hipError_t e;
     if (c.tile_rows == 16) {
-        e = run_attention<few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), s);
+        e = run_attention<few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), c.p.split ? (int)sizeof(Plan) : 0, s);
     } else if (c.tile_rows == 32) {
-        e = run_attention<few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), s);
+        e = run_attention<few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.p.split ? (int)sizeof(Plan) : 0, s);
     } else if (c.tile_rows == kManyRows) {
-        e = run_attention<many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), s);
+        e = run_attention<many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.p.split ? (int)sizeof(Plan) : 0, s);
     } else if constexpr (DP < 256) {
-        e = run_attention<wide_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kWideWaves, wide_stage_bytes<DP>(), s);
+        e = run_attention<wide_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kWideWaves, wide_stage_bytes<DP>(), c.p.split ? (int)sizeof(Plan) : 0, s);
     } else {
         e = hipErrorInvalidValue;  // no such tile: plan_call
     }

@@ -14,6 +14,8 @@
 // tile sees is clamped to one that is seen, as there.
 #include "paged_attention_parts.h"
 
+#include <type_traits>
+
 using namespace pw4;
 
 namespace {
@@ -27,7 +29,7 @@ struct Fp4Params : Params {
 
 // The cache's elements one at a time, as the products take them.
 struct Fp4Keys {
-    static constexpr bool kRepeats = false;
+    static constexpr bool kRepeats = false, kFresh = true;
     template <bool BF16>
     static __device__ __forceinline__ float element(const Fp4Params& a, const uint16_t* plane, int head, uint32_t page,
                                                     uint32_t row, int d) {
@@ -69,8 +71,7 @@ template <int DP>
 struct Lane {
     uint32_t codes[Quarter<DP>::kExps], exps[Quarter<DP>::kExps];
     bool there[Quarter<DP>::kExps];
-    __device__ __forceinline__ explicit Lane(const Fp4Params& a) {
-        const int g = (threadIdx.x & 63) >> 4;
+    __device__ __forceinline__ Lane(const Fp4Params& a, int g) {
 #pragma unroll
         for (int h = 0; h < Quarter<DP>::kExps; ++h) {
             const int first = g * (DP / 4) + h * 32;  // element
@@ -106,7 +107,7 @@ struct Loader {
     Lane<DP> lane;
     Lane<DP> rows;  // with row c of 16 ahead
     int c;
-    __device__ __forceinline__ explicit Loader(const Fp4Params& a) : lane(a), rows(a), c(threadIdx.x & 15) {
+    __device__ __forceinline__ Loader(const Fp4Params& a, int l) : lane(a, l >> 4), rows(a, l >> 4), c(l & 15) {
 #pragma unroll
         for (int h = 0; h < Quarter<DP>::kExps; ++h) {
             rows.codes[h] += c * a.row_codes;
@@ -158,15 +159,27 @@ __device__ __forceinline__ u32x4 widen(const Lane<DP>& l, const Quarter<DP>& q, 
                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3))};
     }
 }
-// A lane's quarter of row r of a stage (rows of DP 16-bit elements, 16-byte units placed by XOR with
-// `swizzle`), widened.
+// Where quarter g of row r of a stage begins, in bytes: rows of DP 16-bit elements, their 16-byte
+// units placed by XOR with `swizzle`; word i is (i << 4) away by XOR.
+template <int DP>
+__device__ __forceinline__ uint32_t quarter_at(int g, int r, int swizzle) {
+    return r * DP * 2 + ((g * Quarter<DP>::kWords) ^ swizzle) * 16;
+}
+// The quarter, widened.
 template <bool BF16, int DP>
-__device__ __forceinline__ void store_quarter(uint8_t* stage, int r, int swizzle, const Lane<DP>& l, const Quarter<DP>& q) {
-    const int g = (threadIdx.x & 63) >> 4;
+__device__ __forceinline__ void store_quarter(uint8_t* stage, uint32_t at, const Lane<DP>& l, const Quarter<DP>& q) {
 #pragma unroll
     for (int i = 0; i < Quarter<DP>::kWords; ++i) {
-        *reinterpret_cast<u32x4*>(stage + r * DP * 2 + ((g * Quarter<DP>::kWords + i) ^ swizzle) * 16) = widen<BF16, DP>(l, q, i);
+        *reinterpret_cast<u32x4*>(stage + (at ^ (i << 4))) = widen<BF16, DP>(l, q, i);
     }
+}
+
+// The transposing read at LDS[at + i * STEP].
+template <int STEP>
+__device__ __forceinline__ u32x2 transposed(uint32_t at, int i) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    using Lds = __attribute__((address_space(3))) s16x4*;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(uintptr_t)at + i * (STEP / 8)));
 }
 
 // ---- few rows --------------------------------------------------------------------
@@ -175,6 +188,7 @@ __device__ __forceinline__ void store_quarter(uint8_t* stage, int r, int swizzle
 // V through 32 rows of LDS of its own (no barrier); the next block's codes are under way during the
 // softmax and the second product.
 constexpr int kFewKeys = 32;
+constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
 constexpr int kFewWaves = DP == 256 ? 2 : 4;
 template <int DP>
@@ -190,7 +204,12 @@ constexpr int few_stage_bytes() {
 
 // Waves on a SIMD that a kernel's registers are held to.
 template <int DP, int MT>
-constexpr int kFewOccupancy = DP == 256 ? 1 : DP == 128 ? MT == 1 ? 3 : 2 : MT == 1 ? 4 : 2;
+constexpr int kFewOccupancy = DP == 64 ? MT == 1 ? 5 : 3 : DP == 128 ? MT == 1 ? 4 : 2 : MT == 1 ? 2 : 1;
+// Its workgroups on a CU, by these and by LDS (160 KB), with `plan` bytes behind the stages.
+template <int DP, int MT>
+int few_slots(int plan) {
+    return std::min(kFewOccupancy<DP, MT> * 4 / kFewWaves<DP>, (160 << 10) / (few_stage_bytes<DP, MT>() + plan));
+}
 
 template <bool BF16, int DP, int MT, bool CAP>
 __global__ __launch_bounds__(kFewWaves<DP> * 64) __attribute__((amdgpu_waves_per_eu(kFewOccupancy<DP, MT>)))
@@ -199,16 +218,24 @@ void fp4_few_rows_kernel(const Fp4Params a) {
     constexpr int KS = DP / 32;       // steps of 32 head elements
     constexpr int DT = DP / 16;       // tiles of 16 output elements
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Plan& plan = *reinterpret_cast<Plan*>(smem + few_stage_bytes<DP, MT>());
     uint8_t* const stage = smem + wave * kFewStage<DP>;
-    const Loader<DP> from(a);
     const float k = unit<CAP>(a);
 
-    Pieces<MR, kFewKeys, UNIT, WAVES, true> piece;
+    Pieces<MR, kFewKeys, UNIT, WAVES, true, true> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
+        // (made anew for each piece: held through all of them, what depends on it takes registers)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int c = lane & 15, g = lane >> 4;
+        const Loader<DP> from(a, lane);
+        // LDS places, the second 16 rows' as the first's: the lane's quarter of V's row c; of 4 rows from 4 g on,
+        // the columns of tile 0 (of tile d: d << 5 away by XOR)
+        const uint32_t v_to = quarter_at<DP>(g, c, v_swizzle<DP, false>(c));
+        const int vr = 4 * g + c / 4;
+        const uint32_t v_at = lds_addr(stage) + vr * DP * 2 + (((c % 4) / 2 ^ v_swizzle<DP, false>(vr)) * 16) + (c & 1) * 8;
         const Tile& t = piece.t;
         const int head = piece.head, u0 = piece.u0, u1 = piece.u1, slot = piece.slot;
         const Source src = source_of(a, t, head);
@@ -275,8 +302,7 @@ void fp4_few_rows_kernel(const Fp4Params a) {
             }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                const int r = kt * 16 + c;
-                store_quarter<BF16, DP>(stage, r, v_swizzle<DP, false>(r), from.lane, vq[kt]);
+                store_quarter<BF16, DP>(stage + kt * 16 * DP * 2, v_to, from.lane, vq[kt]);
             }
             if (i + 1 < mine) {  // the ids of the block after next ahead of the next one's codes: loads return in order
                 const uint32_t id0 = ids[0], id1 = ids[1];
@@ -293,12 +319,15 @@ void fp4_few_rows_kernel(const Fp4Params a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = s[mt][e / 4][e % 4];
                 cap_scores<CAP, 8>(a, x);
+                if (masked) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
-                    x[e] = masked & ((key < row_lo[mt]) | (key >= row_hi[mt])) ? -kInf : x[e];
-                    top = fmaxf(top, x[e]);
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = key0 + (e / 4) * 16 + 4 * g + e % 4;
+                        x[e] = (key < row_lo[mt]) | (key >= row_hi[mt]) ? -kInf : x[e];
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, x[e]);
                 top = max_halves(max_quarters(top));
                 const float m_new = fmaxf(m[mt], top);
                 if (__any((m_new - m[mt]) * k > kSlack)) {
@@ -318,18 +347,27 @@ void fp4_few_rows_kernel(const Fp4Params a) {
                 for (int e = 0; e < 4; ++e) p[mt][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
             }
             // O^T += V^T P^T: step slot 8 g + j is key 4 g + j (j < 4) or 16 + 4 g + j - 4
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
+            uint32_t v_now = v_at;
+            asm volatile("" : "+v"(v_now));  // the tiles' places are computed, not held
+            auto read_v = [&](int d) {
                 u32x4 vf;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt) {
-                    const int r = kt * 16 + 4 * g + c / 4, unit = 2 * d + (c % 4) / 2;
-                    const u32x2 h = read_transposed(stage + r * DP * 2 + ((unit ^ v_swizzle<DP, false>(r)) * 16) + (c & 1) * 8);
+                    const u32x2 h = transposed<16 * DP * 2>(v_now ^ (d << 5), kt);
                     vf[2 * kt] = h[0];
                     vf[2 * kt + 1] = h[1];
                 }
+                return vf;
+            };
+            u32x4 vf[kAhead];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) o[mt][d] = mfma16x16x32<BF16>(vf, p[mt], o[mt][d]);
+            for (int d = 0; d < kAhead; ++d) vf[d] = read_v(d);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][d] = mfma16x16x32<BF16>(vf[d % kAhead], p[mt], o[mt][d]);
+                if (d + kAhead < DT) vf[d % kAhead] = read_v(d + kAhead);
             }
             asm volatile("" ::: "memory");
         }
@@ -345,7 +383,6 @@ void fp4_few_rows_kernel(const Fp4Params a) {
 // Four waves of 32 query rows each over blocks of 64 keys that they share in LDS as 16-bit elements,
 // two stages: each wave widens 16 keys of a block, whose codes came during the block before.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
-constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
 constexpr int kManyStage = 2 * kManyKeys * DP * 2;
 template <int DP>
@@ -363,8 +400,10 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, h = lane >> 5;
     Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
-    const Loader<DP> from(a);
+    const Loader<DP> from(a, lane);
     const int copied = wave * COPY + (lane & 15);  // the lane's key of a block
+    const uint32_t k_to = quarter_at<DP>(lane >> 4, copied, k_swizzle<DP>(copied));
+    const uint32_t v_to = quarter_at<DP>(lane >> 4, copied, v_swizzle<DP, true>(copied));
     const float k = unit<CAP>(a);
     // LDS places of the lane's operands in a stage: K's unit 2 st + h of row c lies st << 5 (in
     // bits 5 up) away by XOR; V's 4 rows from 4 h on, at columns of tile d, d << 6 away
@@ -397,8 +436,8 @@ void fp4_many_rows_kernel(const Fp4Params a) {
         auto load = [&](int i) { from.template load<true, true>(a, src, begin + i * KEYS + wave * COPY, id, kq, vq); };
         auto store = [&](int i) {
             uint8_t* const to = smem + (i & 1) * kManyStage<DP>;
-            store_quarter<BF16, DP>(to, copied, k_swizzle<DP>(copied), from.lane, kq);
-            store_quarter<BF16, DP>(to + kManyStage<DP> / 2, copied, v_swizzle<DP, true>(copied), from.lane, vq);
+            store_quarter<BF16, DP>(to, k_to, from.lane, kq);
+            store_quarter<BF16, DP>(to + kManyStage<DP> / 2, v_to, from.lane, vq);
         };
         if (blocks > 0) {
             id = page(0);
@@ -505,6 +544,7 @@ void fp4_many_rows_kernel(const Fp4Params a) {
 struct Call {
     Fp4Params p;
     int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128
+    int plan;                  // bytes of LDS behind the kernel's stages
     int64_t tiles;             // at most
     size_t bytes;
 };
@@ -535,8 +575,17 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const bool few = c.tile_rows <= 32;
     c.tiles = few ? p.batch : tiles_of(c.tile_rows);
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
+    // what a split call holds in LDS: a plan, or the tiles of few sequences
+    c.plan = !few || p.batch > 64 ? (int)sizeof(Plan) : 64 * (int)sizeof(Tile);
     // workgroups that run at once
-    const int slots = few ? (c.dp == 256 ? 2 : c.tile_rows == 32 ? 2 : c.dp == 128 ? 3 : 4) * cus : c.dp != 256 ? 2 * cus : cus;
+    const auto few_at_once = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        return c.dp == 64 ? few_slots<64, MT>(c.plan) : c.dp == 128 ? few_slots<128, MT>(c.plan) : few_slots<256, MT>(c.plan);
+    };
+    const int slots = cus * (c.tile_rows == 16   ? few_at_once(std::integral_constant<int, 1>{})
+                             : c.tile_rows == 32 ? few_at_once(std::integral_constant<int, 2>{})
+                             : c.dp != 256       ? 2
+                                                 : 1);
     // units of a tile: of the keys that a window leaves its rows, or all
     const int64_t most_keys =
         p.window == 0 ? p.max_len
@@ -550,6 +599,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
                         : few ? most_units > (8 * c.tiles * p.kv_heads <= cus ? 7 : 4 * c.tiles * p.kv_heads <= cus ? 16 : 22)
                               : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
     p.split = wanted && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
+    if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
     if (p.split) {
         c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
@@ -562,17 +612,18 @@ template <bool BF16, int DP, bool CAP>
 hipError_t launch(const Call& c, hipStream_t s) {
     hipError_t e;
     if (c.tile_rows == 16) {
-        e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), s);
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), c.plan, s);
     } else if (c.tile_rows == 32) {
-        e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), s);
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.plan, s);
     } else {
-        e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), s);
+        e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.plan, s);
     }
     if (e != hipSuccess || !c.p.split) return e;
+    const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(c.tile_rows, (int64_t)c.p.max_q * c.p.group));
     if (c.tile_rows == 16) {
-        run_join<16, BF16>(c.p, c.tiles, c.grid, s);
+        run_row_join<16, BF16>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == 32) {
-        run_join<32, BF16>(c.p, c.tiles, c.grid, s);
+        run_row_join<32, BF16>(c.p, c.tiles, rows, c.grid, s);
     } else {
         run_join<kManyRows, BF16>(c.p, c.tiles, c.grid, s);
     }

@@ -6,6 +6,8 @@
 // are computed without matrix instructions:
 //   element<BF16>(params, plane, kv head, page, row of the page, d)   as fp32
 //   kRepeats: a head narrower than the kernel's repeats its elements against zeros
+//   kFresh: what depends on the lane alone is computed at the ends of pieces, rather than ahead of them
+//     and held in registers through their loops
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -350,7 +352,9 @@ struct RowResult {
 };
 template <typename Keys, bool BF16, bool CAP, typename P>
 __device__ __forceinline__ RowResult plain_row(const P& a, int b, int token, int head, int begin, int end) {
-    const int lane = threadIdx.x & 63, kv = head / a.group;
+    int lane = threadIdx.x & 63;
+    if (Keys::kFresh) asm volatile("" : "+v"(lane));
+    const int kv = head / a.group;
     const uint16_t* const q = a.q + token * a.q_token + head * a.q_head;
     RowResult r{-kInf, 0.f, {0.f, 0.f, 0.f, 0.f}};
     for (int j0 = begin; j0 < end; j0 += 64) {
@@ -422,7 +426,9 @@ __device__ __forceinline__ bool values_not_finite(const P& a, const Tile& t, int
     for (int key = max(begin, t.lo); key < min(end, t.hi); ++key) {
         const uint32_t page = min((uint32_t)a.tables[t.b * a.table_stride + page_index(a, key)], (uint32_t)a.num_pages - 1);
         const uint32_t at = key - page_index(a, key) * a.page_size;
-        for (int d = threadIdx.x & 63; d < a.dim; d += 64) {
+        int first = threadIdx.x & 63;
+        if (Keys::kFresh) asm volatile("" : "+v"(first));
+        for (int d = first; d < a.dim; d += 64) {
             const float x = Keys::template element<BF16>(a, a.v, head, page, at, d);
             bad |= x - x != 0.f;
         }
@@ -501,8 +507,9 @@ __device__ __forceinline__ void write_plan(const Params& a, int i, int begin, in
 }
 
 // A workgroup's pieces of work, one after the other: units [u0, u1) of a tile and
-// head, for partial slot `slot`, or the whole of it (-1).  ONE: a sequence has one tile.
-template <int MR, int KEYS, int UNIT, int WAVES, bool ONE>
+// head, for partial slot `slot`, or the whole of it (-1).  ONE: a sequence has one tile;
+// IN_LDS: those of up to 64 sequences are held in LDS, 64 Tiles at the plan's place, and not in registers.
+template <int MR, int KEYS, int UNIT, int WAVES, bool ONE, bool IN_LDS = false>
 struct Pieces {
     Tile t;
     int head, u0, u1, slot;
@@ -538,6 +545,7 @@ struct Pieces {
                 my = tile_of<MR, KEYS>(a, b, 0, sequence(a, b));
                 n = units_of<UNIT>(my);
             }
+            if (IN_LDS) reinterpret_cast<Tile*>(&plan)[b] = my;  // (each wave for itself, and all the same)
             my_end = wave_inclusive_scan(n);
             tiles = a.batch;
             units = __builtin_amdgcn_readlane(my_end, 63);
@@ -603,15 +611,17 @@ struct Pieces {
             const int b = __builtin_ctzll(__ballot(my_end > r));
             first = b ? __builtin_amdgcn_readlane(my_end, b - 1) : 0;
             last = __builtin_amdgcn_readlane(my_end, b);
+            const Tile held = IN_LDS ? reinterpret_cast<const Tile*>(&plan)[b] : my;
+            const auto of_b = [&](int v) { return IN_LDS ? __builtin_amdgcn_readfirstlane(v) : __builtin_amdgcn_readlane(v, b); };
             t.b = b;
-            t.q0 = __builtin_amdgcn_readlane(my.q0, b);
-            t.first_pos = __builtin_amdgcn_readlane(my.first_pos, b);
-            t.len = __builtin_amdgcn_readlane(my.len, b);
+            t.q0 = of_b(held.q0);
+            t.first_pos = of_b(held.first_pos);
+            t.len = of_b(held.len);
             t.row0 = 0;
-            t.rows = __builtin_amdgcn_readlane(my.rows, b);
-            t.lo = __builtin_amdgcn_readlane(my.lo, b);
-            t.hi = __builtin_amdgcn_readlane(my.hi, b);
-            t.base = __builtin_amdgcn_readlane(my.base, b);
+            t.rows = of_b(held.rows);
+            t.lo = of_b(held.lo);
+            t.hi = of_b(held.hi);
+            t.base = of_b(held.base);
         } else {
             const int ti = __builtin_amdgcn_readfirstlane(first_above(plan.unit_end, tiles, r));
             const int b = __builtin_amdgcn_readfirstlane(first_above(plan.seq_end, a.batch, ti));
@@ -638,7 +648,9 @@ __device__ __forceinline__ void join_waves(const P& a, const Tile& t, uint8_t* s
                                            int end, float k, const float (&m)[MT], const float (&z)[MT],
                                            const f32x4 (&o)[MT][DP / 16]) {
     constexpr int MR = 16 * MT, DT = DP / 16;
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    int lane = threadIdx.x & 63;
+    if (Keys::kFresh) asm volatile("" : "+v"(lane));
+    const int c = lane & 15, g = lane >> 4;
     constexpr int kRow = DP + 4;
     float* const join = reinterpret_cast<float*>(smem);
 #pragma unroll
@@ -855,6 +867,82 @@ __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
     if (lane == 0) store_stats<MR, BF16>(a, t, head, row, -1, m2, z);
 }
 
+// The same with a workgroup a row (blockIdx.y), whose waves take the partials in turn: for few rows in
+// many pieces.
+template <int MR, bool BF16>
+__global__ __launch_bounds__(256) void join_row_kernel(const Params a, int grid) {
+    constexpr int WAVES = 4, kAtOnce = 8;
+    __shared__ float s_x[WAVES][256], s_ml[WAVES][2];
+    const int ti = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads, row = blockIdx.y;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const PlanOut::Entry e = reinterpret_cast<const PlanOut::Entry*>(a.plan + PlanOut::kEntries)[ti];
+    const int units = a.plan[PlanOut::kUnits];
+    if (ti >= a.plan[PlanOut::kTiles] || row >= e.rows || e.end <= e.begin) return;
+    const Runs runs(a, units * a.kv_heads, grid);
+    const int w0 = runs.of(head * units + e.begin), n = runs.of(head * units + e.end - 1) - w0 + 1;
+    if (n == 1) return;
+    // partial i: the first run's second slot, then the others' first ones
+    const auto slot = [&](int i) -> int64_t { return 2 * (int64_t)(w0 + i) + (i == 0 ? 1 : 0); };
+    float m2 = -kInf, z = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = wave * kAtOnce; i0 < n; i0 += WAVES * kAtOnce) {
+        float v[kAtOnce][4], m[kAtOnce], l[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int64_t at = slot(min(i0 + u, n - 1)) * MR + row;
+            m[u] = i0 + u < n ? a.part_ml[at * 2] : -kInf;
+            l[u] = i0 + u < n ? a.part_ml[at * 2 + 1] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[u][j] = lane + 64 * j < a.dim ? a.part_o[at * a.dim + lane + 64 * j] : 0.f;
+        }
+        float top = m2;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) top = fmaxf(top, m[u]);
+        const float scale = m2 == -kInf ? 0.f : __builtin_amdgcn_exp2f(m2 - top);
+        z = z == 0.f ? 0.f : z * scale;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = scale == 0.f ? 0.f : x[j] * scale;
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const float w = m[u] == -kInf ? 0.f : __builtin_amdgcn_exp2f(m[u] - top);
+            z += m[u] == -kInf && l[u] == 0.f ? 0.f : m[u] == -kInf ? l[u] - l[u] : w * l[u];  // a sum of NaN has a maximum of -inf
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += w == 0.f ? 0.f : w * v[u][j];  // a run of no weight may hold anything
+        }
+        m2 = top;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s_x[wave][lane + 64 * j] = x[j];
+    if (lane == 0) {
+        s_ml[wave][0] = m2;
+        s_ml[wave][1] = z;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    m2 = -kInf;
+    z = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m2 = fmaxf(m2, s_ml[w][0]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        const float f = s_ml[w][0] == -kInf ? 0.f : __builtin_amdgcn_exp2f(s_ml[w][0] - m2);
+        z += s_ml[w][0] == -kInf ? s_ml[w][1] : f * s_ml[w][1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += f == 0.f ? 0.f : f * s_x[w][lane + 64 * j];
+    }
+    const float inv = z > 0.f ? 1.f / z : z == 0.f ? 0.f : z;
+    Tile t{};
+    t.q0 = e.q0;
+    t.row0 = e.row0;
+    uint16_t* const to = out_row(a, t, head, row);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (lane + 64 * j < a.dim) to[lane + 64 * j] = f32_to_out<BF16>(x[j] * inv);
+    }
+    if (lane == 0) store_stats<MR, BF16>(a, t, head, row, -1, m2, z);
+}
+
 // ---- host ----------------------------------------------------------------------------
 
 inline int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -903,10 +991,10 @@ inline Params params_of(const pw4_paged_attention_args* a) {
 }
 
 // Runs a kernel with more LDS than a kernel may have unasked; the permission is
-// asked for once a kernel and device.
+// asked for once a kernel and device.  `plan`: bytes behind its stages, a Plan's at most.
 template <auto Kernel, typename P>
-hipError_t run_attention(const P& p, int grid, int waves, int stages, hipStream_t s) {
-    const int most = stages + (int)sizeof(Plan), lds = p.split ? most : stages;
+hipError_t run_attention(const P& p, int grid, int waves, int stages, int plan, hipStream_t s) {
+    const int most = stages + (int)sizeof(Plan), lds = stages + plan;
     static std::atomic<uint64_t> allowed{0};
     int dev = 0;
     if (const hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
@@ -924,6 +1012,11 @@ hipError_t run_attention(const P& p, int grid, int waves, int stages, hipStream_
 template <int MR, bool BF16>
 void run_join(const Params& p, int64_t tiles, int grid, hipStream_t s) {
     hipLaunchKernelGGL((join_kernel<MR, BF16>), dim3((unsigned)(tiles * p.kv_heads), MR / 4), dim3(256), 0, s, p, grid);
+}
+
+template <int MR, bool BF16>
+void run_row_join(const Params& p, int64_t tiles, int rows, int grid, hipStream_t s) {
+    hipLaunchKernelGGL((join_row_kernel<MR, BF16>), dim3((unsigned)(tiles * p.kv_heads), rows), dim3(256), 0, s, p, grid);
 }
 
 // The workspace of a split call: partial outputs, their maxima and sums, and the plan.
