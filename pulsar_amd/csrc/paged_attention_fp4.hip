@@ -24,7 +24,8 @@ struct Fp4Params : Params {
     uint32_t row_codes, row_exps;    // bytes of a token's codes, and of its exponents
     uint32_t head_codes, head_exps;  // of a page's of one head
     uint32_t exps_at;                // where a page's exponents begin
-    int32_t flat;                    // pages hold whole runs of 16 keys
+    uint32_t index_magic;            // key / page_size = (2 key * magic) >> (32 + shift), for any page size
+    int32_t index_shift;
 };
 
 // The cache's elements one at a time, as the products take them.
@@ -100,44 +101,25 @@ __device__ __forceinline__ void load_quarter(const uint8_t* codes, const uint8_t
     for (int h = 0; h < Quarter<DP>::kExps; ++h) q.exps[h] = exps[l.exps[h]];
 }
 
-// The lane's quarters of K and V of key c of 16 that begin with `first`, `id` being its page.  Where the
-// 16 lie in one page and all are seen, the row they begin with is uniform.
+// A lane's key of 16: its page's id, which takes a load, and its row of the page.
+struct Key {
+    uint32_t page, row;
+};
+// The lane's quarters of key c of 16 keys, in two steps: where it is, and its codes and exponents.
 template <int DP>
 struct Loader {
     Lane<DP> lane;
-    Lane<DP> rows;  // with row c of 16 ahead
     int c;
-    __device__ __forceinline__ Loader(const Fp4Params& a, int l) : lane(a, l >> 4), rows(a, l >> 4), c(l & 15) {
-#pragma unroll
-        for (int h = 0; h < Quarter<DP>::kExps; ++h) {
-            rows.codes[h] += c * a.row_codes;
-            rows.exps[h] += c * a.row_exps;
-        }
+    __device__ __forceinline__ Loader(const Fp4Params& a, int l) : lane(a, l >> 4), c(l & 15) {}
+    __device__ __forceinline__ Key find(const Fp4Params& a, const Source& s, int first) const {
+        const uint32_t key = clamp_key(s, first + c), index = __umulhi(2 * key, a.index_magic) >> a.index_shift;
+        return Key{(uint32_t)s.table[index], key - index * (uint32_t)a.page_size};
     }
-    __device__ __forceinline__ uint32_t page(const Fp4Params& a, const Source& s, int first) const {
-        return s.table[page_index(a, clamp_key(s, first + c))];
-    }
-    __device__ __forceinline__ bool in_one_page(const Fp4Params& a, const Source& s, int first) const {
-        return a.flat && first >= s.lo && first + 15 <= s.last;
-    }
-    template <bool K, bool V>
-    __device__ __forceinline__ void load(const Fp4Params& a, const Source& s, int first, uint32_t id, Quarter<DP>& k,
-                                         Quarter<DP>& v) const {
-        if (in_one_page(a, s, first)) {
-            const uint32_t page = min((uint32_t)__builtin_amdgcn_readfirstlane(id), s.pages1);
-            const uint32_t row = first - page_index(a, first) * a.page_size;
-            const uint64_t codes = (uint64_t)page * a.page_bytes + (s.codes + row * a.row_codes);
-            const uint64_t exps = (uint64_t)page * a.page_bytes + (s.exps + row * a.row_exps);
-            if (K) load_quarter<DP>(s.k + codes, s.k + exps, rows, k);
-            if (V) load_quarter<DP>(s.v + codes, s.v + exps, rows, v);
-        } else {
-            const int key = clamp_key(s, first + c);
-            const uint32_t row = key - page_index(a, key) * a.page_size;
-            const uint64_t page = (uint64_t)min(id, s.pages1) * a.page_bytes;
-            const uint64_t codes = page + (s.codes + row * a.row_codes), exps = page + (s.exps + row * a.row_exps);
-            if (K) load_quarter<DP>(s.k + codes, s.k + exps, lane, k);
-            if (V) load_quarter<DP>(s.v + codes, s.v + exps, lane, v);
-        }
+    // `plane` with the head's place in a page: codes, exponents
+    __device__ __forceinline__ void load(const Fp4Params& a, const Source& s, const uint8_t* plane, const Key& key,
+                                         Quarter<DP>& q) const {
+        const uint8_t* const page = plane + (uint64_t)min(key.page, s.pages1) * a.page_bytes;
+        load_quarter<DP>(page + (s.codes + __umul24(key.row, a.row_codes)), page + (s.exps + __umul24(key.row, a.row_exps)), lane, q);
     }
 };
 
@@ -243,19 +225,20 @@ void fp4_few_rows_kernel(const Fp4Params a) {
         const int blocks = end > begin ? (end - begin + kFewKeys - 1) / kFewKeys : 0;
         const int mine = (blocks - wave + WAVES - 1) / WAVES;  // blocks wave, wave + WAVES, ...
         auto first_of = [&](int i) { return begin + (wave + i * WAVES) * kFewKeys; };
-        uint32_t ids[2] = {0, 0};  // of the next block's keys c and 16 + c
-        auto pages = [&](int i) {
+        Key keys[2] = {};  // of the block that is loaded next, c and 16 + c
+        auto find = [&](int i) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) ids[kt] = from.page(a, src, first_of(i) + kt * 16);
+            for (int kt = 0; kt < 2; ++kt) keys[kt] = from.find(a, src, first_of(i) + kt * 16);
         };
         Quarter<DP> kq[2], vq[2];
-        auto load = [&](int i, uint32_t id0, uint32_t id1) {
+        auto load = [&](const Key& key0, const Key& key1) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                from.template load<true, true>(a, src, first_of(i) + kt * 16, kt ? id1 : id0, kq[kt], vq[kt]);
+                from.load(a, src, src.k, kt ? key1 : key0, kq[kt]);
+                from.load(a, src, src.v, kt ? key1 : key0, vq[kt]);
             }
         };
-        if (mine > 0) pages(0);
+        if (mine > 0) find(0);
         u32x4 q[MT][KS];
         int row_lo[MT], row_hi[MT];  // keys that the lane's row sees
 #pragma unroll
@@ -283,8 +266,8 @@ void fp4_few_rows_kernel(const Fp4Params a) {
             for (int d = 0; d < DT; ++d) o[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (mine > 0) {
-            load(0, ids[0], ids[1]);
-            if (mine > 1) pages(1);
+            load(keys[0], keys[1]);
+            if (mine > 1) find(1);
         }
         for (int i = 0; i < mine; ++i) {
             const int key0 = first_of(i);
@@ -304,10 +287,10 @@ void fp4_few_rows_kernel(const Fp4Params a) {
             for (int kt = 0; kt < 2; ++kt) {
                 store_quarter<BF16, DP>(stage + kt * 16 * DP * 2, v_to, from.lane, vq[kt]);
             }
-            if (i + 1 < mine) {  // the ids of the block after next ahead of the next one's codes: loads return in order
-                const uint32_t id0 = ids[0], id1 = ids[1];
-                if (i + 2 < mine) pages(i + 2);
-                load(i + 1, id0, id1);
+            if (i + 1 < mine) {  // the pages of the block after next ahead of the next one's codes: loads return in order
+                const Key now0 = keys[0], now1 = keys[1];
+                if (i + 2 < mine) find(i + 2);
+                load(now0, now1);
             }
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");  // a wave's LDS operations stay in this order
@@ -430,23 +413,26 @@ void fp4_many_rows_kernel(const Fp4Params a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
         float m = -kInf, z = 0.f;
-        uint32_t id = 0;  // the page of the lane's key of the block that is loaded next
+        Key key{};  // the lane's, of the block that is loaded next
         Quarter<DP> kq, vq;
-        auto page = [&](int i) { return from.page(a, src, begin + i * KEYS + wave * COPY); };
-        auto load = [&](int i) { from.template load<true, true>(a, src, begin + i * KEYS + wave * COPY, id, kq, vq); };
+        auto find = [&](int i) { return from.find(a, src, begin + i * KEYS + wave * COPY); };
+        auto load = [&] {
+            from.load(a, src, src.k, key, kq);
+            from.load(a, src, src.v, key, vq);
+        };
         auto store = [&](int i) {
             uint8_t* const to = smem + (i & 1) * kManyStage<DP>;
             store_quarter<BF16, DP>(to, k_to, from.lane, kq);
             store_quarter<BF16, DP>(to + kManyStage<DP> / 2, v_to, from.lane, vq);
         };
         if (blocks > 0) {
-            id = page(0);
-            load(0);
-            if (blocks > 1) id = page(1);
+            key = find(0);
+            load();
+            if (blocks > 1) key = find(1);
             store(0);
             if (blocks > 1) {
-                load(1);
-                if (blocks > 2) id = page(2);
+                load();
+                if (blocks > 2) key = find(2);
             }
         }
         for (int i = 0; i < blocks; ++i) {
@@ -455,9 +441,9 @@ void fp4_many_rows_kernel(const Fp4Params a) {
             if (i + 1 < blocks) {
                 store(i + 1);
                 if (i + 2 < blocks) {
-                    const uint32_t then = i + 3 < blocks ? page(i + 3) : 0;
-                    load(i + 2);
-                    id = then;
+                    const Key then = i + 3 < blocks ? find(i + 3) : Key{};
+                    load();
+                    key = then;
                 }
             }
             const int key0 = begin + i * KEYS;
@@ -539,11 +525,182 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     clear_rest(a);
 }
 
+// ---- a great many rows -----------------------------------------------------------------
+
+// Eight waves of 32 rows, two on each SIMD, that take turns: while waves 0 to 3 are in their products
+// (scores of block i + 1, outputs of block i), waves 4 to 7 make the probabilities of a block, and the
+// other way round (measured against waves without turns in paged_attention.hip).  Waves 0 to 3 widen K,
+// waves 4 to 7 V, 16 keys each of a block, beside their probabilities; the codes come a block ahead.
+constexpr int kWideWaves = 8, kWideRows = 32 * kWideWaves, kWideRing = 3;
+template <int DP>
+constexpr int kWideBlock = kManyKeys * DP * 2;  // bytes of K, or of V
+template <int DP>
+constexpr int wide_stage_bytes() { return 2 * kWideRing * kWideBlock<DP>; }
+
+template <bool BF16, int DP, bool CAP>
+__global__ __launch_bounds__(kWideWaves * 64) __attribute__((amdgpu_waves_per_eu(2)))
+void fp4_wide_rows_kernel(const Fp4Params a) {
+    constexpr int MR = kWideRows, KEYS = kManyKeys, KS = DP / 16, DT = DP / 32;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
+    Plan& plan = *reinterpret_cast<Plan*>(smem + wide_stage_bytes<DP>());
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const bool late = wave >= 4;  // half a turn behind, and widens V
+    const Loader<DP> from(a, lane);
+    const int copied = (wave & 3) * 16 + (lane & 15);  // the lane's key of a block
+    uint8_t* const my_ring = smem + (late ? kWideRing * kWideBlock<DP> : 0);
+    const uint32_t to = quarter_at<DP>(lane >> 4, copied, late ? v_swizzle<DP, true>(copied) : k_swizzle<DP>(copied));
+    const float k = unit<CAP>(a);
+    const uint32_t k_at = (uint32_t)(c * DP * 2 + ((h ^ k_swizzle<DP>(c)) * 16));
+    const int vr = 4 * h + ((c & 15) >> 2);
+    const uint32_t v_at = (uint32_t)(vr * DP * 2 + ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) +
+                                     (c & 1) * 8);
+    Pieces<MR, KEYS, KEYS, kWideWaves, false> piece;
+    piece.start(a, plan);
+    while (piece.next(a, plan)) {
+        const Tile& t = piece.t;
+        const int head = piece.head, slot = piece.slot;
+        const Source src = source_of(a, t, head);
+        const uint8_t* const plane = late ? src.v : src.k;
+        const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
+        const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        const WaveRows<KEYS> r(a, t, wave);
+        const int mine0 = begin + (wave & 3) * 16;  // of block 0, the first key that the wave widens
+        Quarter<DP> raw;
+        Key key{};  // the lane's, of the block that is loaded next
+        auto find = [&](int i) { return from.find(a, src, mine0 + i * KEYS); };
+        auto load = [&] { from.load(a, src, plane, key, raw); };
+        auto store = [&](int place) { store_quarter<BF16, DP>(my_ring + place * kWideBlock<DP>, to, from.lane, raw); };
+        if (blocks > 0) key = find(0);
+        u32x4 q[KS];
+        load_query<KS>(a, r.mine, head, c, h, 2, q);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[st]));  // here, not waited for in the loop
+        f32x16 o[DT], s[2];
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+        u32x4 p[4];
+        float m = -kInf, z = 0.f;
+        if (blocks > 0) {
+            // blocks 0 and 1 into the ring, block 2's codes and block 3's pages under way
+            load();
+            if (blocks > 1) key = find(1);
+            store(0);
+            if (blocks > 1) {
+                load();
+                if (blocks > 2) key = find(2);
+                store(1);
+            }
+            if (blocks > 2) {
+                load();
+                if (blocks > 3) key = find(3);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (late) asm volatile("s_barrier" ::: "memory");
+            int place = 2;  // ring place of block i + 3
+            for (int i = -1; i < blocks; ++i) {
+                // ---- products: scores of block i + 1, outputs of block i
+                const int next = begin + (i + 1) * KEYS;
+                const int place_next = place == 2 ? 0 : place + 1;  // of blocks i + 1 (and i + 4)
+                const int place_now = place;                        // of blocks i (and i + 3)
+                const bool do_next = i + 1 < blocks && r.sees(next), do_now = i >= 0 && r.sees(next - KEYS);
+                __builtin_amdgcn_s_setprio(1);
+                if (__builtin_expect(do_next, 1)) {
+                    const uint8_t* const st_at = smem + place_next * kWideBlock<DP>;
+                    auto read_k = [&](int n) {
+                        return *reinterpret_cast<const u32x4*>(st_at + (k_at ^ ((n / 2) << 5)) + (n % 2) * 32 * DP * 2);
+                    };
+                    u32x4 kf[kAhead];
+#pragma unroll
+                    for (int n = 0; n < kAhead; ++n) kf[n] = read_k(n);
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[kt][e] = 0.f;
+#pragma unroll
+                    for (int n = 0; n < 2 * KS; ++n) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
+                        if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
+                    }
+                }
+                if (__builtin_expect(do_now, 1)) {
+                    const uint8_t* const st_at = smem + (kWideRing + place_now) * kWideBlock<DP>;
+                    auto read_v = [&](int n) {
+                        const uint8_t* const at = st_at + (v_at ^ ((n % DT) << 6)) + (n / DT) * 16 * DP * 2;
+                        const u32x2 y0 = read_transposed(at), y1 = read_transposed(at + 8 * DP * 2);
+                        return u32x4{y0[0], y0[1], y1[0], y1[1]};
+                    };
+                    u32x4 vf[kAhead];
+#pragma unroll
+                    for (int n = 0; n < kAhead; ++n) vf[n] = read_v(n);
+#pragma unroll
+                    for (int n = 0; n < 4 * DT; ++n) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        o[n % DT] = mfma32x32x16<BF16>(vf[n % kAhead], p[n / DT], o[n % DT]);
+                        if (n + kAhead < 4 * DT) vf[n % kAhead] = read_v(n + kAhead);
+                    }
+                }
+                __builtin_amdgcn_s_setprio(0);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                // ---- block i + 3 into the ring, the codes of block i + 4; probabilities of block i + 1
+                if (__builtin_expect(i + 3 < blocks, 1)) {
+                    store(place_now);
+                    if (i + 4 < blocks) {
+                        const Key then = i + 5 < blocks ? find(i + 5) : Key{};
+                        load();
+                        key = then;
+                    }
+                }
+                if (__builtin_expect(do_next, 1)) {
+                    cap_scores<CAP, 16>(a, s[0]);
+                    cap_scores<CAP, 16>(a, s[1]);
+                    r.mask(next, h, s);
+                    float top = -kInf;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[kt][e]);
+                    top = max_halves(top);
+                    const float m_new = fmaxf(m, top);
+                    if (__builtin_expect(__any((m_new - m) * k > kSlack), 0)) {
+                        const float scale = __builtin_amdgcn_exp2f((m - (m_new == -kInf ? 0.f : m_new)) * k);
+                        z *= scale;
+#pragma unroll
+                        for (int d = 0; d < DT; ++d) o[d] *= scale;
+                        m = m_new;
+                    }
+                    const float shift = m == -kInf ? -kLift<BF16> : shift_of<BF16>(m, k);
+#pragma unroll
+                    for (int st = 0; st < 4; ++st) {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            x[e] = __builtin_amdgcn_exp2f(s[st / 2][(st % 2) * 8 + e] * k - shift);
+                            z += x[e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[st][e] = pack2<BF16>(x[2 * e], x[2 * e + 1]);
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                place = place_next;
+            }
+            if (!late) asm volatile("s_barrier" ::: "memory");
+        }
+        store_rows<Fp4Keys, BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held_max<BF16>(m, k), z, o);
+        __syncthreads();  // every wave is done with the ring
+    }
+    clear_rest(a);
+}
+
 // ---- host ----------------------------------------------------------------------------
 
 struct Call {
     Fp4Params p;
-    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128
+    int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128 or 256
     int plan;                  // bytes of LDS behind the kernel's stages
     int64_t tiles;             // at most
     size_t bytes;
@@ -564,14 +721,21 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.head_codes = (uint32_t)a->page_size * p.row_codes;
     p.head_exps = (uint32_t)a->page_size * p.row_exps;
     p.exps_at = (uint32_t)a->kv_heads * p.head_codes;
-    p.flat = a->page_size % 16 == 0;
+    // (a power of two 2^n has 2^(31 - n) and 0; else as Params' division, with 2 key)
+    p.index_magic = p.page_shift >= 0 ? 0x80000000u >> p.page_shift : p.page_magic;
+    p.index_shift = p.page_shift >= 0 ? 0 : p.page_magic_shift + 1;
     const int64_t rows = (int64_t)p.max_q * p.group;
     c.dp = padded_dim(a->head_dim);
     const int cus = device_cus();
     const auto tiles_of = [&](int tile_rows) {
         return std::min(a->num_tokens * p.group / tile_rows + p.batch, p.batch * ceil_div(rows, tile_rows));
     };
-    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kManyRows;
+    // 256-row tiles run at the higher rate, but only one to a CU
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32
+                  : c.dp == 256 || tiles_of(kWideRows) * p.kv_heads < cus ? kManyRows : kWideRows;
+    if (const char* const forced = plan_override("PW4_ATTN_TILE"); forced && c.tile_rows > 32 && c.dp != 256) {
+        c.tile_rows = forced[0] == '2' ? kWideRows : kManyRows;
+    }
     const bool few = c.tile_rows <= 32;
     c.tiles = few ? p.batch : tiles_of(c.tile_rows);
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
@@ -584,8 +748,8 @@ Call plan_call(const pw4_paged_attention_args* a) {
     };
     const int slots = cus * (c.tile_rows == 16   ? few_at_once(std::integral_constant<int, 1>{})
                              : c.tile_rows == 32 ? few_at_once(std::integral_constant<int, 2>{})
-                             : c.dp != 256       ? 2
-                                                 : 1);
+                             : c.tile_rows == kManyRows && c.dp != 256 ? 2
+                                                                       : 1);
     // units of a tile: of the keys that a window leaves its rows, or all
     const int64_t most_keys =
         p.window == 0 ? p.max_len
@@ -615,8 +779,12 @@ hipError_t launch(const Call& c, hipStream_t s) {
         e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), c.plan, s);
     } else if (c.tile_rows == 32) {
         e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.plan, s);
-    } else {
+    } else if (c.tile_rows == kManyRows) {
         e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.plan, s);
+    } else if constexpr (DP < 256) {
+        e = run_attention<fp4_wide_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kWideWaves, wide_stage_bytes<DP>(), c.plan, s);
+    } else {
+        e = hipErrorInvalidValue;  // no such tile: plan_call
     }
     if (e != hipSuccess || !c.p.split) return e;
     const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(c.tile_rows, (int64_t)c.p.max_q * c.p.group));
@@ -624,8 +792,10 @@ hipError_t launch(const Call& c, hipStream_t s) {
         run_row_join<16, BF16>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == 32) {
         run_row_join<32, BF16>(c.p, c.tiles, rows, c.grid, s);
-    } else {
+    } else if (c.tile_rows == kManyRows) {
         run_join<kManyRows, BF16>(c.p, c.tiles, c.grid, s);
+    } else {
+        run_join<kWideRows, BF16>(c.p, c.tiles, c.grid, s);
     }
     return hipGetLastError();
 }
