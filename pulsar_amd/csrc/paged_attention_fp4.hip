@@ -730,10 +730,23 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const auto tiles_of = [&](int tile_rows) {
         return std::min(a->num_tokens * p.group / tile_rows + p.batch, p.batch * ceil_div(rows, tile_rows));
     };
-    // 256-row tiles run at the higher rate, but only one to a CU
+    // keys that a tile's rows see at most: those that a window leaves, or all
+    const auto keys_of = [&](int64_t tile_rows) {
+        return p.window == 0 ? p.max_len
+                             : std::min<int64_t>(p.max_len, (int64_t)p.window + (std::min(tile_rows, rows) + p.group - 2) / p.group);
+    };
+    // 256-row tiles run at the higher rate, but only one to a CU: for heads of 96 and 128 where they are long
+    // and either fill the chip almost twice or, of chunks far into their sequences, are alike.  128 and 256
+    // rows, us, 32 heads on 8 of 128: a prompt of 2048 tokens 62 and 71, of 4096 165 and 151, of 8192 584 and
+    // 550, 16 of 512 83 and 97, 4 of 4000 in a window of 1024 305 and 318; 8 chunks of 1024 at 8000 keys, 8
+    // heads, 300 and 259, a prompt of 8192 there 205 and 240.  (Heads of 64: 367 and 437 for a prompt of 8192;
+    // three waves of 128-row tiles share a SIMD.)
+    const int64_t wide_tiles = tiles_of(kWideRows) * p.kv_heads;
+    const bool alike = p.max_len / 4 >= p.max_q;
     c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32
-                  : c.dp == 256 || tiles_of(kWideRows) * p.kv_heads < cus ? kManyRows : kWideRows;
-    if (const char* const forced = plan_override("PW4_ATTN_TILE"); forced && c.tile_rows > 32 && c.dp != 256) {
+                  : c.dp == 128 && 4 * wide_tiles >= (alike ? 4 : 7) * cus && keys_of(kWideRows) >= 24 * kManyKeys ? kWideRows
+                                                                                                                  : kManyRows;
+    if (const char* const forced = plan_override("PW4_ATTN_TILE"); forced && c.tile_rows > 32 && c.dp == 128) {
         c.tile_rows = forced[0] == '2' ? kWideRows : kManyRows;
     }
     const bool few = c.tile_rows <= 32;
@@ -750,18 +763,26 @@ Call plan_call(const pw4_paged_attention_args* a) {
                              : c.tile_rows == 32 ? few_at_once(std::integral_constant<int, 2>{})
                              : c.tile_rows == kManyRows && c.dp != 256 ? 2
                                                                        : 1);
-    // units of a tile: of the keys that a window leaves its rows, or all
-    const int64_t most_keys =
-        p.window == 0 ? p.max_len
-                      : std::min<int64_t>(p.max_len, (int64_t)p.window + (std::min<int64_t>(c.tile_rows, rows) + p.group - 2) / p.group);
-    const int64_t most_units = ceil_div(most_keys, unit) + 1;
+    const int64_t most_units = ceil_div(keys_of(c.tile_rows), unit) + 1;  // of a tile
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
     p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
+    // Whether the keys are split.  A few rows: whole, a workgroup takes 0.5, 0.7 and 1.3 us a unit (heads of
+    // 64 and 128, units of 128 keys; of 256, of 64); the split, a second launch, and the partial outputs' way
+    // through memory, which grow with the tiles.  8 key-value heads, sequences of one length, whole and split, us:
+    //   heads of 64   1 of 1100 keys 9.5 and 10.2, of 1600 11.6 and 10.2; 8 of 2400 15.3 and 15.3, of 4000 22 and 17;
+    //                 32 of 4000 27 and 29
+    //   heads of 128  1 of 777 10.4 and 11.0, of 1100 12.0 and 11.1; 8 of 1600 15.6 and 15.5, of 4000 32 and 19;
+    //                 16 of 2400 22 and 24, of 4000 33 and 24; 32 of 6000 48 and 48, of 8000 68 and 59
+    //   heads of 256  1 of 200 11.8 and 13.2, of 400 15.5 and 13.1; 16 of 777 23 and 25, of 1100 30 and 24
+    // Many rows: the longest tile against the work's share of a place, the join and the partial outputs.  Heads of
+    // 128, tiles of all heads and their keys, whole and split, us: 6 of 777 26 and 31, of 8000 172 and 34; 48 of 4000
+    // 96 and 50; 88 of 1000 31 and 43; 128 of 4000 98 and 70; 176 of 5000 119 and 100; 224 of 1000 31 and 61.
+    const int64_t work = c.tiles * p.kv_heads;
     const char* const forced_split = plan_override("PW4_ATTN_SPLIT");
     const bool wanted = forced_split ? forced_split[0] == '1'
-                        : few ? most_units > (8 * c.tiles * p.kv_heads <= cus ? 7 : 4 * c.tiles * p.kv_heads <= cus ? 16 : 22)
-                              : 2 * c.tiles * p.kv_heads <= slots && most_units > 2 * p.min_units;
+                        : few ? most_units > (c.dp == 256 ? 5 + 20 * work / cus : 9 + 28 * work / cus)
+                              : most_units * (slots - work) > slots * (c.dp == 256 ? 14 + work / 16 : 16 + work / 7);
     p.split = wanted && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
@@ -781,7 +802,7 @@ hipError_t launch(const Call& c, hipStream_t s) {
         e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.plan, s);
     } else if (c.tile_rows == kManyRows) {
         e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.plan, s);
-    } else if constexpr (DP < 256) {
+    } else if constexpr (DP == 128) {
         e = run_attention<fp4_wide_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kWideWaves, wide_stage_bytes<DP>(), c.plan, s);
     } else {
         e = hipErrorInvalidValue;  // no such tile: plan_call
