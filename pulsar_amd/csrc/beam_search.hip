@@ -18,6 +18,7 @@ using namespace pw4;
 namespace {
 
 constexpr int kMaxBeams = 32;
+constexpr int kWaves = 16;  // of the second launch, a wave a beam
 
 struct SelectArgs {
     SliceArgs s;
@@ -27,6 +28,8 @@ struct SelectArgs {
     int32_t* out_rows;
     int64_t* out_tokens;
     uint8_t* out_ended;
+    double* totals;    // workspace [rows, width], more than kWaves beams: the beams' lists
+    uint64_t* keys;
     int32_t beams, width;
 };
 
@@ -55,35 +58,60 @@ struct Lists {
     int length[kMaxBeams];
 };
 
-template <int WAVES>
+// Beam `row`'s continuations as a list, by a wave: totals and keys of logit and token, best first.  Returns
+// the list's length.
+template <int JOIN>
+__device__ __forceinline__ int make_list(const SelectArgs& a, int row, uint64_t* join, double* totals, uint64_t* keys) {
+    const int lane = threadIdx.x & 63, per = a.s.top_k;
+    const double score = a.scores[row];
+    if (a.s.passed != nullptr && a.s.passed[row] != 0) {
+        if (lane == 0) totals[0] = score == score ? score : kLowest;
+        return 1;
+    }
+    const double lse = join_lse(a.s.sums + (int64_t)row * a.s.slices, a.s.slices);
+    join_tops<JOIN>(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, join, [&](int place, uint64_t key) {
+        const double total = score + ((double)unordered((uint32_t)(key >> 32)) - lse);
+        keys[place] = key;
+        totals[place] = total == total ? total : kLowest;
+    });
+    return per;
+}
+
+// The lists of more beams than a workgroup has waves, a wave a list, to the workspace: with two lists a
+// wave, each a chain of loads behind the last, 32 beams of 32003 logits took 21 us in one workgroup; with
+// this launch 7 and 7.
+__global__ __launch_bounds__(kThreads) void list_kernel(const SelectArgs a) {
+    __shared__ uint64_t s_join[kThreads / 64][kJoin];
+    const int row = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    if (row >= a.s.tokens) return;
+    make_list<kJoin>(a, row, s_join[threadIdx.x >> 6], a.totals + (int64_t)row * a.width, a.keys + (int64_t)row * a.width);
+}
+
+// A search's lists, made here (a wave a beam) or read, MADE, from the workspace, become one.
+template <int WAVES, bool MADE>
 __global__ __launch_bounds__(WAVES * 64) void select_kernel(const SelectArgs a) {
-    constexpr int JOIN = WAVES > 4 ? 128 : kJoin;
+    constexpr int JOIN = MADE ? 1 : WAVES > 4 ? 128 : kJoin;
     __shared__ uint64_t s_join[WAVES][JOIN];
     __shared__ uint64_t s_key[kMaxBeams * kMaxTop];
     __shared__ Lists s_lists[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row0 = blockIdx.x * a.beams, per = a.s.top_k;
-    for (int k = wave; k < a.beams; k += WAVES) {
-        const int row = row0 + k;
-        const bool ended = a.s.passed != nullptr && a.s.passed[row] != 0;
-        const double score = a.scores[row];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int row0 = blockIdx.x * a.beams;
+    if constexpr (MADE) {
         Lists& l = s_lists[0];
-        const int at = k * a.width;
-        if (lane == 0) l.length[k] = ended ? 1 : per;
-        if (ended) {
-            if (lane == 0) {
-                l.total[at] = score == score ? score : kLowest;
-                l.which[at] = at;
-            }
-            continue;
+        for (int i = tid; i < a.beams * a.width; i += WAVES * 64) {
+            const int64_t at = (int64_t)row0 * a.width + i;
+            l.total[i] = a.totals[at];
+            l.which[i] = i;
+            s_key[i] = a.keys[at];
         }
-        const double lse = join_lse(a.s.sums + (int64_t)row * a.s.slices, a.s.slices);
-        join_tops<JOIN>(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, s_join[wave], [&](int place, uint64_t key) {
-            const double total = score + ((double)unordered((uint32_t)(key >> 32)) - lse);
-            s_key[at + place] = key;
-            l.total[at + place] = total == total ? total : kLowest;
-            l.which[at + place] = at + place;
-        });
+        if (tid < a.beams) l.length[tid] = a.s.passed != nullptr && a.s.passed[row0 + tid] != 0 ? 1 : a.s.top_k;
+    } else {
+        Lists& l = s_lists[0];
+        for (int k = wave; k < a.beams; k += WAVES) {
+            const int at = k * a.width, length = make_list<JOIN>(a, row0 + k, s_join[wave], l.total + at, s_key + at);
+            for (int i = tid & 63; i < a.width; i += 64) l.which[at + i] = at + i;
+            if ((tid & 63) == 0) l.length[k] = length;
+        }
     }
     // Neighbouring lists become one, of `width` candidates at most, until one is left: a candidate's
     // place there is its own and how many of the other list are ahead of it.
@@ -167,7 +195,8 @@ size_t pw4_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t voca
         return 0;
     }
     const int64_t rows = batch * beams, slices = slices_of(rows, vocab);
-    return sums_bytes(rows, slices) + (size_t)(rows * slices * std::min(width, vocab)) * 8;
+    return sums_bytes(rows, slices) + (size_t)(rows * slices * std::min(width, vocab)) * 8 +
+           (beams > kWaves ? (size_t)(rows * width) * 16 : 0);
 }
 
 int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,
@@ -193,7 +222,9 @@ int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams,
                             reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + sums_bytes(rows, slices)),
                             row_stride, (int32_t)rows, (int32_t)vocab, (int32_t)std::min(width, vocab), slices,
                             (int32_t)ceil_div(vocab, slices)};
-    const SelectArgs a{slicing, scores, end_token, out_scores, out_rows, out_tokens, out_ended, (int32_t)beams, (int32_t)width};
+    double* const totals = reinterpret_cast<double*>(slicing.top + rows * slices * slicing.top_k);
+    const SelectArgs a{slicing, scores, end_token, out_scores, out_rows, out_tokens, out_ended, totals,
+                       reinterpret_cast<uint64_t*>(totals + rows * width), (int32_t)beams, (int32_t)width};
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const dim3 grid(slices, (unsigned)rows);
     const auto run = [&](auto dt) {
@@ -211,11 +242,13 @@ int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams,
     } else {
         run(std::integral_constant<int, PW4_DTYPE_F32>{});
     }
-    // a wave a beam, or two where there are more than 16
     if (beams <= 4) {
-        hipLaunchKernelGGL(select_kernel<4>, dim3((unsigned)batch), dim3(4 * 64), 0, s, a);
+        hipLaunchKernelGGL((select_kernel<4, false>), dim3((unsigned)batch), dim3(4 * 64), 0, s, a);
+    } else if (beams <= kWaves) {
+        hipLaunchKernelGGL((select_kernel<kWaves, false>), dim3((unsigned)batch), dim3(kWaves * 64), 0, s, a);
     } else {
-        hipLaunchKernelGGL(select_kernel<16>, dim3((unsigned)batch), dim3(16 * 64), 0, s, a);
+        hipLaunchKernelGGL(list_kernel, dim3((unsigned)ceil_div(rows, kThreads / 64)), dim3(kThreads), 0, s, a);
+        hipLaunchKernelGGL((select_kernel<kWaves, true>), dim3((unsigned)batch), dim3(kWaves * 64), 0, s, a);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? PW4_OK : report_hip_error(e);
