@@ -1,9 +1,10 @@
 """Beam search over a paged cache, with W4A16 linears.
 
 A small decoder with random int4 weights reads a prompt in chunks, and then keeps the `beams` likeliest
-continuations: each step scores the next tokens (token_logprobs gives the top alternatives of every
-beam), forks the rows of the beams that go on, frees the others' pages, and attends over what the rows
-share.  At the end the pool is compacted.
+continuations.  Each step appends the new tokens' keys, rotated on the way, to the cache (in 16 bits or in
+4), attends over what the rows share, selects the beams that go on and reorders the cache's rows and the
+tokens found so far to follow them; the host queues all of it and waits once, at the end.  Then the pool is
+compacted.
 
     python examples/branching_decode.py
 """
@@ -51,7 +52,8 @@ class Decoder:
         return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(x.dtype)
 
     def forward(self, tokens: torch.Tensor, pos: torch.Tensor, attend) -> torch.Tensor:
-        """Logits [T, vocab] of tokens at positions pos; attend(layer, q, k, v) -> [T, heads, dim]."""
+        """Logits [T, vocab] of tokens at positions pos; attend(layer, q, k, v) -> [T, heads, dim], which
+        rotates q and k by itself where pos is None."""
         def norm(x):
             return torch.nn.functional.rms_norm(x.float(), x.shape[-1:]).half()
 
@@ -59,74 +61,72 @@ class Decoder:
         split = [self.heads * self.dim, self.kv_heads * self.dim, self.kv_heads * self.dim]
         for i, layer in enumerate(self.layers):
             q, k, v = (t.unflatten(-1, (-1, self.dim)) for t in layer["qkv"](norm(x)).split(split, dim=-1))
-            o = attend(i, self.rope(q, pos), self.rope(k, pos), v)
+            if pos is not None:
+                q, k = self.rope(q, pos), self.rope(k, pos)
+            o = attend(i, q, k, v)
             x = x + layer["o"](o.flatten(1))
             x = x + layer["down"](layer["gate_up"](norm(x)))
         return norm(x) @ self.head.t()
 
 
-def paged(cache: PagedKVCache, step: Step):
+def paged(cache: PagedKVCache, step: Step, rope: torch.Tensor):
     def attend(layer, q, k, v):
-        cache.write(layer, k, v, step)
-        return cache.attend(layer, q, step)
+        return cache.attend(layer, cache.append(layer, q, k, v, step, rope), step)
 
     return attend
-
-
-def room(missing: torch.Tensor, what: str) -> None:
-    """Raises where the cache had no room: it took nothing then, and the rows are as they were."""
-    if int(missing):
-        raise RuntimeError(f"{what}: {int(missing)} pages (or table columns) too few")
 
 
 def beam_search(model: Decoder, cache: PagedKVCache, prompt: torch.Tensor, beams: int, steps: int, chunk: int = 48):
     """The `beams` likeliest continuations found, [(log probability, tokens)], likeliest first, and the
     prompt's own log probabilities.  Uses rows 0 to 2 * beams - 1 of the cache."""
     dev, n = prompt.device, prompt.numel()
-    scored = []
+    rope = ops.rope_table(n + steps, model.dim, device=dev)
+    scored, lacked = [], []
     for at in range(0, n, chunk):  # the prompt, in chunks, into row 0
         tokens = prompt[at:at + chunk]
         step = cache.extend([tokens.numel()] + [0] * (cache.rows - 1))
-        room(step.missing, "prompt")
-        logits = model.forward(tokens, torch.arange(at, at + tokens.numel(), device=dev), paged(cache, step))
+        lacked.append(step.missing)
+        logits = model.forward(tokens, None, paged(cache, step, rope))
         after = torch.full_like(tokens, -1)  # the token that follows each one, none behind the last
         after[:min(tokens.numel(), n - at - 1)] = prompt[at + 1:at + chunk + 1]
-        lp, _, _, top, ids = ops.token_logprobs(logits, after, beams)
-        scored.append(lp)
-    alive = [(float(top[-1, j]), 0, [int(ids[-1, j])]) for j in range(beams)]  # (score, row that it continues, tokens)
-    rows, spare = list(range(beams)), list(range(beams, 2 * beams))
-    held = [0]
+        scored.append(ops.token_logprobs(logits, after, 0)[0])
+    scores, rows, tokens = ops.beam_select(logits[-1:], torch.zeros(1, 1, device=dev), beams)
+    found = tokens.new_zeros(beams, steps)
+    found[:, 0] = tokens[0]
+    held, halves = [0], (list(range(beams)), list(range(beams, 2 * beams)))
     for i in range(1, steps + 1):
         # every beam goes on in a row of its own, which shares its parent's full pages
-        room(cache.fork([row for _, row, _ in alive], spare), "fork")
-        cache.free(held)
-        held, spare = spare, rows
-        rows = held
+        lacked.append(cache.reorder(rows, held, halves[i % 2]))
+        held = halves[i % 2]
         if i == steps:
             break
         step = cache.extend([1 if r in held else 0 for r in range(cache.rows)])
-        room(step.missing, "next tokens")
-        tokens = torch.tensor([t[-1] for _, _, t in alive], device=dev)
-        logits = model.forward(tokens, torch.full((beams,), n + i - 1, device=dev), paged(cache, step))
-        _, _, _, top, ids = ops.token_logprobs(logits, torch.full_like(tokens, -1), beams)
-        top, ids = top.tolist(), ids.tolist()
-        grown = [(s + top[b][j], held[b], t + [ids[b][j]]) for b, (s, _, t) in enumerate(alive) for j in range(beams)]
-        alive = sorted(grown, key=lambda g: -g[0])[:beams]
-    return [(s, t) for s, _, t in alive], torch.cat(scored)
+        lacked.append(step.missing)
+        # the step's tokens stand in the order of the rows, as the beams do
+        logits = model.forward(tokens[0], None, paged(cache, step, rope))
+        scores, rows, tokens = ops.beam_select(logits, scores)
+        found, = ops.beam_reorder([found], rows)
+        found[:, i] = tokens[0]
+    lacked = torch.cat(lacked).tolist()
+    if any(lacked):  # the cache took nothing then, and what was computed since means nothing
+        raise RuntimeError(f"too few pages (or table columns), by step: {lacked}")
+    return list(zip(scores[0].tolist(), found.tolist())), torch.cat(scored)
 
 
 def main() -> None:
     torch.manual_seed(1)
     model = Decoder()
-    cache = PagedKVCache(layers=2, pages=256, page_size=16, kv_heads=2, head_dim=64, rows=8, max_seq_len=512,
-                         dtype=torch.float16)
     prompt = torch.randint(0, 1003, (150,), device="cuda:0")
-    found, scored = beam_search(model, cache, prompt, beams=4, steps=12)
-    print(f"prompt: {prompt.numel()} tokens, mean log probability {float(scored[:-1].mean()):.3f}")
-    for score, tokens in found:
-        print(f"{score:9.3f}  {tokens}")
-    used = cache.compact()
-    print(f"pages in use: {int(used)} of {cache.ref_counts.numel()}, the pool's first ones after compacting")
+    for bits in (16, 4):
+        cache = PagedKVCache(layers=2, pages=256, page_size=16, kv_heads=2, head_dim=64, rows=8, max_seq_len=512,
+                             dtype=torch.float16, bits=bits)
+        found, scored = beam_search(model, cache, prompt, beams=4, steps=12)
+        print(f"keys and values in {bits} bits, {cache.pool[0, 0].numel() * cache.pool.element_size()} bytes a page and plane")
+        print(f"prompt: {prompt.numel()} tokens, mean log probability {float(scored[:-1].mean()):.3f}")
+        for score, tokens in found:
+            print(f"{score:9.3f}  {tokens}")
+        used = cache.compact()
+        print(f"pages in use: {int(used)} of {cache.ref_counts.numel()}, the pool's first ones after compacting")
 
 
 if __name__ == "__main__":

@@ -1,8 +1,9 @@
 """A paged key-value cache for the layers of a model, over the operators of pulsar_amd.ops.
 
 The pool holds keys and values of every layer as planes of one tensor, [2 * layers, pages,
-page_size, kv_heads, head_dim] (with bits=4 bytes, the last dimension head_dim / 2 + head_dim / 32), so a page id names the same page in all of them and forking, copying
-and compacting are one call for the whole model.  The book-keeping -- reference counts, block tables,
+page_size, kv_heads, head_dim] (with bits=4 bytes, the last dimension head_dim / 2 + head_dim / 32), so
+a page id names the same page in all of them and forking, copying and compacting are one call for the
+whole model.  The book-keeping -- reference counts, block tables,
 lengths -- is on the device and changes in place; the host keeps only an upper bound of each row's
 length, which sizes the attention's grid.  No method but `lengths` waits for the device.  Methods that
 take lists copy them to the device when they are called, so they do not belong into a captured graph;
@@ -33,6 +34,7 @@ class Step:
     max_q_len: int
     max_seq_len: int
     positions: torch.Tensor | None = None  # of the tokens, int64: PagedKVCache.positions
+    changes: int = -1  # the cache's, when the step was taken
 
 
 class PagedKVCache:
@@ -57,6 +59,7 @@ class PagedKVCache:
         self.block_tables = torch.full((rows, -(-max_seq_len // page_size)), -1, **ints)
         self.seq_lens = torch.zeros(rows, **ints)
         self._most = [0] * rows  # at most so many tokens in each row
+        self._changes = 0  # calls that may have changed a row's length
 
     def layer(self, index: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values of a layer, [pages, page_size, kv_heads, head_dim] (bytes with bits=4)."""
@@ -80,7 +83,8 @@ class PagedKVCache:
         most = self.block_tables.shape[1] * self.page_size  # an extend past a row's table is refused
         self._most = [min(m + c, most) for m, c in zip(self._most, counts)]
         seen = [m for m, c in zip(self._most, counts) if c]
-        return Step(list(counts), cu_q, slots, missing, max(counts), max(seen, default=0))
+        self._changes += 1
+        return Step(list(counts), cu_q, slots, missing, max(counts), max(seen, default=0), changes=self._changes)
 
     def lengths(self) -> list[int]:
         """Each row's tokens, read from the device: this waits for it.  The host's bounds of the rows are
@@ -90,8 +94,11 @@ class PagedKVCache:
         return list(self._most)
 
     def positions(self, step: Step) -> torch.Tensor:
-        """The positions of a step's tokens in their rows, int64 [T], made once a step."""
+        """The positions of a step's tokens in their rows, int64 [T], made once a step from the rows' lengths:
+        before the next step, and before rows are forked, reordered or freed."""
         if step.positions is None:
+            if step.changes != self._changes:
+                raise ValueError("PagedKVCache.positions: the rows have changed since the step was taken")
             n = step.cu_q[1:] - step.cu_q[:-1]
             tokens = step.slots.shape[0]
             row = torch.repeat_interleave(n, output_size=tokens)
@@ -111,7 +118,7 @@ class PagedKVCache:
                interleaved: bool = False) -> torch.Tensor:
         """Rotates the step's queries and keys by their positions in their rows (ops.paged_cache_append's
         rotation, `rope` of at least as many positions as a row has), stores the keys and values and returns
-        the queries.  The positions are taken when a step's first layer is appended: before the next step."""
+        the queries.  The step's positions are taken with the first layer."""
         append = ops.paged_cache_append if self.bits == 16 else ops.paged_cache_append_fp4
         return append(q, k, v, *self.layer(layer), step.slots, rope, self.positions(step), interleaved)
 
@@ -138,30 +145,39 @@ class PagedKVCache:
         missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens, src_rows, dst_rows)
         for s, d in zip(src, dst):
             self._most[d] = self._most[s]
+        self._changes += 1
         return missing
 
     def reorder(self, rows: torch.Tensor, live: list[int], spare: list[int]) -> torch.Tensor:
-        """Beams go on: row spare[i] becomes a copy of row live[rows[i]], rows being int32 on the device
-        (ops.beam_select's of one search), and the rows `live` are given back.  Returns the free pages that
-        lacked (int32 [1]), in which case nothing changed.  The rows `spare` are empty."""
+        """Beams go on: row spare[i] becomes a copy of row live[rows[i]], and the rows `live` are given back.
+        `rows` is int32 on the device, ops.beam_select's rows where live[j] is what row j of its logits
+        belongs to; where one names none of `live`, spare[i] stays empty.  Returns the free pages that lacked
+        (int32 [1]), in which case no row changed, but that what the rows `spare` held is given back first."""
         if len(set(spare)) != len(spare) or set(live) & set(spare) or rows.numel() != len(spare):
             raise ValueError("PagedKVCache.reorder: a spare row for each of rows, each once and not live")
-        if any(self._most[s] for s in spare):
-            raise ValueError("PagedKVCache.reorder: the spare rows must be empty")
-        from_rows, to_rows = self._rows(live, "reorder"), self._rows(spare, "reorder")
+        n = len(live)
+        ints = self._rows(live + spare, "reorder")
+        shifted, to_rows = ints[:n] + 1, ints[n:]
+        if any(self._most[r] for r in spare):
+            ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, to_rows)
+        # a row outside becomes 0 and so -1, a pair that fork passes over
         missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens,
-                                       ops.beam_reorder([from_rows], rows)[0], to_rows)
-        # nothing goes where nothing was copied: row -1 is none
-        ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, torch.where(missing == 0, from_rows, -1))
+                                       ops.beam_reorder([shifted], rows)[0] - 1, to_rows)
+        # nothing goes where nothing was copied: a row below 0 is none
+        ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens,
+                             torch.sub(ints[:n], missing, alpha=self.rows))
+        # (the bounds of `live` stay: the host does not know whether there was room)
         most = max((self._most[r] for r in live), default=0)
         for r in spare:
             self._most[r] = most
+        self._changes += 1
         return missing
 
     def free(self, rows: list[int]) -> None:
         ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, self._rows(rows, "free"))
         for r in rows:
             self._most[r] = 0
+        self._changes += 1
 
     def compact(self) -> torch.Tensor:
         """Moves the pages in use to the pool's start; returns how many there are (int32 [1])."""
