@@ -173,16 +173,20 @@ struct ReorderArgs {
 };
 
 template <typename V>
-__global__ __launch_bounds__(kThreads) void reorder_kernel(const ReorderArgs a) {
+__device__ __forceinline__ void copy_piece(const ReorderArgs& a, int64_t piece) {
     int s = 0;
-    while (s + 1 < a.count && (int64_t)blockIdx.x >= a.end[s]) ++s;
-    const int64_t item = blockIdx.x - (s ? a.end[s - 1] : 0);
+    while (s + 1 < a.count && piece >= a.end[s]) ++s;
+    const int64_t item = piece - (s ? a.end[s - 1] : 0);
     const int64_t i = item / a.pieces[s], begin = (item - i * a.pieces[s]) * kPiece;
     const int64_t row = a.rows[i], bytes = min(kPiece, a.row_bytes[s] - begin);
     const bool there = row >= 0 && row < a.num_rows[s];
     const V* const from = reinterpret_cast<const V*>(a.src[s] + (there ? row : 0) * a.row_bytes[s] + begin);
     V* const to = reinterpret_cast<V*>(a.dst[s] + i * a.row_bytes[s] + begin);
     for (int e = threadIdx.x; e < bytes / (int)sizeof(V); e += kThreads) to[e] = there ? from[e] : V{};
+}
+template <typename V>
+__global__ __launch_bounds__(kThreads) void reorder_kernel(const ReorderArgs a) {
+    for (int64_t piece = blockIdx.x; piece < a.end[a.count - 1]; piece += gridDim.x) copy_piece<V>(a, piece);
 }
 
 }  // namespace
@@ -284,7 +288,7 @@ int pw4_beam_reorder(const pw4_beam_state* states, int64_t count, const int32_t*
             all |= (uint64_t)(uintptr_t)st.src | (uint64_t)(uintptr_t)st.dst | (uint64_t)st.row_bytes;
         }
         if (a.count == 0) break;
-        const dim3 grid((unsigned)items);
+        const dim3 grid((unsigned)std::min<int64_t>(items, 1 << 22));  // (2^32 threads are too many)
         if ((all & 15) == 0) {
             hipLaunchKernelGGL(reorder_kernel<u32x4>, grid, dim3(kThreads), 0, s, a);
         } else if ((all & 3) == 0) {

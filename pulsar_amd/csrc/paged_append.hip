@@ -27,6 +27,7 @@ using namespace pw4;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMostGroups = 1 << 22;  // of a launch of a workgroup a token: 2^32 threads are too many
 
 struct Heads {
     const uint16_t* from;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendArgs a) {
     if (turns && t.known) {
         float cf[8], sf[8];
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {  // (a row of the table is only 4-byte aligned where rot is)
+        for (int e = 0; e < 8; e += 4) {
             *reinterpret_cast<f32x4*>(cf + e) = *reinterpret_cast<const f32x4*>(t.table + 8 * u + e);
             *reinterpret_cast<f32x4*>(sf + e) = *reinterpret_cast<const f32x4*>(t.table + half + 8 * u + e);
         }
@@ -289,11 +290,10 @@ struct Turn {
     }
 };
 
-// Token blockIdx.x; of its heads blockIdx.y's share.  A thread has eight neighbouring elements of a head;
-// four threads have a block of 32.
+// Tokens blockIdx.x, + gridDim.x, ...; of their heads blockIdx.y's share.  A thread has eight neighbouring
+// elements of a head; four threads have a block of 32.
 template <bool BF16, bool FP4>
-__global__ __launch_bounds__(kThreads) void append_any_kernel(const AppendArgs a) {
-    const int token = blockIdx.x;
+__device__ __forceinline__ void append_token(const AppendArgs& a, int token) {
     const int units = a.dim / 8, at_once = kThreads / units;
     const int first = threadIdx.x / units, d0 = (threadIdx.x - first * units) * 8;
     if (first >= at_once) return;
@@ -331,6 +331,10 @@ __global__ __launch_bounds__(kThreads) void append_any_kernel(const AppendArgs a
         for (int e = 0; e < 8; ++e) to[d0 + e] = !t.known ? 0 : turns ? f32_to_out<BF16>(f[e]) : own[e];
     }
 }
+template <bool BF16, bool FP4>
+__global__ __launch_bounds__(kThreads) void append_any_kernel(const AppendArgs a) {
+    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) append_token<BF16, FP4>(a, (int)token);
+}
 
 struct ReadArgs {
     const uint8_t* k_cache;
@@ -340,13 +344,13 @@ struct ReadArgs {
     uint16_t* v;
     int64_t page_bytes, places;
     uint32_t row_codes, row_exps, exps_at;
-    int32_t kv_heads, dim, page_size;
+    int32_t kv_heads, dim, page_size, tokens;
 };
 
 // A token's keys' and values' words of eight codes.
 template <bool BF16>
-__global__ __launch_bounds__(kThreads) void read_kernel(const ReadArgs a) {
-    const int token = blockIdx.x, units = a.dim / 8, items = 2 * a.kv_heads * units;
+__device__ __forceinline__ void read_token(const ReadArgs& a, int token) {
+    const int units = a.dim / 8, items = 2 * a.kv_heads * units;
     const int64_t slot = a.slots[token];
     const bool there = slot >= 0 && slot < a.places;
     const uint32_t page = there ? (uint32_t)slot / (uint32_t)a.page_size : 0;
@@ -375,6 +379,10 @@ __global__ __launch_bounds__(kThreads) void read_kernel(const ReadArgs a) {
         }
         *reinterpret_cast<u32x4*>((is_v ? a.v : a.k) + ((int64_t)token * a.kv_heads + at) * a.dim + d0) = out;
     }
+}
+template <bool BF16>
+__global__ __launch_bounds__(kThreads) void read_kernel(const ReadArgs a) {
+    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x) read_token<BF16>(a, (int)token);
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -454,8 +462,8 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
         if (!vec) {
             const int64_t passes = ceil_div(heads, kThreads / (a->head_dim / 8));
             const int64_t shares = a->num_tokens * passes <= 8 * device_cus() ? passes : 1;
-            hipLaunchKernelGGL((append_any_kernel<BF16, FP4>), dim3((unsigned)a->num_tokens, (unsigned)shares), dim3(kThreads), 0,
-                               s, p);
+            hipLaunchKernelGGL((append_any_kernel<BF16, FP4>), dim3((unsigned)std::min(a->num_tokens, kMostGroups), (unsigned)shares),
+                               dim3(kThreads), 0, s, p);
             return;
         }
         // Rows of lanes of a workgroup, and how many of them share a token: all, each with a head, where
@@ -500,10 +508,10 @@ int pw4_paged_cache_read_fp4(const void* k_cache, const void* v_cache, const int
     const ReadArgs a{static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), slots,
                      static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), page_stride, num_pages * page_size,
                      (uint32_t)head_dim / 2, (uint32_t)head_dim / 32, (uint32_t)(kv_heads * page_size * (head_dim / 2)),
-                     (int32_t)kv_heads, (int32_t)head_dim, (int32_t)page_size};
+                     (int32_t)kv_heads, (int32_t)head_dim, (int32_t)page_size, (int32_t)num_tokens};
     const int64_t passes = ceil_div(2 * kv_heads * (head_dim / 8), kThreads);
     const int64_t shares = num_tokens * passes <= 8 * device_cus() ? passes : 1;
-    const dim3 grid((unsigned)num_tokens, (unsigned)std::min<int64_t>(shares, 65535));
+    const dim3 grid((unsigned)std::min(num_tokens, kMostGroups), (unsigned)shares);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (dtype == PW4_DTYPE_BF16) {
         hipLaunchKernelGGL(read_kernel<true>, grid, dim3(kThreads), 0, s, a);

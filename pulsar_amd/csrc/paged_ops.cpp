@@ -74,7 +74,6 @@ void check_cache(const char* op, const char* name, const at::Tensor& c) {
                 " must be contiguous in its last dimension");
 }
 
-
 void check_half(const char* op, const char* name, const at::Tensor& t) {
     TORCH_CHECK(t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, op, ": ", name,
                 " must be fp16 or bf16");
@@ -538,7 +537,7 @@ std::vector<at::Tensor> beam_reorder_cuda(at::TensorList states, const at::Tenso
     for (const at::Tensor& t : states) {
         check_device(op, rows, {&t});
         TORCH_CHECK(t.dim() >= 1, op, ": states must be at least 1-D");
-        in.push_back(t.contiguous());
+        in.push_back(t.resolve_conj().resolve_neg().contiguous());
         at::DimVector sizes(t.sizes());
         sizes[0] = n;
         out.push_back(fresh(sizes, t.scalar_type(), rows));

@@ -306,6 +306,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
 def rope_table(positions: int, rot: int, base: float = 10000.0, device="cuda:0") -> torch.Tensor:
     """Cosines and sines fp32 [positions, rot] of the angles p base^(-2 i / rot), i < rot / 2, as
     paged_cache_append takes them; the angles are fp64, so far positions are as good as near ones."""
+    if rot % 2 or rot < 0 or positions < 0:
+        raise ValueError(f"rope_table: positions and rot must not be negative and rot even, got {positions} and {rot}")
     half = rot // 2
     rate = base ** (-torch.arange(half, dtype=torch.float64, device=device) / max(half, 1))
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * rate

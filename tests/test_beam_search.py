@@ -427,3 +427,22 @@ def test_writes_stay_in_the_outputs_and_the_workspace(batch, beams, vocab, width
     for a, b in zip((out, rows, tokens), want):
         assert torch.equal(a[:-16].view(b.shape), b) and bool((a[-16:] == 7).all())
     assert bool((ws[n:] == 0x5a).all())
+
+
+@pytest.mark.gpu
+def test_reorder_of_more_rows_than_a_launch_has_workgroups():
+    n = (1 << 24) + 3
+    rows = torch.arange(n, dtype=torch.int32, device=DEV).remainder(7) - 1
+    state = torch.arange(5, dtype=torch.int16, device=DEV) + 100
+    out, = ops.beam_reorder([state], rows)
+    assert torch.equal(out, torch.where((rows >= 0) & (rows < 5), state[rows.clamp(0, 4).long()], 0))
+
+
+@pytest.mark.gpu
+def test_reorder_of_views_that_stand_for_other_values():
+    """Conjugate and negative views hold other numbers than their memory does."""
+    x = torch.randn(5, 3, dtype=torch.complex64, generator=gen(1)).to(DEV)
+    rows = torch.tensor([4, 0, 0], dtype=torch.int32, device=DEV)
+    got = ops.beam_reorder([x.conj(), x.conj().imag, x], rows)
+    for g, w in zip(got, (x.conj(), x.conj().imag, x)):
+        assert torch.equal(g, w[rows.long()])

@@ -428,3 +428,55 @@ def test_opcheck():
     a = _good(4)
     torch.library.opcheck(torch.ops.pulsar.paged_cache_read_fp4.default, (a["k_cache"], a["v_cache"], a["slots"], B),
                           test_utils=utils)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,rot", [(32, 16), (64, 16), (64, 48), (96, 48), (128, 16), (128, 112), (160, 144), (176, 80),
+                                     (224, 96), (256, 208)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotations_that_end_inside_blocks(dim, rot, interleaved):
+    """Vectors of a block of 32 stand with their mates, or where the head has them: the block's exponent is of both."""
+    t, page = 37, 20
+    q, k, v, positions, rope = _case(t, 5, 3, dim, rot, B, dim + rot)
+    k = (k * torch.exp2(torch.randint(-6, 7, k.shape, generator=gen(3)).float())).to(B)  # blocks that differ
+    slots = torch.randperm(3 * page, generator=gen(1))[:t]
+    args = (slots.to(DEV), rope.to(DEV), positions.to(DEV), interleaved)
+    want, size = rotate_ref(k, rope, positions, interleaved)
+    pool = torch.zeros(2, 3, page, 3, dim, dtype=B, device=DEV)
+    check16(ops.paged_cache_append(q.to(DEV), k.to(DEV), v.to(DEV), pool[0], pool[1], *args),
+            *rotate_ref(q, rope, positions, interleaved), B)
+    check16(pool[0].view(-1, 3, dim)[slots.to(DEV)], want, size, B)
+    if dim % 32:
+        return
+    four = to_dev(new_pool(2, 3, page, 3, dim))
+    ops.paged_cache_append_fp4(None, k.to(DEV), v.to(DEV), four[0], four[1], *args)
+    got = ops.paged_cache_read_fp4(four[0], four[1], slots.to(DEV), B)
+    assert torch.equal(got[0].cpu().double(), fp4_round(want.float())[2])
+    assert torch.equal(got[1].cpu().double(), fp4_round(v)[2])
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_has_workgroups():
+    """2^24 workgroups of 256 threads are more than one launch may have."""
+    t, page = (1 << 24) + 3, 64
+    pages = -(-t // page)
+    slots = torch.arange(t, device=DEV).flip(0)
+    k = torch.arange(t, device=DEV).remainder(2039).half()[:, None, None].expand(t, 1, 8)
+    v = torch.arange(t, device=DEV).remainder(1021).half()[:, None, None].expand(t, 1, 8)
+    pool = torch.zeros(2, pages, page, 1, 8, dtype=H, device=DEV)  # heads of 8: one element at a time
+    ops.paged_cache_append(None, k, v, pool[0], pool[1], slots)
+    flat = pool.view(2, -1, 1, 8)[:, :t].flip(1)
+    assert torch.equal(flat[0], k) and torch.equal(flat[1], v)
+    del pool, flat
+    four = torch.zeros(2, pages, page * 32, dtype=torch.uint8, device=DEV)[:, :, :page * 17].unflatten(2, (page, 1, 17))
+    k4, v4 = ((x % 4)[:, :, :1].expand(t, 1, 32) for x in (k, v))  # exact in 4 bits
+    ops.paged_cache_append_fp4(None, k4, v4, four[0], four[1], slots)
+    got = ops.paged_cache_read_fp4(four[0], four[1], slots, H)
+    assert torch.equal(got[0], k4) and torch.equal(got[1], v4)
+
+
+def test_rope_table_refusals():
+    for positions, rot in ((4, 3), (-1, 4), (4, -2)):
+        with pytest.raises(ValueError, match="rope_table"):
+            ops.rope_table(positions, rot, device="cpu")
+    assert ops.rope_table(0, 4, device="cpu").shape == (0, 4) and ops.rope_table(3, 0, device="cpu").shape == (3, 0)
