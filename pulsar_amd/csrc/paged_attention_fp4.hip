@@ -193,7 +193,8 @@ int few_slots(int plan) {
     return std::min(kFewOccupancy<DP, MT> * 4 / kFewWaves<DP>, (160 << 10) / (few_stage_bytes<DP, MT>() + plan));
 }
 
-template <bool BF16, int DP, int MT, bool CAP>
+// ONE: a sequence has one tile; else the call is not split.
+template <bool BF16, int DP, int MT, bool CAP, bool ONE>
 __global__ __launch_bounds__(kFewWaves<DP> * 64) __attribute__((amdgpu_waves_per_eu(kFewOccupancy<DP, MT>)))
 void fp4_few_rows_kernel(const Fp4Params a) {
     constexpr int WAVES = kFewWaves<DP>, MR = 16 * MT, UNIT = kFewUnit<DP>;
@@ -205,7 +206,7 @@ void fp4_few_rows_kernel(const Fp4Params a) {
     uint8_t* const stage = smem + wave * kFewStage<DP>;
     const float k = unit<CAP>(a);
 
-    Pieces<MR, kFewKeys, UNIT, WAVES, true, true> piece;
+    Pieces<MR, kFewKeys, UNIT, WAVES, ONE, ONE> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         // (made anew for each piece: held through all of them, what depends on it takes registers)
@@ -301,7 +302,7 @@ void fp4_few_rows_kernel(const Fp4Params a) {
                 float x[8], top = -kInf;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = s[mt][e / 4][e % 4];
-                cap_scores<CAP, 8>(a, x);
+                cap_scores<CAP, 8, true>(a, x);
                 if (masked) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -467,8 +468,8 @@ void fp4_many_rows_kernel(const Fp4Params a) {
                 s[n % 2] = mfma32x32x16<BF16>(kf[n % kAhead], q[n / 2], s[n % 2]);
                 if (n + kAhead < 2 * KS) kf[n % kAhead] = read_k(n + kAhead);
             }
-            cap_scores<CAP, 16>(a, s[0]);
-            cap_scores<CAP, 16>(a, s[1]);
+            cap_scores<CAP, 16, true>(a, s[0]);
+            cap_scores<CAP, 16, true>(a, s[1]);
             r.mask(key0, h, s);
             float top = -kInf;
 #pragma unroll
@@ -655,8 +656,8 @@ void fp4_wide_rows_kernel(const Fp4Params a) {
                     }
                 }
                 if (__builtin_expect(do_next, 1)) {
-                    cap_scores<CAP, 16>(a, s[0]);
-                    cap_scores<CAP, 16>(a, s[1]);
+                    cap_scores<CAP, 16, true>(a, s[0]);
+                    cap_scores<CAP, 16, true>(a, s[1]);
                     r.mask(next, h, s);
                     float top = -kInf;
 #pragma unroll
@@ -701,6 +702,7 @@ void fp4_wide_rows_kernel(const Fp4Params a) {
 struct Call {
     Fp4Params p;
     int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128 or 256
+    bool narrow;               // tiles of 32 rows where a sequence has several
     int plan;                  // bytes of LDS behind the kernel's stages
     int64_t tiles;             // at most
     size_t bytes;
@@ -743,14 +745,28 @@ Call plan_call(const pw4_paged_attention_args* a) {
     // three waves of 128-row tiles share a SIMD.)
     const int64_t wide_tiles = tiles_of(kWideRows) * p.kv_heads;
     const bool alike = p.max_len / 4 >= p.max_q;
-    c.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32
+    // 32-row tiles, whose waves have keys of their own, take less than half of 128-row tiles' time for one, but are
+    // four times as many, each with the keys to widen: for up to two a CU, over keys that are enough to tell and
+    // too few to split 128-row tiles for.  32 and 128 rows (those whole or split, as below), us, heads of 64 / 128:
+    //   18 tiles (6) of 300 keys 13.3 and 12.1 / 16.8 and 15.8, of 450 14.2 and 14.8 / 17.8 and 19.7, of 1200 18.9 and
+    //   23.9 / 24 and 31, of 2400 25.6 and 24.4 / 33 and 31; 252 (84) of 1200 19.6 and 25.5 / 25 and 35, of 3200 32 and
+    //   39 / 42 and 50, of 4000 38 and 42 / 50 and 54; 324 (108) of 800 21.0 and 20.8 / 27 and 28, of 2400 35 and 44 /
+    //   47 and 66, of 4000 51 and 49 / 65 and 64; 512 (128) of 1200 24.7 and 25.8 / 32 and 35, of 4000 50 and 54 / 65
+    //   and 71, of 6000 68 and 66 / 87 and 88; 576 (144) of 2400 44 and 43 / 70 and 64
+    const int64_t narrow_tiles = tiles_of(32) * p.kv_heads, narrow_keys = keys_of(32);
+    bool narrow = narrow_tiles <= cus ? narrow_keys >= 400 && (narrow_keys - 2048) * cus <= 2304 * narrow_tiles
+                                      : narrow_tiles <= 2 * cus && narrow_keys >= 1000 &&
+                                            (narrow_keys - 1280) * cus <= 1664 * narrow_tiles;
+    const char* const forced_tile = plan_override("PW4_ATTN_TILE");
+    if (forced_tile) narrow = forced_tile[0] == '3';
+    narrow = narrow && rows > 32 && c.dp != 256;
+    c.tile_rows = rows <= 16 ? 16 : rows <= 32 || narrow ? 32
                   : c.dp == 128 && 4 * wide_tiles >= (alike ? 4 : 7) * cus && keys_of(kWideRows) >= 24 * kManyKeys ? kWideRows
                                                                                                                   : kManyRows;
-    if (const char* const forced = plan_override("PW4_ATTN_TILE"); forced && c.tile_rows > 32 && c.dp == 128) {
-        c.tile_rows = forced[0] == '2' ? kWideRows : kManyRows;
-    }
+    if (forced_tile && c.tile_rows > 32 && c.dp == 128) c.tile_rows = forced_tile[0] == '2' ? kWideRows : kManyRows;
     const bool few = c.tile_rows <= 32;
-    c.tiles = few ? p.batch : tiles_of(c.tile_rows);
+    c.narrow = narrow;
+    c.tiles = few && !narrow ? p.batch : tiles_of(c.tile_rows);
     const int unit = !few ? kManyKeys : c.dp == 64 ? kFewUnit<64> : c.dp == 128 ? kFewUnit<128> : kFewUnit<256>;
     // what a split call holds in LDS: a plan, or the tiles of few sequences
     c.plan = !few || p.batch > 64 ? (int)sizeof(Plan) : 64 * (int)sizeof(Tile);
@@ -783,7 +799,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const bool wanted = forced_split ? forced_split[0] == '1'
                         : few ? most_units > (c.dp == 256 ? 5 + 20 * work / cus : 9 + 28 * work / cus)
                               : most_units * (slots - work) > slots * (c.dp == 256 ? 14 + work / 16 : 16 + work / 7);
-    p.split = wanted && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
+    p.split = wanted && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
     if (p.split) {
@@ -797,9 +813,15 @@ template <bool BF16, int DP, bool CAP>
 hipError_t launch(const Call& c, hipStream_t s) {
     hipError_t e;
     if (c.tile_rows == 16) {
-        e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), c.plan, s);
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 1, CAP, true>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 1>(), c.plan, s);
+    } else if (c.tile_rows == 32 && !c.narrow) {
+        e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP, true>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.plan, s);
     } else if (c.tile_rows == 32) {
-        e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), c.plan, s);
+        if constexpr (DP != 256) {
+            e = run_attention<fp4_few_rows_kernel<BF16, DP, 2, CAP, false>>(c.p, c.grid, kFewWaves<DP>, few_stage_bytes<DP, 2>(), 0, s);
+        } else {
+            e = hipErrorInvalidValue;  // no such tile: plan_call
+        }
     } else if (c.tile_rows == kManyRows) {
         e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.plan, s);
     } else if constexpr (DP == 128) {

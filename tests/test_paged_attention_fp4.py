@@ -139,7 +139,7 @@ def test_few_rows_whole_and_split(plan, dim, new, split, units):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("split,units", [(0, None), (1, 1), (1, 3)])
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [32, 128, 256])
 @pytest.mark.parametrize("dim,dtype", [(64, H), (128, B), (96, B), (256, H)])
 def test_many_rows_whole_and_split(plan, dim, dtype, tile, split, units):
     plan(split, units, tile)
@@ -147,6 +147,17 @@ def test_many_rows_whole_and_split(plan, dim, dtype, tile, split, units):
     _run([900, 333], [200, 333], heads=1, group=3, dim=dim, dtype=dtype, window=150, cap=4.0, page=8, seed=dim)
     _run([1000, 50], [70, 50], heads=1, group=7, dim=dim, dtype=dtype, page=24, window=300, seed=dim)
     _run([500], [499], heads=3, group=1, dim=dim, dtype=dtype, page=7, extra=5, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_chunks_of_middling_size(dim, dtype):
+    """A few chunks over some hundred to some thousand keys: tiles of 32 rows, by the rule."""
+    _run([1500, 800, 0, 2], [100, 60, 0, 2], heads=2, group=4, dim=dim, dtype=dtype, seed=dim)
+    _run([2900, 450, 777], [33, 130, 1], heads=4, group=7, dim=dim, dtype=dtype, page=24, cap=5.0, extra=3, seed=dim)
+    _run([1300] * 9, [40] * 9, heads=8, group=4, dim=dim, dtype=dtype, seed=dim)  # more of them than CUs
+    _run([3000, 100], [90, 100], heads=1, group=3, dim=dim, dtype=dtype, window=500, seed=dim)
 
 
 @pytest.mark.gpu
@@ -206,7 +217,7 @@ def test_pages_behind_the_window_may_be_gone(new):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("split,tile", [(None, None), (0, 256), (1, 128)])
+@pytest.mark.parametrize("split,tile", [(None, None), (0, 256), (1, 128), (None, 32)])
 @pytest.mark.parametrize("new,group", [(7, 1), (40, 1), (40, 4), (300, 2)])
 @pytest.mark.parametrize("dim", [64, 96])
 def test_values_of_nan_reach_only_the_queries_that_see_them(plan, new, group, dim, split, tile):
@@ -231,7 +242,7 @@ def test_values_of_nan_reach_only_the_queries_that_see_them(plan, new, group, di
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("split", [0, 1])
-@pytest.mark.parametrize("new,tile", [(1, None), (7, None), (60, 128), (200, 256)])
+@pytest.mark.parametrize("new,tile", [(1, None), (7, None), (60, 128), (200, 256), (60, 32)])
 def test_nan_scores_have_a_nan_lse(plan, new, tile, split):
     """A query of NaN, and a key with a block of NaN for the queries that see it: out and lse are NaN, and
     no other row's change."""
@@ -356,7 +367,7 @@ def test_page_ids_outside_the_pool_read_its_last_page(new, name):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("split", [0, 1])
-@pytest.mark.parametrize("most,tile", [(0, None), (1, None), (5, None), (40, 128), (90, 256)])
+@pytest.mark.parametrize("most,tile", [(0, None), (1, None), (5, None), (40, 128), (90, 256), (40, 32), (90, 32)])
 def test_queries_past_max_q_len_are_empty(plan, most, tile, split):
     plan(split, 1, tile)
     lens, new, dim = [300, 150, 2, 40], [100, 150, 2, 0], 64
@@ -528,7 +539,7 @@ def test_no_sequences_and_a_far_bound(new):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("split", [0, 1])
-@pytest.mark.parametrize("tile,new", [(None, 1), (None, 7), (128, 40), (256, 150)])
+@pytest.mark.parametrize("tile,new", [(None, 1), (None, 7), (128, 40), (256, 150), (32, 40)])
 @pytest.mark.parametrize("dim", [64, 96, 256])
 def test_writes_stay_in_the_outputs_and_the_workspace(plan, dim, tile, new, split):
     """The C entry on buffers with a margin behind each."""
@@ -549,7 +560,7 @@ def test_writes_stay_in_the_outputs_and_the_workspace(plan, dim, tile, new, spli
               max_seq_len=900, scale=dim ** -0.5, dtype=1)
     lib = _lib()
     size = lib.pw4_paged_attention_fp4_workspace_size(ctypes.byref(a))
-    assert (size > 0) == bool(split)
+    assert (size > 0) == (split == 1 and not (tile == 32 and dim < 256))  # (tiles of 32 rows are not split)
     ws = torch.full((size + 256,), 0x5a, dtype=torch.uint8, device=DEV)
     torch.cuda.synchronize()
     assert lib.pw4_paged_attention_fp4(ctypes.byref(a), ws.data_ptr(), size, None) == 0
