@@ -64,12 +64,19 @@ template <int JOIN>
 __device__ __forceinline__ int make_list(const SelectArgs& a, int row, uint64_t* join, double* totals, uint64_t* keys) {
     const int lane = threadIdx.x & 63, per = a.s.top_k;
     const double score = a.scores[row];
-    if (a.s.passed != nullptr && a.s.passed[row] != 0) {
+    const SliceSums* const sums = a.s.sums + (int64_t)row * a.s.slices;
+    const uint64_t* const tops = a.s.top + (int64_t)row * a.s.slices * per;
+    // one trip to memory: the lines that the steps below read one after the other
+    const uint64_t line = tops[min(lane * 16, a.s.slices * per - 1)];
+    const float sum = sums[min(lane, a.s.slices - 1)].m;
+    const bool passed = a.s.passed != nullptr && a.s.passed[row] != 0;
+    asm volatile("" ::"v"(line), "v"(sum));
+    if (passed) {
         if (lane == 0) totals[0] = score == score ? score : kLowest;
         return 1;
     }
-    const double lse = join_lse(a.s.sums + (int64_t)row * a.s.slices, a.s.slices);
-    join_tops<JOIN>(a.s.top + (int64_t)row * a.s.slices * per, a.s.slices, per, join, [&](int place, uint64_t key) {
+    const double lse = join_lse(sums, a.s.slices);
+    join_tops<JOIN>(tops, a.s.slices, per, join, [&](int place, uint64_t key) {
         const double total = score + ((double)unordered((uint32_t)(key >> 32)) - lse);
         keys[place] = key;
         totals[place] = total == total ? total : kLowest;
