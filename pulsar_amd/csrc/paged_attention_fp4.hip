@@ -206,7 +206,7 @@ void fp4_few_rows_kernel(const Fp4Params a) {
     uint8_t* const stage = smem + wave * kFewStage<DP>;
     const float k = unit<CAP>(a);
 
-    Pieces<MR, kFewKeys, UNIT, WAVES, ONE, ONE> piece;
+    Pieces<MR, kFewKeys, UNIT, WAVES, ONE, ONE, !ONE> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         // (made anew for each piece: held through all of them, what depends on it takes registers)
@@ -395,7 +395,7 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     const int vr = 4 * h + ((c & 15) >> 2);
     const uint32_t v_at = (uint32_t)(kManyStage<DP> / 2 + vr * DP * 2 +
                                      ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) + (c & 1) * 8);
-    Pieces<MR, KEYS, KEYS, WAVES, false> piece;
+    Pieces<MR, KEYS, KEYS, WAVES, false, false, true> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
@@ -556,7 +556,7 @@ void fp4_wide_rows_kernel(const Fp4Params a) {
     const int vr = 4 * h + ((c & 15) >> 2);
     const uint32_t v_at = (uint32_t)(vr * DP * 2 + ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) +
                                      (c & 1) * 8);
-    Pieces<MR, KEYS, KEYS, kWideWaves, false> piece;
+    Pieces<MR, KEYS, KEYS, kWideWaves, false, false, true> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
@@ -802,6 +802,9 @@ Call plan_call(const pw4_paged_attention_args* a) {
     p.split = wanted && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
     if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
+    // (6 chunks in a window of 1024, 270 tiles, those of the fifth chunk a third as long: 38 us, in the sequences'
+    // order 50)
+    p.order = p.batch > 1 && p.batch <= 64 && c.grid > cus;
     if (p.split) {
         c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
         c.bytes = partial_bytes(c.grid, c.tile_rows, p.dim);

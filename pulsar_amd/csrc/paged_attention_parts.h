@@ -56,6 +56,7 @@ struct Params {
     int32_t flat;            // 2: pages of a power of two of keys, 16 at least; 1: of a multiple of 8
     int32_t min_units;       // split: units (blocks of keys) a workgroup takes at least
     int32_t split;           // 1: runs of units over the grid; 0: a workgroup a tile and head
+    int32_t order;           // whole: up to 64 sequences are taken by the lengths of their tiles (Pieces' ORDER)
 };
 
 // ---- small device parts ------------------------------------------------------
@@ -519,7 +520,9 @@ __device__ __forceinline__ void write_plan(const Params& a, int i, int begin, in
 // A workgroup's pieces of work, one after the other: units [u0, u1) of a tile and
 // head, for partial slot `slot`, or the whole of it (-1).  ONE: a sequence has one tile;
 // IN_LDS: those of up to 64 sequences are held in LDS, 64 Tiles at the plan's place, and not in registers.
-template <int MR, int KEYS, int UNIT, int WAVES, bool ONE, bool IN_LDS = false>
+// ORDER: of whole tiles more than run alone on a CU, the sequences with the longer ones come first, so that
+// those that have to share one, or come late, are short.
+template <int MR, int KEYS, int UNIT, int WAVES, bool ONE, bool IN_LDS = false, bool ORDER = false>
 struct Pieces {
     Tile t;
     int head, u0, u1, slot;
@@ -542,6 +545,23 @@ struct Pieces {
         t.lo = __builtin_amdgcn_readfirstlane(t.lo);
         t.hi = __builtin_amdgcn_readfirstlane(t.hi);
         t.base = __builtin_amdgcn_readfirstlane(t.base);
+    }
+
+    // Lane b of a wave has sequence b and its number of tiles: now the sequence that is b-th by its first and
+    // last tile's units.
+    __device__ __forceinline__ void by_length(const Params& a, int& b, int& n) const {
+        int units = 0, place = b;
+        if (n > 0) {
+            const Sequence s = sequence(a, b);
+            units = units_of<KEYS>(tile_of<MR, KEYS>(a, b, 0, s)) + units_of<KEYS>(tile_of<MR, KEYS>(a, b, n - 1, s));
+        }
+        if (b < a.batch) place = 0;
+        for (int other = 0; other < a.batch; ++other) {
+            const int theirs = __builtin_amdgcn_readlane(units, other);
+            place += b < a.batch && (theirs > units || (theirs == units && other < b));
+        }
+        n = __builtin_amdgcn_ds_permute(place * 4, n);
+        b = __builtin_amdgcn_ds_permute(place * 4, b);
     }
 
     // Every thread of the workgroup calls these two.
@@ -599,13 +619,14 @@ struct Pieces {
             }
             int before = 0;
             for (int b0 = 0; b0 < a.batch; b0 += 64) {
-                const int b = b0 + lane;
-                const int mine = b < a.batch ? (sequence(a, b).n * a.group + MR - 1) / MR : 0;
+                int b = b0 + lane;
+                int mine = b < a.batch ? (sequence(a, b).n * a.group + MR - 1) / MR : 0;
+                if (ORDER && a.order) by_length(a, b, mine);
                 const int upto = before + wave_inclusive_scan(mine);
                 const uint64_t past = __ballot(upto > rank);
                 if (past != 0) {
                     const int l = __builtin_ctzll(past);
-                    set_tile(a, b0 + l, __builtin_amdgcn_readlane(upto, l) - 1 - rank);
+                    set_tile(a, __builtin_amdgcn_readlane(b, l), __builtin_amdgcn_readlane(upto, l) - 1 - rank);
                     u1 = units_of<UNIT>(t);
                     return true;
                 }

@@ -156,8 +156,22 @@ def test_chunks_of_middling_size(dim, dtype):
     """A few chunks over some hundred to some thousand keys: tiles of 32 rows, by the rule."""
     _run([1500, 800, 0, 2], [100, 60, 0, 2], heads=2, group=4, dim=dim, dtype=dtype, seed=dim)
     _run([2900, 450, 777], [33, 130, 1], heads=4, group=7, dim=dim, dtype=dtype, page=24, cap=5.0, extra=3, seed=dim)
-    _run([1300] * 9, [40] * 9, heads=8, group=4, dim=dim, dtype=dtype, seed=dim)  # more of them than CUs
+    if dim == 64:
+        _run([1100] * 9, [40] * 9, heads=8, group=4, dim=dim, dtype=dtype, seed=dim)  # more of them than CUs
     _run([3000, 100], [90, 100], heads=1, group=3, dim=dim, dtype=dtype, window=500, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,tile", [(2, 32), (7, 128), (63, 256), (64, 32), (64, 128), (65, 128)])
+def test_sequences_of_mixed_lengths(plan, batch, tile):
+    """More tiles than CUs: up to 64 sequences are taken by their tiles' lengths, whatever their order; some
+    have no new tokens, and some no keys."""
+    plan(0, None, tile)
+    rows = torch.randint(0, 40, (batch,), generator=gen(batch)) * 300 // (batch + 10)
+    new = [0 if i % 5 == 3 else int(n) for i, n in enumerate(rows)]
+    new[-1] = 700 if batch < 10 else 90
+    lens = [n + int(p) for n, p in zip(new, torch.randint(0, 300, (batch,), generator=gen(1)))]
+    _run(lens, new, heads=8, group=2, dim=128 if tile == 256 else 64, window=200 * (batch % 2), seed=batch)
 
 
 @pytest.mark.gpu
