@@ -7,8 +7,15 @@
 // sums added in fp64, and its best candidates in order.  No beam gives more than `width` of the
 // new ones, so width times beams candidates are left, in lists that fall by total, which are
 // merged pair by pair: a candidate's place in the merged list is its own and, by bisection,
-// how many of the other list are ahead.  Totals are fp64: scores of some hundred tokens have fp32 steps of 1e-5, within which
-// beams would tie.
+// how many of the other list are ahead.  Totals are fp64: scores of some hundred tokens have fp32
+// steps of 1e-5, within which beams would tie.
+//
+// 32 searches of 8 beams over 100003 bf16 logits (51 MB) take 14 us for the first launch (3.7 TB/s; vector
+// units busy 37% of the cycles, waves waiting 53%), 7.4 for the second and 3.8 to reorder 500 tokens a
+// beam; 23.5 a call of both.  The second launch is a chain of steps by one workgroup a search, waves
+// waiting 83% of their time; one that ranked every candidate against all others took 111 us for 32
+// beams, merging 34, and with the lists made in a launch of their own 26, all three launches and the
+// reordering.
 #include "logit_slices.h"
 
 #include <type_traits>
@@ -179,6 +186,8 @@ struct ReorderArgs {
     int32_t count;
 };
 
+// A row's piece of a state: 16 KB a workgroup, so that short rows of many beams and long rows of few
+// both spread.
 template <typename V>
 __device__ __forceinline__ void copy_piece(const ReorderArgs& a, int64_t piece) {
     int s = 0;

@@ -12,6 +12,15 @@
 // operand as it is, q's elements being put in the same order; V goes to LDS (and K too, where
 // waves share it), from where it is read transposed.  A key index outside what some row of the
 // tile sees is clamped to one that is seen, as there.
+//
+// Three kernels, by the rows of a tile (plan_call has the rules and both sides' times); their bounds on
+// an MI355X, heads of 128, 4 query heads on each of 8 key-value heads, bf16:
+//   16, 32   waves with keys of their own.  Memory: 16 tokens over 2 to 32 thousand keys, 200 MB, 41 us (4.9
+//            TB/s, what a copy reaches) and 5.8 for the join; vector units 43% busy, half of it widening.
+//   128      four waves share blocks of 64 keys.  Latency, with a wave or two on a SIMD: 6 chunks of 101 and
+//            707 tokens in a window of 1024 keys (heads of 64, a cap), 35 us.
+//   256      eight waves in turns.  A prompt of 8192 tokens 530 to 560 us, 1.0 PFLOP/s: matrix cores 43% and
+//            vector units 49% busy; over 16-bit keys 515, the rest is the widening.
 #include "paged_attention_parts.h"
 
 #include <type_traits>
@@ -166,9 +175,11 @@ __device__ __forceinline__ u32x2 transposed(uint32_t at, int i) {
 
 // ---- few rows --------------------------------------------------------------------
 
-// Up to 16 MT query rows.  Each wave takes blocks of 32 keys of its own: K straight from registers,
-// V through 32 rows of LDS of its own (no barrier); the next block's codes are under way during the
-// softmax and the second product.
+// 16 MT query rows, of a sequence that has no more or one of its tiles.  Each wave takes blocks of 32 keys
+// of its own: K straight from registers, V through 32 rows of LDS of its own (no barrier); the next block's
+// codes are under way during the softmax and the second product.  Memory is hidden by waves, so registers
+// are held to four a SIMD (16 rows, heads of 128; 53 us for 200 MB of keys where two had 76) and to three (32
+// rows; 79 us where two had 85), for which the queries lie in LDS.
 constexpr int kFewKeys = 32;
 constexpr int kAhead = 4;  // operands read ahead of their products
 template <int DP>
@@ -178,15 +189,18 @@ constexpr int kFewUnit = kFewKeys * kFewWaves<DP>;
 template <int DP>
 constexpr int kFewStage = kFewKeys * DP * 2;  // V of a block, bytes
 
+// Whether the queries lie in LDS, operand by operand, rather than in every wave's registers.
+template <int DP, int MT>
+constexpr bool kQueryInLds = DP == 128 && MT == 2;
 template <int DP, int MT>
 constexpr int few_stage_bytes() {
-    const int stages = kFewWaves<DP> * kFewStage<DP>, join = kFewWaves<DP> * 16 * MT * (DP + 4) * 4;
+    const int stages = kFewWaves<DP> * kFewStage<DP> + (kQueryInLds<DP, MT> ? 16 * MT * DP * 2 : 0), join = kFewWaves<DP> * 16 * (DP + 4) * 4;  // 16 rows at a time
     return stages > join ? stages : join;
 }
 
 // Waves on a SIMD that a kernel's registers are held to.
 template <int DP, int MT>
-constexpr int kFewOccupancy = DP == 64 ? MT == 1 ? 5 : 3 : DP == 128 ? MT == 1 ? 4 : 2 : MT == 1 ? 2 : 1;
+constexpr int kFewOccupancy = DP == 64 ? MT == 1 ? 5 : 3 : DP == 128 ? MT == 1 ? 4 : 3 : MT == 1 ? 2 : 1;
 // Its workgroups on a CU, by these and by LDS (160 KB), with `plan` bytes behind the stages.
 template <int DP, int MT>
 int few_slots(int plan) {
@@ -246,13 +260,23 @@ void fp4_few_rows_kernel(const Fp4Params a) {
         for (int mt = 0; mt < MT; ++mt) {
             load_query<KS>(a, t, head, mt * 16 + c, g * KS, 1, q[mt]);
         }
+        constexpr bool QLDS = kQueryInLds<DP, MT>;
+        u32x4* const q_lds = reinterpret_cast<u32x4*>(smem + WAVES * kFewStage<DP>);
+        if constexpr (QLDS) {  // operand (mt, st) of a lane: 64 lanes side by side
+            static_assert(MT * KS % WAVES == 0, "the waves store as many each");
+#pragma unroll
+            for (int i = 0; i < MT * KS; ++i) {
+                if (i % WAVES == wave) q_lds[i * 64 + lane] = q[i / KS][i % KS];
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int pos = t.first_pos + (t.row0 + mt * 16 + c) / a.group;
             row_hi[mt] = min(pos + 1, t.hi);
             row_lo[mt] = a.window > 0 ? pos + 1 - a.window : 0;
 #pragma unroll
-            for (int st = 0; st < KS; ++st) asm volatile("" : "+v"(q[mt][st]));  // here, not waited for in the loop
+            for (int st = 0; st < KS && !QLDS; ++st) asm volatile("" : "+v"(q[mt][st]));  // here, not waited for in the loop
         }
         // blocks inside [all_lo, all_hi) are seen by every row of the tile
         const int all_hi = min(t.first_pos + t.row0 / a.group + 1, t.hi);
@@ -274,15 +298,31 @@ void fp4_few_rows_kernel(const Fp4Params a) {
             const int key0 = first_of(i);
             f32x4 s[MT][2];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
+            for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) s[mt][kt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (QLDS) {
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
-                    const u32x4 kf = widen<BF16, DP>(from.lane, kq[kt], st);
+                    u32x4 qf[MT];
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, q[mt][st], s[mt][kt]);
+                    for (int mt = 0; mt < MT; ++mt) qf[mt] = q_lds[(mt * KS + st) * 64 + lane];
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) {
+                        const u32x4 kf = widen<BF16, DP>(from.lane, kq[kt], st);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, qf[mt], s[mt][kt]);
+                    }
                 }
+            } else {
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int st = 0; st < KS; ++st) {
+                        const u32x4 kf = widen<BF16, DP>(from.lane, kq[kt], st);
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) s[mt][kt] = mfma16x16x32<BF16>(kf, q[mt][st], s[mt][kt]);
+                    }
             }
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
@@ -356,7 +396,7 @@ void fp4_few_rows_kernel(const Fp4Params a) {
             asm volatile("" ::: "memory");
         }
         __syncthreads();  // every wave is done with its stage
-        join_waves<Fp4Keys, BF16, DP, MT, WAVES, CAP>(a, t, smem, wave, head, slot, begin, end, k, m, z, o);
+        join_waves<Fp4Keys, BF16, DP, MT, WAVES, CAP, MT>(a, t, smem, wave, head, slot, begin, end, k, m, z, o);
         __syncthreads();  // the stages are used again
     }
     clear_rest(a);
@@ -799,7 +839,8 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const bool wanted = forced_split ? forced_split[0] == '1'
                         : few ? most_units > (c.dp == 256 ? 5 + 20 * work / cus : 9 + 28 * work / cus)
                               : most_units * (slots - work) > slots * (c.dp == 256 ? 14 + work / 16 : 16 + work / 7);
-    p.split = wanted && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles && c.tiles * p.kv_heads * most_units < INT_MAX;
+    p.split = wanted && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles &&
+              c.tiles * p.kv_heads * most_units < INT_MAX;
     if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
     // (6 chunks in a window of 1024, 270 tiles, those of the fifth chunk a third as long: 38 us, in the sequences'
@@ -834,10 +875,15 @@ hipError_t launch(const Call& c, hipStream_t s) {
     }
     if (e != hipSuccess || !c.p.split) return e;
     const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(c.tile_rows, (int64_t)c.p.max_q * c.p.group));
+    // A wave a row to join where rows are enough, a workgroup where not.  Both launches, workgroup and wave, us,
+    // heads of 128: 16 tokens over 2 to 32 thousand keys (512 rows) 46 and 48, two of each 48 and 50, four (2048) 54
+    // and 53, eight 76 and 72, eight of 48 sequences 173 and 156, one of each (1536) 128 and 125; eight of 2 sequences
+    // (512) 45 and 55.
+    const bool wave_a_row = rows * c.tiles * c.p.kv_heads >= 6 * device_cus();
     if (c.tile_rows == 16) {
-        run_row_join<16, BF16>(c.p, c.tiles, rows, c.grid, s);
+        wave_a_row ? run_join<16, BF16>(c.p, c.tiles, c.grid, s) : run_row_join<16, BF16>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == 32) {
-        run_row_join<32, BF16>(c.p, c.tiles, rows, c.grid, s);
+        wave_a_row ? run_join<32, BF16>(c.p, c.tiles, c.grid, s) : run_row_join<32, BF16>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == kManyRows) {
         run_join<kManyRows, BF16>(c.p, c.tiles, c.grid, s);
     } else {

@@ -673,57 +673,64 @@ struct Pieces {
 
 // The waves of a few-rows workgroup, each with keys of its own, join in LDS: rows of DP + 4
 // floats (maximum, sum behind the outputs) from `smem` on.  o[mt][d] holds elements 16 d + 4 g
-// .. + 3 of row 16 mt + c, m its maximum, z the lane's share of its sum, over keys [begin, end).
-template <typename Keys, bool BF16, int DP, int MT, int WAVES, bool CAP, typename P>
+// .. + 3 of row 16 mt + c, m its maximum, z the lane's share of its sum, over keys [begin, end).  PARTS: the rows
+// go through LDS in so many parts, in as much less of it.
+template <typename Keys, bool BF16, int DP, int MT, int WAVES, bool CAP, int PARTS = 1, typename P>
 __device__ __forceinline__ void join_waves(const P& a, const Tile& t, uint8_t* smem, int wave, int head, int slot, int begin,
                                            int end, float k, const float (&m)[MT], const float (&z)[MT],
                                            const f32x4 (&o)[MT][DP / 16]) {
-    constexpr int MR = 16 * MT, DT = DP / 16;
+    constexpr int MR = 16 * MT, DT = DP / 16, PR = MR / PARTS;
+    static_assert(MT % PARTS == 0, "whole tiles of 16 rows");
     int lane = threadIdx.x & 63;
     if (Keys::kFresh) asm volatile("" : "+v"(lane));
     const int c = lane & 15, g = lane >> 4;
     constexpr int kRow = DP + 4;
     float* const join = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        float* const row = join + (wave * MR + mt * 16 + c) * kRow;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + 4 * g) = o[mt][d];
-        const float all = sum_halves(sum_quarters(z[mt]));
-        if (g == 0) {
-            row[DP] = held_max<BF16>(m[mt], k);
-            row[DP + 1] = all;
-        }
-    }
-    __syncthreads();
     bool bad = false;
-    for (int row = wave; row < t.rows; row += WAVES) {
-        float m2 = -kInf, sum = 0.f, w[WAVES];
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) m2 = fmaxf(m2, join[(v * MR + row) * kRow + DP]);
+    for (int part = 0; part < PARTS; ++part) {
+        if (part > 0) __syncthreads();
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) {
-            const float mv = join[(v * MR + row) * kRow + DP];
-            w[v] = mv == -kInf ? 0.f : __builtin_amdgcn_exp2f(mv - m2);
-            sum += w[v] * join[(v * MR + row) * kRow + DP + 1];
+        for (int mt = part * MT / PARTS; mt < (part + 1) * MT / PARTS; ++mt) {
+            float* const row = join + (wave * PR + mt * 16 - part * PR + c) * kRow;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(row + d * 16 + 4 * g) = o[mt][d];
+            const float all = sum_halves(sum_quarters(z[mt]));
+            if (g == 0) {
+                row[DP] = held_max<BF16>(m[mt], k);
+                row[DP + 1] = all;
+            }
         }
-        const float inv = slot >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        uint16_t* const to = slot >= 0 ? nullptr : out_row(a, t, head, row);
-        for (int d = lane; d < a.dim; d += 64) {
-            float x = 0.f;
+        __syncthreads();
+        for (int row = part * PR + wave; row < min(t.rows, (part + 1) * PR); row += WAVES) {
+            const float* const of_row = join + (row - part * PR) * kRow;  // wave v's is v * PR rows on
+            float m2 = -kInf, sum = 0.f, w[WAVES];
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) m2 = fmaxf(m2, of_row[v * PR * kRow + DP]);
 #pragma unroll
             for (int v = 0; v < WAVES; ++v) {
-                if (w[v] != 0.f) x += w[v] * join[(v * MR + row) * kRow + d];
+                const float mv = of_row[v * PR * kRow + DP];
+                w[v] = mv == -kInf ? 0.f : __builtin_amdgcn_exp2f(mv - m2);
+                sum += w[v] * of_row[v * PR * kRow + DP + 1];
             }
-            bad |= x - x != 0.f;
-            if (slot >= 0) {
-                a.part_o[((int64_t)slot * MR + row) * a.dim + d] = x;
-            } else {
-                to[d] = f32_to_out<BF16>(x * inv);
+            const float inv = slot >= 0 ? 1.f : sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+            uint16_t* const to = slot >= 0 ? nullptr : out_row(a, t, head, row);
+            for (int d = lane; d < a.dim; d += 64) {
+                float x = 0.f;
+#pragma unroll
+                for (int v = 0; v < WAVES; ++v) {
+                    if (w[v] != 0.f) x += w[v] * of_row[v * PR * kRow + d];
+                }
+                bad |= x - x != 0.f;
+                if (slot >= 0) {
+                    a.part_o[((int64_t)slot * MR + row) * a.dim + d] = x;
+                } else {
+                    to[d] = f32_to_out<BF16>(x * inv);
+                }
             }
+            if (lane == 0) store_stats<MR, BF16>(a, t, head, row, slot, m2, sum);
+            bad |= sum - sum != 0.f;
         }
-        if (lane == 0) store_stats<MR, BF16>(a, t, head, row, slot, m2, sum);
-        bad |= sum - sum != 0.f;
     }
     if (__any(bad) && must_repeat<Keys, BF16>(a, t, head, DP)) {
         for (int row = wave; row < t.rows; row += WAVES) {
