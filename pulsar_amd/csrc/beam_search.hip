@@ -10,9 +10,9 @@
 // how many of the other list are ahead.  Totals are fp64: scores of some hundred tokens have fp32
 // steps of 1e-5, within which beams would tie.
 //
-// 32 searches of 8 beams over 100003 bf16 logits (51 MB) take 14 us for the first launch (3.7 TB/s; vector
-// units busy 37% of the cycles, waves waiting 53%), 7.4 for the second and 3.8 to reorder 500 tokens a
-// beam; 23.5 a call of both.  The second launch is a chain of steps by one workgroup a search, waves
+// 32 searches of 8 beams, a fifth of them ended, over 100003 bf16 logits (41 MB) take 14 us for the first
+// launch (3.0 TB/s; vector units busy 36% of the cycles, waves waiting 52%), 7.3 for the second and 3.7 to
+// reorder 500 tokens a beam; 24 a call of both.  The second launch is a chain of steps by one workgroup a search, waves
 // waiting 83% of their time; one that ranked every candidate against all others took 111 us for 32
 // beams, merging 34, and with the lists made in a launch of their own 26, all three launches and the
 // reordering.

@@ -16,11 +16,11 @@
 // Three kernels, by the rows of a tile (plan_call has the rules and both sides' times); their bounds on
 // an MI355X, heads of 128, 4 query heads on each of 8 key-value heads, bf16:
 //   16, 32   waves with keys of their own.  Memory: 16 tokens over 2 to 32 thousand keys, 200 MB, 41 us (4.9
-//            TB/s, what a copy reaches) and 5.8 for the join; vector units 43% busy, half of it widening.
+//            TB/s, what a copy reaches) and 5.8 for the join; vector units 42% busy.
 //   128      four waves share blocks of 64 keys.  Latency, with a wave or two on a SIMD: 6 chunks of 101 and
 //            707 tokens in a window of 1024 keys (heads of 64, a cap), 35 us.
 //   256      eight waves in turns.  A prompt of 8192 tokens 530 to 560 us, 1.0 PFLOP/s: matrix cores 43% and
-//            vector units 49% busy; over 16-bit keys 515, the rest is the widening.
+//            vector units 48% busy; over 16-bit keys 515, the rest is the widening.
 #include "paged_attention_parts.h"
 
 #include <type_traits>
