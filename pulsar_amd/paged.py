@@ -93,6 +93,11 @@ class PagedKVCache:
         self._most = self.seq_lens.tolist()
         return list(self._most)
 
+    def _check(self, x: torch.Tensor, what: str) -> None:
+        # 4 bits hold magnitudes of bf16 that fp16 has not, and do not know which they are of
+        if self.bits == 4 and x.dtype != self.dtype:
+            raise ValueError(f"PagedKVCache.{what}: the cache is of {self.dtype}, got {x.dtype}")
+
     def positions(self, step: Step) -> torch.Tensor:
         """The positions of a step's tokens in their rows, int64 [T], made once a step from the rows' lengths:
         before the next step, and before rows are forked, reordered or freed."""
@@ -109,6 +114,7 @@ class PagedKVCache:
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, step: Step) -> None:
         """Stores the step's keys and values [T, kv_heads, head_dim] of a layer."""
+        self._check(k, "write")
         if self.bits == 16:
             ops.paged_cache_write(k, v, *self.layer(layer), step.slots)
         else:
@@ -119,12 +125,14 @@ class PagedKVCache:
         """Rotates the step's queries and keys by their positions in their rows (ops.paged_cache_append's
         rotation, `rope` of at least as many positions as a row has), stores the keys and values and returns
         the queries.  The step's positions are taken with the first layer."""
+        self._check(k, "append")
         append = ops.paged_cache_append if self.bits == 16 else ops.paged_cache_append_fp4
         return append(q, k, v, *self.layer(layer), step.slots, rope, self.positions(step), interleaved)
 
     def attend(self, layer: int, q: torch.Tensor, step: Step, **options):
         """Attention of the step's queries [T, q_heads, head_dim] over their rows, with the options of
         ops.paged_attention."""
+        self._check(q, "attend")
         attention = ops.paged_attention if self.bits == 16 else ops.paged_attention_fp4
         return attention(q, *self.layer(layer), self.block_tables, self.seq_lens, step.cu_q, step.max_q_len,
                          step.max_seq_len, **options)

@@ -229,6 +229,11 @@ def test_refusals():
     cache = PagedKVCache(1, 4, 7, 3, 96, 4, 64, device="cpu", bits=4)
     assert cache.pool.dtype == torch.uint8 and cache.pool.shape == (2, 4, 7, 3, 51)
     assert cache.pool.stride(1) == 1072 and cache.pool.stride(0) == 4 * 1072
+    k = torch.zeros(0, 3, 96, dtype=H)  # a cache of bf16
+    for call in (lambda: cache.write(0, k, k, None), lambda: cache.append(0, k, k, k, None, None),
+                 lambda: cache.attend(0, k, None)):
+        with pytest.raises(ValueError, match="cache is of torch.bfloat16, got torch.float16"):
+            call()
     rows = torch.zeros(2, dtype=torch.int32)
     for live, spare in (([0, 1], [2, 2]), ([0, 1], [1, 2]), ([0, 1], [2]), ([0, 1], [1, 2, 3])):
         with pytest.raises(ValueError, match="spare row"):
