@@ -165,12 +165,12 @@ class PagedKVCache:
             raise ValueError("PagedKVCache.reorder: a spare row for each of rows, each once and not live")
         n = len(live)
         ints = self._rows(live + spare, "reorder")
-        shifted, to_rows = ints[:n] + 1, ints[n:]
+        to_rows = ints[n:]
+        # a row outside becomes 0 and so -1, a pair that fork passes over
+        from_rows = ops.beam_reorder([ints[:n] + 1], rows)[0] - 1
         if any(self._most[r] for r in spare):
             ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens, to_rows)
-        # a row outside becomes 0 and so -1, a pair that fork passes over
-        missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens,
-                                       ops.beam_reorder([shifted], rows)[0] - 1, to_rows)
+        missing = ops.paged_cache_fork(self.pool, self.ref_counts, self.block_tables, self.seq_lens, from_rows, to_rows)
         # nothing goes where nothing was copied: a row below 0 is none
         ops.paged_cache_free(self.ref_counts, self.block_tables, self.seq_lens,
                              torch.sub(ints[:n], missing, alpha=self.rows))

@@ -192,6 +192,9 @@ def test_reorder():
     assert int(cache.reorder(rows(0, 1, 1), [4, 5], [1, 2, 3])) == 0  # rows whose bounds a refusal left
     assert cache.lengths() == [0, 11, 11, 11, 0, 0]
     cache.extend([0, 0, 0, 0, 0, 20])
+    with pytest.raises(RuntimeError, match="int32"):  # refused with nothing changed
+        cache.reorder(rows(2).long(), [1, 2, 3], [5])
+    assert cache.lengths() == [0, 11, 11, 11, 0, 20]
     assert int(cache.reorder(rows(2), [1, 2, 3], [5])) == 0  # a spare row in use gives its pages back
     assert cache.lengths() == [0, 0, 0, 0, 0, 11] and int(cache.ref_counts.sum()) == 2
 
