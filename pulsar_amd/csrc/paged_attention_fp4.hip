@@ -744,6 +744,7 @@ struct Call {
     int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128 or 256
     bool narrow;               // tiles of 32 rows where a sequence has several
     int plan;                  // bytes of LDS behind the kernel's stages
+    int64_t pieces;            // split: that a tile's keys are in, about, the longest tile's
     int64_t tiles;             // at most
     size_t bytes;
 };
@@ -822,7 +823,11 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const int64_t most_units = ceil_div(keys_of(c.tile_rows), unit) + 1;  // of a tile
     const char* const forced = plan_override("PW4_ATTN_UNITS");
     const int forced_units = forced ? std::atoi(forced) : 0;
-    p.min_units = forced_units > 0 ? forced_units : few ? 1 : 8;
+    // A few rows: pieces of one unit make long joins of long sequences.  Pieces of 1 and 4 units (16 waves to join,
+    // below), us, 4 query heads on each of 2 key-value heads of 128: 65000 keys 27 and 18.4, six tokens there 37 and
+    // 26; one head, 131072 keys 36 and 20; 8 heads, 16000 keys 21.7 and 17.6; of 3 units, 8000 keys 15.4 and 14.1,
+    // 6000 15.1 and 16.4.
+    p.min_units = forced_units > 0 ? forced_units : !few ? 8 : most_units > 96 ? 4 : most_units > 50 ? 3 : 1;
     // Whether the keys are split.  A few rows: whole, a workgroup takes 0.5, 0.7 and 1.3 us a unit (heads of
     // 64 and 128, units of 128 keys; of 256, of 64); the split, a second launch, and the partial outputs' way
     // through memory, which grow with the tiles.  8 key-value heads, sequences of one length, whole and split, us:
@@ -849,6 +854,7 @@ Call plan_call(const pw4_paged_attention_args* a) {
     if (p.split) {
         c.grid = (int)std::min<int64_t>(slots, ceil_div(c.tiles * p.kv_heads * most_units, p.min_units));
         c.bytes = partial_bytes(c.grid, c.tile_rows, p.dim);
+        c.pieces = most_units / std::max<int64_t>(p.min_units, c.tiles * p.kv_heads * most_units / c.grid);
     }
     return c;
 }
@@ -878,12 +884,18 @@ hipError_t launch(const Call& c, hipStream_t s) {
     // A wave a row to join where rows are enough, a workgroup where not.  Both launches, workgroup and wave, us,
     // heads of 128: 16 tokens over 2 to 32 thousand keys (512 rows) 46 and 48, two of each 48 and 50, four (2048) 54
     // and 53, eight 76 and 72, eight of 48 sequences 173 and 156, one of each (1536) 128 and 125; eight of 2 sequences
-    // (512) 45 and 55.
+    // (512) 45 and 55.  Sixteen waves to that workgroup where a tile is in many pieces: 131072 keys of one head in
+    // 256 20 and with four waves 28, 65000 of two in 127 18.4 and 20.9; 16000 of eight in 31 18.7 and 17.6.
+    const bool long_joins = c.pieces > 48;
     const bool wave_a_row = rows * c.tiles * c.p.kv_heads >= 6 * device_cus();
     if (c.tile_rows == 16) {
-        wave_a_row ? run_join<16, BF16>(c.p, c.tiles, c.grid, s) : run_row_join<16, BF16>(c.p, c.tiles, rows, c.grid, s);
+        wave_a_row   ? run_join<16, BF16>(c.p, c.tiles, c.grid, s)
+        : long_joins ? run_row_join<16, BF16, 16>(c.p, c.tiles, rows, c.grid, s)
+                     : run_row_join<16, BF16, 4>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == 32) {
-        wave_a_row ? run_join<32, BF16>(c.p, c.tiles, c.grid, s) : run_row_join<32, BF16>(c.p, c.tiles, rows, c.grid, s);
+        wave_a_row   ? run_join<32, BF16>(c.p, c.tiles, c.grid, s)
+        : long_joins ? run_row_join<32, BF16, 16>(c.p, c.tiles, rows, c.grid, s)
+                     : run_row_join<32, BF16, 4>(c.p, c.tiles, rows, c.grid, s);
     } else if (c.tile_rows == kManyRows) {
         run_join<kManyRows, BF16>(c.p, c.tiles, c.grid, s);
     } else {

@@ -907,9 +907,9 @@ __global__ __launch_bounds__(256) void join_kernel(const Params a, int grid) {
 
 // The same with a workgroup a row (blockIdx.y), whose waves take the partials in turn: for few rows in
 // many pieces.
-template <int MR, bool BF16>
-__global__ __launch_bounds__(256) void join_row_kernel(const Params a, int grid) {
-    constexpr int WAVES = 4, kAtOnce = 8;
+template <int MR, bool BF16, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void join_row_kernel(const Params a, int grid) {
+    constexpr int kAtOnce = 8;
     __shared__ float s_x[WAVES][256], s_ml[WAVES][2];
     const int ti = blockIdx.x / a.kv_heads, head = blockIdx.x % a.kv_heads, row = blockIdx.y;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -1052,9 +1052,10 @@ void run_join(const Params& p, int64_t tiles, int grid, hipStream_t s) {
     hipLaunchKernelGGL((join_kernel<MR, BF16>), dim3((unsigned)(tiles * p.kv_heads), MR / 4), dim3(256), 0, s, p, grid);
 }
 
-template <int MR, bool BF16>
+template <int MR, bool BF16, int WAVES>
 void run_row_join(const Params& p, int64_t tiles, int rows, int grid, hipStream_t s) {
-    hipLaunchKernelGGL((join_row_kernel<MR, BF16>), dim3((unsigned)(tiles * p.kv_heads), rows), dim3(256), 0, s, p, grid);
+    hipLaunchKernelGGL((join_row_kernel<MR, BF16, WAVES>), dim3((unsigned)(tiles * p.kv_heads), rows), dim3(WAVES * 64), 0, s,
+                       p, grid);
 }
 
 // The workspace of a split call: partial outputs, their maxima and sums, and the plan.

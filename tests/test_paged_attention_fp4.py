@@ -127,6 +127,16 @@ def test_long_context_is_split():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,length", [(64, 30000), (128, 26000), (256, 14000)])
+@pytest.mark.parametrize("new,dtype", [(1, B), (5, H)])
+def test_sequences_in_many_pieces(dim, length, new, dtype):
+    """Pieces by the hundred to join, and a short sequence beside them."""
+    out, lse = _run([length, 7], [new, new], heads=1, group=4, dim=dim, dtype=dtype, seed=dim)
+    again = _run([length, 7], [new, new], heads=1, group=4, dim=dim, dtype=dtype, seed=dim)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("split,units", [(0, None), (1, 1), (1, 3)])
 @pytest.mark.parametrize("new", [1, 6])
 @pytest.mark.parametrize("dim", [64, 128, 256])
