@@ -405,15 +405,21 @@ void fp4_few_rows_kernel(const Fp4Params a) {
 // ---- many rows --------------------------------------------------------------------
 
 // Four waves of 32 query rows each over blocks of 64 keys that they share in LDS as 16-bit elements,
-// two stages: each wave widens 16 keys of a block, whose codes came during the block before.
+// two stages: each wave widens 16 keys of a block, whose codes came during the block before.  With two
+// GROUPS of four waves, each with stages of its own, the blocks go to them in turn, and the second
+// group's outputs reach the first one's through LDS at the end: for whole tiles too few to give a SIMD
+// a second wave.
 constexpr int kManyWaves = 4, kManyRows = 32 * kManyWaves;
 template <int DP>
 constexpr int kManyStage = 2 * kManyKeys * DP * 2;
-template <int DP>
-constexpr int many_stage_bytes() { return 2 * kManyStage<DP>; }
+template <int DP, int GROUPS>
+constexpr int many_stage_bytes() {
+    const int stages = GROUPS * 2 * kManyStage<DP>, join = kManyRows * (DP + 4) * 4;
+    return GROUPS > 1 && join > stages ? join : stages;
+}
 
-template <bool BF16, int DP, bool CAP>
-__global__ __launch_bounds__(kManyWaves * 64) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
+template <bool BF16, int DP, bool CAP, int GROUPS>
+__global__ __launch_bounds__(GROUPS * kManyWaves * 64) __attribute__((amdgpu_waves_per_eu(DP == 256 ? 1 : 2)))
 void fp4_many_rows_kernel(const Fp4Params a) {
     constexpr int WAVES = kManyWaves, MR = kManyRows, KEYS = kManyKeys;
     constexpr int KS = DP / 16;      // steps of 16 head elements
@@ -421,9 +427,11 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     constexpr int COPY = KEYS / WAVES;
     static_assert(COPY == 16, "a load takes 16 keys");
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // (nothing else is: it starts at 0)
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES;
+    const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES : 0;
     const int c = lane & 31, h = lane >> 5;
-    Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP>());
+    Plan& plan = *reinterpret_cast<Plan*>(smem + many_stage_bytes<DP, GROUPS>());
+    uint8_t* const stages = smem + group * 2 * kManyStage<DP>;
     const Loader<DP> from(a, lane);
     const int copied = wave * COPY + (lane & 15);  // the lane's key of a block
     const uint32_t k_to = quarter_at<DP>(lane >> 4, copied, k_swizzle<DP>(copied));
@@ -435,14 +443,16 @@ void fp4_many_rows_kernel(const Fp4Params a) {
     const int vr = 4 * h + ((c & 15) >> 2);
     const uint32_t v_at = (uint32_t)(kManyStage<DP> / 2 + vr * DP * 2 +
                                      ((((c >> 4) * 2 + ((c & 3) >> 1)) ^ v_swizzle<DP, true>(vr)) * 16) + (c & 1) * 8);
-    Pieces<MR, KEYS, KEYS, WAVES, false, false, true> piece;
+    Pieces<MR, KEYS, KEYS, GROUPS * WAVES, false, false, true> piece;
     piece.start(a, plan);
     while (piece.next(a, plan)) {
         const Tile& t = piece.t;
         const int head = piece.head, slot = piece.slot;
         const Source src = source_of(a, t, head);
         const int begin = t.base + piece.u0 * KEYS, end = min(t.hi, t.base + piece.u1 * KEYS);
-        const int blocks = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        const int all = end > begin ? (end - begin + KEYS - 1) / KEYS : 0;
+        const int rounds = (all + GROUPS - 1) / GROUPS, blocks = (all - group + GROUPS - 1) / GROUPS;  // the group's
+        auto first_of = [&](int i) { return begin + (i * GROUPS + group) * KEYS; };
         const WaveRows<KEYS> r(a, t, wave);
         u32x4 q[KS];
         load_query<KS>(a, r.mine, head, c, h, 2, q);
@@ -456,13 +466,13 @@ void fp4_many_rows_kernel(const Fp4Params a) {
         float m = -kInf, z = 0.f;
         Key key{};  // the lane's, of the block that is loaded next
         Quarter<DP> kq, vq;
-        auto find = [&](int i) { return from.find(a, src, begin + i * KEYS + wave * COPY); };
+        auto find = [&](int i) { return from.find(a, src, first_of(i) + wave * COPY); };
         auto load = [&] {
             from.load(a, src, src.k, key, kq);
             from.load(a, src, src.v, key, vq);
         };
         auto store = [&](int i) {
-            uint8_t* const to = smem + (i & 1) * kManyStage<DP>;
+            uint8_t* const to = stages + (i & 1) * kManyStage<DP>;
             store_quarter<BF16, DP>(to, k_to, from.lane, kq);
             store_quarter<BF16, DP>(to + kManyStage<DP> / 2, v_to, from.lane, vq);
         };
@@ -476,7 +486,7 @@ void fp4_many_rows_kernel(const Fp4Params a) {
                 if (blocks > 2) key = find(2);
             }
         }
-        for (int i = 0; i < blocks; ++i) {
+        for (int i = 0; i < rounds; ++i) {
             // block i is there, and every wave is done with block i - 1
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (i + 1 < blocks) {
@@ -487,9 +497,9 @@ void fp4_many_rows_kernel(const Fp4Params a) {
                     key = then;
                 }
             }
-            const int key0 = begin + i * KEYS;
-            if (!r.sees(key0)) continue;
-            const uint8_t* const st_at = smem + (i & 1) * kManyStage<DP>;
+            const int key0 = first_of(i);
+            if (i >= blocks || !r.sees(key0)) continue;
+            const uint8_t* const st_at = stages + (i & 1) * kManyStage<DP>;
             f32x16 s[2];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -560,7 +570,38 @@ void fp4_many_rows_kernel(const Fp4Params a) {
                 }
             }
         }
-        store_rows<Fp4Keys, BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held_max<BF16>(m, k), z, o);
+        float held = held_max<BF16>(m, k);
+        if constexpr (GROUPS > 1) {
+            constexpr int kLane = 16 * DT + 2;  // floats of a lane: outputs, maximum, sum
+            float* const theirs = reinterpret_cast<float*>(smem) + wave * kLane * 64 + lane;
+            __syncthreads();  // every wave is done with the stages
+            if (group == 1) {
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) theirs[(16 * d + e) * 64] = o[d][e];
+                theirs[16 * DT * 64] = held;
+                theirs[(16 * DT + 1) * 64] = z;
+            }
+            __syncthreads();
+            if (group == 0) {
+                const float m1 = theirs[16 * DT * 64], z1 = theirs[(16 * DT + 1) * 64], top = fmaxf(held, m1);
+                // (a maximum of -inf: no key, or scores of NaN, which the sum has then)
+                const float f0 = held == -kInf ? 0.f : __builtin_amdgcn_exp2f(held - top);
+                const float f1 = m1 == -kInf ? 0.f : __builtin_amdgcn_exp2f(m1 - top);
+                z = (held == -kInf ? z : f0 * z) + (m1 == -kInf ? z1 : f1 * z1);
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        o[d][e] = (f0 == 0.f ? 0.f : f0 * o[d][e]) + (f1 == 0.f ? 0.f : f1 * theirs[(16 * d + e) * 64]);
+                    }
+                held = top;
+            }
+        }
+        if (group == 0) {
+            store_rows<Fp4Keys, BF16, DP, MR, CAP>(a, t, r, wave, head, slot, begin, end, held, z, o);
+        }
         __syncthreads();  // every wave is done with the stages
     }
     clear_rest(a);
@@ -742,6 +783,7 @@ void fp4_wide_rows_kernel(const Fp4Params a) {
 struct Call {
     Fp4Params p;
     int dp, tile_rows, grid;   // tile_rows: 16 or 32 (few rows), 128 or 256
+    int groups;                // of 128 rows: of waves that share a tile's keys
     bool narrow;               // tiles of 32 rows where a sequence has several
     int plan;                  // bytes of LDS behind the kernel's stages
     int64_t pieces;            // split: that a tile's keys are in, about, the longest tile's
@@ -844,7 +886,16 @@ Call plan_call(const pw4_paged_attention_args* a) {
     const bool wanted = forced_split ? forced_split[0] == '1'
                         : few ? most_units > (c.dp == 256 ? 5 + 20 * work / cus : 9 + 28 * work / cus)
                               : most_units * (slots - work) > slots * (c.dp == 256 ? 14 + work / 16 : 16 + work / 7);
-    p.split = wanted && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles &&
+    // Whole tiles of 128 rows that leave CUs idle: two groups of waves.  One and two, us, heads of 64 / 128: 6 tiles of
+    // 300 keys 12.0 and 13.4 / 15.8 and 18.0, of 777 20.0 and 19.5 / 26.8 and 26.6; 132 of 1500 30.7 and 26.8 / 42 and
+    // 38; 176 of 2000 39 and 33 / 55 and 48, of 5000 81 and 65 / 116 and 95; more than CUs, 336 of 1500, 42 and 50 / 61
+    // and 73.
+    const char* const forced_groups = plan_override("PW4_ATTN_GROUPS");
+    c.groups = c.tile_rows != kManyRows || c.dp == 256 ? 1
+               : forced_groups                         ? forced_groups[0] - '0'
+               : !wanted && work <= cus && keys_of(kManyRows) >= 900 ? 2
+                                                                      : 1;
+    p.split = wanted && c.groups == 1 && !narrow && c.tiles > 0 && p.batch <= kMaxSplitTiles && c.tiles <= kMaxSplitTiles &&
               c.tiles * p.kv_heads * most_units < INT_MAX;
     if (!p.split) c.plan = 0;
     c.grid = (int)(c.tiles * p.kv_heads);
@@ -873,7 +924,12 @@ hipError_t launch(const Call& c, hipStream_t s) {
             e = hipErrorInvalidValue;  // no such tile: plan_call
         }
     } else if (c.tile_rows == kManyRows) {
-        e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP>(), c.plan, s);
+        if (c.groups == 1 || DP == 256) {
+            e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP, 1>>(c.p, c.grid, kManyWaves, many_stage_bytes<DP, 1>(), c.plan, s);
+        } else {
+            constexpr int G = DP < 256 ? 2 : 1;
+            e = run_attention<fp4_many_rows_kernel<BF16, DP, CAP, G>>(c.p, c.grid, G * kManyWaves, many_stage_bytes<DP, G>(), c.plan, s);
+        }
     } else if constexpr (DP == 128) {
         e = run_attention<fp4_wide_rows_kernel<BF16, DP, CAP>>(c.p, c.grid, kWideWaves, wide_stage_bytes<DP>(), c.plan, s);
     } else {

@@ -185,6 +185,46 @@ def test_sequences_of_mixed_lengths(plan, batch, tile):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype", [(64, H), (64, B), (96, B), (128, H), (128, B)])
+def test_tiles_of_two_groups_of_waves(plan, monkeypatch, dim, dtype):
+    """Blocks in turn: none, one, an even and an odd number of them, and rows that see those of one group only."""
+    plan(0, None, 128)
+    monkeypatch.setenv("PW4_ATTN_GROUPS", "2")
+    _run([600, 257, 64, 400, 0, 65], [600, 129, 1, 90, 0, 65], heads=2, group=2, dim=dim, dtype=dtype, seed=dim)
+    _run([900, 333, 128], [200, 333, 70], heads=1, group=3, dim=dim, dtype=dtype, window=30, cap=4.0, page=8, seed=dim)
+    _run([500], [499], heads=3, group=1, dim=dim, dtype=dtype, page=7, extra=5, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunks_of_whole_tiles(dim):
+    """Two groups of waves by the rule."""
+    _run([1500, 1300, 1200], [200, 200, 200], heads=8, group=4, dim=dim, window=1000, seed=dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("groups", [1, 2])
+def test_infinite_values_with_groups_of_waves(plan, monkeypatch, groups):
+    """A block of NaN in a key of either group's blocks reaches only the queries that see it."""
+    plan(0, None, 128)
+    monkeypatch.setenv("PW4_ATTN_GROUPS", str(groups))
+    lens, new, dim = [400], 300, 64
+    for j in (120, 190, 399):
+        def edit(ks, vs):
+            vs[0][j, 0, 3] = math.inf
+            ks[0][j - 20, 0, 40] = math.nan
+
+        kc, vc, tables, ks, vs = fp4_kv(lens, 16, 1, dim, B, 8, edit=edit)
+        q = torch.randn(new, 2, dim, generator=gen(9)).to(B).to(DEV)
+        out, lse = ops.paged_attention_fp4(q, kc, vc, tables, _i32(lens), offsets([new]).to(DEV), new, lens[0],
+                                           return_lse=True)
+        ref = attention_ref(q.cpu(), ks[0], vs[0], lens[0], new, dim ** -0.5, 0, 0.0)
+        fine = torch.arange(100, 400) < j - 20  # the queries that see no key of NaN
+        check_attention(out.cpu()[fine], lse.cpu()[fine], [r[fine] for r in ref], dim, lens[0], B)
+        assert bool(out.cpu()[~fine].isnan().all()) and bool(lse.cpu()[~fine].isnan().all())
+
+
+@pytest.mark.gpu
 def test_magnitudes():
     """Blocks of very different exponents, and of zeros."""
     for dtype, lo, hi in ((B, -30, 30), (H, -10, 9)):
