@@ -34,7 +34,7 @@ using namespace pw4;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int64_t kMostGroups = 1 << 22;  // of a launch of a workgroup a token: 2^32 threads are too many
+constexpr int64_t kMostGroups = 1 << 22;  // of a launch: threads are counted in 32 bits, and past 2^32 tokens are lost
 
 struct Heads {
     const uint16_t* from;
@@ -479,11 +479,24 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
         const int64_t rows = kThreads / 64 * (64 / (a->head_dim / 16));
         const bool few = a->num_tokens * heads <= 8 * device_cus() * rows;
         p.abreast = (int32_t)std::min<int64_t>(few ? rows : std::min<int64_t>(8, rows), heads);
-        const dim3 grid((unsigned)ceil_div(a->num_tokens, rows / p.abreast), (unsigned)(few ? ceil_div(heads, p.abreast) : 1));
-        if (p.interleaved || !turns) {
-            hipLaunchKernelGGL((append_kernel<BF16, FP4, true>), grid, dim3(kThreads), 0, s, p);
-        } else {
-            hipLaunchKernelGGL((append_kernel<BF16, FP4, false>), grid, dim3(kThreads), 0, s, p);
+        const int64_t at_once = rows / p.abreast, most = kMostGroups * at_once;  // tokens of a workgroup, of a launch
+        for (int64_t first = 0; first < a->num_tokens; first += most) {
+            AppendArgs part = p;
+            part.tokens = (int32_t)std::min(most, a->num_tokens - first);
+            part.slots += first;
+            if (turns) part.positions += first;
+            part.k.from += first * part.k.token;
+            part.v.from += first * part.v.token;
+            if (q) {
+                part.q.from += first * part.q.token;
+                part.q_out += first * a->q_heads * a->head_dim;
+            }
+            const dim3 grid((unsigned)ceil_div(part.tokens, at_once), (unsigned)(few ? ceil_div(heads, p.abreast) : 1));
+            if (p.interleaved || !turns) {
+                hipLaunchKernelGGL((append_kernel<BF16, FP4, true>), grid, dim3(kThreads), 0, s, part);
+            } else {
+                hipLaunchKernelGGL((append_kernel<BF16, FP4, false>), grid, dim3(kThreads), 0, s, part);
+            }
         }
     };
     const auto with_bits = [&](auto bf16) { fp4 ? run(bf16, std::true_type{}) : run(bf16, std::false_type{}); };
