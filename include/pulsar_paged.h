@@ -54,7 +54,9 @@ extern "C" {
  *            sized by them, longer sequences are cut to them (keys past
  *            max_seq_len are not seen, queries past max_q_len come out empty)
  * scale and softcap are finite.  A sequence has fewer than 2^31 - 1024 rows (new
- * tokens times the query heads of a key-value head).  head_dim: a multiple of 8 up to 256.  Pointers
+ * tokens times the query heads of a key-value head), and a call fewer than 2^32
+ * threads, else PW4_ERR_SHAPE: 128 to 512 for each tile of up to 16 to 256 rows of
+ * a sequence and key-value head, 2 million sequences of a token with 8 heads.  head_dim: a multiple of 8 up to 256.  Pointers
  * 16-byte aligned, strides multiples of 8, row_stride below 2^24. */
 typedef struct pw4_paged_attention_args {
     const void* q;

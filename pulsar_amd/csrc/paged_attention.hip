@@ -794,7 +794,9 @@ int pw4_paged_attention(const pw4_paged_attention_args* args, void* workspace, s
     if (const int rc = check(args)) return rc;
     if (args->num_tokens == 0) return PW4_OK;
     Call c = plan_call(args);
-    if (c.grid > 65535 * 4096 || c.tiles * c.p.kv_heads > INT_MAX) return PW4_ERR_SHAPE;
+    const int waves = c.tile_rows > kManyRows ? kWideWaves : c.tile_rows > 32 ? kManyWaves
+                      : c.dp == 64 ? kFewWaves<64> : c.dp == 128 ? kFewWaves<128> : kFewWaves<256>;
+    if (!fits_a_launch(c.tiles * c.p.kv_heads, waves)) return PW4_ERR_SHAPE;
     if (c.bytes > 0) {
         if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < c.bytes) {
             return PW4_ERR_WORKSPACE;

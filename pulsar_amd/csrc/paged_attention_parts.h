@@ -1028,6 +1028,10 @@ inline Params params_of(const pw4_paged_attention_args* a) {
     return p;
 }
 
+// Whether a launch may have so many workgroups: the device counts threads in 32 bits, and runs what is left of
+// the count without an error.
+inline bool fits_a_launch(int64_t groups, int waves) { return groups <= UINT32_MAX / (waves * 64); }
+
 // Runs a kernel with more LDS than a kernel may have unasked; the permission is
 // asked for once a kernel and device.  `plan`: bytes behind its stages, a Plan's at most.
 template <auto Kernel, typename P>
