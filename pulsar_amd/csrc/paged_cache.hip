@@ -614,9 +614,12 @@ int pw4_paged_cache_free(int32_t* ref_counts, int64_t num_pages, int32_t* block_
     if (!small(n) || table_width > 65535 * 256) return PW4_ERR_SHAPE;
     if (n == 0 || rows == 0) return PW4_OK;
     const unsigned cols = (unsigned)std::max<int64_t>(1, ceil_div(table_width, 256));
-    hipLaunchKernelGGL(free_kernel, dim3((unsigned)n, cols), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
-                       ref_counts, (int)num_pages, block_tables, (int)rows, (int)table_width, table_stride, seq_lens,
-                       which);
+    constexpr int64_t kMost = 1 << 22;  // workgroups of a launch: threads are counted in 32 bits, the rest is lost
+    for (int64_t first = 0; first < n; first += kMost) {
+        hipLaunchKernelGGL(free_kernel, dim3((unsigned)std::min(kMost, n - first), cols), dim3(256), 0,
+                           reinterpret_cast<hipStream_t>(stream), ref_counts, (int)num_pages, block_tables, (int)rows,
+                           (int)table_width, table_stride, seq_lens, which + first);
+    }
     return check_launch();
 }
 
