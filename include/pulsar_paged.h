@@ -187,9 +187,10 @@ int pw4_paged_cache_compact(const pw4_page_pool* pool, int32_t* ref_counts, int3
  * byte i); then, heads and tokens in the same order, head_dim / 32 exponents:
  * page_size * kv_heads * head_dim * 17 / 32 bytes.  head_dim is a multiple of 32 up to 256.
  *
- * Values round to the block 2^e whose largest magnitude is in [3.5, 7) 2^e (e from -127; with
- * dtype fp16 up to 13, so that what is held is finite in fp16), and there to the nearest code,
- * of two the even one: each is off by 2^e at most, half a step.  A block with a NaN or an
+ * Values round to the block 2^e whose largest magnitude is in [3.5, 7) 2^e (e from -127 up to 13
+ * with dtype fp16 and 125 with bf16, so that what is held is finite in the type), and there to
+ * the nearest code, of two the even one: each is off by 2^e at most, half a step, and those
+ * above 7 * 2^13, 7 * 2^125, are cut off to 6 * 2^13, 6 * 2^125.  A block with a NaN or an
  * infinity becomes NaN.
  *
  * Caches are pages of one layer, page_stride bytes apart, 16-byte aligned; row_stride and
@@ -200,7 +201,8 @@ int pw4_paged_cache_append_fp4(const pw4_paged_append_args* args, pw4_stream_t s
 
 /* paged_cache_read_fp4: the values that slots of one layer's 4-bit caches hold, k and v
  * [num_tokens, kv_heads, head_dim] contiguous, each rounded once to dtype (fp16 or bf16; exact
- * unless it is subnormal there); 0 for a slot outside the pool. */
+ * unless it is subnormal in fp16, or of another writer's exponent past the above); 0 for a slot
+ * outside the pool. */
 int pw4_paged_cache_read_fp4(const void* k_cache, const void* v_cache, const int64_t* slots, void* k, void* v,
                              int64_t num_tokens, int64_t kv_heads, int64_t head_dim, int64_t num_pages,
                              int64_t page_size, int64_t page_stride, int dtype, pw4_stream_t stream);

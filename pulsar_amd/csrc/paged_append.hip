@@ -462,7 +462,7 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
     p.rot = (int32_t)a->rot;
     p.page_size = (int32_t)a->page_size;
     p.interleaved = a->interleaved != 0;
-    p.exp_limit = a->dtype == PW4_DTYPE_F16 ? 127 + 13 : 254;
+    p.exp_limit = a->dtype == PW4_DTYPE_F16 ? 127 + 13 : 127 + 125;  // 6 * 2^e is finite in the type, 4 * 2^(e + 1) is not
     p.tokens = (int32_t)a->num_tokens;
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const auto run = [&](auto bf16, auto four) {

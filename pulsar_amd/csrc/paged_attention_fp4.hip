@@ -3,7 +3,8 @@
 //
 // A key is codes times powers of two, one for each 32 elements.  The conversion
 // instructions take both (v_cvt_scalef32_pk_*_fp4: two elements each), and every value
-// that a code stands for is exact in 16 bits, so the products see the cache's own
+// that the append stores is exact in 16 bits but for fp16's subnormal ones, which are
+// rounded as reading them back rounds them; so the products see the cache's own
 // numbers and the rest is the attention over a 16-bit cache: rows, tiles, transposed
 // products and splitting are those of paged_attention.hip.
 //

@@ -344,8 +344,9 @@ def paged_cache_append_fp4(q: torch.Tensor | None, k: torch.Tensor, v: torch.Ten
     """paged_cache_append into 4-bit caches uint8 [pages, page_size, kv_heads, head_dim / 2 + head_dim / 32].
 
     A block of 32 elements of k (rotated, in fp32) or v is rounded to 2^e times 4-bit floats, its largest
-    magnitude in [3.5, 7) 2^e: each element is off by 2^e at most.  In fp16 e is 13 at most, which cuts
-    magnitudes above 6 * 2^13 off.  A block with a NaN or an infinity becomes NaN."""
+    magnitude in [3.5, 7) 2^e: each element is off by 2^e at most.  In fp16 e is 13 at most and in bf16 125, so
+    that what is held is finite: magnitudes above 7 * 2^e are cut off to 6 * 2^e there.  A block with a NaN or an
+    infinity becomes NaN."""
     out = _paged_cache_append_fp4(q, k, v, k_cache, v_cache, slots, rope, positions, interleaved)
     return None if q is None else out
 
