@@ -5,7 +5,8 @@ page_size, kv_heads, head_dim] (with bits=4 bytes, the last dimension head_dim /
 a page id names the same page in all of them and forking, copying and compacting are one call for the
 whole model.  The book-keeping -- reference counts, block tables,
 lengths -- is on the device and changes in place; the host keeps only an upper bound of each row's
-length, which sizes the attention's grid.  No method but `lengths` waits for the device.  Methods that
+length, which sizes the attention's grid.  No method but `lengths` waits for the device, and `append` where
+that bound does not tell whether its table of rotations is long enough.  Methods that
 take lists copy them to the device when they are called, so they do not belong into a captured graph;
 the operators may.
 
@@ -35,6 +36,7 @@ class Step:
     max_seq_len: int
     positions: torch.Tensor | None = None  # of the tokens, int64: PagedKVCache.positions
     changes: int = -1  # the cache's, when the step was taken
+    reach: int | None = None  # positions that its stored tokens need of a table: read where max_seq_len is too high
 
 
 class PagedKVCache:
@@ -124,10 +126,21 @@ class PagedKVCache:
                interleaved: bool = False) -> torch.Tensor:
         """Rotates the step's queries and keys by their positions in their rows (ops.paged_cache_append's
         rotation, `rope` of at least as many positions as a row has), stores the keys and values and returns
-        the queries.  The step's positions are taken with the first layer."""
+        the queries.  The step's positions are taken with the first layer.
+
+        A table that ends before a token that would be stored raises ValueError, and nothing is stored.  The
+        bound step.max_seq_len tells mostly; where it is above the table's rows the positions are read, once a
+        step, which waits for the device (not while a graph is captured: a table is taken as it is there)."""
         self._check(k, "append")
+        positions = self.positions(step)
+        if rope.dim() == 2 and rope.shape[0] < step.max_seq_len and not torch.cuda.is_current_stream_capturing():
+            if step.reach is None:
+                stored = torch.where(step.slots >= 0, positions, -1)
+                step.reach = 1 + int(stored.max()) if stored.numel() else 0
+            if rope.shape[0] < step.reach:
+                raise ValueError(f"PagedKVCache.append: rope has {rope.shape[0]} positions, a row {step.reach}")
         append = ops.paged_cache_append if self.bits == 16 else ops.paged_cache_append_fp4
-        return append(q, k, v, *self.layer(layer), step.slots, rope, self.positions(step), interleaved)
+        return append(q, k, v, *self.layer(layer), step.slots, rope, positions, interleaved)
 
     def attend(self, layer: int, q: torch.Tensor, step: Step, **options):
         """Attention of the step's queries [T, q_heads, head_dim] over their rows, with the options of
