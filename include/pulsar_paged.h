@@ -244,7 +244,8 @@ int pw4_token_logprobs(const void* logits, int dtype, int64_t num_tokens, int64_
  * beam, then by logit, then by token, the lower first.  A total that is NaN counts as -inf.
  * ended (bytes, NULL: none): a beam whose byte is not 0 has one continuation, end_token with its score
  * as it is; its logits are not read.  out_ended (with ended): whether the new beam continues one that
- * had ended, or its token is end_token.
+ * had ended, or its token is end_token.  end_token (read with ended) is a token, or -1: no token ends a
+ * beam then, and -1 stands for the next token of those that have ended, not to be looked up.
  * beams and width from 1 to 32, width at most beams * vocab, with ended at most beams. */
 size_t pw4_beam_select_workspace_size(int64_t batch, int64_t beams, int64_t vocab, int64_t width);
 int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams, int64_t vocab, int64_t row_stride,

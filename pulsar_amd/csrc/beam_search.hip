@@ -225,6 +225,7 @@ int pw4_beam_select(const void* logits, int dtype, int64_t batch, int64_t beams,
                     size_t workspace_bytes, pw4_stream_t stream) {
     if (batch < 0 || beams <= 0 || vocab <= 0 || width <= 0) return PW4_ERR_ARG;
     if (dtype != PW4_DTYPE_F16 && dtype != PW4_DTYPE_BF16 && dtype != PW4_DTYPE_F32) return PW4_ERR_ARG;
+    if (ended != nullptr && (end_token < -1 || end_token >= vocab)) return PW4_ERR_ARG;
     if (beams > kMaxBeams || width > kMaxTop || vocab > INT_MAX / 2 || batch > 65535 / beams || width > beams * vocab ||
         (ended != nullptr && width > beams) || row_stride < vocab) {
         return PW4_ERR_SHAPE;

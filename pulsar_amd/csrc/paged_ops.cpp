@@ -504,6 +504,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select_cuda(cons
     TORCH_CHECK(!ended || (ended->scalar_type() == at::kBool && ended->sizes() == scores.sizes()), op,
                 ": ended must be bool [batch, beams]");
     TORCH_CHECK(!ended || W <= K, op, ": with ended, width must be at most beams");
+    TORCH_CHECK(!ended || (end_token >= -1 && end_token < V), op, ": end_token must be a token, or -1 for none");
     DeviceGuard guard(logits.device());
     const at::Tensor x = (V == 1 || logits.stride(1) == 1) && (B * K <= 1 || logits.stride(0) >= V) ? logits
                                                                                                   : logits.contiguous();

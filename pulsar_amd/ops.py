@@ -410,6 +410,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, width: int | None = 
         scores: fp32 [batch, beams], beams up to 32.
         width: up to 32, with `ended` at most beams.
         ended: bool [batch, beams].
+        end_token: with `ended`, the token that ends a beam; or -1, none: no new beam ends by its token, and those
+            that have ended go on with -1, which the caller replaces before it looks tokens up.
 
     Returns:
         (scores fp32, rows int32, tokens int64), each [batch, width]: rows are those of logits that the new
