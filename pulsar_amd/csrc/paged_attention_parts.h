@@ -271,6 +271,12 @@ __device__ __forceinline__ Sequence sequence(const Params& a, int b) {
     return s;
 }
 
+// The first key that a query at `pos` sees.  (A query before the first key sees none; its window's end, taken as
+// that of position 0, stays in 32 bits.)
+__device__ __forceinline__ int lowest_key(const Params& a, int pos) {
+    return a.window > 0 ? max(0, max(pos, 0) + 1 - a.window) : 0;
+}
+
 // A tile: query rows [row0, row0 + rows) of a sequence; keys [lo, hi) are those
 // that some row sees, and blocks of keys start at `base`.
 struct Tile {
@@ -287,7 +293,7 @@ __device__ __forceinline__ Tile tile_of(const Params& a, int b, int t, const Seq
     r.rows = min(MR, s.n * a.group - r.row0);
     const int first = s.first_pos + r.row0 / a.group, last = s.first_pos + (r.row0 + max(r.rows, 1) - 1) / a.group;
     r.hi = max(0, min(last + 1, s.len));
-    r.lo = a.window > 0 ? max(0, first + 1 - a.window) : 0;
+    r.lo = lowest_key(a, first);
     if (r.lo >= r.hi) r.lo = r.hi = 0;  // no key
     r.base = r.lo / KEYS * KEYS;
     return r;
@@ -767,7 +773,7 @@ struct WaveRows {
         const int pos1 = t.first_pos + (mine.row0 + max(mine.rows, 1) - 1) / a.group;
         const int pos = t.first_pos + (mine.row0 + (int)(threadIdx.x & 31)) / a.group;
         mine.hi = mine.rows > 0 ? max(0, min(pos1 + 1, t.hi)) : 0;
-        mine.lo = a.window > 0 ? max(0, pos0 + 1 - a.window) : 0;
+        mine.lo = lowest_key(a, pos0);
         all_hi = min(pos0 + 1, t.hi);
         all_lo = a.window > 0 ? pos1 + 1 - a.window : 0;
         row_hi = min(pos + 1, t.hi);
