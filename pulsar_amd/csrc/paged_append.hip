@@ -5,7 +5,8 @@
 // A thread has sixteen elements of a head, eight and the eight that they are paired with, at a
 // number of the token's heads in turn, with the pairs' cosines and sines in registers; the next
 // head's elements are under way meanwhile.  What vectors of eight do not fit (odd rotations, odd
-// addresses) is done one element at a time by append_any_kernel.
+// addresses) is done one element at a time by append_any_kernel: 16384 tokens, 32 heads on 8 of 80, of which 20 or
+// 40 elements rotate, take 131 us (1.9 TB/s), and 56 (4.6) where all 80 do.
 //
 // Rotations are fp64: the product of an element and an fp32 cosine is exact there, so the sum is
 // rounded once and a 4-bit cache's exponent and codes, which stand next to borders, do not depend
@@ -355,7 +356,7 @@ struct ReadArgs {
 };
 
 // A token's keys' and values' words of eight codes.  (16384 tokens of twice 8 heads of 96, 64 MB in
-// and out, 19 us; waves waiting for memory 63% of their time.)
+// and out, 18.5 us, 3.5 TB/s; waves waiting for memory 63% of their time.)
 template <bool BF16>
 __device__ __forceinline__ void read_token(const ReadArgs& a, int token) {
     const int units = a.dim / 8, items = 2 * a.kv_heads * units;
@@ -469,13 +470,20 @@ int append(const pw4_paged_append_args* a, bool fp4, pw4_stream_t stream) {
         constexpr bool BF16 = decltype(bf16)::value, FP4 = decltype(four)::value;
         if (!vec) {
             const int64_t passes = ceil_div(heads, kThreads / (a->head_dim / 8));
+            // Several workgroups a token and one, us, heads of 80, 20 elements rotated: 1 token 3.6 and 4.3, 64 3.9 and
+            // 4.6, 256 4.9 and 4.9, 512 7.4 and 7.0, 1024 (the last one shared) 12.4 and 10.0, 2048 22 and 17.
             const int64_t shares = a->num_tokens * passes <= 8 * device_cus() ? passes : 1;
             hipLaunchKernelGGL((append_any_kernel<BF16, FP4>), dim3((unsigned)std::min(a->num_tokens, kMostGroups), (unsigned)shares),
                                dim3(kThreads), 0, s, p);
             return;
         }
         // Rows of lanes of a workgroup, and how many of them share a token: all, each with a head, where
-        // tokens are few; else 8, so that a row's cosines serve several heads.
+        // tokens are few; else 8, so that a row's cosines serve several heads.  A head a row and 8 rows a token, us,
+        // 32 heads on 8 (the rule goes over between the last two of each): heads of 128, 64 tokens 3.0 and 6.2, 512
+        // 5.8 and 8.6, 1024 9.1 and 9.3, 2048 13.6 and 11.7, into 4 bits 3.6 and 6.8, 6.4 and 9.0, 10.5 and 9.8, 16.6
+        // and 12.0; of 256, 512 tokens 8.9 and 9.3, 1024 13.2 and 12.1.  16384 tokens by 2, 4, 8, 16 and 32 rows a
+        // token: heads of 128 92, 87, 83, 79 and 85, into 4 bits 80, 76, 75, 78 and 99; of 96 75, 72, 64, 68 and 80;
+        // of 256, 16 on 4, 88, 83, 80, 85 and 85; of 64, 14 on 2, 22, 19, 21, 24 and 23.
         const int64_t rows = kThreads / 64 * (64 / (a->head_dim / 16));
         const bool few = a->num_tokens * heads <= 8 * device_cus() * rows;
         p.abreast = (int32_t)std::min<int64_t>(few ? rows : std::min<int64_t>(8, rows), heads);
@@ -531,6 +539,8 @@ int pw4_paged_cache_read_fp4(const void* k_cache, const void* v_cache, const int
                      (uint32_t)head_dim / 2, (uint32_t)head_dim / 32, (uint32_t)(kv_heads * page_size * (head_dim / 2)),
                      (int32_t)kv_heads, (int32_t)head_dim, (int32_t)page_size, (int32_t)num_tokens};
     const int64_t passes = ceil_div(2 * kv_heads * (head_dim / 8), kThreads);
+    // Several workgroups a token and one, us, 8 heads of 256: 1 token 2.06 and 2.18, 64 2.22 and 2.49, 256 2.48 and
+    // 2.69, 512 3.1 and 3.1, 4096 10.8 and 9.3; of 128, 1 token 1.92 and 2.01, 256 2.24 and 2.36.
     const int64_t shares = num_tokens * passes <= 8 * device_cus() ? passes : 1;
     const dim3 grid((unsigned)std::min(num_tokens, kMostGroups), (unsigned)shares);
     const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
